@@ -44,7 +44,8 @@ typedef enum SplashStatus {
 typedef enum SplashDType {
   SPLASH_BF16 = 0,
   SPLASH_F32 = 1,
-  SPLASH_F8E4M3 = 2
+  SPLASH_F8E4M3 = 2,
+  SPLASH_F16 = 3
 } SplashDType;
 
 /* (batch, heads, seq, head_dim) view of device memory. */
@@ -443,6 +444,97 @@ int splash_exchange_push(const SplashExchangeArgs* args, void* cuda_stream);
  * array — order them, or use splash_bwd with separate workspaces. */
 #define SPLASH_STATIC_SCRATCH_MAX_ROWS (1 << 20)
 int splash_bwd_static_scratch(const SplashBwdArgs* args, void* cuda_stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Quantised key / value cache: written token by token, read back, and attended to in place.  No
+ * counterpart in the reference, which has no cache (it dequantises quantised operands before its
+ * attention, tokamax/_src/quantization.py:75-78).
+ *
+ * Tokens lie in pages of `page_size` tokens (a power of two, 16 at least); a token's place is its slot,
+ * page * page_size + offset.  Each array is contiguous and 16-byte aligned:
+ *   k_codes [n_pages, kv_heads, page_size, row bytes]   row bytes: row_k / 2 (int4) or row_k (e4m3)
+ *   k_scales, int4: bf16 [n_pages, kv_heads, page_size, row_k / group, 2], a zero and a scale for each group of
+ *                   channels; e4m3: bf16 [n_pages, kv_heads, page_size], the scale of the row
+ *   v_codes, v_scales: the same with row_v.
+ * A row is padded from head_dim to row_k channels, (row_k, row_v) being one of (64, 64), (96, 96), (128, 128),
+ * (192, 128), (192, 192), (256, 256) (splash_cache_row_widths picks one).
+ *   int4: channel c is the low (c even) or high half of byte c / 2; value = zero + scale * code, with
+ *         zero = bf16(least), scale = bf16((most - least) / 15) over the group, code = round((x - zero) / scale)
+ *         clamped to 0 .. 15 (0 where scale is 0), all of it in 32 bits, ties to even
+ *   e4m3: value = scale * code, scale = bf16(amax / 448), code = e4m3(x / scale), saturating
+ * A group (row) with a value that is not finite is held, and read back, as NaN.
+ * ---------------------------------------------------------------------------------------- */
+typedef enum SplashCacheFormat { SPLASH_CACHE_INT4 = 0, SPLASH_CACHE_E4M3 = 1 } SplashCacheFormat;
+
+typedef struct SplashKvCache {
+  void* k_codes;
+  void* k_scales;
+  void* v_codes;
+  void* v_scales;
+  int64_t n_pages;
+  int32_t format;               /* SplashCacheFormat */
+  int32_t page_size, kv_heads;
+  int32_t group;                /* int4: 32, 64 or 128 channels, dividing row_k and row_v; e4m3: ignored */
+  int32_t head_dim, head_dim_v; /* multiples of 8, at most 256 */
+  int32_t row_k, row_v;
+} SplashKvCache;
+
+/* The padded widths of rows of head_dim and head_dim_v channels. */
+int splash_cache_row_widths(int32_t head_dim, int32_t head_dim_v, int32_t* row_k, int32_t* row_v);
+
+/* Writes k [batch, kv_heads, tokens, head_dim] and v [.., head_dim_v] (one type of bf16, f16, f32; strides multiples
+ * of 8 elements) into the slots [batch, tokens] (row stride slot_stride).  A slot outside 0 .. n_pages * page_size - 1
+ * (-1, say) means that the token is not kept.  Of two tokens of one call with the same slot either may remain, or a row
+ * of one beside a row of the other. */
+typedef struct SplashCacheAppendArgs {
+  SplashKvCache cache;
+  SplashTensor k, v;
+  const void* slots;
+  int32_t slots_are_64;         /* 1: int64, 0: int32 */
+  int64_t slot_stride;
+} SplashCacheAppendArgs;
+int splash_cache_append(const SplashCacheAppendArgs* args, void* cuda_stream);
+
+/* Writes the first lengths[b] tokens of the sequences to k [batch, kv_heads, max_len, head_dim] and v [.., head_dim_v]
+ * (one type of bf16, f16, f32; values are rounded to it once); zeros behind them.  page_table [batch, n_table] int32
+ * (row stride table_stride): the page of tokens i * page_size ..; tokens on a page outside 0 .. n_pages - 1, and
+ * those that the table does not reach, read as zeros.  lengths [batch] int32 on the device. */
+typedef struct SplashCacheReadArgs {
+  SplashKvCache cache;
+  SplashTensor k, v;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t n_table;
+  const int32_t* lengths;
+} SplashCacheReadArgs;
+int splash_cache_read(const SplashCacheReadArgs* args, void* cuda_stream);
+
+/* Attention of the newest q_len tokens of each sequence over the cache: o = softmax(mask(scale * q k^T)) v on the
+ * dequantised rows, fp32 accumulation, q [batch, q_heads, q_len, head_dim] and o [.., head_dim_v] of one type, bf16 or
+ * f16.  Query i of sequence b stands at position lengths[b] - q_len + i and sees the keys at j <= position, with
+ * window >= 0 also j >= position - window, except those on pages outside the cache or that the table does not reach.  q head h reads kv head
+ * h / (q_heads / kv_heads).  soft_cap, sinks, logsumexp, max_logits, mask_value: as for splash_fwd.  A row that sees
+ * nothing is zeros, its logsumexp and max_logits the mask value (with a sink: the sink's logit).
+ * The grid, and with it the order of sums, follows from sizes and lengths alone: results repeat bit for bit. */
+typedef struct SplashCacheAttendArgs {
+  SplashKvCache cache;
+  SplashTensor q, o;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t n_table;
+  const int32_t* lengths;
+  float* logsumexp;             /* fp32 [batch, q_heads, q_len], or NULL */
+  float* max_logits;            /* the same, or NULL */
+  const float* sinks;           /* fp32 [q_heads], or NULL */
+  float scale, soft_cap;        /* soft_cap 0: off */
+  int32_t window;               /* negative: none */
+  float mask_value;
+  void* workspace;              /* splash_cache_attend_workspace_bytes, 16-byte aligned; need not be zeroed */
+  size_t workspace_bytes;
+} SplashCacheAttendArgs;
+int splash_cache_attend(const SplashCacheAttendArgs* args, void* cuda_stream);
+/* Reads the sizes in `args`, nothing on the device; 0 for sizes that splash_cache_attend refuses. */
+size_t splash_cache_attend_workspace_bytes(const SplashCacheAttendArgs* args);
 
 /* Copies the 4-word device error record to host (synchronises the stream) and maps it to a
  * status: SPLASH_OK or SPLASH_ERR_KERNEL_TIMEOUT.  record_out may be NULL. */

@@ -1,0 +1,363 @@
+"""The quantised key / value cache against its definition in 64 bits: rows written and read back, attention over them."""
+import math
+
+import pytest
+import torch
+
+from oracle import kv_cache_ref
+from tokamax_b200 import kv_cache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+ROUNDOFF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}  # half a step of the type, at most, of a value
+FORMATS = [("int4", 32), ("int4", 64), ("int4", 128), ("e4m3", None)]
+
+
+class Store:
+  """A cache with sequences of the given lengths on scattered pages, and what it should hold."""
+
+  def __init__(self, lengths, *, heads=2, d=64, d_v=None, fmt="int4", group=32, page=16, dtype=torch.bfloat16, seed=0, spare=0,
+               keys=None, values=None):
+    g = torch.Generator().manual_seed(seed)
+    d_v = d if d_v is None else d_v
+    used = [-(-n // page) for n in lengths]
+    order = torch.randperm(sum(used) + 1 + spare, generator=g).tolist()
+    width = max(max(used), 1)
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(used):
+      table[b, :n] = torch.tensor(order[at:at + n], dtype=torch.int32)
+      at += n
+    self.fmt, self.group, self.d, self.d_v, self.heads, self.page = fmt, group, d, d_v, heads, page
+    self.lengths_list = lengths
+    self.cache = kv_cache.make_kv_cache(len(order), page, heads, d, d_v, fmt=fmt, group_size=group, device=DEV)
+    self.table, self.lengths = table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    longest = max(max(lengths), 1)
+    make = lambda c: torch.randn(len(lengths), heads, longest, c, generator=g)  # noqa: E731
+    k = make(d) + torch.randn(1, heads, 1, d, generator=g) ** 3  # some channels of a head carry an offset
+    v = make(d_v) * torch.exp(torch.randn(len(lengths), heads, longest, 1, generator=g))
+    self.k, self.v = (x.to(dtype) for x in (k if keys is None else keys(k), v if values is None else values(v)))
+    positions = torch.arange(longest)[None, :].expand(len(lengths), -1)
+    positions = torch.where(positions < torch.tensor(lengths)[:, None], positions, -1).to(DEV)
+    self.slots = kv_cache.slots_of(self.cache, self.table, positions)
+    kv_cache.append(self.cache, self.k.to(DEV), self.v.to(DEV), self.slots)
+
+  def held(self, b):
+    n = self.lengths_list[b]
+    return tuple(kv_cache_ref.held(x[b, :, :n], self.fmt, self.group) for x in (self.k, self.v))
+
+
+def _check_read(store, dtype, max_len):
+  k, v = kv_cache.read(store.cache, store.table, store.lengths, max_len, dtype=dtype)
+  for b, n in enumerate(store.lengths_list):
+    n = min(n, max_len)
+    for got, ref in zip((k[b], v[b]), store.held(b)):
+      assert got.dtype == dtype and not got[:, n:].any()
+      # zero + scale * code is rounded to 32 bits once (zero and the product are exact), then to dtype
+      assert torch.equal(got[:, :n].cpu(), ref[:, :n].float().to(dtype))
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("d,d_v", [(64, 64), (80, 80), (96, 96), (128, 128), (128, 64), (192, 128), (160, 160), (256, 256), (8, 8)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_come_back_as_the_format_holds_them(fmt, group, d, d_v, dtype):
+  try:
+    store = Store([0, 1, 77, 33], heads=3, d=d, d_v=d_v, fmt=fmt, group=group, page=32, dtype=dtype)
+  except ValueError as e:
+    assert "group_size" in str(e) and group in (64, 128)
+    return
+  _check_read(store, torch.float32, 77)
+  _check_read(store, dtype, 96)
+  _check_read(store, torch.bfloat16, 50)  # shorter than the sequences
+
+
+def test_f32_rows_are_held_to_within_half_a_step():
+  """In 32 bits x / scale may fall on the other side of a tie than in 64: a step more, for values within rounding of one."""
+  for fmt, group in FORMATS:
+    store = Store([300], heads=2, d=128, fmt=fmt, group=group, page=64, dtype=torch.float32)
+    k, v = kv_cache.read(store.cache, store.table, store.lengths, 300, dtype=torch.float32)
+    for got, ref, x in zip((k[0], v[0]), store.held(0), (store.k[0], store.v[0])):
+      off = (got.cpu().double() - ref).abs() > 2.0 ** -22 * (1 + ref.abs())
+      assert off.float().mean() <= 1e-4, fmt
+      if fmt == "int4":
+        parts = x.double().unflatten(-1, (-1, group))
+        scale = ((parts.amax(-1) - parts.amin(-1)) / 15).repeat_interleave(group, -1)
+        # half a step; a scale rounded down leaves the last code 15 * 2^-9 of a step short; the zero's own rounding
+        bound = scale * (0.5 + 15 * 2.0 ** -9) * (1 + 2.0 ** -8) + 2.0 ** -8 * parts.amin(-1).abs().repeat_interleave(group, -1)
+        assert ((got.cpu().double() - x.double()).abs() <= bound).all()
+
+
+def test_tokens_of_a_projection_are_written_through_their_strides():
+  store = Store([40, 23], heads=2, d=64, group=64)
+  fresh = Store([40, 23], heads=2, d=64, group=64, seed=1)
+  qkv = torch.zeros(2, 40, 3, 2, 64, dtype=torch.bfloat16, device=DEV)
+  qkv[:, :, 1] = store.k.to(DEV).transpose(1, 2)
+  qkv[:, :, 2] = store.v.to(DEV).transpose(1, 2)
+  k, v = qkv[:, :, 1].transpose(1, 2), qkv[:, :, 2].transpose(1, 2)
+  assert not k.is_contiguous()
+  slots = kv_cache.slots_of(fresh.cache, fresh.table, torch.where(store.slots >= 0, torch.arange(40, device=DEV)[None], -1))
+  odd = torch.full((2, 81), -7, dtype=torch.int32, device=DEV)[:, ::2][:, :40]  # int32, every second element
+  odd.copy_(slots)
+  kv_cache.append(fresh.cache, k, v, odd)
+  fresh.k, fresh.v = store.k, store.v
+  _check_read(fresh, torch.float32, 40)
+  odd_k = torch.zeros(2, 2, 40, 65, dtype=torch.bfloat16, device=DEV)[..., 1:]  # rows that start between 16-byte boundaries
+  odd_k.copy_(k)
+  kv_cache.append(fresh.cache, odd_k, v, slots)
+  _check_read(fresh, torch.float32, 40)
+
+
+def test_slots_outside_the_cache_are_not_kept():
+  store = Store([16, 16], heads=1, d=64, spare=2)
+  before = [t.clone() for t in (store.cache.k_codes, store.cache.k_scales, store.cache.v_codes, store.cache.v_scales)]
+  n = store.cache.n_pages * 16
+  slots = torch.tensor([[-1, n, n + 5, -(1 << 40), 1 << 40]], device=DEV)
+  x = torch.randn(1, 1, 5, 64, device=DEV)
+  kv_cache.append(store.cache, x, x, slots)
+  kv_cache.append(store.cache, x[:, :, :3], x[:, :, :3], slots[:, :3].int())
+  for a, t in zip(before, (store.cache.k_codes, store.cache.k_scales, store.cache.v_codes, store.cache.v_scales)):
+    assert torch.equal(a, t)
+
+
+def test_pages_outside_the_cache_read_as_zeros_and_are_not_seen():
+  store = Store([70, 64, 100], heads=2, d=64, spare=3)
+  table = store.table.clone()
+  table[0, 1], table[1, 0], table[2, 2], table[2, 6] = -1, store.cache.n_pages, 2 ** 31 - 1, -5
+  k, _ = kv_cache.read(store.cache, table, store.lengths, 100, dtype=torch.float32)
+  whole, _ = kv_cache.read(store.cache, store.table, store.lengths, 100, dtype=torch.float32)
+  seen = torch.ones(3, 100, dtype=torch.bool)
+  seen[0, 16:32], seen[1, :16], seen[2, 32:48], seen[2, 96:] = False, False, False, False
+  assert torch.equal(k, torch.where(seen[:, None, :, None].to(DEV), whole, 0.0))
+  _check_attend(store, q_heads=4, t=3, seen=seen, table=table)
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+def test_groups_with_values_that_are_not_finite_are_nan_and_constant_ones_exact(fmt, group):
+  def spoil(x):
+    x[0, 0, 0, 3] = math.inf
+    x[0, 0, 1, 70] = -math.inf
+    x[0, 1, 2, 127] = math.nan
+    x[0, 1, 3] = 0.0
+    x[0, 1, 4] = 1.5
+    x[0, 1, 5] = -0.0
+    return x
+
+  store = Store([6], heads=2, d=128, fmt=fmt, group=group, keys=spoil, values=spoil)
+  k, v = kv_cache.read(store.cache, store.table, store.lengths, 6, dtype=torch.float32)
+  for got, ref in zip((k[0], v[0]), store.held(0)):
+    assert torch.equal(got.cpu().isnan(), ref.isnan()) and int(ref.isnan().sum()) > 0
+    # values near 1.5 of an e4m3 row are a step of its scale's rounding away; an int4 group of one value is exact
+    assert torch.allclose(got.cpu().double().nan_to_num(), ref.nan_to_num(), rtol=2.0 ** -22, atol=0)
+  if fmt == "int4":
+    assert (k[0, 1, 4] == 1.5).all() and not k[0, 1, 3].any()
+
+
+# ----------------------------------------------------------------------------------------------
+# attention
+# ----------------------------------------------------------------------------------------------
+def _check_attend(store, *, q_heads, t=1, window=None, soft_cap=None, sinks=None, seen=None, table=None, dtype=torch.bfloat16,
+                  q_scale=1.5, scale=None, seed=5):
+  g = torch.Generator().manual_seed(seed)
+  scale = store.d ** -0.5 if scale is None else scale
+  q = (torch.randn(len(store.lengths_list), t, q_heads, store.d, generator=g) * q_scale).to(dtype).transpose(1, 2)
+  o, res = kv_cache.attend(store.cache, q.to(DEV), store.table if table is None else table, store.lengths, logits_scale=scale,
+                           local_window_size=window, logits_soft_cap=soft_cap,
+                           sinks=None if sinks is None else sinks.to(DEV), save_residuals=True)
+  assert o.dtype == dtype and o.shape == (*q.shape[:3], store.d_v)
+  for b, n in enumerate(store.lengths_list):
+    k, v = store.held(b)
+    moved = kv_cache_ref.products(store.v[b, :, :n], store.fmt, store.group)
+    ref, lse, top, size, moved = kv_cache_ref.attend(q[b].double(), k, v, scale=scale, window=window, soft_cap=soft_cap, sinks=sinks,
+                                                     seen=None if seen is None else seen[b, :n], weights=moved)
+    # Rounding: of P * scale to f16, 2^-11 of each term (plus a little for sums in 32 bits: 2^-18); of logits, 2^-24 of each
+    # of some hundred partial sums of size |q| |k| scale, which moves each p, and with it o, by up to twice that in all; of
+    # o to its type.
+    logits = (q[b].double().norm(dim=-1).max() * (k.norm(dim=-1).max() if n else 0.0) * scale).clamp_min(1.0)
+    slack = 2.0 ** -18 * logits
+    err = (o[b].cpu().double() - ref).abs()
+    before = (ROUNDOFF[torch.float16] + 2.0 ** -18) * moved + 2 * slack * size + 1e-9
+    least = 2.0 ** -25 if dtype == torch.float16 else 0.0  # half a step of f16's subnormals
+    bound = before + ROUNDOFF[dtype] * (ref.abs() + before) + least
+    assert (err <= bound).all(), (b, n, float(err.max()), float((err / bound).max()))
+    for got, want in ((res["logsumexp"], lse), (res["max_logits"], top)):
+      got, dead = got[b].cpu().double(), want == kv_cache_ref.MASK_VALUE
+      assert (got[dead] <= -2e38).all() and not o[b].cpu()[dead].any()
+      assert ((got - want).abs()[~dead] <= slack + 2.0 ** -20 * (1 + want.abs()[~dead])).all()
+  return o
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("d,d_v", [(64, 64), (80, 80), (96, 96), (128, 128), (128, 64), (192, 128), (160, 160), (256, 256), (8, 8)])
+@pytest.mark.parametrize("q_heads,t", [(2, 1), (6, 1), (16, 1), (10, 5)])
+def test_attention_of_every_shape(fmt, group, d, d_v, q_heads, t):
+  try:
+    store = Store([0, 1, 7, 63, 64, 65, 700], d=d, d_v=d_v, fmt=fmt, group=group, page=16)
+  except ValueError as e:
+    assert "group_size" in str(e) and group in (64, 128)
+    return
+  _check_attend(store, q_heads=q_heads, t=t)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 256])
+@pytest.mark.parametrize("fmt", ["int4", "e4m3"])
+@pytest.mark.parametrize("lengths", [[2900], [257, 4097], list(range(3, 43))])
+def test_rows_shared_by_many_ctas_and_ctas_with_many_rows(page, fmt, lengths):
+  store = Store(lengths, heads=1, d=128, fmt=fmt, group=64 if fmt == "int4" else None, page=page)
+  first = _check_attend(store, q_heads=4)
+  again = _check_attend(store, q_heads=4)
+  assert torch.equal(first, again)
+
+
+@pytest.mark.parametrize("fmt", ["int4", "e4m3"])
+@pytest.mark.parametrize("window", [0, 1, 15, 100, 5000])
+@pytest.mark.parametrize("t", [1, 9])
+def test_window(fmt, window, t):
+  store = Store([1, 8, 9, 100, 1000, 1300], d=64, fmt=fmt, group=32 if fmt == "int4" else None)
+  _check_attend(store, q_heads=4, t=t, window=window)
+
+
+@pytest.mark.parametrize("fmt", ["int4", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_soft_cap_and_sinks(fmt, dtype):
+  store = Store([0, 1, 33, 900, 2000], d=128, fmt=fmt, group=64 if fmt == "int4" else None, page=64, dtype=dtype)
+  sinks = torch.tensor([0.5, -1.0, 2.0, 30.0, -40.0, 0.0])
+  _check_attend(store, q_heads=6, soft_cap=5.0, dtype=dtype)
+  _check_attend(store, q_heads=6, sinks=sinks, dtype=dtype)
+  _check_attend(store, q_heads=6, t=2, soft_cap=30.0, sinks=sinks, window=64, dtype=dtype)
+
+
+def test_sizes_of_scales_and_queries():
+  """Tokens whose values differ by powers of ten, queries that are large, small and zero."""
+  for fmt, group in FORMATS:
+    gain = torch.tensor([1e-3, 1.0, 30.0, 0.0, 200.0]).repeat(140)[None, None, :700, None]
+    store = Store([700, 5], d=128, fmt=fmt, group=group, values=lambda v: v * gain)  # pylint: disable=cell-var-from-loop
+    for q_scale, scale in ((1.5, None), (3e-3, 10.0), (900.0, 2e-4), (0.0, 1.0)):
+      _check_attend(store, q_heads=4, t=2, q_scale=q_scale, scale=scale)
+    alike = Store([300], d=128, fmt=fmt, group=group, values=lambda v: v * 3e-6)
+    _check_attend(alike, q_heads=4)
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+def test_what_lies_in_places_that_are_not_seen_has_no_part(fmt, group):
+  """NaN behind the end of a sequence, in pages that nobody holds, and in keys that a window leaves out."""
+  store = Store([50, 21], d=128, fmt=fmt, group=group, page=64, spare=2)
+  clean = _check_attend(store, q_heads=4, t=2, window=20)
+  store.cache.k_scales.view(torch.int16)[store.cache.k_scales == 0] = 0x7fff  # everything never written
+  store.cache.v_scales.view(torch.int16)[store.cache.v_scales == 0] = 0x7fff
+  bad = torch.full((1, 2, 1, 128), math.nan, device=DEV)
+  kv_cache.append(store.cache, bad, bad, store.slots[:1, 5:6])  # in sequence 0, far outside the window
+  assert torch.equal(clean, _attend_again(store, 4, 2, 20))
+  kv_cache.append(store.cache, bad, bad, store.slots[:1, 48:49])  # query 0 stands at 48: both rows see it
+  o = _attend_again(store, 4, 2, 20)
+  assert o[0].isnan().all() and torch.equal(o[1], clean[1])
+  kv_cache.append(store.cache, store.k[:1, :, 48:49].to(DEV), store.v[:1, :, 48:49].to(DEV), store.slots[:1, 48:49])
+  kv_cache.append(store.cache, bad, bad, store.slots[:1, 49:50])  # the newest key: not seen by the query before it
+  o = _attend_again(store, 4, 2, 20)
+  assert torch.equal(o[0, :, 0], clean[0, :, 0]) and o[0, :, 1].isnan().all()
+
+
+def _attend_again(store, q_heads, t, window):
+  g = torch.Generator().manual_seed(5)
+  q = (torch.randn(len(store.lengths_list), t, q_heads, store.d, generator=g) * 1.5).to(torch.bfloat16).transpose(1, 2)
+  return kv_cache.attend(store.cache, q.to(DEV), store.table, store.lengths, logits_scale=store.d ** -0.5, local_window_size=window)
+
+
+def test_lengths_beyond_the_page_table_and_below_zero():
+  store = Store([64, 64], d=64, page=16)
+  lengths = torch.tensor([80, -3], dtype=torch.int32, device=DEV)  # the table holds 64 tokens
+  q = torch.randn(2, 2, 1, 64, device=DEV, dtype=torch.bfloat16)
+  o = kv_cache.attend(store.cache, q, store.table, lengths, logits_scale=0.1)
+  want = kv_cache.attend(store.cache, q, store.table, store.lengths, logits_scale=0.1)
+  assert torch.equal(o[0], want[0]) and not o[1].any()
+  k, _ = kv_cache.read(store.cache, store.table, lengths, 96)
+  assert k[0, :, 63].any() and not k[0, :, 64:].any() and not k[1].any()
+
+
+def test_queries_through_their_strides_and_nothing_at_all():
+  store = Store([90, 31], d=64, group=64)
+  q = torch.randn(2, 4, 3, 64, device=DEV, dtype=torch.bfloat16)
+  call = lambda x: kv_cache.attend(store.cache, x, store.table, store.lengths, logits_scale=0.1)  # noqa: E731
+  want = call(q)
+  wide = torch.zeros(2, 3, 9, 72, device=DEV, dtype=torch.bfloat16)
+  wide[:, :, 2:6, :64] = q.transpose(1, 2)
+  assert torch.equal(call(wide[:, :, 2:6, :64].transpose(1, 2)), want)
+  odd = torch.zeros(2, 4, 3, 67, device=DEV, dtype=torch.bfloat16)[..., 3:]
+  odd.copy_(q)
+  assert torch.equal(call(odd), want)
+  assert call(q[:, :, :0]).shape == (2, 4, 0, 64)
+  empty = store.lengths[:0]
+  assert kv_cache.attend(store.cache, q[:0], store.table[:0], empty).shape == (0, 4, 3, 64)
+  assert kv_cache.read(store.cache, store.table, store.lengths, 0)[0].shape == (2, 2, 0, 64)
+  kv_cache.append(store.cache, q[:, :2, :0], q[:, :2, :0], store.slots[:, :0])
+
+
+def test_offsets_beyond_32_bits():
+  """Codes of the pages at the end lie more than 2^32 bytes from the first."""
+  page, heads, d = 4096, 8, 256
+  n_pages = (1 << 32) // (page * heads * d) + 2
+  cache = kv_cache.make_kv_cache(n_pages, page, heads, d, fmt="e4m3", device=DEV)
+  g = torch.Generator(device=DEV).manual_seed(0)
+  k, v = (torch.randn(1, heads, 100, d, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+  table = torch.tensor([[n_pages - 1], [0]], dtype=torch.int32, device=DEV)
+  lengths = torch.tensor([100, 100], dtype=torch.int32, device=DEV)
+  positions = torch.arange(100, device=DEV)[None]
+  for row in range(2):
+    kv_cache.append(cache, k, v, kv_cache.slots_of(cache, table[row:row + 1], positions))
+  q = torch.randn(1, heads, 1, d, generator=g, device=DEV).to(torch.bfloat16).expand(2, -1, -1, -1)
+  o = kv_cache.attend(cache, q, table, lengths, logits_scale=d ** -0.5)
+  back, _ = kv_cache.read(cache, table, lengths, 100)
+  assert torch.equal(o[0], o[1]) and torch.equal(back[0], back[1]) and back[0].any()
+  assert torch.equal(back[0].cpu().double(), kv_cache_ref.held(k[0], "e4m3", None).to(torch.bfloat16).double())
+
+
+def test_streams_and_graphs():
+  store = Store([500, 900, 40], d=128, group=64, page=64)
+  q = torch.randn(3, 4, 1, 128, device=DEV, dtype=torch.bfloat16)
+  call = lambda: kv_cache.attend(store.cache, q, store.table, store.lengths, logits_scale=0.1)  # noqa: E731
+  want = call()
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    outs = [call() for _ in range(20)]
+  mine = [call() for _ in range(20)]  # two streams at a time: each call has a workspace of its own
+  side.synchronize()
+  assert all(torch.equal(o, want) for o in outs + mine)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    kv_cache.append(store.cache, q[:, :2], q[:, :2], store.slots[:, :1])
+    o = call()
+  short = torch.tensor([17, 0, 40], dtype=torch.int32, device=DEV)
+  store.lengths.copy_(short)  # lengths change between replays
+  graph.replay()
+  kv_cache.append(store.cache, q[:, :2], q[:, :2], store.slots[:, :1])
+  assert torch.equal(o, call()) and not o[1].any()
+
+
+def test_refusals():
+  store = Store([20, 20], d=64)
+  cache, table, lengths = store.cache, store.table, store.lengths
+  q = torch.zeros(2, 4, 1, 64, device=DEV, dtype=torch.bfloat16)
+  k = torch.zeros(2, 2, 1, 64, device=DEV, dtype=torch.bfloat16)
+  slots = store.slots[:, :1]
+  for bad in (lambda: kv_cache.attend(cache, q[:, :3], table, lengths), lambda: kv_cache.attend(cache, q[..., :32], table, lengths),
+              lambda: kv_cache.attend(cache, q[0], table, lengths), lambda: kv_cache.attend(cache, q, table, lengths[:1]),
+              lambda: kv_cache.attend(cache, q, table.long(), lengths), lambda: kv_cache.attend(cache, q, table, lengths.long()),
+              lambda: kv_cache.attend(cache, q, table.cpu(), lengths), lambda: kv_cache.attend(cache, q.cpu(), table, lengths),
+              lambda: kv_cache.attend(cache, q, table, lengths, local_window_size=-1),
+              lambda: kv_cache.attend(cache, q, table, lengths, logits_soft_cap=0.0),
+              lambda: kv_cache.attend(cache, q, table, lengths, sinks=torch.zeros(3, device=DEV)),
+              lambda: kv_cache.append(cache, k, k[..., :32], slots), lambda: kv_cache.append(cache, k, k.float(), slots),
+              lambda: kv_cache.append(cache, k, k, slots.float()), lambda: kv_cache.append(cache, k, k, slots[:1]),
+              lambda: kv_cache.append(cache, k[:, :1], k[:, :1], slots), lambda: kv_cache.append(cache, k, k, slots.cpu()),
+              lambda: kv_cache.read(cache, table, lengths[:1], 20), lambda: kv_cache.read(cache, table, lengths, -1),
+              lambda: kv_cache.read(cache, table[0], lengths, 20)):
+    with pytest.raises(ValueError):
+      bad()
+  for bad in (lambda: kv_cache.attend(cache, q.float(), table, lengths), lambda: kv_cache.append(cache, k.double(), k.double(), slots),
+              lambda: kv_cache.read(cache, table, lengths, 20, dtype=torch.int32),
+              lambda: kv_cache.attend(cache, q.clone().requires_grad_(True), table, lengths),
+              lambda: kv_cache.append(cache, k.clone().requires_grad_(True), k, slots)):
+    with pytest.raises(NotImplementedError):
+      bad()
+  with torch.no_grad():
+    kv_cache.attend(cache, q.clone().requires_grad_(True), table, lengths)

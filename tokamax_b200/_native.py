@@ -31,6 +31,8 @@ SOURCES = (
     "dynamic_schedule.cu",
     "ring_merge.cu",
     "exchange.cu",
+    "cache_rows.cu",
+    "cache_attend_sm100.cu",
     "splash_xla_ffi.cc",  # handlers compile only where xla/ffi/api/ffi.h is on the include path
 )
 
@@ -211,6 +213,61 @@ class SplashExchangeArgs(C.Structure):
   ]
 
 
+class SplashKvCache(C.Structure):
+  _fields_ = [
+      ("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p), ("v_scales", C.c_void_p),
+      ("n_pages", C.c_int64),
+      ("format", C.c_int32),
+      ("page_size", C.c_int32), ("kv_heads", C.c_int32),
+      ("group", C.c_int32),
+      ("head_dim", C.c_int32), ("head_dim_v", C.c_int32),
+      ("row_k", C.c_int32), ("row_v", C.c_int32),
+  ]
+
+
+CACHE_INT4, CACHE_E4M3 = 0, 1  # SplashCacheFormat
+
+
+class SplashCacheAppendArgs(C.Structure):
+  _fields_ = [
+      ("cache", SplashKvCache),
+      ("k", SplashTensor), ("v", SplashTensor),
+      ("slots", C.c_void_p),
+      ("slots_are_64", C.c_int32),
+      ("slot_stride", C.c_int64),
+  ]
+
+
+class SplashCacheReadArgs(C.Structure):
+  _fields_ = [
+      ("cache", SplashKvCache),
+      ("k", SplashTensor), ("v", SplashTensor),
+      ("page_table", C.c_void_p),
+      ("table_stride", C.c_int64),
+      ("n_table", C.c_int32),
+      ("lengths", C.c_void_p),
+  ]
+
+
+class SplashCacheAttendArgs(C.Structure):
+  _fields_ = [
+      ("cache", SplashKvCache),
+      ("q", SplashTensor), ("o", SplashTensor),
+      ("page_table", C.c_void_p),
+      ("table_stride", C.c_int64),
+      ("n_table", C.c_int32),
+      ("lengths", C.c_void_p),
+      ("logsumexp", C.c_void_p),
+      ("max_logits", C.c_void_p),
+      ("sinks", C.c_void_p),
+      ("scale", C.c_float), ("soft_cap", C.c_float),
+      ("window", C.c_int32),
+      ("mask_value", C.c_float),
+      ("workspace", C.c_void_p),
+      ("workspace_bytes", C.c_size_t),
+  ]
+
+
 # name -> (restype, argtypes); every function include/splash_b200.h declares.
 _PROTOTYPES = {
     "splash_maskinfo_build": (C.c_int, [C.POINTER(SplashMaskNode), C.c_int32, C.c_int64, C.c_int64,
@@ -243,6 +300,11 @@ _PROTOTYPES = {
     "splash_bwd": (C.c_int, [C.POINTER(SplashBwdArgs), C.c_void_p]),
     "splash_bwd_static_scratch": (C.c_int, [C.POINTER(SplashBwdArgs), C.c_void_p]),
     "splash_exchange_push": (C.c_int, [C.POINTER(SplashExchangeArgs), C.c_void_p]),
+    "splash_cache_row_widths": (C.c_int, [C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
+    "splash_cache_append": (C.c_int, [C.POINTER(SplashCacheAppendArgs), C.c_void_p]),
+    "splash_cache_read": (C.c_int, [C.POINTER(SplashCacheReadArgs), C.c_void_p]),
+    "splash_cache_attend": (C.c_int, [C.POINTER(SplashCacheAttendArgs), C.c_void_p]),
+    "splash_cache_attend_workspace_bytes": (C.c_size_t, [C.POINTER(SplashCacheAttendArgs)]),
     "splash_read_error": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_uint32 * 4)]),
     "splash_probe_bounded_wait": (C.c_int, [C.c_void_p, C.c_int64, C.c_uint32, C.c_void_p]),
     "splash_xla_ffi_compiled": (C.c_int, []),
@@ -362,6 +424,8 @@ def host():
         spec.loader.exec_module(module)
         module.bind_library(*(C.cast(getattr(handle, name), C.c_void_p).value for name in (
             "splash_fwd_shard", "splash_bwd_shard", "splash_bwd_workspace_bytes", "splash_bwd_fused_workspace_bytes")))
+        module.bind_cache_library(*(C.cast(getattr(handle, name), C.c_void_p).value for name in (
+            "splash_cache_append", "splash_cache_read", "splash_cache_attend", "splash_cache_attend_workspace_bytes")))
         module.bind_check(check)
         _host = module
   return _host

@@ -268,10 +268,204 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention(const std::shared_ptr<T
   return {out[0], out[1], out[2]};
 }
 
+// ------------------------------------------------------------------------------------------------------------------
+// the quantised key / value cache (kv_cache.py): checks of arguments, results, launches
+// ------------------------------------------------------------------------------------------------------------------
+struct CacheLibrary {
+  int (*append)(const SplashCacheAppendArgs*, void*) = nullptr;
+  int (*read)(const SplashCacheReadArgs*, void*) = nullptr;
+  int (*attend)(const SplashCacheAttendArgs*, void*) = nullptr;
+  size_t (*attend_workspace_bytes)(const SplashCacheAttendArgs*) = nullptr;
+} cache_lib;
+
+void bind_cache_library(uintptr_t append, uintptr_t read, uintptr_t attend, uintptr_t attend_workspace_bytes) {
+  cache_lib.append = reinterpret_cast<decltype(cache_lib.append)>(append);
+  cache_lib.read = reinterpret_cast<decltype(cache_lib.read)>(read);
+  cache_lib.attend = reinterpret_cast<decltype(cache_lib.attend)>(attend);
+  cache_lib.attend_workspace_bytes = reinterpret_cast<decltype(cache_lib.attend_workspace_bytes)>(attend_workspace_bytes);
+}
+
+// A cache's description, with the tensors that it lies in.
+struct KvCache {
+  SplashKvCache desc{};
+  at::Tensor k_codes, k_scales, v_codes, v_scales;
+
+  KvCache(at::Tensor k_codes_in, at::Tensor k_scales_in, at::Tensor v_codes_in, at::Tensor v_scales_in, int format, int group,
+          int head_dim, int head_dim_v, int row_k, int row_v)
+      : k_codes(std::move(k_codes_in)), k_scales(std::move(k_scales_in)), v_codes(std::move(v_codes_in)), v_scales(std::move(v_scales_in)) {
+    for (const at::Tensor* t : {&k_codes, &k_scales, &v_codes, &v_scales})
+      TORCH_CHECK_VALUE(t->is_contiguous() && t->device() == k_codes.device(), "the arrays of a cache are contiguous, on one device");
+    desc.k_codes = k_codes.data_ptr();
+    desc.k_scales = k_scales.data_ptr();
+    desc.v_codes = v_codes.data_ptr();
+    desc.v_scales = v_scales.data_ptr();
+    desc.n_pages = k_codes.size(0);
+    desc.kv_heads = (int32_t)k_codes.size(1);
+    desc.page_size = (int32_t)k_codes.size(2);
+    desc.format = format;
+    desc.group = group;
+    desc.head_dim = head_dim;
+    desc.head_dim_v = head_dim_v;
+    desc.row_k = row_k;
+    desc.row_v = row_v;
+  }
+};
+
+void require_on_gpu(const at::Tensor& t, const KvCache& cache, const char* name) {
+  TORCH_CHECK(cache.k_codes.is_cuda(), "a cache on ", cache.k_codes.device(), ": the kernels need a CUDA device");
+  TORCH_CHECK_VALUE(t.device() == cache.k_codes.device(), name, " is on ", t.device(), ", the cache on ", cache.k_codes.device());
+}
+
+// The result of a cache's operator cannot be differentiated: refused rather than cut off from its inputs without a word.
+void require_no_grad(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+                              " requires a gradient: the cache's operators have none (call them under torch.no_grad())");
+}
+
+SplashTensor describe_row_tensor(const at::Tensor& t, const char* name, bool f32_too) {
+  SplashTensor d{};
+  const auto type = t.scalar_type();
+  TORCH_CHECK_NOT_IMPLEMENTED(type == at::kBFloat16 || type == at::kHalf || (f32_too && type == at::kFloat), name, ": ", type,
+                              " is not built (bfloat16, float16", f32_too ? ", float32)" : ")");
+  d.dtype = type == at::kBFloat16 ? SPLASH_BF16 : type == at::kHalf ? SPLASH_F16 : SPLASH_F32;
+  d.data = t.data_ptr();
+  for (int i = 0; i < 4; ++i) d.size[i] = t.size(i), d.stride[i] = t.stride(i);
+  return d;
+}
+
+// Raises what `status` stands for; called with the interpreter's lock held.
+void check_cache_call(int status, const char* what) {
+  if (status == 0) return;
+  TORCH_CHECK_NOT_IMPLEMENTED(status != SPLASH_ERR_UNSUPPORTED, what, ": not built for these sizes or types");
+  Py_XDECREF(PyObject_CallFunction(check_status, "is", status, what));
+  throw python_error();
+}
+
+template <typename Fn>
+int on_stream_of(const at::Tensor& t, Fn&& call) {
+  const WithoutGil release;
+  const c10::OptionalDeviceGuard guard(t.device());
+  return call(static_cast<void*>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()));
+}
+
+void cache_append(const KvCache& cache, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& slots_in) {
+  const SplashKvCache& c = cache.desc;
+  TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.dim() == 4 && slots_in.dim() == 2, "expected k and v of [B, H, T, D] and slots of [B, T]");
+  TORCH_CHECK_VALUE(k_in.size(1) == c.kv_heads && k_in.size(3) == c.head_dim && v_in.size(3) == c.head_dim_v, "k ", k_in.sizes(), " / v ",
+                    v_in.sizes(), " do not match a cache of ", c.kv_heads, " heads of ", c.head_dim, " / ", c.head_dim_v, " channels");
+  TORCH_CHECK_VALUE(v_in.sizes().slice(0, 3) == k_in.sizes().slice(0, 3) && slots_in.size(0) == k_in.size(0) && slots_in.size(1) == k_in.size(2),
+                    "k ", k_in.sizes(), ", v ", v_in.sizes(), " and slots ", slots_in.sizes(), " do not match");
+  TORCH_CHECK_VALUE(k_in.scalar_type() == v_in.scalar_type(), "k and v have one type, got ", k_in.scalar_type(), " and ", v_in.scalar_type());
+  const auto type = slots_in.scalar_type();
+  TORCH_CHECK_VALUE(type == at::kInt || type == at::kLong, "slots are int32 or int64, got ", type);
+  require_on_gpu(k_in, cache, "k");
+  require_on_gpu(v_in, cache, "v");
+  require_on_gpu(slots_in, cache, "slots");
+  require_no_grad(k_in, "k");
+  require_no_grad(v_in, "v");
+  SplashCacheAppendArgs a{};
+  a.cache = c;
+  if (slots_in.numel() == 0) return;
+  const at::Tensor k = usable(k_in), v = usable(v_in), slots = slots_in.stride(1) == 1 || slots_in.size(1) == 1 ? slots_in : slots_in.contiguous();
+  a.k = describe_row_tensor(k, "k", true);
+  a.v = describe_row_tensor(v, "v", true);
+  a.slots = slots.data_ptr();
+  a.slots_are_64 = type == at::kLong;
+  a.slot_stride = slots.stride(0);
+  check_cache_call(on_stream_of(k, [&](void* stream) { return cache_lib.append(&a, stream); }), "splash_cache_append");
+}
+
+// A page table [B, pages] and the lengths [B] of the sequences, as the kernels take them.
+template <typename Args>
+at::Tensor set_pages(Args& a, const KvCache& cache, const at::Tensor& table_in, const at::Tensor& lengths) {
+  TORCH_CHECK_VALUE(table_in.dim() == 2 && lengths.dim() == 1 && table_in.size(0) == lengths.size(0), "page table ", table_in.sizes(),
+                    " and lengths ", lengths.sizes(), " do not match: expected [B, pages] and [B]");
+  TORCH_CHECK_VALUE(table_in.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt, "the page table and the lengths are int32");
+  require_on_gpu(table_in, cache, "the page table");
+  require_on_gpu(lengths, cache, "lengths");
+  TORCH_CHECK_VALUE(lengths.size(0) <= 1 || lengths.stride(0) == 1, "lengths are contiguous");
+  const at::Tensor table = table_in.size(1) <= 1 || table_in.stride(1) == 1 ? table_in : table_in.contiguous();
+  TORCH_CHECK_VALUE(table.size(1) >= 1 && table.size(1) <= INT32_MAX, "a page table of ", table.size(1), " pages");
+  a.cache = cache.desc;
+  a.page_table = static_cast<const int32_t*>(table.data_ptr());
+  a.table_stride = table.stride(0);
+  a.n_table = (int32_t)table.size(1);
+  a.lengths = static_cast<const int32_t*>(lengths.data_ptr());
+  return table;
+}
+
+std::tuple<at::Tensor, at::Tensor> cache_read(const KvCache& cache, const at::Tensor& table_in, const at::Tensor& lengths, int64_t max_len,
+                                              at::ScalarType type) {
+  const SplashKvCache& c = cache.desc;
+  SplashCacheReadArgs a{};
+  const at::Tensor table = set_pages(a, cache, table_in, lengths);
+  TORCH_CHECK_VALUE(max_len >= 0, "max_len is not negative, got ", max_len);
+  const auto options = cache.k_codes.options().dtype(type);
+  const at::Tensor k = at::empty({lengths.size(0), c.kv_heads, max_len, c.head_dim}, options);
+  const at::Tensor v = at::empty({lengths.size(0), c.kv_heads, max_len, c.head_dim_v}, options);
+  a.k = describe_row_tensor(k, "dtype", true);
+  a.v = describe_row_tensor(v, "dtype", true);
+  if (k.numel() != 0)
+    check_cache_call(on_stream_of(k, [&](void* stream) { return cache_lib.read(&a, stream); }), "splash_cache_read");
+  return {k, v};
+}
+
+std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at::Tensor& q_in, const at::Tensor& table_in,
+                                                  const at::Tensor& lengths, double scale, std::optional<int64_t> window,
+                                                  std::optional<double> soft_cap, const Maybe& sinks_in, double mask_value, bool residuals) {
+  const SplashKvCache& c = cache.desc;
+  TORCH_CHECK_VALUE(q_in.dim() == 4 && q_in.size(3) == c.head_dim && q_in.size(1) % c.kv_heads == 0, "q ", q_in.sizes(),
+                    " does not match a cache of ", c.kv_heads, " heads of ", c.head_dim, " channels: expected [B, heads, T, D]");
+  SplashCacheAttendArgs a{};
+  const at::Tensor table = set_pages(a, cache, table_in, lengths);
+  TORCH_CHECK_VALUE(q_in.size(0) == lengths.size(0), "q of ", q_in.size(0), " sequences, lengths of ", lengths.size(0));
+  TORCH_CHECK_VALUE(!window.has_value() || (*window >= 0 && *window <= INT32_MAX), "local_window_size is not negative");
+  TORCH_CHECK_VALUE(!soft_cap.has_value() || *soft_cap > 0, "logits_soft_cap is positive");
+  require_on_gpu(q_in, cache, "q");
+  require_no_grad(q_in, "q");
+  const int64_t b = q_in.size(0), heads = q_in.size(1), t = q_in.size(2);
+  Maybe sinks;
+  if (sinks_in.has_value()) {
+    TORCH_CHECK_VALUE(sinks_in->dim() == 1 && sinks_in->size(0) == heads, "sinks ", sinks_in->sizes(), " for ", heads, " q heads");
+    require_on_gpu(*sinks_in, cache, "sinks");
+    require_no_grad(*sinks_in, "sinks");
+    sinks = sinks_in->to(at::kFloat).contiguous();
+    a.sinks = static_cast<const float*>(sinks->data_ptr());
+  }
+  const at::Tensor q = usable(q_in);
+  a.q = describe_row_tensor(q, "q", false);
+  // (like q, it keeps q's dense stride order)
+  const at::Tensor o = c.head_dim_v == c.head_dim ? at::empty_like(q) : at::empty({b, heads, t, c.head_dim_v}, q.options());
+  a.o = describe_row_tensor(o, "o", false);
+  Maybe lse, max_logits;
+  if (residuals) {
+    lse = at::empty({b, heads, t}, q.options().dtype(at::kFloat));
+    max_logits = at::empty({b, heads, t}, q.options().dtype(at::kFloat));
+    a.logsumexp = static_cast<float*>(lse->data_ptr());
+    a.max_logits = static_cast<float*>(max_logits->data_ptr());
+  }
+  if (o.numel() == 0) return {o, lse, max_logits};
+  a.scale = (float)scale;
+  a.soft_cap = (float)soft_cap.value_or(0.0);
+  a.window = window.has_value() ? (int32_t)*window : -1;
+  a.mask_value = (float)mask_value;
+  a.workspace_bytes = cache_lib.attend_workspace_bytes(&a);
+  const at::Tensor workspace = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
+  a.workspace = workspace.data_ptr();
+  check_cache_call(on_stream_of(q, [&](void* stream) { return cache_lib.attend(&a, stream); }), "splash_cache_attend");
+  return {o, lse, max_logits};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_splash_torch, m) {
   m.def("bind_library", &bind_library);
+  m.def("bind_cache_library", &bind_cache_library);
+  pybind11::class_<KvCache>(m, "KvCache")
+      .def(pybind11::init<at::Tensor, at::Tensor, at::Tensor, at::Tensor, int, int, int, int, int, int>());
+  m.def("cache_append", torch::wrap_pybind_function(cache_append));
+  m.def("cache_read", torch::wrap_pybind_function(cache_read));
+  m.def("cache_attend", torch::wrap_pybind_function(cache_attend));
   m.def("forward", torch::wrap_pybind_function(forward));
   m.def("backward", torch::wrap_pybind_function(backward));
   m.def("bind_check", [](pybind11::object check) { check_status = check.release().ptr(); });
