@@ -45,10 +45,10 @@ struct AttendParams {
   const float* sinks;
   // workspace: for each CTA two items it may share with others, sums [rows][row_v], then max and sum [2][rows]
   float* parts;
-  int64_t* starts;  // [batch + 1] first unit of each sequence
+  int64_t* starts;  // [batch + 1] where each sequence begins, in the measure of shares
   int64_t q_stride_b, q_stride_h, q_stride_s, o_stride_b, o_stride_h, o_stride_s, table_stride, n_pages;
   float scale, soft_cap, mask_value;
-  int32_t batch, q_heads, kv_heads, heads_per_kv, q_len, row_tiles, n_table, page_size, page_shift, group, group_shift, dtype;
+  int32_t batch, q_heads, kv_heads, heads_per_kv, q_len, row_tiles, n_table, page_size, page_shift, dtype;
   int32_t head_dim, head_dim_v, window, min_share;
 };
 
@@ -69,6 +69,15 @@ __device__ __forceinline__ void cp_async_wait() {
 __device__ __forceinline__ void ldmatrix_x2(uint32_t addr, uint32_t& a, uint32_t& b) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+               : "r"(addr)
+               : "memory");
+}
 __device__ __forceinline__ void ldmatrix_x2_trans(uint32_t addr, uint32_t& a, uint32_t& b) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
 }
@@ -88,23 +97,25 @@ __device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddep
 // ------------------------------------------------------------------------------------------
 // sizes
 // ------------------------------------------------------------------------------------------
-// kK, kV: padded widths of a row; kN: blocks of eight query rows
-template <int kFormat_, int kK_, int kV_, int kN_>
+// kK, kV: padded widths of a row; kG: channels of a group (int4); kN: blocks of eight query rows
+template <int kFormat_, int kK_, int kV_, int kG_, int kN_>
 struct AttendShape {
   static constexpr int kFormat = kFormat_, kK = kK_, kV = kV_, kN = kN_;
   static constexpr bool kInt4 = kFormat == SPLASH_CACHE_INT4;
   static constexpr int kRows = 8 * kN;
   static constexpr int kRowK = cache_row_bytes(kFormat, kK), kRowV = cache_row_bytes(kFormat, kV);
   // tokens of a unit: about 4 KB, which a warp has in flight for each stage
-  static constexpr int kUnit = kRowK + kRowV <= 64 ? 64 : kRowK + kRowV <= 128 ? 32 : 16;
+  static constexpr int kUnit = kN > 2 ? 16 : kRowK + kRowV <= 64 && kN == 1 ? 64 : kRowK + kRowV <= 128 ? 32 : 16;
   static constexpr int kTiles = kUnit / 16;
   // channels that 16 bytes of codes hold, and MMA steps (16 channels) over them
   static constexpr int kChunk = kInt4 ? 32 : 16, kSteps = kChunk / 16;
+  static constexpr int kGroupsK = kInt4 ? kK / kG_ : 1, kGroupsV = kInt4 ? kV / kG_ : 1;
   static constexpr int kChunksK = kK / kChunk, kChunksV = kV / kChunk;
-  static constexpr int kScaleK = kInt4 ? 4 * (kK / 32) : 2, kScaleV = kInt4 ? 4 * (kV / 32) : 2;  // at most
-  static constexpr int kStageBytes = kUnit * (kRowK + kRowV + kScaleK + kScaleV);
-  static constexpr int kStages = 3;
-  static constexpr int kGroupsK = kInt4 ? kK / 32 : 1, kGroupsV = kInt4 ? kV / 32 : 1;  // at most
+  static constexpr int kPerGroupK = kChunksK / kGroupsK, kPerGroupV = kChunksV / kGroupsV;
+  static constexpr int kScaleK = cache_scale_bytes(kFormat, kK, kG_), kScaleV = cache_scale_bytes(kFormat, kV, kG_);
+  static constexpr int kStageBytes = (kUnit * (kRowK + kRowV + kScaleK + kScaleV) + 127) / 128 * 128;
+  static constexpr int kStages = 2;
+  static constexpr int kResident = kN == 1 && kV <= 128 ? 2 : 1;  // CTAs of an SM
   // shared memory
   static constexpr int kFragBytes = kK / 16 * kN * 256;            // q as fragments
   static constexpr int kQSums = kFragBytes;                        // [kGroupsK][kRows] sums of q over a group
@@ -118,18 +129,79 @@ struct AttendShape {
 };
 
 // Where in a stage 16-byte piece c of row r lies: so that eight consecutive rows' piece c are in eight different bank groups.
+// The low bits of c, those in kTurn, are turned by the row.
 template <int kRowBytes>
-__device__ __forceinline__ int piece_at(int r, int c) {
-  constexpr int kPieces = kRowBytes / 16;
-  const int turn = kPieces % 8 == 0 ? r & 7 : kPieces % 4 == 0 ? (r >> 1) & 3 : kPieces % 2 == 0 ? (r >> 2) & 1 : 0;
-  return r * kRowBytes + ((c ^ turn) << 4);
+struct Pieces {
+  static constexpr int kEach = kRowBytes / 16;
+  static constexpr int kTurn = kEach % 8 == 0 ? 7 : kEach % 4 == 0 ? 3 : kEach % 2 == 0 ? 1 : 0;
+  static constexpr int kShift = kEach % 8 == 0 ? 0 : kEach % 4 == 0 ? 1 : 2;
+  static __device__ __forceinline__ int row_at(int r) { return r * kRowBytes + ((r >> kShift & kTurn) << 4); }
+  // `row`: the address of row_at() in an area that starts at a multiple of 128
+  static __device__ __forceinline__ uint32_t at(uint32_t row, int c) { return (row ^ ((c & kTurn) << 4)) + ((c & ~kTurn) << 4); }
+};
+
+// Sixteen rows of the tile at `place` to `to` (a multiple of 128), 16 bytes a lane and step.
+template <int kRowBytes>
+__device__ __forceinline__ void copy_rows(uint32_t to, const uint8_t* codes, uint32_t place, int lane) {
+  using P = Pieces<kRowBytes>;
+  const uint8_t* const from = codes + ((uint64_t)place * (16 * kRowBytes) + lane * 16);
+  constexpr bool kAlike = 32 % P::kEach == 0 && 32 / P::kEach % 8 == 0;  // every step's rows are turned alike
+  const uint32_t first = to + P::at(P::row_at(lane / P::kEach), lane % P::kEach);
+#pragma unroll
+  for (int j = 0; j < (kRowBytes + 31) / 32; ++j) {
+    const int piece = j * 32 + lane;
+    const uint32_t at = kAlike ? first + j * 512 : to + P::at(P::row_at(piece / P::kEach), piece % P::kEach);
+    if (kRowBytes % 32 == 0 || piece < kRowBytes) cp_async16(at, from + j * 512);
+  }
 }
+
+// A 16-byte piece of the rows of kTiles tiles: words of rows g and g + 8.  `at`: this lane's row of the first two tiles.
+template <int kTiles, int kRowBytes>
+__device__ __forceinline__ void load_tiles(uint32_t at, uint32_t (&words)[kTiles][2]) {
+  if constexpr (kTiles == 1) {
+    ldmatrix_x2(at, words[0][0], words[0][1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kTiles; i += 2) ldmatrix_x4(at + i * 16 * kRowBytes, words[i][0], words[i][1], words[i + 1][0], words[i + 1][1]);
+  }
+}
+
+// kCount consecutive words of shared memory, kCount * 4 bytes from a multiple of that times any number.
+template <int kCount>
+__device__ __forceinline__ void load_words(uint32_t (&w)[kCount], const uint32_t* from) {
+  if constexpr (kCount % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < kCount; i += 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(from + i);
+      w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+    }
+  } else if constexpr (kCount % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < kCount; i += 2) {
+      const uint2 x = *reinterpret_cast<const uint2*>(from + i);
+      w[i] = x.x, w[i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) w[i] = from[i];
+  }
+}
+
+constexpr float kNoMaximum = -1.0e30f;  // of a row that has seen no key yet: finite, so that differences are
+constexpr float kSlack = 8.f;           // how far (in units of log2) logits may pass the maximum that P is taken against
+constexpr int kUnitLog2 = 5;            // P * scale is below 2^(kSlack + 1 + kUnitLog2) = 2^14
+constexpr uint32_t kLeastTop = 87u << 23;  // 2^-40
 
 // ------------------------------------------------------------------------------------------
 // shares
 // ------------------------------------------------------------------------------------------
+// What a CTA spends on an item beside its units, in units: shares are equal in the sum of both.  (Looking up the item, q as
+// fragments, the first keys' latency, the warps' sums together: about what 20 of their units take.)
+constexpr int kItemCost = 20;
+
 struct Keys {  // of a sequence: tokens [lo, hi) in whole units from lo, which is a multiple of kUnit
   int lo, hi, units;
+  __device__ int cost() const { return units > 0 ? units + kItemCost : 0; }
 };
 template <int kUnit>
 __device__ __forceinline__ Keys keys_of(const AttendParams& p, int length) {
@@ -147,7 +219,7 @@ __host__ __device__ inline int64_t share_of(int64_t total, int ctas, int min_sha
 }
 
 struct Start {  // where a CTA's share begins
-  int64_t total, before;  // units of all sequences (for one head and row tile), and before sequence b
+  int64_t total, before;  // cost of all sequences (for one head and row tile), and before sequence b
   int b;
 };
 
@@ -157,7 +229,7 @@ __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
   const int per_sequence = p.kv_heads * p.row_tiles;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t total = 0, mine = 0;  // mine: of the sequences that this thread counts when there is one round of them
-  for (int b = tid; b < p.batch; b += kAttendThreads) total += (mine = keys_of<kUnit>(p, __ldg(p.lengths + b)).units);
+  for (int b = tid; b < p.batch; b += kAttendThreads) total += (mine = keys_of<kUnit>(p, __ldg(p.lengths + b)).cost());
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
   if (lane == 0) scratch[warp] = total;
@@ -172,7 +244,7 @@ __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
   int64_t carry = 0;
   for (int base = 0; base < p.batch; base += kAttendThreads) {
     const int b = base + tid;
-    if (base > 0 || p.batch > kAttendThreads) mine = b < p.batch ? keys_of<kUnit>(p, __ldg(p.lengths + b)).units : 0;
+    if (base > 0 || p.batch > kAttendThreads) mine = b < p.batch ? keys_of<kUnit>(p, __ldg(p.lengths + b)).cost() : 0;
     if (b >= p.batch) mine = 0;
     int64_t sum = mine;
 #pragma unroll
@@ -211,13 +283,34 @@ __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
 // What a row's sums become: the output row, or a part of it in the workspace.  `m` in units of log2, with the sink in it.
 __device__ __forceinline__ void add_sink(float sink, float& m, float& l) {
   const float s = sink * kLog2e, top = fmaxf(m, s);
-  l = l * (m > -INFINITY ? ex2(m - top) : 0.f) + ex2(s - top);
+  l = l * ex2(m - top) + ex2(s - top);
   m = top;
 }
 
+// Eight channels of a row, from the sums of all its keys.
+__device__ __forceinline__ void finish_row(const AttendParams& p, int b, int head, int row, int d, float (&x)[8], float m, float l) {
+  const int i = row / p.heads_per_kv, h = head * p.heads_per_kv + row % p.heads_per_kv;
+  float weight = 1.f;
+  if (p.sinks != nullptr) {
+    const float own = m;
+    add_sink(__ldg(p.sinks + h), m, l);
+    weight = ex2(own - m);
+  }
+  weight = l == 0.f ? 0.f : weight / l;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) x[k] *= weight;
+  if (d < p.head_dim_v) store8(p.o, p.dtype, b * p.o_stride_b + h * p.o_stride_h + i * p.o_stride_s + d, x);
+  if (d == 0) {
+    const int64_t to = ((int64_t)b * p.q_heads + h) * p.q_len + i;
+    if (p.lse != nullptr) p.lse[to] = l == 0.f ? p.mask_value : (m + __log2f(l)) * kLn2;
+    if (p.max_logits != nullptr) p.max_logits[to] = l == 0.f ? p.mask_value : m * kLn2;
+  }
+}
+
 template <typename Shape>
-__global__ void __launch_bounds__(kAttendThreads) cache_attend_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend_kernel(const __grid_constant__ AttendParams p) {
   constexpr int kN = Shape::kN, kRows = Shape::kRows, kUnit = Shape::kUnit, kTiles = Shape::kTiles, kSteps = Shape::kSteps;
+  constexpr int kGroupsK = Shape::kGroupsK, kGroupsV = Shape::kGroupsV;
   constexpr bool kInt4 = Shape::kInt4;
   extern __shared__ __align__(128) uint8_t smem[];
   float* const q_sums = reinterpret_cast<float*>(smem + Shape::kQSums);
@@ -238,84 +331,81 @@ __global__ void __launch_bounds__(kAttendThreads) cache_attend_kernel(const __gr
   const int64_t first_unit = at;
   int b = start.b;
   int64_t before = start.before * per_sequence;  // units before sequence b
-  const uint32_t ring = smem_u32(smem + Shape::kRing) + warp * (Shape::kStages * Shape::kStageBytes);
-  const int groups_k = kInt4 ? Shape::kK >> p.group_shift : 1, groups_v = kInt4 ? Shape::kV >> p.group_shift : 1;
-  const int chunk_mask = kInt4 ? (p.group >> 5) - 1 : 0;  // chunks of a group, less one
-  const int scale_bytes_k = kInt4 ? 4 * groups_k : 2, scale_bytes_v = kInt4 ? 4 * groups_v : 2;
+  uint8_t* const ring = smem + Shape::kRing + warp * (Shape::kStages * Shape::kStageBytes);
+  const uint32_t ring_at = smem_u32(ring);
   const int heads = p.heads_per_kv;
 
   while (at < end) {
     Keys keys = keys_of<kUnit>(p, __ldg(p.lengths + b));
-    while (at >= before + (int64_t)keys.units * per_sequence) {  // (sequences without keys are passed over)
-      before += (int64_t)keys.units * per_sequence;
+    while (at >= before + (int64_t)keys.cost() * per_sequence) {  // (sequences without keys are passed over)
+      before += (int64_t)keys.cost() * per_sequence;
       keys = keys_of<kUnit>(p, __ldg(p.lengths + ++b));
     }
     const int length = __ldg(p.lengths + b);
-    const int item = (int)((at - before) / keys.units);  // of this sequence: head * row_tiles + row tile
+    const int item = (int)((at - before) / keys.cost());  // of this sequence: head * row_tiles + row tile
     const int head = item / p.row_tiles, row0 = item % p.row_tiles * kRows;
-    const int64_t item_first = before + (int64_t)item * keys.units;
-    const int u0 = (int)(at - item_first), u1 = (int)min((int64_t)keys.units, end - item_first);
+    const int64_t item_first = before + (int64_t)item * keys.cost() + kItemCost;  // of its first unit
+    const int u0 = (int)max(at - item_first, (int64_t)0), u1 = (int)min((int64_t)keys.units, end - item_first);
+    at = item_first + u1;
+    if (u1 <= 0) break;  // (the share ends before the item's keys)
     const int n_rows = min(kRows, p.q_len * heads - row0);
     const int32_t* const table = p.page_table + b * p.table_stride;
 
     // ---- keys on their way: unit u of this item into a stage ----
-    // A unit's pages are looked up one turn ahead (lane i has tile i's).
-    int next_page = -1;
-    auto look_up = [&](int u) {
-      const int token = keys.lo + u * kUnit + lane * 16;
-      next_page = u < u1 && lane < kTiles && token < keys.hi ? __ldg(table + (token >> p.page_shift)) : -1;
-      if (next_page >= p.n_pages) next_page = -1;
+    // Pages are looked up for kTurns of a warp's units at a time, a batch ahead: lane i has where tile i of the batch lies,
+    // in tiles of the whole cache.
+    constexpr uint32_t kNowhere = ~0u;
+    constexpr int kTurns = 32 / kTiles;
+    auto look_up = [&](int turn) -> uint32_t {
+      const int u = u0 + warp + (turn + lane / kTiles) * kAttendWarps, token = keys.lo + u * kUnit + lane % kTiles * 16;
+      const int page = u < u1 && token < keys.hi ? __ldg(table + (token >> p.page_shift)) : -1;
+      return page >= 0 && page < p.n_pages ? ((uint32_t)(page * p.kv_heads + head) << (p.page_shift - 4)) + ((token & (p.page_size - 1)) >> 4)
+                                           : kNowhere;
     };
-    // Returns a bit for each tile of the unit that has no page (its keys are not seen).
-    auto fetch = [&](int u, int stage) -> uint32_t {
-      uint32_t missing = 0;
-      if (u < u1) {
-        const uint32_t to = ring + stage * Shape::kStageBytes;
+    uint32_t places = look_up(0), next_places = look_up(kTurns);
+    uint32_t absent = __ballot_sync(~0u, places == kNowhere);  // a bit for each tile of the batch that has no page
+    auto copy_tile = [&](uint32_t place, uint32_t to, int i) {
+      const uint32_t to_v = to + kUnit * Shape::kRowK, to_scales = to_v + kUnit * Shape::kRowV;
+      copy_rows<Shape::kRowK>(to + i * 16 * Shape::kRowK, p.k_codes, place, lane);
+      copy_rows<Shape::kRowV>(to_v + i * 16 * Shape::kRowV, p.v_codes, place, lane);
+      if (lane < Shape::kScaleK)
+        cp_async16(to_scales + i * Shape::kScaleK * 16 + lane * 16, p.k_scales + ((uint64_t)place * (Shape::kScaleK * 16) + lane * 16));
+      if (lane < Shape::kScaleV)
+        cp_async16(to_scales + kUnit * Shape::kScaleK + i * Shape::kScaleV * 16 + lane * 16,
+                   p.v_scales + ((uint64_t)place * (Shape::kScaleV * 16) + lane * 16));
+    };
+    // Starts the copies of the warp's unit number `turn`; called for each in turn.  Returns a bit for each of its tiles that
+    // has no page (its keys are not seen).
+    auto fetch = [&](int turn, int stage) -> uint32_t {
+      const int first = turn % kTurns * kTiles;
+      if (first == 0 && turn > 0) {
+        places = next_places;
+        absent = __ballot_sync(~0u, places == kNowhere);
+        next_places = look_up(turn + kTurns);
+      }
+      const uint32_t missing = absent >> first & ((1u << kTiles) - 1);
+      const uint32_t to = ring_at + stage * Shape::kStageBytes;
+      if (missing == 0) {
 #pragma unroll
+        for (int i = 0; i < kTiles; ++i) copy_tile(__shfl_sync(~0u, places, first + i), to, i);
+      } else if (u0 + warp + turn * kAttendWarps < u1) {
         for (int i = 0; i < kTiles; ++i) {
-          const int page = __shfl_sync(~0u, next_page, i);
-          if (page < 0) {
-            missing |= 1u << i;
+          const uint32_t place = __shfl_sync(~0u, places, first + i);
+          if (!(missing >> i & 1)) {
+            copy_tile(place, to, i);
+          } else if (!kInt4) {
             // P is 0 there, but 0 times what lay there before need not be (codes of four bits are numbers always)
-            if (!kInt4) {
-#pragma unroll
-              for (int j = 0; j < Shape::kRowV / 32; ++j)
-                cp_async16_zeros(to + kUnit * Shape::kRowK + i * 16 * Shape::kRowV + (j * 32 + lane) * 16, p.v_codes);
-            }
-            continue;
+            for (int j = lane; j < Shape::kRowV; j += 32) cp_async16_zeros(to + kUnit * Shape::kRowK + i * 16 * Shape::kRowV + j * 16, p.v_codes);
           }
-          const int token = keys.lo + u * kUnit + i * 16;
-          const int64_t row = ((int64_t)page * p.kv_heads + head) * p.page_size + (token & (p.page_size - 1));
-          const uint8_t* const k = p.k_codes + row * Shape::kRowK;
-          const uint8_t* const v = p.v_codes + row * Shape::kRowV;
-#pragma unroll
-          for (int j = 0; j < (Shape::kRowK + 31) / 32; ++j) {
-            const int piece = j * 32 + lane;
-            if (Shape::kRowK % 32 == 0 || piece < Shape::kRowK)
-              cp_async16(to + piece_at<Shape::kRowK>(i * 16 + piece / (Shape::kRowK / 16), piece % (Shape::kRowK / 16)), k + piece * 16);
-          }
-#pragma unroll
-          for (int j = 0; j < (Shape::kRowV + 31) / 32; ++j) {
-            const int piece = j * 32 + lane;
-            if (Shape::kRowV % 32 == 0 || piece < Shape::kRowV)
-              cp_async16(to + kUnit * Shape::kRowK + piece_at<Shape::kRowV>(i * 16 + piece / (Shape::kRowV / 16), piece % (Shape::kRowV / 16)),
-                         v + piece * 16);
-          }
-          const uint32_t scales = to + kUnit * (Shape::kRowK + Shape::kRowV);
-          if (lane < scale_bytes_k) cp_async16(scales + i * 16 * scale_bytes_k + lane * 16, p.k_scales + row * scale_bytes_k + lane * 16);
-          if (lane < scale_bytes_v)
-            cp_async16(scales + kUnit * Shape::kScaleK + i * 16 * scale_bytes_v + lane * 16, p.v_scales + row * scale_bytes_v + lane * 16);
         }
       }
       cp_async_commit();
-      look_up(u + kAttendWarps);
       return missing;
     };
-    static_assert(Shape::kStages == 3);
-    look_up(u0 + warp);
-    uint32_t missing[3];
-    missing[0] = fetch(u0 + warp, 0);
-    missing[1] = fetch(u0 + warp + kAttendWarps, 1);
+    constexpr int kAhead = Shape::kStages - 1;  // units on their way while one is worked on
+    uint32_t missing[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) missing[i] = fetch(i, i);
 
     // ---- q as fragments; a warp a row ----
     for (int r = warp; r < kRows; r += kAttendWarps) {
@@ -329,9 +419,9 @@ __global__ void __launch_bounds__(kAttendThreads) cache_attend_kernel(const __gr
       for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-      // the power of two that brings `top` to 2^14 .. 2^15, within 2^-100 .. 2^100
+      // the power of two that brings `top` to 2^14 .. 2^15, within 2^-100 .. 2^100; with the sign of the logits' scale
       const int e = min(max((int)(__float_as_uint(top) >> 23), 41), 227);
-      const float up = __uint_as_float((uint32_t)(268 - e) << 23), down = __uint_as_float((uint32_t)(e - 14) << 23);
+      const float up = copysignf(__uint_as_float((uint32_t)(268 - e) << 23), p.scale), down = __uint_as_float((uint32_t)(e - 14) << 23);
       uint16_t h16[8];
       float sum = 0.f;
 #pragma unroll
@@ -355,273 +445,322 @@ __global__ void __launch_bounds__(kAttendThreads) cache_attend_kernel(const __gr
         }
       }
       if (kInt4) {
-        for (int d = 1; d < p.group / 8; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        if ((lane & (p.group / 8 - 1)) == 0 && lane * 8 < Shape::kK)
-          q_sums[(lane * 8 >> p.group_shift) * kRows + r] = sum * 0x1p-24f;  // in the units of the products of codes
+        constexpr int kLanes = Shape::kPerGroupK * 4;  // of a group
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        if (lane % kLanes == 0 && lane * 8 < Shape::kK)
+          q_sums[lane / kLanes * kRows + r] = sum * 0x1p-24f;  // in the units of the products of codes
       }
-      if (lane == 0) factors[r] = p.scale * down * (kInt4 ? 0x1p24f : 1.f) * (p.soft_cap > 0.f ? 1.f : kLog2e);
+      if (lane == 0) factors[r] = fmaxf(fabsf(p.scale) * down * (kInt4 ? 0x1p24f : 1.f) * (p.soft_cap > 0.f ? 1.f : kLog2e), 1e-37f);
     }
     __syncthreads();
 
     // ---- this lane's columns: rows nb * 8 + t4 * 2 and the next ----
-    float m[kN][2], l[kN][2], factor[kN][2];
-    int last[kN][2];  // position of the query
+    float m[kN][2], base[kN][2], l[kN][2], factor[kN][2], highest[kN][2];  // highest: of this lane's logits
     float o[Shape::kChunksV][kSteps][kN][4] = {};
-    float zeros[Shape::kGroupsV][kN][2] = {};
-    uint32_t top = 20u << 23;  // the largest scale of V seen (as bits), rounded down to a power of two
-    int last_least = INT32_MAX, last_most = INT32_MIN;
+    float zeros[kGroupsV][kN][2] = {};
+    // The largest scale of V seen, as bits, rounded down to a power of two (2^-40 at least).  P is taken in units of `unit` =
+    // 2^kUnitLog2 / top throughout: in l, the zeros' sums and O.
+    uint32_t top = kLeastTop;
 #pragma unroll
     for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int r = nb * 8 + t4 * 2 + j;
-        m[nb][j] = -INFINITY;
+        m[nb][j] = base[nb][j] = highest[nb][j] = kNoMaximum;
         l[nb][j] = 0.f;
-        factor[nb][j] = factors[r];
-        last[nb][j] = length - p.q_len + (row0 + min(r, n_rows - 1)) / heads;
+        factor[nb][j] = p.soft_cap > 0.f ? 1.f : factors[nb * 8 + t4 * 2 + j];
       }
-    last_least = length - p.q_len + row0 / heads;
-    last_most = length - p.q_len + (row0 + n_rows - 1) / heads;
+    // units of which every row sees every key: whole_lo .. whole_hi - 1
+    const int whole_hi = (min(length - p.q_len + row0 / heads + 1, keys.hi) - keys.lo) / kUnit;
+    const int whole_lo = p.window < 0 ? 0 : max(length - p.q_len + (row0 + n_rows - 1) / heads - p.window - keys.lo + kUnit - 1, 0) / kUnit;
 
     const uint2* const frags = reinterpret_cast<const uint2*>(smem) + lane;
-    int stage = 0;
-    for (int u = u0 + warp; u < u1; u += kAttendWarps) {
-      cp_async_wait<1>();
+    // where a lane's rows of matrices begin: K, the next tile's in the upper half of the warp; V, the next piece's
+    const uint32_t lane_k = Pieces<Shape::kRowK>::row_at(kTiles > 1 ? lane : lane & 15);
+    const uint32_t lane_v = kUnit * Shape::kRowK + Pieces<Shape::kRowV>::at(Pieces<Shape::kRowV>::row_at(lane & 15), Pieces<Shape::kRowV>::kTurn > 0 ? lane >> 4 : 0) +
+                            (Pieces<Shape::kRowV>::kTurn > 0 ? 0 : (lane >> 4) * 16);
+    int stage = 0, turn = 0;
+    for (int u = u0 + warp; u < u1; u += kAttendWarps, ++turn) {
+      cp_async_wait<kAhead - 1>();
       __syncwarp();
       const uint32_t none = missing[0];
-      missing[0] = missing[1];
-      missing[1] = fetch(u + 2 * kAttendWarps, stage == 0 ? 2 : stage - 1);
-      const uint32_t from = ring + stage * Shape::kStageBytes;
-      const uint8_t* const scales_k = smem + (from - smem_u32(smem)) + kUnit * (Shape::kRowK + Shape::kRowV);
+#pragma unroll
+      for (int i = 0; i + 1 < kAhead; ++i) missing[i] = missing[i + 1];
+      missing[kAhead - 1] = fetch(turn + kAhead, stage == 0 ? kAhead : stage - 1);
+      const uint32_t from_k = ring_at + stage * Shape::kStageBytes + lane_k, from_v = ring_at + stage * Shape::kStageBytes + lane_v;
+      const uint8_t* const scales_k = ring + stage * Shape::kStageBytes + kUnit * (Shape::kRowK + Shape::kRowV);
       const uint8_t* const scales_v = scales_k + kUnit * Shape::kScaleK;
-      stage = stage == 2 ? 0 : stage + 1;
+      stage = stage == kAhead ? 0 : stage + 1;
 
       // ---- S ----
       float s[kTiles][kN][4];
-      float acc[kTiles][kN][4];
+      if constexpr (kInt4) {
+        uint32_t pairs[kTiles][2][kGroupsK];
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i)
+        for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-        for (int nb = 0; nb < kN; ++nb)
+          for (int half = 0; half < 2; ++half)
+            load_words<kGroupsK>(pairs[i][half], reinterpret_cast<const uint32_t*>(scales_k) + (i * 16 + half * 8 + g) * kGroupsK);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][nb][j] = acc[i][nb][j] = 0.f;
+        for (int group = 0; group < kGroupsK; ++group) {
+          float acc[kTiles][kN][4] = {};
 #pragma unroll
-      for (int c = 0; c < Shape::kChunksK; ++c) {
-        uint2 qf[kSteps][kN];
+          for (int cc = 0; cc < Shape::kPerGroupK; ++cc) {
+            const int c = group * Shape::kPerGroupK + cc;
+            uint2 qf[2][kN];
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k)
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int nb = 0; nb < kN; ++nb) qf[k][nb] = frags[((c * kSteps + k) * kN + nb) * 32];
+              for (int nb = 0; nb < kN; ++nb) qf[k][nb] = frags[((c * 2 + k) * kN + nb) * 32];
+            uint32_t words[kTiles][2];
+            load_tiles<kTiles, Shape::kRowK>(Pieces<Shape::kRowK>::at(from_k, c), words);
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          uint32_t w0, w1;  // rows g and g + 8: word t4 of the 16 bytes
-          ldmatrix_x2(from + piece_at<Shape::kRowK>(i * 16 + (lane & 15), c), w0, w1);
-          if (kInt4) {
-            const uint32_t a[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
-            w0 >>= 8;
-            w1 >>= 8;
-            const uint32_t a2[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+            for (int i = 0; i < kTiles; ++i) {
+              uint32_t w0 = words[i][0], w1 = words[i][1];  // rows g and g + 8: word t4 of the 16 bytes
+              const uint32_t a[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+              w0 >>= 8;
+              w1 >>= 8;
+              const uint32_t a2[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
 #pragma unroll
-            for (int nb = 0; nb < kN; ++nb) {
-              mma_f16(acc[i][nb], a, qf[0][nb].x, qf[0][nb].y);
-              mma_f16(acc[i][nb], a2, qf[kSteps - 1][nb].x, qf[kSteps - 1][nb].y);
+              for (int nb = 0; nb < kN; ++nb) {
+                mma_f16(acc[i][nb], a, qf[0][nb].x, qf[0][nb].y);
+                mma_f16(acc[i][nb], a2, qf[1][nb].x, qf[1][nb].y);
+              }
             }
-          } else {
-            const uint32_t a[4] = {e4m3x2_to_f16x2(w0), e4m3x2_to_f16x2(w1), e4m3x2_to_f16x2(w0 >> 16), e4m3x2_to_f16x2(w1 >> 16)};
-#pragma unroll
-            for (int nb = 0; nb < kN; ++nb) mma_f16(acc[i][nb], a, qf[0][nb].x, qf[0][nb].y);
           }
-        }
-        if (kInt4 && (c & chunk_mask) == chunk_mask) {  // the end of a group
-          const int group = (c * 32) >> p.group_shift;
           float2 sums[kN];
 #pragma unroll
           for (int nb = 0; nb < kN; ++nb) sums[nb] = *reinterpret_cast<const float2*>(q_sums + group * kRows + nb * 8 + t4 * 2);
 #pragma unroll
           for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t pair = reinterpret_cast<const uint32_t*>(scales_k)[(i * 16 + half * 8 + g) * groups_k + group];
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t pair = pairs[i][j >> 1][group];
               const float zero = bf16_bits_to_float(pair), scale = __uint_as_float(pair & 0xffff0000u);
 #pragma unroll
               for (int nb = 0; nb < kN; ++nb) {
-                s[i][nb][half * 2] = fmaf(zero, sums[nb].x, fmaf(scale, acc[i][nb][half * 2], s[i][nb][half * 2]));
-                s[i][nb][half * 2 + 1] = fmaf(zero, sums[nb].y, fmaf(scale, acc[i][nb][half * 2 + 1], s[i][nb][half * 2 + 1]));
-                acc[i][nb][half * 2] = acc[i][nb][half * 2 + 1] = 0.f;
+                const float sum = j & 1 ? sums[nb].y : sums[nb].x;
+                const float part = group == 0 ? zero * sum : fmaf(zero, sum, s[i][nb][j]);
+                s[i][nb][j] = fmaf(scale, acc[i][nb][j], part);
               }
             }
         }
-      }
-      // logits in units of log2
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float scale = 1.f;
-          if (!kInt4) scale = bf16_bits_to_float(reinterpret_cast<const uint16_t*>(scales_k)[i * 16 + half * 8 + g]);
-#pragma unroll
-          for (int nb = 0; nb < kN; ++nb)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float& x = s[i][nb][half * 2 + j];
-              x = kInt4 ? x * factor[nb][j] : acc[i][nb][half * 2 + j] * scale * factor[nb][j];
-              if (p.soft_cap > 0.f) {  // cap * tanh(x / cap), tanh y = 1 - 2 / (exp(2 y) + 1)
-                const float e = ex2(x * (2.f * kLog2e / p.soft_cap));
-                x = (p.soft_cap * kLog2e) * (1.f - __fdividef(2.f, e + 1.f));
-              }
-            }
-        }
-
-      // ---- what is seen ----
-      const int token0 = keys.lo + u * kUnit;
-      const bool whole = none == 0 && token0 + kUnit - 1 <= min(last_least, keys.hi - 1) && (p.window < 0 || token0 >= last_most - p.window);
-      uint32_t seen = ~0u;  // a bit for each of s, where not whole: tile, block, element
-      if (!whole) {
-        seen = 0;
+      } else {
 #pragma unroll
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
           for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int token = token0 + i * 16 + (j >> 1) * 8 + g, position = last[nb][j & 1];
+            for (int j = 0; j < 4; ++j) s[i][nb][j] = 0.f;
+#pragma unroll
+        for (int c = 0; c < Shape::kChunksK; ++c) {
+          uint2 qf[kN];
+#pragma unroll
+          for (int nb = 0; nb < kN; ++nb) qf[nb] = frags[(c * kN + nb) * 32];
+          uint32_t words[kTiles][2];
+          load_tiles<kTiles, Shape::kRowK>(Pieces<Shape::kRowK>::at(from_k, c), words);
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+            const uint32_t w0 = words[i][0], w1 = words[i][1];
+            const uint32_t a[4] = {e4m3x2_to_f16x2(w0), e4m3x2_to_f16x2(w1), e4m3x2_to_f16x2(w0 >> 16), e4m3x2_to_f16x2(w1 >> 16)};
+#pragma unroll
+            for (int nb = 0; nb < kN; ++nb) mma_f16(s[i][nb], a, qf[nb].x, qf[nb].y);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float scale = bf16_bits_to_float(reinterpret_cast<const uint16_t*>(scales_k)[i * 16 + half * 8 + g]);
+#pragma unroll
+            for (int nb = 0; nb < kN; ++nb) {
+              s[i][nb][half * 2] *= scale;
+              s[i][nb][half * 2 + 1] *= scale;
+            }
+          }
+      }
+      if (p.soft_cap > 0.f) {  // cap * tanh(x / cap) in units of log2, tanh y = 1 - 2 / (exp(2 y) + 1)
+        const float inside = 2.f * kLog2e / p.soft_cap, outside = p.soft_cap * kLog2e;
+#pragma unroll
+        for (int nb = 0; nb < kN; ++nb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float f = factors[nb * 8 + t4 * 2 + (j & 1)] * inside;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) s[i][nb][j] = outside - __fdividef(2.f * outside, ex2(s[i][nb][j] * f) + 1.f);
+          }
+      }
+
+      // ---- what is seen ----
+      const int token0 = keys.lo + u * kUnit;
+      const bool whole = none == 0 && u >= whole_lo && u < whole_hi;
+      uint32_t seen = ~0u;  // a bit for each of s, where not whole: tile, block, element
+      if (!whole) {
+        seen = 0;
+#pragma unroll
+        for (int nb = 0; nb < kN; ++nb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int position = length - p.q_len + (row0 + min(nb * 8 + t4 * 2 + (j & 1), n_rows - 1)) / heads;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+              const int token = token0 + i * 16 + (j >> 1) * 8 + g;
               const bool keep = !(none >> i & 1) && token < keys.hi && token <= position && (p.window < 0 || token >= position - p.window);
               if (keep)
                 seen |= 1u << ((i * kN + nb) * 4 + j);
               else
                 s[i][nb][j] = -INFINITY;
             }
+          }
       }
       static_assert(kTiles * kN * 4 <= 32);
 
-      // ---- running maximum, P ----
-      float alpha[kN][2];
-      bool grew = false;
+      // ---- the maximum that P is taken against: raised where a logit passes it by more than kSlack ----
+      bool grows = false;
+      float most[kN][2];
 #pragma unroll
       for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float top_s = -INFINITY;
+          float x = fmaxf(s[0][nb][j], s[0][nb][2 + j]);
 #pragma unroll
-          for (int i = 0; i < kTiles; ++i) top_s = max3(top_s, s[i][nb][j], s[i][nb][2 + j]);
-          top_s = fmaxf(top_s, __shfl_xor_sync(~0u, top_s, 4));
-          top_s = fmaxf(top_s, __shfl_xor_sync(~0u, top_s, 8));
-          top_s = fmaxf(top_s, __shfl_xor_sync(~0u, top_s, 16));
-          const float next = fmaxf(m[nb][j], top_s);
-          grew = grew || next > m[nb][j];
-          alpha[nb][j] = m[nb][j] > -INFINITY ? ex2(m[nb][j] - next) : 0.f;
-          m[nb][j] = next;
-          const float base = next > -INFINITY ? next : 0.f;
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float& x = s[i][nb][half * 2 + j];
-              x = ex2(x - base);
-              sum += x;
-            }
-          l[nb][j] = l[nb][j] * alpha[nb][j] + sum;
+          for (int i = 1; i < kTiles; ++i) x = max3(x, s[i][nb][j], s[i][nb][2 + j]);
+          most[nb][j] = x * factor[nb][j];
+          highest[nb][j] = fmaxf(highest[nb][j], most[nb][j]);
+          grows = grows || most[nb][j] > m[nb][j] + kSlack;
         }
-
-      // ---- the power of two that P * scale is taken in ----
-      uint32_t largest = 0;
+      // ---- and the power of two that P * scale is taken in: lowered where a scale passes `top` by a factor of two ----
+      uint32_t own_top[(kUnit + 31) / 32][kGroupsV];  // a lane a token
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i)
+      for (int i = 0; i < kUnit; i += 32) {
+        const int token = kUnit < 32 ? lane & (kUnit - 1) : i + lane;
+        if constexpr (kInt4)
+          load_words<kGroupsV>(own_top[i / 32], reinterpret_cast<const uint32_t*>(scales_v) + token * kGroupsV);
+        else
+          own_top[i / 32][0] = (uint32_t)reinterpret_cast<const uint16_t*>(scales_v)[token] << 16;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int token = i * 16 + half * 8 + g;
-          // (lanes t4 = 0 .. 3 have the same token: each looks at a quarter of its groups)
-          if (kInt4) {
-            for (int group = t4; group < groups_v; group += 4) {
-              const uint32_t pair = reinterpret_cast<const uint32_t*>(scales_v)[token * groups_v + group];
-              if ((whole || (!(none >> i & 1) && token0 + token < keys.hi)) && pair < 0x7f800000u) largest = max(largest, pair);
+        for (int group = 0; group < kGroupsV; ++group) grows = grows || own_top[i / 32][group] >= top + (1u << 23);
+      }
+      if (__any_sync(~0u, grows)) {
+        uint32_t largest = 0;
+#pragma unroll
+        for (int i = 0; i < kUnit; i += 32) {
+          const int token = kUnit < 32 ? lane & (kUnit - 1) : i + lane;
+          if (whole || (!(none >> (token >> 4) & 1) && token0 + token < keys.hi)) {
+#pragma unroll
+            for (int group = 0; group < kGroupsV; ++group) {
+              const uint32_t x = own_top[i / 32][group];
+              largest = max(largest, x < 0x7f800000u ? x : 0u);  // (not NaN)
             }
-          } else {
-            const uint32_t bits = (uint32_t)reinterpret_cast<const uint16_t*>(scales_v)[token] << 16;
-            if ((whole || (!(none >> i & 1) && token0 + token < keys.hi)) && bits < 0x7f800000u) largest = max(largest, bits);
           }
         }
-      largest = __reduce_max_sync(~0u, largest) & 0x7f800000u;
-      float rise = 1.f;  // what sums so far are multiplied by when it changes
-      if (largest > top) {
-        rise = __uint_as_float((uint32_t)max(127 - (int)((largest - top) >> 23), 0) << 23);
+        largest = max(__reduce_max_sync(~0u, largest) & 0x7f800000u, top);
+        const float rise = __uint_as_float((uint32_t)max(127 - (int)((largest - top) >> 23), 0) << 23);
         top = largest;
-      }
-      const float unit = __uint_as_float((267u << 23) - top);  // 2^13 / 2^exponent(top)
-      if (__any_sync(~0u, grew) || rise != 1.f) {
+        const float unit_log2 = (float)(kUnitLog2 + 127 - (int)(top >> 23));
 #pragma unroll
         for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float a = alpha[nb][j] * rise;
+            float x = fmaxf(m[nb][j], most[nb][j]);
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+            const float alpha = ex2(m[nb][j] - x) * rise;
+            m[nb][j] = x;
+            base[nb][j] = x - unit_log2;
+            l[nb][j] *= alpha;
 #pragma unroll
             for (int c = 0; c < Shape::kChunksV; ++c)
 #pragma unroll
               for (int k = 0; k < kSteps; ++k) {
-                o[c][k][nb][j] *= a;
-                o[c][k][nb][2 + j] *= a;
+                o[c][k][nb][j] *= alpha;
+                o[c][k][nb][2 + j] *= alpha;
               }
 #pragma unroll
-            for (int c = 0; c < Shape::kGroupsV; ++c) zeros[c][nb][j] *= alpha[nb][j];
+            for (int c = 0; c < kGroupsV; ++c) zeros[c][nb][j] *= alpha;
           }
       }
+#pragma unroll
+      for (int nb = 0; nb < kN; ++nb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+            s[i][nb][j] = ex2(fmaf(s[i][nb][j], factor[nb][j & 1], -base[nb][j & 1]));
+            l[nb][j & 1] += s[i][nb][j];
+          }
 
       // ---- O ----
-      const uint32_t from_v = from + kUnit * Shape::kRowK;
+      auto accumulate = [&](auto masked) {
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        uint32_t pf[kN][2];  // P * scale as the MMAs' second operand
+        for (int i = 0; i < kTiles; ++i) {
+          uint32_t pairs[2][kGroupsV], words[4];
 #pragma unroll
-        for (int c = 0; c < Shape::kChunksV; ++c) {
-          if (kInt4 ? (c & chunk_mask) == 0 : c == 0) {  // the start of a group
-            const int group = kInt4 ? (c * 32) >> p.group_shift : 0;
+          for (int half = 0; half < 2; ++half) {
+            const int token = i * 16 + half * 8 + g;
+            if constexpr (kInt4)
+              load_words<kGroupsV>(pairs[half], reinterpret_cast<const uint32_t*>(scales_v) + token * kGroupsV);
+            else
+              pairs[half][0] = (uint32_t)reinterpret_cast<const uint16_t*>(scales_v)[token] << 16;
+          }
+#pragma unroll
+          for (int group = 0; group < kGroupsV; ++group) {
+            uint32_t pf[kN][2];  // P * scale as the MMAs' second operand
             float scale[2], zero[2];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const int token = i * 16 + half * 8 + g;
-              if (kInt4) {
-                const uint32_t pair = reinterpret_cast<const uint32_t*>(scales_v)[token * groups_v + group];
-                zero[half] = bf16_bits_to_float(pair);
-                scale[half] = __uint_as_float(pair & 0xffff0000u) * unit;
-              } else {
-                scale[half] = bf16_bits_to_float(reinterpret_cast<const uint16_t*>(scales_v)[token]) * unit;
-              }
+              scale[half] = __uint_as_float(pairs[half][group] & 0xffff0000u);
+              zero[half] = bf16_bits_to_float(pairs[half][group]);
             }
 #pragma unroll
             for (int nb = 0; nb < kN; ++nb) {
               float x[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                x[j] = s[i][nb][j] * scale[j >> 1];
-                float z = kInt4 ? s[i][nb][j] * zero[j >> 1] : 0.f;
-                if (!whole && !(seen >> ((i * kN + nb) * 4 + j) & 1)) x[j] = z = 0.f;  // (whatever lies there, NaN too)
-                if (kInt4) zeros[c][nb][j & 1] += z;
+                const bool dead = decltype(masked)::value && !(seen >> ((i * kN + nb) * 4 + j) & 1);
+                x[j] = dead ? 0.f : s[i][nb][j] * scale[j >> 1];  // (whatever lies there, NaN too)
+                if (kInt4 && !dead) zeros[group][nb][j & 1] = fmaf(s[i][nb][j], zero[j >> 1], zeros[group][nb][j & 1]);
               }
               pf[nb][0] = movmatrix(pack_f16(x[0], x[1]));
               pf[nb][1] = movmatrix(pack_f16(x[2], x[3]));
             }
-          }
-          uint32_t w0, w1;  // tokens 2 * t4 and the next (w1: + 8), 16 bits each from byte 2 * g of the piece
-          ldmatrix_x2_trans(from_v + piece_at<Shape::kRowV>(i * 16 + (lane & 15), c), w0, w1);
-          if (kInt4) {
-            const uint32_t a[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
-            w0 >>= 8;
-            w1 >>= 8;
-            const uint32_t a2[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
 #pragma unroll
-            for (int nb = 0; nb < kN; ++nb) {
-              mma_f16(o[c][0][nb], a, pf[nb][0], pf[nb][1]);
-              mma_f16(o[c][kSteps - 1][nb], a2, pf[nb][0], pf[nb][1]);
+            for (int cc = 0; cc < Shape::kPerGroupV; ++cc) {
+              const int c = group * Shape::kPerGroupV + cc;
+              // tokens 2 * t4 and the next (w1: + 8), 16 bits each from byte 2 * g of the piece; two pieces at a time
+              if (c % 2 == 0) {
+                const uint32_t at = Pieces<Shape::kRowV>::at(from_v, c) + i * 16 * Shape::kRowV;
+                if (c + 1 < Shape::kChunksV)
+                  ldmatrix_x4_trans(at, words[0], words[1], words[2], words[3]);
+                else
+                  ldmatrix_x2_trans(at, words[0], words[1]);
+              }
+              uint32_t w0 = words[c % 2 * 2], w1 = words[c % 2 * 2 + 1];
+              if constexpr (kInt4) {
+                const uint32_t a[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+                w0 >>= 8;
+                w1 >>= 8;
+                const uint32_t a2[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+#pragma unroll
+                for (int nb = 0; nb < kN; ++nb) {
+                  mma_f16(o[c][0][nb], a, pf[nb][0], pf[nb][1]);
+                  mma_f16(o[c][1][nb], a2, pf[nb][0], pf[nb][1]);
+                }
+              } else {
+                const uint32_t x0 = __byte_perm(w0, 0, 0x3120), x1 = __byte_perm(w1, 0, 0x3120);
+                const uint32_t a[4] = {e4m3x2_to_f16x2(x0), e4m3x2_to_f16x2(x0 >> 16), e4m3x2_to_f16x2(x1), e4m3x2_to_f16x2(x1 >> 16)};
+#pragma unroll
+                for (int nb = 0; nb < kN; ++nb) mma_f16(o[c][0][nb], a, pf[nb][0], pf[nb][1]);
+              }
             }
-          } else {
-            const uint32_t x0 = __byte_perm(w0, 0, 0x3120), x1 = __byte_perm(w1, 0, 0x3120);
-            const uint32_t a[4] = {e4m3x2_to_f16x2(x0), e4m3x2_to_f16x2(x0 >> 16), e4m3x2_to_f16x2(x1), e4m3x2_to_f16x2(x1 >> 16)};
-#pragma unroll
-            for (int nb = 0; nb < kN; ++nb) mma_f16(o[c][0][nb], a, pf[nb][0], pf[nb][1]);
           }
         }
-      }
+      };
+      if (whole)
+        accumulate(std::false_type{});
+      else
+        accumulate(std::true_type{});
       __syncwarp();
     }
     cp_async_wait<0>();  // (nothing is in flight here that anyone waits for; the ring's place is about to be written)
@@ -635,64 +774,66 @@ __global__ void __launch_bounds__(kAttendThreads) cache_attend_kernel(const __gr
         sum += __shfl_xor_sync(~0u, sum, 4);
         sum += __shfl_xor_sync(~0u, sum, 8);
         sum += __shfl_xor_sync(~0u, sum, 16);
-        l[nb][j] = sum;
+        float high = highest[nb][j];
+        high = fmaxf(high, __shfl_xor_sync(~0u, high, 4));
+        high = fmaxf(high, __shfl_xor_sync(~0u, high, 8));
+        high = fmaxf(high, __shfl_xor_sync(~0u, high, 16));
         if (kInt4) {
 #pragma unroll
-          for (int c = 0; c < Shape::kGroupsV; ++c) {
+          for (int c = 0; c < kGroupsV; ++c) {
             float z = zeros[c][nb][j];
             z += __shfl_xor_sync(~0u, z, 4);
             z += __shfl_xor_sync(~0u, z, 8);
             z += __shfl_xor_sync(~0u, z, 16);
-            if (lane < 4) warp_zeros[(warp * Shape::kGroupsV + c) * kRows + nb * 8 + t4 * 2 + j] = z;
+            if (lane < 4) warp_zeros[(warp * kGroupsV + c) * kRows + nb * 8 + t4 * 2 + j] = z;
           }
         }
         if (lane < 4) {
-          warp_max[warp * kRows + nb * 8 + t4 * 2 + j] = m[nb][j];
-          warp_sum[warp * kRows + nb * 8 + t4 * 2 + j] = sum;
+          warp_max[warp * kRows + nb * 8 + t4 * 2 + j] = high;
+          warp_sum[warp * kRows + nb * 8 + t4 * 2 + j] = sum * ex2(base[nb][j] - high);
         }
       }
     __syncthreads();
     {
       float* const join = reinterpret_cast<float*>(smem + Shape::kRing) + warp * (kRows * Shape::kV);
-      const float back = __uint_as_float(top - (13u << 23)) * (kInt4 ? 0x1p24f : 1.f);  // 1 / unit
+      constexpr float kBack = kInt4 ? 0x1p24f : 1.f;  // of products of codes
 #pragma unroll
       for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int r = nb * 8 + t4 * 2 + j;
-          float most = -INFINITY;
+          float most = kNoMaximum;
 #pragma unroll
           for (int w = 0; w < kAttendWarps; ++w) most = fmaxf(most, warp_max[w * kRows + r]);
-          const float weight = m[nb][j] > -INFINITY ? ex2(m[nb][j] - most) : 0.f;
+          const float weight = ex2(base[nb][j] - most);
 #pragma unroll
           for (int c = 0; c < Shape::kChunksV; ++c) {
-            if (kInt4) {
-              const float4 x = make_float4(o[c][0][nb][j] * back, o[c][0][nb][2 + j] * (back * 0.0625f),
-                                           o[c][kSteps - 1][nb][j] * back, o[c][kSteps - 1][nb][2 + j] * (back * 0.0625f));
-              const float z = warp_zeros[(warp * Shape::kGroupsV + (c & ~chunk_mask)) * kRows + r];
+            if constexpr (kInt4) {
+              const float4 x = make_float4(o[c][0][nb][j] * kBack, o[c][0][nb][2 + j] * (kBack * 0.0625f),
+                                           o[c][1][nb][j] * kBack, o[c][1][nb][2 + j] * (kBack * 0.0625f));
+              const float z = warp_zeros[(warp * kGroupsV + c / Shape::kPerGroupV) * kRows + r];
               *reinterpret_cast<float4*>(join + r * Shape::kV + c * 32 + g * 4) =
                   make_float4((x.x + z) * weight, (x.y + z) * weight, (x.z + z) * weight, (x.w + z) * weight);
             } else {
               *reinterpret_cast<float2*>(join + r * Shape::kV + c * 16 + g * 2) =
-                  make_float2(o[c][0][nb][j] * back * weight, o[c][0][nb][2 + j] * back * weight);
+                  make_float2(o[c][0][nb][j] * weight, o[c][0][nb][2 + j] * weight);
             }
           }
         }
     }
     __syncthreads();
     const bool alone = u0 == 0 && u1 == keys.units;
-    // sums of this CTA: its first item in place 0, its last in place 1 (an item that is both and not whole: 0)
-    float* const part = p.parts + ((int64_t)blockIdx.x * 2 + (at == first_unit ? 0 : 1)) * (kRows * (Shape::kV + 2));
+    // sums of this CTA: an item that began before its share in place 0, one that goes on behind it in place 1 (both: 0)
+    float* const part = p.parts + ((int64_t)blockIdx.x * 2 + (item_first > first_unit ? 1 : 0)) * (kRows * (Shape::kV + 2));
     for (int id = tid; id < n_rows * (Shape::kV / 8); id += kAttendThreads) {
       const int r = id / (Shape::kV / 8), d = id % (Shape::kV / 8) * 8;
       float x[8] = {};
-      float most = -INFINITY, sum = 0.f;
+      float most = kNoMaximum, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kAttendWarps; ++w) most = fmaxf(most, warp_max[w * kRows + r]);
 #pragma unroll
       for (int w = 0; w < kAttendWarps; ++w) {
-        const float mine = warp_max[w * kRows + r];
-        sum += mine > -INFINITY ? warp_sum[w * kRows + r] * ex2(mine - most) : 0.f;
+        sum += warp_sum[w * kRows + r] * ex2(warp_max[w * kRows + r] - most);
         const float4* const from = reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem + Shape::kRing) + (w * kRows + r) * Shape::kV + d);
         const float4 lo = from[0], hi = from[1];
         x[0] += lo.x, x[1] += lo.y, x[2] += lo.z, x[3] += lo.w, x[4] += hi.x, x[5] += hi.y, x[6] += hi.z, x[7] += hi.w;
@@ -707,25 +848,8 @@ __global__ void __launch_bounds__(kAttendThreads) cache_attend_kernel(const __gr
         }
         continue;
       }
-      const int row = row0 + r, i = row / heads, h = head * heads + row % heads;
-      if (p.sinks != nullptr) {
-        const float own = most;
-        add_sink(__ldg(p.sinks + h), most, sum);
-        const float weight = own > -INFINITY ? ex2(own - most) : 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] *= weight;
-      }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = sum == 0.f ? 0.f : x[k] * inv;
-      if (d < p.head_dim_v) store8(p.o, p.dtype, b * p.o_stride_b + h * p.o_stride_h + i * p.o_stride_s + d, x);
-      if (d == 0) {
-        const int64_t to = ((int64_t)b * p.q_heads + h) * p.q_len + i;
-        if (p.lse != nullptr) p.lse[to] = sum == 0.f ? p.mask_value : (most + __log2f(sum)) * kLn2;
-        if (p.max_logits != nullptr) p.max_logits[to] = sum == 0.f ? p.mask_value : most * kLn2;
-      }
+      finish_row(p, b, head, row0 + r, d, x, most, sum);
     }
-    at = item_first + u1;
     __syncthreads();  // before q's place, the statistics and the ring are written again
   }
 }
@@ -733,54 +857,93 @@ __global__ void __launch_bounds__(kAttendThreads) cache_attend_kernel(const __gr
 // ------------------------------------------------------------------------------------------
 // items that several CTAs have worked on, and items without keys
 // ------------------------------------------------------------------------------------------
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 256;
 
-// blockIdx.x: row tile of an item (fastest) and head; y: sequence.  A thread has eight channels of a row.
+// blockIdx.x: row tile of an item (fastest) and head; y: sequence; z: rows z, z + gridDim.z ..  Threads have eight channels
+// of a row; where there are more threads than that, several have the same and take every n-th part.
 template <int kRows, int kV>
 __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const __grid_constant__ AttendParams p, int ctas) {
+  constexpr int kEach = kV / 8, kSlices = kJoinThreads / kEach;  // threads of a row, and of it in turn
+  constexpr int kPart = kRows * (kV + 2);
+  __shared__ float sums[kSlices][kV];
+  __shared__ float stats[2][kSlices];
   grid_dependency_wait();
   const int per_sequence = p.kv_heads * p.row_tiles;
+  const int slice = threadIdx.x / kEach, d = threadIdx.x % kEach * 8;
+  const int64_t share = share_of(p.starts[p.batch] * per_sequence, ctas, p.min_share);
   for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
-    const int64_t before = p.starts[b], units = p.starts[b + 1] - before;
-    const int64_t share = share_of(p.starts[p.batch] * per_sequence, ctas, p.min_share);
-    const int64_t first = before * per_sequence + blockIdx.x * units;  // unit of this item
-    const int64_t c0 = first / share, c1 = units > 0 ? (first + units - 1) / share : c0 - 1;
+    const int64_t before = p.starts[b], cost = p.starts[b + 1] - before;
+    const int64_t first = before * per_sequence + blockIdx.x * cost + kItemCost;  // unit of this item
+    const int64_t c0 = first / share, c1 = cost > 0 ? (first + cost - kItemCost - 1) / share : c0 - 1;
     if (c0 == c1) continue;  // written already
     const int head = blockIdx.x / p.row_tiles, row0 = blockIdx.x % p.row_tiles * kRows;
     const int n_rows = min(kRows, p.q_len * p.heads_per_kv - row0);
-    for (int id = threadIdx.x; id < n_rows * (kV / 8); id += kJoinThreads) {
-      const int r = id / (kV / 8), d = id % (kV / 8) * 8;
-      const int row = row0 + r, i = row / p.heads_per_kv, h = head * p.heads_per_kv + row % p.heads_per_kv;
-      float most = -INFINITY, sum = 0.f, x[8] = {};
-      for (int64_t c = c0; c <= c1; ++c) {
-        // the first CTA has the item last in its share, unless it starts there
-        const float* const part = p.parts + (c * 2 + (c * share < first ? 1 : 0)) * (kRows * (kV + 2));
-        const float m = part[kRows * kV + r], l = part[kRows * (kV + 1) + r];
-        const float4* const from = reinterpret_cast<const float4*>(part + r * kV + d);
-        const float4 lo = from[0], hi = from[1];
-        const float top = fmaxf(most, m);
-        const float old = most > -INFINITY ? ex2(most - top) : 0.f, fresh = m > -INFINITY ? ex2(m - top) : 0.f;
-        const float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    for (int r = blockIdx.z; r < n_rows; r += gridDim.z) {
+      float most = kNoMaximum, sum = 0.f, x[8] = {};
+      if (slice < kSlices) {
+        const float* part = p.parts + (c0 + slice) * (2 * kPart);
+        constexpr int kAtOnce = 4;  // parts whose loads are in flight together
+        for (int64_t c = c0 + slice; c <= c1; c += kSlices * kAtOnce) {
+          float m[kAtOnce], l[kAtOnce];
+          float4 lo[kAtOnce], hi[kAtOnce];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = x[k] * old + y[k] * fresh;
-        sum = sum * old + l * fresh;
-        most = top;
-      }
-      if (p.sinks != nullptr) {
-        const float own = most;
-        add_sink(__ldg(p.sinks + h), most, sum);
-        const float weight = own > -INFINITY ? ex2(own - most) : 0.f;
+          for (int k = 0; k < kAtOnce; ++k) {
+            const int64_t at = c + k * kSlices;
+            m[k] = kNoMaximum;
+            l[k] = 0.f;
+            lo[k] = hi[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (at > c1) continue;
+            // the first CTA has the item last in its share, unless it starts there
+            const float* const from = part + k * (kSlices * 2 * kPart) + (at * share < first ? kPart : 0);
+            m[k] = from[kRows * kV + r];
+            l[k] = from[kRows * (kV + 1) + r];
+            lo[k] = *reinterpret_cast<const float4*>(from + r * kV + d);
+            hi[k] = *reinterpret_cast<const float4*>(from + r * kV + d + 4);
+          }
+          part += kAtOnce * (kSlices * 2 * kPart);
+          float top = most;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] *= weight;
-      }
+          for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, m[k]);
+          const float old = ex2(most - top);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = sum == 0.f ? 0.f : x[k] / sum;
-      if (d < p.head_dim_v) store8(p.o, p.dtype, b * p.o_stride_b + h * p.o_stride_h + i * p.o_stride_s + d, x);
-      if (d == 0) {
-        const int64_t to = ((int64_t)b * p.q_heads + h) * p.q_len + i;
-        if (p.lse != nullptr) p.lse[to] = sum == 0.f ? p.mask_value : (most + __log2f(sum)) * kLn2;
-        if (p.max_logits != nullptr) p.max_logits[to] = sum == 0.f ? p.mask_value : most * kLn2;
+          for (int k = 0; k < 8; ++k) x[k] *= old;
+          sum *= old;
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k) {
+            const float weight = ex2(m[k] - top);
+            const float y[8] = {lo[k].x, lo[k].y, lo[k].z, lo[k].w, hi[k].x, hi[k].y, hi[k].z, hi[k].w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(y[i], weight, x[i]);
+            sum = fmaf(l[k], weight, sum);
+          }
+          most = top;
+        }
+        *reinterpret_cast<float4*>(&sums[slice][d]) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(&sums[slice][d + 4]) = make_float4(x[4], x[5], x[6], x[7]);
+        if (d == 0) {
+          stats[0][slice] = most;
+          stats[1][slice] = sum;
+        }
       }
+      __syncthreads();
+      if (slice == 0) {
+        float top = most;
+#pragma unroll
+        for (int k = 1; k < kSlices; ++k) top = fmaxf(top, stats[0][k]);
+        const float own = ex2(most - top);
+        sum *= own;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= own;
+#pragma unroll
+        for (int k = 1; k < kSlices; ++k) {
+          const float weight = ex2(stats[0][k] - top);
+          sum = fmaf(stats[1][k], weight, sum);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = fmaf(sums[k][d + i], weight, x[i]);
+        }
+        finish_row(p, b, head, row0 + r, d, x, top, sum);
+      }
+      __syncthreads();
     }
   }
 }
@@ -788,10 +951,6 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const _
 // ------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------
-struct AttendPlan {
-  int rows, ctas;
-};
-
 template <typename Shape>
 static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   auto kernel = cache_attend_kernel<Shape>;
@@ -800,7 +959,10 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   kernel<<<ctas, kAttendThreads, Shape::kSmem, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return SPLASH_ERR_CUDA;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3((unsigned)(p.kv_heads * p.row_tiles), (unsigned)(p.batch < 65535 ? p.batch : 65535));
+  // (a block a row where there are few items: each has many parts then)
+  const int64_t items = (int64_t)p.kv_heads * p.row_tiles * p.batch;
+  config.gridDim = dim3((unsigned)(p.kv_heads * p.row_tiles), (unsigned)(p.batch < 65535 ? p.batch : 65535),
+                        items * Shape::kRows <= 4 * kSms ? Shape::kRows : 1);
   config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
   cudaLaunchAttribute attribute{};
@@ -814,35 +976,48 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
 // CTAs that the GPU holds at a time
 template <typename Shape>
 constexpr int resident() {
-  return kSms * (Shape::kSmem <= 113 * 1024 ? 2 : 1);
+  return kSms * Shape::kResident;
 }
 
 // Calls fn with the shape that a call takes.
 template <typename Fn>
 static int with_shape(const SplashCacheAttendArgs& a, Fn&& fn) {
+  using std::integral_constant;
   const SplashKvCache& c = a.cache;
   const int64_t rows = a.q.size[2] * (a.q.size[1] / c.kv_heads);
-  auto pick = [&](auto format) {
-    constexpr int kF = decltype(format)::value;
-    auto wide = [&](auto k, auto v) {
-      constexpr int kK = decltype(k)::value, kV = decltype(v)::value;
-      // eight rows a CTA, or sixteen, which unpack the codes once for twice as many
-      if (rows <= 8 || kV > 128) return fn(AttendShape<kF, kK, kV, 1>{});
-      return fn(AttendShape<kF, kK, kV, kV <= 128 ? 2 : 1>{});
-    };
-    using std::integral_constant;
-    switch (c.row_k) {
-      case 64: return wide(integral_constant<int, 64>{}, integral_constant<int, 64>{});
-      case 96: return wide(integral_constant<int, 96>{}, integral_constant<int, 96>{});
-      case 128: return wide(integral_constant<int, 128>{}, integral_constant<int, 128>{});
-      case 192:
-        return c.row_v == 128 ? wide(integral_constant<int, 192>{}, integral_constant<int, 128>{})
-                              : wide(integral_constant<int, 192>{}, integral_constant<int, 192>{});
-      default: return wide(integral_constant<int, 256>{}, integral_constant<int, 256>{});
+  auto pick = [&](auto format, auto k, auto v, auto group) {
+    constexpr int kF = decltype(format)::value, kK = decltype(k)::value, kV = decltype(v)::value, kG = decltype(group)::value;
+    // Rows go in as few tiles as can be: the codes are read and unpacked again for each.
+    constexpr int kMost = kV <= 128 ? 4 : 1;
+    const int64_t tiles = (rows + 8 * kMost - 1) / (8 * kMost), blocks = (rows + 8 * tiles - 1) / (8 * tiles);
+    if constexpr (kMost > 1) {
+      if (blocks == 2) return fn(AttendShape<kF, kK, kV, kG, 2>{});
+      if (blocks == 3) return fn(AttendShape<kF, kK, kV, kG, 3>{});
+      if (blocks == 4) return fn(AttendShape<kF, kK, kV, kG, 4>{});
     }
+    return fn(AttendShape<kF, kK, kV, kG, 1>{});
   };
-  return c.format == SPLASH_CACHE_INT4 ? pick(std::integral_constant<int, SPLASH_CACHE_INT4>{})
-                                       : pick(std::integral_constant<int, SPLASH_CACHE_E4M3>{});
+  auto wide = [&](auto k, auto v) {
+    constexpr int kK = decltype(k)::value, kV = decltype(v)::value;
+    if (c.format == SPLASH_CACHE_E4M3) return pick(integral_constant<int, SPLASH_CACHE_E4M3>{}, k, v, integral_constant<int, 32>{});
+    constexpr integral_constant<int, SPLASH_CACHE_INT4> int4;
+    if constexpr (kK % 128 == 0 && kV % 128 == 0) {
+      if (c.group == 128) return pick(int4, k, v, integral_constant<int, 128>{});
+    }
+    if constexpr (kK % 64 == 0 && kV % 64 == 0) {
+      if (c.group == 64) return pick(int4, k, v, integral_constant<int, 64>{});
+    }
+    return pick(int4, k, v, integral_constant<int, 32>{});
+  };
+  switch (c.row_k) {
+    case 64: return wide(integral_constant<int, 64>{}, integral_constant<int, 64>{});
+    case 96: return wide(integral_constant<int, 96>{}, integral_constant<int, 96>{});
+    case 128: return wide(integral_constant<int, 128>{}, integral_constant<int, 128>{});
+    case 192:
+      return c.row_v == 128 ? wide(integral_constant<int, 192>{}, integral_constant<int, 128>{})
+                            : wide(integral_constant<int, 192>{}, integral_constant<int, 192>{});
+    default: return wide(integral_constant<int, 256>{}, integral_constant<int, 256>{});
+  }
 }
 
 static int check_attend(const SplashCacheAttendArgs& a) {
@@ -856,7 +1031,8 @@ static int check_attend(const SplashCacheAttendArgs& a) {
   if (a.q.size[3] != c.head_dim || a.o.size[3] != c.head_dim_v || a.q.size[1] % c.kv_heads != 0) return SPLASH_ERR_INVALID_ARGUMENT;
   if (a.page_table == nullptr || a.lengths == nullptr || a.n_table <= 0 || a.table_stride < 0) return SPLASH_ERR_INVALID_ARGUMENT;
   if (!(a.soft_cap >= 0.f)) return SPLASH_ERR_INVALID_ARGUMENT;
-  if (a.q.size[0] > (1 << 24) || a.q.size[1] > (1 << 20) || a.q.size[2] > (1 << 20) || a.q.size[1] * a.q.size[2] > (1 << 26))
+  if (a.q.size[0] > (1 << 24) || a.q.size[1] > (1 << 20) || a.q.size[2] > (1 << 20) || a.q.size[1] * a.q.size[2] > (1 << 26) ||
+      c.n_pages * c.kv_heads > 0x7fffffffll / (c.page_size / 16))  // (tiles of 16 tokens are counted in 32 bits)
     return SPLASH_ERR_TOO_LARGE;
   return SPLASH_OK;
 }
@@ -897,8 +1073,6 @@ static int cache_attend(const SplashCacheAttendArgs& a, cudaStream_t stream) {
   p.n_table = a.n_table;
   p.page_size = c.page_size;
   p.page_shift = log2_of(c.page_size);
-  p.group = c.format == SPLASH_CACHE_INT4 ? c.group : 32;
-  p.group_shift = log2_of(p.group);
   p.dtype = a.q.dtype;
   p.head_dim = c.head_dim;
   p.head_dim_v = c.head_dim_v;

@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "splash_common.cuh"
 
 namespace sb {
@@ -19,6 +21,18 @@ __host__ __device__ constexpr int cache_scale_bytes(int format, int width, int g
 
 __device__ __forceinline__ float bf16_bits_to_float(uint32_t bits) { return __uint_as_float(bits << 16); }
 
+// Two bf16 or f16 values of a word.
+__device__ __forceinline__ void unpack16(int dtype, uint32_t w, float& lo, float& hi) {
+  if (dtype == SPLASH_BF16) {
+    lo = bf16_bits_to_float(w);
+    hi = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+  }
+}
+
 // Eight values of one of the three element types from 16-byte aligned memory, and back.
 __device__ __forceinline__ void load8(const void* base, int dtype, int64_t at, float (&x)[8]) {
   if (dtype == SPLASH_F32) {
@@ -30,16 +44,7 @@ __device__ __forceinline__ void load8(const void* base, int dtype, int64_t at, f
   const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
   const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (dtype == SPLASH_BF16) {
-      x[2 * i] = __uint_as_float(words[i] << 16);
-      x[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
-    } else {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&words[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  }
+  for (int i = 0; i < 4; ++i) unpack16(dtype, words[i], x[2 * i], x[2 * i + 1]);
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
