@@ -529,11 +529,12 @@ typedef struct SplashCacheAttendArgs {
   float scale, soft_cap;        /* soft_cap 0: off */
   int32_t window;               /* negative: none */
   float mask_value;
-  void* workspace;              /* splash_cache_attend_workspace_bytes, 16-byte aligned; need not be zeroed */
+  void* workspace;              /* splash_cache_attend_workspace_bytes, 16-byte aligned; need not be zeroed; NULL if 0 */
   size_t workspace_bytes;
 } SplashCacheAttendArgs;
 int splash_cache_attend(const SplashCacheAttendArgs* args, void* cuda_stream);
-/* Reads the sizes in `args`, nothing on the device; 0 for sizes that splash_cache_attend refuses. */
+/* Reads the sizes in `args`, nothing on the device; 0 where no workspace is needed (short page tables or windows), and for
+ * sizes that splash_cache_attend refuses. */
 size_t splash_cache_attend_workspace_bytes(const SplashCacheAttendArgs* args);
 
 /* Copies the 4-word device error record to host (synchronises the stream) and maps it to a

@@ -94,7 +94,7 @@ CACHE_FAULTS = [("cache.k_codes", None, -1), ("cache.v_scales", 4104, -1), ("cac
     ("SplashCacheReadArgs", "page_table", None, -1), ("SplashCacheReadArgs", "n_table", 0, -1), ("SplashCacheReadArgs", "k.size.0", 2, -1),
     ("SplashCacheAttendArgs", "q.dtype", 1, -2), ("SplashCacheAttendArgs", "q.size.1", 3, -1), ("SplashCacheAttendArgs", "lengths", None, -1),
     ("SplashCacheAttendArgs", "soft_cap", -1.0, -1), ("SplashCacheAttendArgs", "soft_cap", float("nan"), -1),
-    ("SplashCacheAttendArgs", "workspace", None, -1), ("SplashCacheAttendArgs", "o.size.3", 56, -1)])
+    ("SplashCacheAttendArgs", "o.size.3", 56, -1)])
 def test_c_entry_points_refuse_before_they_touch_the_gpu(kind, path, value, status):
   fn = {"SplashCacheAppendArgs": "splash_cache_append", "SplashCacheReadArgs": "splash_cache_read",
         "SplashCacheAttendArgs": "splash_cache_attend"}[kind]
@@ -104,11 +104,16 @@ def test_c_entry_points_refuse_before_they_touch_the_gpu(kind, path, value, stat
 
 def test_workspace():
   lib = _native.lib()
-  size = lib.splash_cache_attend_workspace_bytes(C.byref(_args("SplashCacheAttendArgs")))
+  short = _args("SplashCacheAttendArgs")  # two pages: every item is one CTA's
+  assert lib.splash_cache_attend_workspace_bytes(C.byref(short)) == 0
+  a = _spoilt("SplashCacheAttendArgs", "n_table", 4096)
+  assert lib.splash_cache_attend_workspace_bytes(C.byref(a)) == 0  # (a window of 0: each query sees its own key)
+  a.window = -1
+  size = lib.splash_cache_attend_workspace_bytes(C.byref(a))
   assert 0 < size < 64 << 20
+  assert lib.splash_cache_attend(C.byref(a), None) == -1  # it has none
   assert lib.splash_cache_attend_workspace_bytes(C.byref(_spoilt("SplashCacheAttendArgs", "q.size.1", 3))) == 0
   assert lib.splash_cache_attend_workspace_bytes(None) == 0
-  a = _args("SplashCacheAttendArgs")
   a.workspace, a.workspace_bytes = 4096, size - 1
   assert lib.splash_cache_attend(C.byref(a), None) == -1
 

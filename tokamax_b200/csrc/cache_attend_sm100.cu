@@ -24,12 +24,13 @@
 // item in turn, each with a ring of its own in shared memory (cp.async; no barrier between warps while keys stream), and
 // join their sums at the end of the item.  An item that more than one CTA has worked on is joined by a second kernel, from
 // sums in the workspace, in the order of the CTAs: results do not depend on who comes first.
+#include <atomic>
+
 #include "cache_common.cuh"
 
 namespace sb {
 
-constexpr int kAttendWarps = 8;
-constexpr int kAttendThreads = kAttendWarps * 32;
+constexpr int kWarps = 4, kMostWarps = 8;  // of a CTA; kMostWarps where there are few items and each is one CTA's
 
 struct AttendParams {
   const uint8_t* k_codes;
@@ -49,7 +50,8 @@ struct AttendParams {
   int64_t q_stride_b, q_stride_h, q_stride_s, o_stride_b, o_stride_h, o_stride_s, table_stride, n_pages;
   float scale, soft_cap, mask_value;
   int32_t batch, q_heads, kv_heads, heads_per_kv, q_len, row_tiles, n_table, page_size, page_shift, dtype;
-  int32_t head_dim, head_dim_v, window, min_share;
+  int32_t head_dim, head_dim_v, window, item_cost, min_share;  // item_cost, min_share: in units
+  bool whole;  // every item is one CTA's
 };
 
 // ------------------------------------------------------------------------------------------
@@ -104,8 +106,14 @@ struct AttendShape {
   static constexpr bool kInt4 = kFormat == SPLASH_CACHE_INT4;
   static constexpr int kRows = 8 * kN;
   static constexpr int kRowK = cache_row_bytes(kFormat, kK), kRowV = cache_row_bytes(kFormat, kV);
-  // tokens of a unit: about 4 KB, which a warp has in flight for each stage
-  static constexpr int kUnit = kN > 2 ? 16 : kRowK + kRowV <= 64 && kN == 1 ? 64 : kRowK + kRowV <= 128 ? 32 : 16;
+  // Tokens of a unit.  A warp has a unit in flight while it works on another: about 4 KB (a quarter more or less with what 16
+  // tokens are), which fills the shared memory of an SM with 16 warps.  Where the rows' sums leave registers for 8 or 12 warps,
+  // a unit may be 8 KB (e4m3, head dim 128, 24 rows, 16 sequences of 1000 .. 8192 tokens: 63 -> 60 us), unless the logits
+  // of 32 tokens do not fit beside the sums (int4, whose scales take registers too).
+  static constexpr int kRowBytes = kRowK + kRowV;
+  static constexpr int kUnit = kN > 2   ? (kInt4 ? (kRowBytes <= 64 && kN == 3 ? 32 : 16) : kRowBytes <= 256 ? 32 : 16)
+                               : kN == 2 ? (kRowBytes <= (kInt4 ? 128 : 256) ? 32 : 16)
+                                         : (kRowBytes <= 64 ? 64 : kRowBytes <= 128 ? 32 : 16);
   static constexpr int kTiles = kUnit / 16;
   // channels that 16 bytes of codes hold, and MMA steps (16 channels) over them
   static constexpr int kChunk = kInt4 ? 32 : 16, kSteps = kChunk / 16;
@@ -115,17 +123,19 @@ struct AttendShape {
   static constexpr int kScaleK = cache_scale_bytes(kFormat, kK, kG_), kScaleV = cache_scale_bytes(kFormat, kV, kG_);
   static constexpr int kStageBytes = (kUnit * (kRowK + kRowV + kScaleK + kScaleV) + 127) / 128 * 128;
   static constexpr int kStages = 2;
-  static constexpr int kResident = kN == 1 && kV <= 128 ? 2 : 1;  // CTAs of an SM
+  static constexpr int kRegisters = kV * kN / 4 + 90;  // sums, and about what else a thread holds
+  static constexpr int kResident = 65536 / (kWarps * 32 * (kRegisters < 128 ? 128 : kRegisters));  // CTAs of an SM
+  static constexpr int kMostRegisters = kResident >= 4 ? 128 : kResident == 3 ? 168 : 255;
   // shared memory
   static constexpr int kFragBytes = kK / 16 * kN * 256;            // q as fragments
   static constexpr int kQSums = kFragBytes;                        // [kGroupsK][kRows] sums of q over a group
   static constexpr int kFactors = kQSums + kGroupsK * kRows * 4;   // [kRows] what S is multiplied by
-  static constexpr int kStats = kFactors + kRows * 4;              // [2][kAttendWarps][kRows] maxima and sums of the warps
-  static constexpr int kZeros = kStats + 2 * kAttendWarps * kRows * 4;  // [kAttendWarps][kGroupsV][kRows]
-  static constexpr int kRing = (kZeros + kAttendWarps * kGroupsV * kRows * 4 + 127) / 128 * 128;
-  static constexpr int kRingBytes = kAttendWarps * kStages * kStageBytes;
-  static constexpr int kJoinBytes = kAttendWarps * kRows * kV * 4;  // in the ring's place once it has run dry
-  static constexpr int kSmem = kRing + (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes);
+  static constexpr int kStats = kFactors + kRows * 4;              // [2][kMostWarps][kRows] maxima and sums of the warps
+  static constexpr int kZeros = kStats + 2 * kMostWarps * kRows * 4;  // [kMostWarps][kGroupsV][kRows]
+  static constexpr int kRing = (kZeros + kMostWarps * kGroupsV * kRows * 4 + 127) / 128 * 128;
+  static constexpr int kRingBytes = kStages * kStageBytes;  // of a warp
+  static constexpr int kJoinBytes = kRows * kV * 4;         // the same, in the ring's place once it has run dry
+  static constexpr int smem(int warps) { return kRing + warps * (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes); }
 };
 
 // Where in a stage 16-byte piece c of row r lies: so that eight consecutive rows' piece c are in eight different bank groups.
@@ -195,13 +205,14 @@ constexpr uint32_t kLeastTop = 87u << 23;  // 2^-40
 // ------------------------------------------------------------------------------------------
 // shares
 // ------------------------------------------------------------------------------------------
-// What a CTA spends on an item beside its units, in units: shares are equal in the sum of both.  (Looking up the item, q as
-// fragments, the first keys' latency, the warps' sums together: about what 20 of their units take.)
-constexpr int kItemCost = 20;
+// What a CTA spends on an item beside its units, in tokens: shares are equal in the sum of both.  (Looking up the item, q as
+// fragments, the first keys' latency, the warps' sums together.)
+constexpr int kItemTokens = 320;
+constexpr int kWholeTokens = 1024, kWholeItems = 64;
 
 struct Keys {  // of a sequence: tokens [lo, hi) in whole units from lo, which is a multiple of kUnit
   int lo, hi, units;
-  __device__ int cost() const { return units > 0 ? units + kItemCost : 0; }
+  __device__ int cost(const AttendParams& p) const { return units > 0 ? units + p.item_cost : 0; }
 };
 template <int kUnit>
 __device__ __forceinline__ Keys keys_of(const AttendParams& p, int length) {
@@ -223,28 +234,28 @@ struct Start {  // where a CTA's share begins
   int b;
 };
 
-// All threads; `scratch`: 2 * kAttendWarps + 3 words of shared memory of 8 bytes.
+// All threads of a CTA of kWarps; `scratch`: 2 * kWarps + 2 words of shared memory of 8 bytes.
 template <int kUnit>
 __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
   const int per_sequence = p.kv_heads * p.row_tiles;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t total = 0, mine = 0;  // mine: of the sequences that this thread counts when there is one round of them
-  for (int b = tid; b < p.batch; b += kAttendThreads) total += (mine = keys_of<kUnit>(p, __ldg(p.lengths + b)).cost());
+  for (int b = tid; b < p.batch; b += (kWarps * 32)) total += (mine = keys_of<kUnit>(p, __ldg(p.lengths + b)).cost(p));
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
   if (lane == 0) scratch[warp] = total;
   __syncthreads();
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kAttendWarps; ++w) total += scratch[w];
+  for (int w = 0; w < kWarps; ++w) total += scratch[w];
   const int64_t share = share_of(total * per_sequence, gridDim.x, p.min_share);
   const int64_t at = (int64_t)blockIdx.x * share;
   const bool keep = blockIdx.x == 0;  // this CTA writes down where the sequences start
-  int64_t* found = scratch + 2 * kAttendWarps;
+  int64_t* found = scratch + 2 * kWarps;
   int64_t carry = 0;
-  for (int base = 0; base < p.batch; base += kAttendThreads) {
+  for (int base = 0; base < p.batch; base += (kWarps * 32)) {
     const int b = base + tid;
-    if (base > 0 || p.batch > kAttendThreads) mine = b < p.batch ? keys_of<kUnit>(p, __ldg(p.lengths + b)).cost() : 0;
+    if (base > 0 || p.batch > (kWarps * 32)) mine = b < p.batch ? keys_of<kUnit>(p, __ldg(p.lengths + b)).cost(p) : 0;
     if (b >= p.batch) mine = 0;
     int64_t sum = mine;
 #pragma unroll
@@ -253,12 +264,12 @@ __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
       if (lane >= d) sum += other;
     }
     __syncthreads();
-    if (lane == 31) scratch[kAttendWarps + warp] = sum;
+    if (lane == 31) scratch[kWarps + warp] = sum;
     __syncthreads();
     int64_t before = carry, round = 0;
 #pragma unroll
-    for (int w = 0; w < kAttendWarps; ++w) {
-      const int64_t s = scratch[kAttendWarps + w];
+    for (int w = 0; w < kWarps; ++w) {
+      const int64_t s = scratch[kWarps + w];
       before += w < warp ? s : 0;
       round += s;
     }
@@ -308,7 +319,7 @@ __device__ __forceinline__ void finish_row(const AttendParams& p, int b, int hea
 }
 
 template <typename Shape>
-__global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __grid_constant__ AttendParams p) {
   constexpr int kN = Shape::kN, kRows = Shape::kRows, kUnit = Shape::kUnit, kTiles = Shape::kTiles, kSteps = Shape::kSteps;
   constexpr int kGroupsK = Shape::kGroupsK, kGroupsV = Shape::kGroupsV;
   constexpr bool kInt4 = Shape::kInt4;
@@ -316,142 +327,186 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
   float* const q_sums = reinterpret_cast<float*>(smem + Shape::kQSums);
   float* const factors = reinterpret_cast<float*>(smem + Shape::kFactors);
   float* const warp_max = reinterpret_cast<float*>(smem + Shape::kStats);
-  float* const warp_sum = warp_max + kAttendWarps * kRows;
+  float* const warp_sum = warp_max + kMostWarps * kRows;
   float* const warp_zeros = reinterpret_cast<float*>(smem + Shape::kZeros);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   grid_dependents_launch();  // the joining kernel may come up beside this one; it waits for its end
 
-  const Start start = find_start<kUnit>(p, reinterpret_cast<int64_t*>(smem));
-  __syncthreads();  // (its scratch is about to be q's place)
   const int per_sequence = p.kv_heads * p.row_tiles;
-  const int64_t all = start.total * per_sequence, share = share_of(all, gridDim.x, p.min_share);
-  int64_t at = (int64_t)blockIdx.x * share;
-  const int64_t end = min(at + share, all);
-  const int64_t first_unit = at;
-  int b = start.b;
-  int64_t before = start.before * per_sequence;  // units before sequence b
-  uint8_t* const ring = smem + Shape::kRing + warp * (Shape::kStages * Shape::kStageBytes);
+  int64_t at, end, before, share_begin;  // in the measure of shares; before: what lies before sequence b
+  int b;
+  if (p.whole) {  // items in turn
+    at = blockIdx.x;
+    end = (int64_t)p.batch * per_sequence;
+  } else {
+    const Start start = find_start<kUnit>(p, reinterpret_cast<int64_t*>(smem));
+    __syncthreads();  // (its scratch is about to be q's place)
+    const int64_t all = start.total * per_sequence, share = share_of(all, gridDim.x, p.min_share);
+    at = share_begin = (int64_t)blockIdx.x * share;
+    end = min(at + share, all);
+    b = start.b;
+    before = start.before * per_sequence;
+  }
+  uint8_t* const ring = smem + Shape::kRing + warp * Shape::kRingBytes;
   const uint32_t ring_at = smem_u32(ring);
+  constexpr int stage_step = Shape::kStageBytes;
+  float* const join = reinterpret_cast<float*>(smem + Shape::kRing);  // the warps' sums
   const int heads = p.heads_per_kv;
 
-  while (at < end) {
-    Keys keys = keys_of<kUnit>(p, __ldg(p.lengths + b));
-    while (at >= before + (int64_t)keys.cost() * per_sequence) {  // (sequences without keys are passed over)
-      before += (int64_t)keys.cost() * per_sequence;
-      keys = keys_of<kUnit>(p, __ldg(p.lengths + ++b));
-    }
-    const int length = __ldg(p.lengths + b);
-    const int item = (int)((at - before) / keys.cost());  // of this sequence: head * row_tiles + row tile
-    const int head = item / p.row_tiles, row0 = item % p.row_tiles * kRows;
-    const int64_t item_first = before + (int64_t)item * keys.cost() + kItemCost;  // of its first unit
-    const int u0 = (int)max(at - item_first, (int64_t)0), u1 = (int)min((int64_t)keys.units, end - item_first);
-    at = item_first + u1;
-    if (u1 <= 0) break;  // (the share ends before the item's keys)
-    const int n_rows = min(kRows, p.q_len * heads - row0);
-    const int32_t* const table = p.page_table + b * p.table_stride;
-
-    // ---- keys on their way: unit u of this item into a stage ----
-    // Pages are looked up for kTurns of a warp's units at a time, a batch ahead: lane i has where tile i of the batch lies,
-    // in tiles of the whole cache.
-    constexpr uint32_t kNowhere = ~0u;
-    constexpr int kTurns = 32 / kTiles;
-    auto look_up = [&](int turn) -> uint32_t {
-      const int u = u0 + warp + (turn + lane / kTiles) * kAttendWarps, token = keys.lo + u * kUnit + lane % kTiles * 16;
-      const int page = u < u1 && token < keys.hi ? __ldg(table + (token >> p.page_shift)) : -1;
-      return page >= 0 && page < p.n_pages ? ((uint32_t)(page * p.kv_heads + head) << (p.page_shift - 4)) + ((token & (p.page_size - 1)) >> 4)
-                                           : kNowhere;
-    };
-    uint32_t places = look_up(0), next_places = look_up(kTurns);
-    uint32_t absent = __ballot_sync(~0u, places == kNowhere);  // a bit for each tile of the batch that has no page
-    auto copy_tile = [&](uint32_t place, uint32_t to, int i) {
-      const uint32_t to_v = to + kUnit * Shape::kRowK, to_scales = to_v + kUnit * Shape::kRowV;
-      copy_rows<Shape::kRowK>(to + i * 16 * Shape::kRowK, p.k_codes, place, lane);
-      copy_rows<Shape::kRowV>(to_v + i * 16 * Shape::kRowV, p.v_codes, place, lane);
-      if (lane < Shape::kScaleK)
-        cp_async16(to_scales + i * Shape::kScaleK * 16 + lane * 16, p.k_scales + ((uint64_t)place * (Shape::kScaleK * 16) + lane * 16));
-      if (lane < Shape::kScaleV)
-        cp_async16(to_scales + kUnit * Shape::kScaleK + i * Shape::kScaleV * 16 + lane * 16,
-                   p.v_scales + ((uint64_t)place * (Shape::kScaleV * 16) + lane * 16));
-    };
-    // Starts the copies of the warp's unit number `turn`; called for each in turn.  Returns a bit for each of its tiles that
-    // has no page (its keys are not seen).
-    auto fetch = [&](int turn, int stage) -> uint32_t {
-      const int first = turn % kTurns * kTiles;
-      if (first == 0 && turn > 0) {
-        places = next_places;
-        absent = __ballot_sync(~0u, places == kNowhere);
-        next_places = look_up(turn + kTurns);
+  // The item that is worked on (or whose keys are on their way): b, item = head * row_tiles + row tile, units u0 .. u1 - 1.
+  int item = 0, u0 = 0, u1 = 0, length = 0;
+  Keys keys{};
+  bool is_last = false;  // its first unit is in this share, so that its sums are those of place 1
+  auto next_item = [&]() -> bool {
+    if (at >= end) return false;
+    if (p.whole) {
+      b = (int)((unsigned)at / (unsigned)per_sequence);
+      item = (int)((unsigned)at % (unsigned)per_sequence);
+      length = __ldg(p.lengths + b);
+      keys = keys_of<kUnit>(p, length);
+      u0 = 0;
+      u1 = keys.units;
+      at += gridDim.x;
+    } else {
+      length = __ldg(p.lengths + b);
+      keys = keys_of<kUnit>(p, length);
+      while (at >= before + (int64_t)keys.cost(p) * per_sequence) {  // (sequences without keys are passed over)
+        before += (int64_t)keys.cost(p) * per_sequence;
+        length = __ldg(p.lengths + ++b);
+        keys = keys_of<kUnit>(p, length);
       }
-      const uint32_t missing = absent >> first & ((1u << kTiles) - 1);
-      const uint32_t to = ring_at + stage * Shape::kStageBytes;
-      if (missing == 0) {
+      item = (int)((at - before) / keys.cost(p));
+      const int64_t first = before + (int64_t)item * keys.cost(p) + p.item_cost;  // of its units
+      u0 = (int)max(at - first, (int64_t)0);
+      u1 = (int)min((int64_t)keys.units, end - first);
+      is_last = first > share_begin;
+      at = first + u1;
+      if (u1 <= 0) return false;  // (the share ends before the item's keys)
+    }
+    return true;
+  };
+
+  // ---- keys on their way ----
+  // Pages are looked up for kTurns of a warp's units at a time, a batch ahead: lane i has where tile i of the batch lies,
+  // in tiles of the whole cache.
+  constexpr uint32_t kNowhere = ~0u;
+  constexpr int kTurns = 32 / kTiles;
+  auto look_up = [&](int turn) -> uint32_t {
+    const int u = u0 + warp + (turn + lane / kTiles) * warps, token = keys.lo + u * kUnit + lane % kTiles * 16;
+    const int page = u < u1 && token < keys.hi ? __ldg(p.page_table + b * p.table_stride + (token >> p.page_shift)) : -1;
+    return page >= 0 && page < p.n_pages ? ((uint32_t)(page * p.kv_heads + item / p.row_tiles) << (p.page_shift - 4)) + ((token & (p.page_size - 1)) >> 4)
+                                         : kNowhere;
+  };
+  uint32_t places, next_places;
+  uint32_t absent;  // a bit for each tile of the batch that has no page
+  auto copy_tile = [&](uint32_t place, uint32_t to, int i) {
+    const uint32_t to_v = to + kUnit * Shape::kRowK, to_scales = to_v + kUnit * Shape::kRowV;
+    copy_rows<Shape::kRowK>(to + i * 16 * Shape::kRowK, p.k_codes, place, lane);
+    copy_rows<Shape::kRowV>(to_v + i * 16 * Shape::kRowV, p.v_codes, place, lane);
+    if (lane < Shape::kScaleK)
+      cp_async16(to_scales + i * Shape::kScaleK * 16 + lane * 16, p.k_scales + ((uint64_t)place * (Shape::kScaleK * 16) + lane * 16));
+    if (lane < Shape::kScaleV)
+      cp_async16(to_scales + kUnit * Shape::kScaleK + i * Shape::kScaleV * 16 + lane * 16,
+                 p.v_scales + ((uint64_t)place * (Shape::kScaleV * 16) + lane * 16));
+  };
+  // Starts the copies of the warp's unit number `turn`; called for each in turn.  Returns a bit for each of its tiles that
+  // has no page (its keys are not seen).
+  auto fetch = [&](int turn, int stage) -> uint32_t {
+    const int first = turn % kTurns * kTiles;
+    if (first == 0 && turn > 0) {
+      places = next_places;
+      absent = __ballot_sync(~0u, places == kNowhere);
+      next_places = look_up(turn + kTurns);
+    }
+    const uint32_t missing = absent >> first & ((1u << kTiles) - 1);
+    const uint32_t to = ring_at + stage * stage_step;
+    if (missing == 0) {
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) copy_tile(__shfl_sync(~0u, places, first + i), to, i);
-      } else if (u0 + warp + turn * kAttendWarps < u1) {
-        for (int i = 0; i < kTiles; ++i) {
-          const uint32_t place = __shfl_sync(~0u, places, first + i);
-          if (!(missing >> i & 1)) {
-            copy_tile(place, to, i);
-          } else if (!kInt4) {
-            // P is 0 there, but 0 times what lay there before need not be (codes of four bits are numbers always)
-            for (int j = lane; j < Shape::kRowV; j += 32) cp_async16_zeros(to + kUnit * Shape::kRowK + i * 16 * Shape::kRowV + j * 16, p.v_codes);
-          }
+      for (int i = 0; i < kTiles; ++i) copy_tile(__shfl_sync(~0u, places, first + i), to, i);
+    } else if (u0 + warp + turn * warps < u1) {
+      for (int i = 0; i < kTiles; ++i) {
+        const uint32_t place = __shfl_sync(~0u, places, first + i);
+        if (!(missing >> i & 1)) {
+          copy_tile(place, to, i);
+        } else if (!kInt4) {
+          // P is 0 there, but 0 times what lay there before need not be (codes of four bits are numbers always)
+          for (int j = lane; j < Shape::kRowV; j += 32) cp_async16_zeros(to + kUnit * Shape::kRowK + i * 16 * Shape::kRowV + j * 16, p.v_codes);
         }
       }
-      cp_async_commit();
-      return missing;
-    };
-    constexpr int kAhead = Shape::kStages - 1;  // units on their way while one is worked on
-    uint32_t missing[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) missing[i] = fetch(i, i);
+    }
+    cp_async_commit();
+    return missing;
+  };
+  constexpr int kAhead = Shape::kStages - 1;  // units on their way while one is worked on
+  static_assert(kAhead == 1);
+  uint32_t missing[kAhead];
+  auto start_item = [&]() {
+    places = look_up(0);
+    next_places = look_up(kTurns);
+    absent = __ballot_sync(~0u, places == kNowhere);
+    missing[0] = fetch(0, 0);
+  };
 
-    // ---- q as fragments; a warp a row ----
-    for (int r = warp; r < kRows; r += kAttendWarps) {
+  while (next_item()) {
+    start_item();
+    const int head = item / p.row_tiles, row0 = item % p.row_tiles * kRows;
+    const int n_rows = min(kRows, p.q_len * heads - row0);
+
+    // ---- q as fragments: kLanes lanes (a power of two that holds the row's width / 8) a row ----
+    // Row r of the tile is query (first_row + r) / heads behind first_query (r and heads are small: the quotient by a product
+    // is exact), q head (first_row + r) % heads of the kv head.
+    const int first_query = row0 / heads, first_row = row0 - first_query * heads;
+    const float per_head = 1.f / (float)heads;
+    auto query_of = [&](int r) { return (int)(((float)(first_row + r) + 0.5f) * per_head); };
+    constexpr int kLanes = Shape::kK <= 64 ? 8 : Shape::kK <= 128 ? 16 : 32, kAtOnce = 32 / kLanes;
+    const int piece = lane % kLanes;
+    for (int r = warp * kAtOnce + lane / kLanes; r < kRows; r += warps * kAtOnce) {
       float x[8] = {};
-      if (r < n_rows && lane * 8 < p.head_dim) {
-        const int row = row0 + r, i = row / heads, h = head * heads + row % heads;
-        load8(p.q, p.dtype, b * p.q_stride_b + h * p.q_stride_h + i * p.q_stride_s + lane * 8, x);
+      if (r < n_rows && piece * 8 < p.head_dim) {
+        const int i = query_of(r), h = head * heads + first_row + r - i * heads;
+        load8(p.q, p.dtype, b * p.q_stride_b + h * p.q_stride_h + (first_query + i) * p.q_stride_s + piece * 8, x);
       }
       float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+      for (int i = 0; i < 8; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+      for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
       // the power of two that brings `top` to 2^14 .. 2^15, within 2^-100 .. 2^100; with the sign of the logits' scale
       const int e = min(max((int)(__float_as_uint(top) >> 23), 41), 227);
       const float up = copysignf(__uint_as_float((uint32_t)(268 - e) << 23), p.scale), down = __uint_as_float((uint32_t)(e - 14) << 23);
-      uint16_t h16[8];
+      __half h16[8];
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const __half h = __float2half_rn(x[i] * up);
-        h16[i] = __half_as_ushort(h);
-        sum += __half2float(h);
-        // int4: the odd codes of a half-word stand four bits higher
-        if (kInt4 && (i & 1)) h16[i] = __half_as_ushort(__float2half_rn(__half2float(h) * 0.0625f));
+        h16[i] = __float2half_rn(x[i] * up);
+        if (kInt4) sum += __half2float(h16[i]);
       }
-      auto two = [&](int lo, int hi) { return (uint32_t)h16[lo] | (uint32_t)h16[hi] << 16; };
-      if (lane * 8 < Shape::kK) {
-        uint2* const frag = reinterpret_cast<uint2*>(smem);
-        const int block = r >> 3, n = r & 7;
-        if (kInt4) {  // a lane's eight channels are one word of codes: steps 2 * (lane / 4) and the next, column lane % 4
-          frag[((lane >> 2) * 2 * kN + block) * 32 + n * 4 + (lane & 3)] = make_uint2(two(0, 4), two(1, 5));
-          frag[(((lane >> 2) * 2 + 1) * kN + block) * 32 + n * 4 + (lane & 3)] = make_uint2(two(2, 6), two(3, 7));
-        } else {  // two words of codes: columns 2 * (lane % 2) and the next of step lane / 2
-          frag[((lane >> 1) * kN + block) * 32 + n * 4 + (lane & 1) * 2] = make_uint2(two(0, 1), two(2, 3));
-          frag[((lane >> 1) * kN + block) * 32 + n * 4 + (lane & 1) * 2 + 1] = make_uint2(two(4, 5), two(6, 7));
+      auto two = [&](int lo, int hi) { return (uint32_t)__half_as_ushort(h16[lo]) | (uint32_t)__half_as_ushort(h16[hi]) << 16; };
+      auto sixteenth = [&](uint32_t pair) {  // int4: the odd codes of a half-word stand four bits higher
+        const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&pair), __float2half2_rn(0.0625f));
+        return *reinterpret_cast<const uint32_t*>(&y);
+      };
+      if (piece * 8 < Shape::kK) {
+        // For each 32 channels, block of rows and lane of the MMA: its part of both steps.
+        uint4* const frag = reinterpret_cast<uint4*>(smem) + ((piece >> 2) * kN + (r >> 3)) * 32 + (r & 7) * 4;
+        if (kInt4) {  // a lane's eight channels are one word of codes, column piece % 4
+          const uint32_t odd = sixteenth(two(1, 5)), odd2 = sixteenth(two(3, 7));
+          frag[piece & 3] = make_uint4(two(0, 4), odd, two(2, 6), odd2);
+        } else {  // two words of codes: columns 2 * (piece % 2) and the next of step piece / 2 % 2
+          uint2* const half = reinterpret_cast<uint2*>(frag + (piece & 1) * 2) + (piece >> 1 & 1);
+          half[0] = make_uint2(two(0, 1), two(2, 3));
+          half[2] = make_uint2(two(4, 5), two(6, 7));
         }
       }
       if (kInt4) {
-        constexpr int kLanes = Shape::kPerGroupK * 4;  // of a group
+        constexpr int kGroupLanes = Shape::kPerGroupK * 4;
 #pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        if (lane % kLanes == 0 && lane * 8 < Shape::kK)
-          q_sums[lane / kLanes * kRows + r] = sum * 0x1p-24f;  // in the units of the products of codes
+        for (int d = 1; d < kGroupLanes; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        if (piece % kGroupLanes == 0 && piece * 8 < Shape::kK)
+          q_sums[piece / kGroupLanes * kRows + r] = sum * 0x1p-24f;  // in the units of the products of codes
       }
-      if (lane == 0) factors[r] = fmaxf(fabsf(p.scale) * down * (kInt4 ? 0x1p24f : 1.f) * (p.soft_cap > 0.f ? 1.f : kLog2e), 1e-37f);
+      if (piece == 0) factors[r] = fmaxf(fabsf(p.scale) * down * (kInt4 ? 0x1p24f : 1.f) * (p.soft_cap > 0.f ? 1.f : kLog2e), 1e-37f);
     }
     __syncthreads();
 
@@ -471,24 +526,25 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
         factor[nb][j] = p.soft_cap > 0.f ? 1.f : factors[nb * 8 + t4 * 2 + j];
       }
     // units of which every row sees every key: whole_lo .. whole_hi - 1
-    const int whole_hi = (min(length - p.q_len + row0 / heads + 1, keys.hi) - keys.lo) / kUnit;
-    const int whole_lo = p.window < 0 ? 0 : max(length - p.q_len + (row0 + n_rows - 1) / heads - p.window - keys.lo + kUnit - 1, 0) / kUnit;
+    const int position0 = length - p.q_len + first_query;  // of the tile's first query
+    const int whole_hi = (min(position0 + 1, keys.hi) - keys.lo) / kUnit;
+    const int whole_lo = p.window < 0 ? 0 : max(position0 + query_of(n_rows - 1) - p.window - keys.lo + kUnit - 1, 0) / kUnit;
 
-    const uint2* const frags = reinterpret_cast<const uint2*>(smem) + lane;
+    const uint4* const frags = reinterpret_cast<const uint4*>(smem) + lane;
     // where a lane's rows of matrices begin: K, the next tile's in the upper half of the warp; V, the next piece's
     const uint32_t lane_k = Pieces<Shape::kRowK>::row_at(kTiles > 1 ? lane : lane & 15);
     const uint32_t lane_v = kUnit * Shape::kRowK + Pieces<Shape::kRowV>::at(Pieces<Shape::kRowV>::row_at(lane & 15), Pieces<Shape::kRowV>::kTurn > 0 ? lane >> 4 : 0) +
                             (Pieces<Shape::kRowV>::kTurn > 0 ? 0 : (lane >> 4) * 16);
     int stage = 0, turn = 0;
-    for (int u = u0 + warp; u < u1; u += kAttendWarps, ++turn) {
+    for (int u = u0 + warp; u < u1; u += warps, ++turn) {
       cp_async_wait<kAhead - 1>();
       __syncwarp();
       const uint32_t none = missing[0];
 #pragma unroll
       for (int i = 0; i + 1 < kAhead; ++i) missing[i] = missing[i + 1];
       missing[kAhead - 1] = fetch(turn + kAhead, stage == 0 ? kAhead : stage - 1);
-      const uint32_t from_k = ring_at + stage * Shape::kStageBytes + lane_k, from_v = ring_at + stage * Shape::kStageBytes + lane_v;
-      const uint8_t* const scales_k = ring + stage * Shape::kStageBytes + kUnit * (Shape::kRowK + Shape::kRowV);
+      const uint32_t from_k = ring_at + stage * stage_step + lane_k, from_v = ring_at + stage * stage_step + lane_v;
+      const uint8_t* const scales_k = ring + stage * stage_step + kUnit * (Shape::kRowK + Shape::kRowV);
       const uint8_t* const scales_v = scales_k + kUnit * Shape::kScaleK;
       stage = stage == kAhead ? 0 : stage + 1;
 
@@ -507,11 +563,9 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
 #pragma unroll
           for (int cc = 0; cc < Shape::kPerGroupK; ++cc) {
             const int c = group * Shape::kPerGroupK + cc;
-            uint2 qf[2][kN];
+            uint4 qf[kN];
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-              for (int nb = 0; nb < kN; ++nb) qf[k][nb] = frags[((c * 2 + k) * kN + nb) * 32];
+            for (int nb = 0; nb < kN; ++nb) qf[nb] = frags[(c * kN + nb) * 32];
             uint32_t words[kTiles][2];
             load_tiles<kTiles, Shape::kRowK>(Pieces<Shape::kRowK>::at(from_k, c), words);
 #pragma unroll
@@ -523,8 +577,8 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
               const uint32_t a2[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
 #pragma unroll
               for (int nb = 0; nb < kN; ++nb) {
-                mma_f16(acc[i][nb], a, qf[0][nb].x, qf[0][nb].y);
-                mma_f16(acc[i][nb], a2, qf[1][nb].x, qf[1][nb].y);
+                mma_f16(acc[i][nb], a, qf[nb].x, qf[nb].y);
+                mma_f16(acc[i][nb], a2, qf[nb].z, qf[nb].w);
               }
             }
           }
@@ -552,11 +606,13 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
           for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[i][nb][j] = 0.f;
+        uint4 qf[kN];
 #pragma unroll
         for (int c = 0; c < Shape::kChunksK; ++c) {
-          uint2 qf[kN];
+          if (c % 2 == 0) {
 #pragma unroll
-          for (int nb = 0; nb < kN; ++nb) qf[nb] = frags[(c * kN + nb) * 32];
+            for (int nb = 0; nb < kN; ++nb) qf[nb] = frags[(c / 2 * kN + nb) * 32];
+          }
           uint32_t words[kTiles][2];
           load_tiles<kTiles, Shape::kRowK>(Pieces<Shape::kRowK>::at(from_k, c), words);
 #pragma unroll
@@ -564,7 +620,7 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
             const uint32_t w0 = words[i][0], w1 = words[i][1];
             const uint32_t a[4] = {e4m3x2_to_f16x2(w0), e4m3x2_to_f16x2(w1), e4m3x2_to_f16x2(w0 >> 16), e4m3x2_to_f16x2(w1 >> 16)};
 #pragma unroll
-            for (int nb = 0; nb < kN; ++nb) mma_f16(s[i][nb], a, qf[nb].x, qf[nb].y);
+            for (int nb = 0; nb < kN; ++nb) mma_f16(s[i][nb], a, c % 2 == 0 ? qf[nb].x : qf[nb].z, c % 2 == 0 ? qf[nb].y : qf[nb].w);
           }
         }
 #pragma unroll
@@ -601,7 +657,7 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
         for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int position = length - p.q_len + (row0 + min(nb * 8 + t4 * 2 + (j & 1), n_rows - 1)) / heads;
+            const int position = position0 + query_of(min(nb * 8 + t4 * 2 + (j & 1), n_rows - 1));
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
               const int token = token0 + i * 16 + (j >> 1) * 8 + g;
@@ -763,7 +819,8 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
         accumulate(std::true_type{});
       __syncwarp();
     }
-    cp_async_wait<0>();  // (nothing is in flight here that anyone waits for; the ring's place is about to be written)
+    cp_async_wait<0>();  // (nothing is in flight that anyone waits for; the place of the stages is about to be written)
+
 
     // ---- the warps' sums together ----
 #pragma unroll
@@ -795,7 +852,7 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
       }
     __syncthreads();
     {
-      float* const join = reinterpret_cast<float*>(smem + Shape::kRing) + warp * (kRows * Shape::kV);
+      float* const own = join + warp * (kRows * Shape::kV);
       constexpr float kBack = kInt4 ? 0x1p24f : 1.f;  // of products of codes
 #pragma unroll
       for (int nb = 0; nb < kN; ++nb)
@@ -803,8 +860,7 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
         for (int j = 0; j < 2; ++j) {
           const int r = nb * 8 + t4 * 2 + j;
           float most = kNoMaximum;
-#pragma unroll
-          for (int w = 0; w < kAttendWarps; ++w) most = fmaxf(most, warp_max[w * kRows + r]);
+          for (int w = 0; w < warps; ++w) most = fmaxf(most, warp_max[w * kRows + r]);
           const float weight = ex2(base[nb][j] - most);
 #pragma unroll
           for (int c = 0; c < Shape::kChunksV; ++c) {
@@ -812,10 +868,10 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
               const float4 x = make_float4(o[c][0][nb][j] * kBack, o[c][0][nb][2 + j] * (kBack * 0.0625f),
                                            o[c][1][nb][j] * kBack, o[c][1][nb][2 + j] * (kBack * 0.0625f));
               const float z = warp_zeros[(warp * kGroupsV + c / Shape::kPerGroupV) * kRows + r];
-              *reinterpret_cast<float4*>(join + r * Shape::kV + c * 32 + g * 4) =
+              *reinterpret_cast<float4*>(own + r * Shape::kV + c * 32 + g * 4) =
                   make_float4((x.x + z) * weight, (x.y + z) * weight, (x.z + z) * weight, (x.w + z) * weight);
             } else {
-              *reinterpret_cast<float2*>(join + r * Shape::kV + c * 16 + g * 2) =
+              *reinterpret_cast<float2*>(own + r * Shape::kV + c * 16 + g * 2) =
                   make_float2(o[c][0][nb][j] * weight, o[c][0][nb][2 + j] * weight);
             }
           }
@@ -824,17 +880,17 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
     __syncthreads();
     const bool alone = u0 == 0 && u1 == keys.units;
     // sums of this CTA: an item that began before its share in place 0, one that goes on behind it in place 1 (both: 0)
-    float* const part = p.parts + ((int64_t)blockIdx.x * 2 + (item_first > first_unit ? 1 : 0)) * (kRows * (Shape::kV + 2));
-    for (int id = tid; id < n_rows * (Shape::kV / 8); id += kAttendThreads) {
+    float* const part = p.parts + ((int64_t)blockIdx.x * 2 + (is_last ? 1 : 0)) * (kRows * (Shape::kV + 2));
+    for (int id = tid; id < n_rows * (Shape::kV / 8); id += blockDim.x) {
       const int r = id / (Shape::kV / 8), d = id % (Shape::kV / 8) * 8;
       float x[8] = {};
       float most = kNoMaximum, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kAttendWarps; ++w) most = fmaxf(most, warp_max[w * kRows + r]);
-#pragma unroll
-      for (int w = 0; w < kAttendWarps; ++w) {
+#pragma unroll 4
+      for (int w = 0; w < warps; ++w) most = fmaxf(most, warp_max[w * kRows + r]);
+#pragma unroll 4
+      for (int w = 0; w < warps; ++w) {
         sum += warp_sum[w * kRows + r] * ex2(warp_max[w * kRows + r] - most);
-        const float4* const from = reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem + Shape::kRing) + (w * kRows + r) * Shape::kV + d);
+        const float4* const from = reinterpret_cast<const float4*>(join + (w * kRows + r) * Shape::kV + d);
         const float4 lo = from[0], hi = from[1];
         x[0] += lo.x, x[1] += lo.y, x[2] += lo.z, x[3] += lo.w, x[4] += hi.x, x[5] += hi.y, x[6] += hi.z, x[7] += hi.w;
       }
@@ -859,57 +915,63 @@ __global__ void __launch_bounds__(kAttendThreads, Shape::kResident) cache_attend
 // ------------------------------------------------------------------------------------------
 constexpr int kJoinThreads = 256;
 
-// blockIdx.x: row tile of an item (fastest) and head; y: sequence; z: rows z, z + gridDim.z ..  Threads have eight channels
-// of a row; where there are more threads than that, several have the same and take every n-th part.
+// blockIdx.x: row tile of an item (fastest) and head; y: sequence.  A thread has eight channels of a row; a row's parts are
+// dealt to as many threads as there are parts for, so that a block takes several rows at a time where they are few.  z: the
+// rows that a block takes are every gridDim.z-th such lot.
 template <int kRows, int kV>
 __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const __grid_constant__ AttendParams p, int ctas) {
-  constexpr int kEach = kV / 8, kSlices = kJoinThreads / kEach;  // threads of a row, and of it in turn
+  constexpr int kEach = kV / 8, kLanes = kJoinThreads / kEach;  // threads of a row's channels; how many such lots
+  constexpr int kMostSlices = kLanes >= 16 ? 16 : 8;
+  static_assert(kLanes >= 8);
   constexpr int kPart = kRows * (kV + 2);
-  __shared__ float sums[kSlices][kV];
-  __shared__ float stats[2][kSlices];
+  __shared__ float sums[kMostSlices][kV];
+  __shared__ float stats[2][kMostSlices];
   grid_dependency_wait();
   const int per_sequence = p.kv_heads * p.row_tiles;
-  const int slice = threadIdx.x / kEach, d = threadIdx.x % kEach * 8;
+  const int lot = threadIdx.x / kEach, d = threadIdx.x % kEach * 8;
   const int64_t share = share_of(p.starts[p.batch] * per_sequence, ctas, p.min_share);
   for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
     const int64_t before = p.starts[b], cost = p.starts[b + 1] - before;
-    const int64_t first = before * per_sequence + blockIdx.x * cost + kItemCost;  // unit of this item
-    const int64_t c0 = first / share, c1 = cost > 0 ? (first + cost - kItemCost - 1) / share : c0 - 1;
+    const int64_t first = before * per_sequence + blockIdx.x * cost + p.item_cost;  // unit of this item
+    const int64_t c0 = first / share, c1 = cost > 0 ? (first + cost - p.item_cost - 1) / share : c0 - 1;
     if (c0 == c1) continue;  // written already
     const int head = blockIdx.x / p.row_tiles, row0 = blockIdx.x % p.row_tiles * kRows;
     const int n_rows = min(kRows, p.q_len * p.heads_per_kv - row0);
-    for (int r = blockIdx.z; r < n_rows; r += gridDim.z) {
+    int slices = 1;
+    while (slices < kMostSlices && slices * 2 <= c1 - c0 + 1) slices *= 2;
+    const int at_once = kMostSlices / slices, slice = lot % slices;
+    for (int r0 = blockIdx.z * at_once; r0 < n_rows; r0 += gridDim.z * at_once) {
+      const int r = r0 + lot / slices;
       float most = kNoMaximum, sum = 0.f, x[8] = {};
-      if (slice < kSlices) {
-        const float* part = p.parts + (c0 + slice) * (2 * kPart);
-        constexpr int kAtOnce = 4;  // parts whose loads are in flight together
-        for (int64_t c = c0 + slice; c <= c1; c += kSlices * kAtOnce) {
-          float m[kAtOnce], l[kAtOnce];
-          float4 lo[kAtOnce], hi[kAtOnce];
+      const bool mine = lot < kMostSlices && r < n_rows;
+      if (mine) {
+        constexpr int kAhead = 4;  // parts whose loads are in flight together
+        for (int64_t c = c0 + slice; c <= c1; c += slices * kAhead) {
+          float m[kAhead], l[kAhead];
+          float4 lo[kAhead], hi[kAhead];
 #pragma unroll
-          for (int k = 0; k < kAtOnce; ++k) {
-            const int64_t at = c + k * kSlices;
+          for (int k = 0; k < kAhead; ++k) {
+            const int64_t at = c + k * slices;
             m[k] = kNoMaximum;
             l[k] = 0.f;
             lo[k] = hi[k] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (at > c1) continue;
             // the first CTA has the item last in its share, unless it starts there
-            const float* const from = part + k * (kSlices * 2 * kPart) + (at * share < first ? kPart : 0);
+            const float* const from = p.parts + at * (2 * kPart) + (at * share < first ? kPart : 0);
             m[k] = from[kRows * kV + r];
             l[k] = from[kRows * (kV + 1) + r];
             lo[k] = *reinterpret_cast<const float4*>(from + r * kV + d);
             hi[k] = *reinterpret_cast<const float4*>(from + r * kV + d + 4);
           }
-          part += kAtOnce * (kSlices * 2 * kPart);
           float top = most;
 #pragma unroll
-          for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, m[k]);
+          for (int k = 0; k < kAhead; ++k) top = fmaxf(top, m[k]);
           const float old = ex2(most - top);
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[k] *= old;
           sum *= old;
 #pragma unroll
-          for (int k = 0; k < kAtOnce; ++k) {
+          for (int k = 0; k < kAhead; ++k) {
             const float weight = ex2(m[k] - top);
             const float y[8] = {lo[k].x, lo[k].y, lo[k].z, lo[k].w, hi[k].x, hi[k].y, hi[k].z, hi[k].w};
 #pragma unroll
@@ -918,32 +980,35 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const _
           }
           most = top;
         }
-        *reinterpret_cast<float4*>(&sums[slice][d]) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(&sums[slice][d + 4]) = make_float4(x[4], x[5], x[6], x[7]);
-        if (d == 0) {
-          stats[0][slice] = most;
-          stats[1][slice] = sum;
-        }
       }
-      __syncthreads();
-      if (slice == 0) {
-        float top = most;
-#pragma unroll
-        for (int k = 1; k < kSlices; ++k) top = fmaxf(top, stats[0][k]);
-        const float own = ex2(most - top);
-        sum *= own;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= own;
-#pragma unroll
-        for (int k = 1; k < kSlices; ++k) {
-          const float weight = ex2(stats[0][k] - top);
-          sum = fmaf(stats[1][k], weight, sum);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = fmaf(sums[k][d + i], weight, x[i]);
+      if (slices > 1) {  // (all threads of the block alike)
+        if (mine && slice > 0) {
+          *reinterpret_cast<float4*>(&sums[lot][d]) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(&sums[lot][d + 4]) = make_float4(x[4], x[5], x[6], x[7]);
+          if (d == 0) {
+            stats[0][lot] = most;
+            stats[1][lot] = sum;
+          }
         }
-        finish_row(p, b, head, row0 + r, d, x, top, sum);
+        __syncthreads();
+        if (mine && slice == 0) {
+          float top = most;
+          for (int k = 1; k < slices; ++k) top = fmaxf(top, stats[0][lot + k]);
+          const float own = ex2(most - top);
+          sum *= own;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= own;
+          for (int k = 1; k < slices; ++k) {
+            const float weight = ex2(stats[0][lot + k] - top);
+            sum = fmaf(stats[1][lot + k], weight, sum);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(sums[lot + k][d + i], weight, x[i]);
+          }
+          most = top;
+        }
+        __syncthreads();
       }
-      __syncthreads();
+      if (mine && slice == 0) finish_row(p, b, head, row0 + r, d, x, most, sum);
     }
   }
 }
@@ -954,15 +1019,24 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const _
 template <typename Shape>
 static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   auto kernel = cache_attend_kernel<Shape>;
-  static_assert(Shape::kSmem <= 227 * 1024);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem) != cudaSuccess) return SPLASH_ERR_CUDA;
-  kernel<<<ctas, kAttendThreads, Shape::kSmem, stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return SPLASH_ERR_CUDA;
-  cudaLaunchConfig_t config{};
-  // (a block a row where there are few items: each has many parts then)
+  static_assert(Shape::smem(kMostWarps) <= 227 * 1024);
+  static std::atomic<uint64_t> ready{0};  // devices that know how much shared memory the kernel takes
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return SPLASH_ERR_CUDA;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem(kMostWarps)) != cudaSuccess) return SPLASH_ERR_CUDA;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int64_t items = (int64_t)p.kv_heads * p.row_tiles * p.batch;
+  const int warps = p.whole && items < 2 * kSms ? kMostWarps : kWarps;
+  kernel<<<p.whole && items < ctas ? (int)items : ctas, warps * 32, Shape::smem(warps), stream>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return SPLASH_ERR_CUDA;
+  if (p.whole) return SPLASH_OK;
+  cudaLaunchConfig_t config{};
+  // (as many blocks of an item as its rows and the GPU have room for: where items are few, each has many parts)
   config.gridDim = dim3((unsigned)(p.kv_heads * p.row_tiles), (unsigned)(p.batch < 65535 ? p.batch : 65535),
-                        items * Shape::kRows <= 4 * kSms ? Shape::kRows : 1);
+                        (unsigned)(items >= 8 * kSms ? 1 : items * Shape::kRows <= 8 * kSms ? Shape::kRows : 8 * kSms / items));
   config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
   cudaLaunchAttribute attribute{};
@@ -1037,6 +1111,16 @@ static int check_attend(const SplashCacheAttendArgs& a) {
   return SPLASH_OK;
 }
 
+// Whether every item is given to one CTA: one launch, no sums in the workspace.
+template <typename Shape>
+static bool is_whole(const SplashCacheAttendArgs& a) {
+  int64_t reach = (int64_t)a.n_table * a.cache.page_size;
+  if (a.window >= 0 && reach > a.window + a.q.size[2]) reach = a.window + a.q.size[2];
+  const int64_t tiles = (a.q.size[2] * (a.q.size[1] / a.cache.kv_heads) + Shape::kRows - 1) / Shape::kRows;
+  const int64_t items = a.q.size[0] * a.cache.kv_heads * tiles;
+  return reach <= (items < kWholeItems ? kWholeTokens : 2 * kWholeTokens) && items <= INT32_MAX;
+}
+
 template <typename Shape>
 static size_t parts_bytes() {
   return (size_t)resident<Shape>() * 2 * Shape::kRows * (Shape::kV + 2) * 4;
@@ -1045,7 +1129,6 @@ static size_t parts_bytes() {
 static int cache_attend(const SplashCacheAttendArgs& a, cudaStream_t stream) {
   if (const int status = check_attend(a)) return status;
   const SplashKvCache& c = a.cache;
-  if (a.workspace == nullptr || (reinterpret_cast<uintptr_t>(a.workspace) & 15u) != 0) return SPLASH_ERR_INVALID_ARGUMENT;
   AttendParams p{};
   p.k_codes = static_cast<const uint8_t*>(c.k_codes);
   p.k_scales = static_cast<const uint8_t*>(c.k_scales);
@@ -1079,13 +1162,19 @@ static int cache_attend(const SplashCacheAttendArgs& a, cudaStream_t stream) {
   p.window = a.window < 0 ? -1 : a.window;
   return with_shape(a, [&](auto shape) -> int {
     using Shape = decltype(shape);
-    const size_t parts = parts_bytes<Shape>();
-    if (a.workspace_bytes < parts + 8 * ((size_t)p.batch + 1)) return SPLASH_ERR_INVALID_ARGUMENT;
     AttendParams own = p;
-    own.parts = static_cast<float*>(a.workspace);
-    own.starts = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(a.workspace) + parts);
+    own.whole = is_whole<Shape>(a);
+    if (!own.whole) {
+      const size_t parts = parts_bytes<Shape>();
+      if (a.workspace == nullptr || (reinterpret_cast<uintptr_t>(a.workspace) & 15u) != 0 ||
+          a.workspace_bytes < parts + 8 * ((size_t)p.batch + 1))
+        return SPLASH_ERR_INVALID_ARGUMENT;
+      own.parts = static_cast<float*>(a.workspace);
+      own.starts = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(a.workspace) + parts);
+    }
     own.row_tiles = (p.q_len * p.heads_per_kv + Shape::kRows - 1) / Shape::kRows;
-    own.min_share = kAttendWarps;
+    own.item_cost = kItemTokens / Shape::kUnit;
+    own.min_share = kWarps;
     return launch<Shape>(own, resident<Shape>(), stream);
   });
 }
@@ -1094,7 +1183,8 @@ static size_t cache_attend_workspace(const SplashCacheAttendArgs& a) {
   if (check_attend(a) != SPLASH_OK) return 0;
   size_t bytes = 0;
   with_shape(a, [&](auto shape) -> int {
-    bytes = parts_bytes<decltype(shape)>() + 8 * ((size_t)a.q.size[0] + 1);
+    using Shape = decltype(shape);
+    if (!is_whole<Shape>(a)) bytes = parts_bytes<Shape>() + 8 * ((size_t)a.q.size[0] + 1);
     return 0;
   });
   return bytes;

@@ -450,8 +450,11 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
   a.window = window.has_value() ? (int32_t)*window : -1;
   a.mask_value = (float)mask_value;
   a.workspace_bytes = cache_lib.attend_workspace_bytes(&a);
-  const at::Tensor workspace = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
-  a.workspace = workspace.data_ptr();
+  at::Tensor workspace;
+  if (a.workspace_bytes != 0) {
+    workspace = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
+    a.workspace = workspace.data_ptr();
+  }
   check_cache_call(on_stream_of(q, [&](void* stream) { return cache_lib.attend(&a, stream); }), "splash_cache_attend");
   return {o, lse, max_logits};
 }
