@@ -172,7 +172,7 @@ def _check_attend(store, *, q_heads, t=1, window=None, soft_cap=None, sinks=None
     # Rounding: of P * scale to f16, 2^-11 of each term (plus a little for sums in 32 bits: 2^-18); of logits, 2^-24 of each
     # of some hundred partial sums of size |q| |k| scale, which moves each p, and with it o, by up to twice that in all; of
     # o to its type.
-    logits = (q[b].double().norm(dim=-1).max() * (k.norm(dim=-1).max() if n else 0.0) * scale).clamp_min(1.0)
+    logits = (q[b].double().norm(dim=-1).max() * (k.norm(dim=-1).max() if n else 0.0) * abs(scale)).clamp_min(1.0)
     slack = 2.0 ** -18 * logits
     err = (o[b].cpu().double() - ref).abs()
     before = (ROUNDOFF[torch.float16] + 2.0 ** -18) * moved + 2 * slack * size + 1e-9
@@ -231,7 +231,7 @@ def test_sizes_of_scales_and_queries():
   for fmt, group in FORMATS:
     gain = torch.tensor([1e-3, 1.0, 30.0, 0.0, 200.0]).repeat(140)[None, None, :700, None]
     store = Store([700, 5], d=128, fmt=fmt, group=group, values=lambda v: v * gain)  # pylint: disable=cell-var-from-loop
-    for q_scale, scale in ((1.5, None), (3e-3, 10.0), (900.0, 2e-4), (0.0, 1.0)):
+    for q_scale, scale in ((1.5, None), (3e-3, 10.0), (900.0, 2e-4), (0.0, 1.0), (1.5, -0.1), (1.5, 0.0)):
       _check_attend(store, q_heads=4, t=2, q_scale=q_scale, scale=scale)
     alike = Store([300], d=128, fmt=fmt, group=group, values=lambda v: v * 3e-6)
     _check_attend(alike, q_heads=4)
@@ -260,6 +260,24 @@ def _attend_again(store, q_heads, t, window):
   g = torch.Generator().manual_seed(5)
   q = (torch.randn(len(store.lengths_list), t, q_heads, store.d, generator=g) * 1.5).to(torch.bfloat16).transpose(1, 2)
   return kv_cache.attend(store.cache, q.to(DEV), store.table, store.lengths, logits_scale=store.d ** -0.5, local_window_size=window)
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("d,d_v", [(64, 64), (96, 96), (128, 128), (192, 128), (160, 160), (256, 256)])
+def test_row_tiles_and_page_tables_of_every_kind(fmt, group, d, d_v):
+  """Up to 32 rows a tile, more in several; short tables (an item is one CTA's), long ones, and very long ones (wide heads then
+  take 16 rows a tile)."""
+  for page, lengths in ((16, [300, 40]), (256, [3000, 0, 17])):
+    try:
+      store = Store(lengths, d=d, d_v=d_v, fmt=fmt, group=group, page=page)
+    except ValueError:
+      assert group in (64, 128)
+      return
+    for q_heads, t in ((2, 3), (4, 6), (6, 7), (8, 8), (4, 19)):
+      _check_attend(store, q_heads=q_heads, t=t)
+    wide = torch.full((len(lengths), (1 << 18) // page), -1, dtype=torch.int32, device=DEV)
+    wide[:, :store.table.shape[1]] = store.table
+    _check_attend(store, q_heads=20, t=2, table=wide)
 
 
 def test_lengths_beyond_the_page_table_and_below_zero():

@@ -1053,6 +1053,14 @@ constexpr int resident() {
   return kSms * Shape::kResident;
 }
 
+// Tokens of a sequence that the page table and the window let queries see.
+static int64_t reach_of(const SplashCacheAttendArgs& a) {
+  const int64_t reach = (int64_t)a.n_table * a.cache.page_size;
+  return a.window >= 0 && reach > a.window + a.q.size[2] ? a.window + a.q.size[2] : reach;
+}
+
+constexpr int64_t kWideTokens = 1 << 18;
+
 // Calls fn with the shape that a call takes.
 template <typename Fn>
 static int with_shape(const SplashCacheAttendArgs& a, Fn&& fn) {
@@ -1061,11 +1069,15 @@ static int with_shape(const SplashCacheAttendArgs& a, Fn&& fn) {
   const int64_t rows = a.q.size[2] * (a.q.size[1] / c.kv_heads);
   auto pick = [&](auto format, auto k, auto v, auto group) {
     constexpr int kF = decltype(format)::value, kK = decltype(k)::value, kV = decltype(v)::value, kG = decltype(group)::value;
-    // Rows go in as few tiles as can be: the codes are read and unpacked again for each.
-    constexpr int kMost = kV <= 128 ? 4 : 1;
-    const int64_t tiles = (rows + 8 * kMost - 1) / (8 * kMost), blocks = (rows + 8 * tiles - 1) / (8 * tiles);
-    if constexpr (kMost > 1) {
-      if (blocks == 2) return fn(AttendShape<kF, kK, kV, kG, 2>{});
+    // Rows go in as few tiles as can be: the codes are read and unpacked again for each.  Sums of 16 rows of over 128 channels
+    // leave an SM 8 warps instead of 12, though, and pay in large calls only (us, one tile of 16 rows against two of 8, head
+    // dim 256: 32 x 8000 .. 30000 tokens, 2 kv heads 122 : 139; 16 x 2000 .. 8000, 4 kv heads 55.1 : 55.4; 12 x 0 .. 10000, 1 kv
+    // head 23.2 : 20.8): from kWideTokens tokens times kv heads that the page tables have room for.
+    constexpr int kMost = kV <= 128 ? 4 : 2;
+    const int64_t most = kV <= 128 || a.q.size[0] * reach_of(a) * c.kv_heads >= kWideTokens ? kMost : 1;
+    const int64_t tiles = (rows + 8 * most - 1) / (8 * most), blocks = (rows + 8 * tiles - 1) / (8 * tiles);
+    if (blocks == 2) return fn(AttendShape<kF, kK, kV, kG, 2>{});
+    if constexpr (kMost > 2) {
       if (blocks == 3) return fn(AttendShape<kF, kK, kV, kG, 3>{});
       if (blocks == 4) return fn(AttendShape<kF, kK, kV, kG, 4>{});
     }
@@ -1114,11 +1126,9 @@ static int check_attend(const SplashCacheAttendArgs& a) {
 // Whether every item is given to one CTA: one launch, no sums in the workspace.
 template <typename Shape>
 static bool is_whole(const SplashCacheAttendArgs& a) {
-  int64_t reach = (int64_t)a.n_table * a.cache.page_size;
-  if (a.window >= 0 && reach > a.window + a.q.size[2]) reach = a.window + a.q.size[2];
   const int64_t tiles = (a.q.size[2] * (a.q.size[1] / a.cache.kv_heads) + Shape::kRows - 1) / Shape::kRows;
   const int64_t items = a.q.size[0] * a.cache.kv_heads * tiles;
-  return reach <= (items < kWholeItems ? kWholeTokens : 2 * kWholeTokens) && items <= INT32_MAX;
+  return reach_of(a) <= (items < kWholeItems ? kWholeTokens : 2 * kWholeTokens) && items <= INT32_MAX;
 }
 
 template <typename Shape>
