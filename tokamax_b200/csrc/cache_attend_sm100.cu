@@ -1069,19 +1069,18 @@ static int with_shape(const SplashCacheAttendArgs& a, Fn&& fn) {
   const int64_t rows = a.q.size[2] * (a.q.size[1] / c.kv_heads);
   auto pick = [&](auto format, auto k, auto v, auto group) {
     constexpr int kF = decltype(format)::value, kK = decltype(k)::value, kV = decltype(v)::value, kG = decltype(group)::value;
-    // Rows go in as few tiles as can be: the codes are read and unpacked again for each.  Sums of 16 rows of over 128 channels
-    // leave an SM 8 warps instead of 12, though, and pay in large calls only (us, one tile of 16 rows against two of 8, head
-    // dim 256: 32 x 8000 .. 30000 tokens, 2 kv heads 122 : 139; 16 x 2000 .. 8000, 4 kv heads 55.1 : 55.4; 12 x 0 .. 10000, 1 kv
-    // head 23.2 : 20.8): from kWideTokens tokens times kv heads that the page tables have room for.
-    constexpr int kMost = kV <= 128 ? 4 : 2;
-    const int64_t most = kV <= 128 || a.q.size[0] * reach_of(a) * c.kv_heads >= kWideTokens ? kMost : 1;
-    const int64_t tiles = (rows + 8 * most - 1) / (8 * most), blocks = (rows + 8 * tiles - 1) / (8 * tiles);
-    if (blocks == 2) return fn(AttendShape<kF, kK, kV, kG, 2>{});
-    if constexpr (kMost > 2) {
-      if (blocks == 3) return fn(AttendShape<kF, kK, kV, kG, 3>{});
-      if (blocks == 4) return fn(AttendShape<kF, kK, kV, kG, 4>{});
+    // Rows go in tiles of up to 16: the codes are read and unpacked again for each tile, but sums of more rows leave an SM
+    // fewer warps.  Two exceptions, us measured:
+    //   17 .. 24 rows of up to 128 channels are one tile (16 sequences of 2048 .. 4096 tokens, 32 / 8 heads of 128, 20 rows,
+    //   int4 48.7 : 52.7, e4m3 44.6 : 49.1 in two tiles of 16; 32 rows in one tile 62.7, in two 55.0);
+    //   rows of over 128 channels go by eight in small calls (one tile of 16 rows against two of 8, head dim 256: 32 x 8000 ..
+    //   30000 tokens, 2 kv heads 122 : 139; 16 x 2000 .. 8000, 4 kv heads 55.1 : 55.4; 12 x 0 .. 10000, 1 kv head 23.2 : 20.8),
+    //   below kWideTokens tokens times kv heads that the page tables have room for.
+    if constexpr (kV <= 128) {
+      if (rows > 16 && rows <= 24) return fn(AttendShape<kF, kK, kV, kG, 3>{});
     }
-    return fn(AttendShape<kF, kK, kV, kG, 1>{});
+    const bool by_eight = rows <= 8 || (kV > 128 && a.q.size[0] * reach_of(a) * c.kv_heads < kWideTokens);
+    return by_eight ? fn(AttendShape<kF, kK, kV, kG, 1>{}) : fn(AttendShape<kF, kK, kV, kG, 2>{});
   };
   auto wide = [&](auto k, auto v) {
     constexpr int kK = decltype(k)::value, kV = decltype(v)::value;
