@@ -130,12 +130,11 @@ struct AttendShape {
   static constexpr int kFragBytes = kK / 16 * kN * 256;            // q as fragments
   static constexpr int kQSums = kFragBytes;                        // [kGroupsK][kRows] sums of q over a group
   static constexpr int kFactors = kQSums + kGroupsK * kRows * 4;   // [kRows] what S is multiplied by
-  static constexpr int kStats = kFactors + kRows * 4;              // [2][kMostWarps][kRows] maxima and sums of the warps
-  static constexpr int kZeros = kStats + 2 * kMostWarps * kRows * 4;  // [kMostWarps][kGroupsV][kRows]
-  static constexpr int kRing = (kZeros + kMostWarps * kGroupsV * kRows * 4 + 127) / 128 * 128;
-  static constexpr int kRingBytes = kStages * kStageBytes;  // of a warp
-  static constexpr int kJoinBytes = kRows * kV * 4;         // the same, in the ring's place once it has run dry
-  static constexpr int smem(int warps) { return kRing + warps * (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes); }
+  static constexpr int kStats = kFactors + kRows * 4;              // [3][kMostWarps][kRows] of the warps, see there
+  static constexpr int kRing = (kStats + 3 * kMostWarps * kRows * 4 + 127) / 128 * 128;
+  // of a warp: its stages, and in their place its sums [kRows][kV] once they have run dry
+  static constexpr int kWarpBytes = kStages * kStageBytes > kRows * kV * 4 ? kStages * kStageBytes : kRows * kV * 4;
+  static constexpr int smem(int warps) { return kRing + warps * kWarpBytes; }
 };
 
 // Where in a stage 16-byte piece c of row r lies: so that eight consecutive rows' piece c are in eight different bank groups.
@@ -326,9 +325,10 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   extern __shared__ __align__(128) uint8_t smem[];
   float* const q_sums = reinterpret_cast<float*>(smem + Shape::kQSums);
   float* const factors = reinterpret_cast<float*>(smem + Shape::kFactors);
-  float* const warp_max = reinterpret_cast<float*>(smem + Shape::kStats);
-  float* const warp_sum = warp_max + kMostWarps * kRows;
-  float* const warp_zeros = reinterpret_cast<float*>(smem + Shape::kZeros);
+  // of each warp and row: the highest logit, what P was taken against, the sum of P (all as that leaves it)
+  float* const warp_high = reinterpret_cast<float*>(smem + Shape::kStats);
+  float* const warp_base = warp_high + kMostWarps * kRows;
+  float* const warp_sum = warp_base + kMostWarps * kRows;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   grid_dependents_launch();  // the joining kernel may come up beside this one; it waits for its end
@@ -348,10 +348,9 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     b = start.b;
     before = start.before * per_sequence;
   }
-  uint8_t* const ring = smem + Shape::kRing + warp * Shape::kRingBytes;
+  uint8_t* const ring = smem + Shape::kRing + warp * Shape::kWarpBytes;
   const uint32_t ring_at = smem_u32(ring);
   constexpr int stage_step = Shape::kStageBytes;
-  float* const join = reinterpret_cast<float*>(smem + Shape::kRing);  // the warps' sums
   const int heads = p.heads_per_kv;
 
   // The item that is worked on (or whose keys are on their way): b, item = head * row_tiles + row tile, units u0 .. u1 - 1.
@@ -820,64 +819,50 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       __syncwarp();
     }
     cp_async_wait<0>();  // (nothing is in flight that anyone waits for; the place of the stages is about to be written)
+    __syncwarp();
 
-
-    // ---- the warps' sums together ----
-#pragma unroll
-    for (int nb = 0; nb < kN; ++nb)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float sum = l[nb][j];
-        sum += __shfl_xor_sync(~0u, sum, 4);
-        sum += __shfl_xor_sync(~0u, sum, 8);
-        sum += __shfl_xor_sync(~0u, sum, 16);
-        float high = highest[nb][j];
-        high = fmaxf(high, __shfl_xor_sync(~0u, high, 4));
-        high = fmaxf(high, __shfl_xor_sync(~0u, high, 8));
-        high = fmaxf(high, __shfl_xor_sync(~0u, high, 16));
-        if (kInt4) {
-#pragma unroll
-          for (int c = 0; c < kGroupsV; ++c) {
-            float z = zeros[c][nb][j];
-            z += __shfl_xor_sync(~0u, z, 4);
-            z += __shfl_xor_sync(~0u, z, 8);
-            z += __shfl_xor_sync(~0u, z, 16);
-            if (lane < 4) warp_zeros[(warp * kGroupsV + c) * kRows + nb * 8 + t4 * 2 + j] = z;
-          }
-        }
-        if (lane < 4) {
-          warp_max[warp * kRows + nb * 8 + t4 * 2 + j] = high;
-          warp_sum[warp * kRows + nb * 8 + t4 * 2 + j] = sum * ex2(base[nb][j] - high);
-        }
-      }
-    __syncthreads();
-    {
-      float* const own = join + warp * (kRows * Shape::kV);
-      constexpr float kBack = kInt4 ? 0x1p24f : 1.f;  // of products of codes
+    // ---- the sums of the warps that had units, each in its own place ----
+    const int active = min(warps, u1 - u0);
+    if (warp < active) {
+      float* const own = reinterpret_cast<float*>(ring);
 #pragma unroll
       for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int r = nb * 8 + t4 * 2 + j;
-          float most = kNoMaximum;
-          for (int w = 0; w < warps; ++w) most = fmaxf(most, warp_max[w * kRows + r]);
-          const float weight = ex2(base[nb][j] - most);
+          float sum = l[nb][j], high = highest[nb][j], z[kGroupsV];
+#pragma unroll
+          for (int c = 0; c < kGroupsV; ++c) z[c] = zeros[c][nb][j];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            sum += __shfl_xor_sync(~0u, sum, d);
+            high = fmaxf(high, __shfl_xor_sync(~0u, high, d));
+            if (kInt4) {
+#pragma unroll
+              for (int c = 0; c < kGroupsV; ++c) z[c] += __shfl_xor_sync(~0u, z[c], d);
+            }
+          }
+          if (g == 0) {
+            warp_high[warp * kRows + r] = high;
+            warp_base[warp * kRows + r] = base[nb][j];
+            warp_sum[warp * kRows + r] = sum;
+          }
 #pragma unroll
           for (int c = 0; c < Shape::kChunksV; ++c) {
             if constexpr (kInt4) {
-              const float4 x = make_float4(o[c][0][nb][j] * kBack, o[c][0][nb][2 + j] * (kBack * 0.0625f),
-                                           o[c][1][nb][j] * kBack, o[c][1][nb][2 + j] * (kBack * 0.0625f));
-              const float z = warp_zeros[(warp * kGroupsV + c / Shape::kPerGroupV) * kRows + r];
+              constexpr float kBack = 0x1p24f;  // of products of codes
+              const float zero = z[c / Shape::kPerGroupV];
               *reinterpret_cast<float4*>(own + r * Shape::kV + c * 32 + g * 4) =
-                  make_float4((x.x + z) * weight, (x.y + z) * weight, (x.z + z) * weight, (x.w + z) * weight);
+                  make_float4(fmaf(o[c][0][nb][j], kBack, zero), fmaf(o[c][0][nb][2 + j], kBack * 0.0625f, zero),
+                              fmaf(o[c][1][nb][j], kBack, zero), fmaf(o[c][1][nb][2 + j], kBack * 0.0625f, zero));
             } else {
-              *reinterpret_cast<float2*>(own + r * Shape::kV + c * 16 + g * 2) =
-                  make_float2(o[c][0][nb][j] * weight, o[c][0][nb][2 + j] * weight);
+              *reinterpret_cast<float2*>(own + r * Shape::kV + c * 16 + g * 2) = make_float2(o[c][0][nb][j], o[c][0][nb][2 + j]);
             }
           }
         }
     }
     __syncthreads();
+    // ---- and together ----
     const bool alone = u0 == 0 && u1 == keys.units;
     // sums of this CTA: an item that began before its share in place 0, one that goes on behind it in place 1 (both: 0)
     float* const part = p.parts + ((int64_t)blockIdx.x * 2 + (is_last ? 1 : 0)) * (kRows * (Shape::kV + 2));
@@ -885,14 +870,16 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       const int r = id / (Shape::kV / 8), d = id % (Shape::kV / 8) * 8;
       float x[8] = {};
       float most = kNoMaximum, sum = 0.f;
+      for (int w = 0; w < active; ++w) most = fmaxf(most, warp_high[w * kRows + r]);
 #pragma unroll 4
-      for (int w = 0; w < warps; ++w) most = fmaxf(most, warp_max[w * kRows + r]);
-#pragma unroll 4
-      for (int w = 0; w < warps; ++w) {
-        sum += warp_sum[w * kRows + r] * ex2(warp_max[w * kRows + r] - most);
-        const float4* const from = reinterpret_cast<const float4*>(join + (w * kRows + r) * Shape::kV + d);
+      for (int w = 0; w < active; ++w) {
+        const float weight = ex2(warp_base[w * kRows + r] - most);
+        const float4* const from = reinterpret_cast<const float4*>(smem + Shape::kRing + w * Shape::kWarpBytes + (r * Shape::kV + d) * 4);
         const float4 lo = from[0], hi = from[1];
-        x[0] += lo.x, x[1] += lo.y, x[2] += lo.z, x[3] += lo.w, x[4] += hi.x, x[5] += hi.y, x[6] += hi.z, x[7] += hi.w;
+        const float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = fmaf(y[k], weight, x[k]);
+        sum = fmaf(warp_sum[w * kRows + r], weight, sum);
       }
       if (!alone) {
         float4* const to = reinterpret_cast<float4*>(part + r * Shape::kV + d);
