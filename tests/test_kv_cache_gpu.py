@@ -209,6 +209,14 @@ def test_rows_shared_by_many_ctas_and_ctas_with_many_rows(page, fmt, lengths):
 
 
 @pytest.mark.parametrize("fmt", ["int4", "e4m3"])
+@pytest.mark.parametrize("most", [90, 2500])  # every item one CTA's, or shares of them all
+def test_more_sequences_than_a_cta_has_threads(fmt, most):
+  lengths = [i * 37 % 90 for i in range(150)] + [most] + [i * 53 % 91 for i in range(149)] + [0, 0]
+  store = Store(lengths, heads=1, d=64, fmt=fmt, group=32 if fmt == "int4" else None, page=16)
+  _check_attend(store, q_heads=2)
+
+
+@pytest.mark.parametrize("fmt", ["int4", "e4m3"])
 @pytest.mark.parametrize("window", [0, 1, 15, 100, 5000])
 @pytest.mark.parametrize("t", [1, 9])
 def test_window(fmt, window, t):

@@ -46,7 +46,7 @@ struct AttendParams {
   const float* sinks;
   // workspace: for each CTA two items it may share with others, sums [rows][row_v], then max and sum [2][rows]
   float* parts;
-  int64_t* starts;  // [batch + 1] where each sequence begins, in the measure of shares
+  int64_t* starts;  // [batch + 1] where each sequence's items begin, in the measure of shares
   int64_t q_stride_b, q_stride_h, q_stride_s, o_stride_b, o_stride_h, o_stride_s, table_stride, n_pages;
   float scale, soft_cap, mask_value;
   int32_t batch, q_heads, kv_heads, heads_per_kv, q_len, row_tiles, n_table, page_size, page_shift, dtype;
@@ -223,68 +223,78 @@ __device__ __forceinline__ Keys keys_of(const AttendParams& p, int length) {
   return k;
 }
 
-__host__ __device__ inline int64_t share_of(int64_t total, int ctas, int min_share) {
-  const int64_t share = (total + ctas - 1) / ctas;
+// a / b for a >= 0, b > 0; 32 bits wide where that is enough (a division of 64 bits takes some hundred cycles).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return (a | b) >> 32 == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+__device__ __forceinline__ int64_t share_of(int64_t total, int ctas, int min_share) {
+  const int64_t share = quotient(total + ctas - 1, ctas);
   return share > min_share ? share : min_share;
 }
 
 struct Start {  // where a CTA's share begins
-  int64_t total, before;  // cost of all sequences (for one head and row tile), and before sequence b
+  int64_t total, before;  // cost of all items, and of those of the sequences before b
+  int64_t share;
   int b;
 };
 
-// All threads of a CTA of kWarps; `scratch`: 2 * kWarps + 2 words of shared memory of 8 bytes.
+// All threads of a CTA of kWarps; `scratch`: kWarps + 2 words of shared memory of 8 bytes.  Sequences go by the threads of a
+// CTA at a time; a second look is taken only where there are more of them than that.
 template <int kUnit>
 __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
-  const int per_sequence = p.kv_heads * p.row_tiles;
+  constexpr int kThreads = kWarps * 32;
+  const int64_t per_sequence = p.kv_heads * p.row_tiles;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t total = 0, mine = 0;  // mine: of the sequences that this thread counts when there is one round of them
-  for (int b = tid; b < p.batch; b += (kWarps * 32)) total += (mine = keys_of<kUnit>(p, __ldg(p.lengths + b)).cost(p));
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
-  if (lane == 0) scratch[warp] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += scratch[w];
-  const int64_t share = share_of(total * per_sequence, gridDim.x, p.min_share);
-  const int64_t at = (int64_t)blockIdx.x * share;
+  int64_t* const found = scratch + kWarps;
   const bool keep = blockIdx.x == 0;  // this CTA writes down where the sequences start
-  int64_t* found = scratch + 2 * kWarps;
-  int64_t carry = 0;
-  for (int base = 0; base < p.batch; base += (kWarps * 32)) {
-    const int b = base + tid;
-    if (base > 0 || p.batch > (kWarps * 32)) mine = b < p.batch ? keys_of<kUnit>(p, __ldg(p.lengths + b)).cost(p) : 0;
-    if (b >= p.batch) mine = 0;
-    int64_t sum = mine;
+  const bool once = p.batch <= kThreads;
+  int64_t total = 0, share = 0, at = 0;
+  for (int look = once ? 1 : 0; look < 2; ++look) {
+    int64_t carry = 0;
+    for (int base = 0; base < p.batch; base += kThreads) {
+      const int b = base + tid;
+      const int64_t mine = b < p.batch ? keys_of<kUnit>(p, __ldg(p.lengths + b)).cost(p) * per_sequence : 0;
+      int64_t sum = mine;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t other = __shfl_up_sync(~0u, sum, d);
-      if (lane >= d) sum += other;
-    }
-    __syncthreads();
-    if (lane == 31) scratch[kWarps + warp] = sum;
-    __syncthreads();
-    int64_t before = carry, round = 0;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t other = __shfl_up_sync(~0u, sum, d);
+        if (lane >= d) sum += other;
+      }
+      if (base > 0 || look > 0) __syncthreads();  // (before what the last round left is written over)
+      if (lane == 31) scratch[warp] = sum;
+      __syncthreads();
+      int64_t before = carry + sum - mine;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const int64_t s = scratch[kWarps + w];
-      before += w < warp ? s : 0;
-      round += s;
-    }
-    before += sum - mine;
-    if (b < p.batch) {
-      if (keep) p.starts[b] = before;
-      if (mine > 0 && at >= before * per_sequence && at < (before + mine) * per_sequence) {
-        found[0] = b;
-        found[1] = before;
+      for (int w = 0; w < kWarps; ++w) {
+        const int64_t s = scratch[w];
+        before += w < warp ? s : 0;
+        carry += s;
+      }
+      if (look == 1) {
+        if (once) {
+          total = carry;
+          share = share_of(total, gridDim.x, p.min_share);
+          at = blockIdx.x * share;
+        }
+        if (b < p.batch) {
+          if (keep) p.starts[b] = before;
+          if (at >= before && at < before + mine) {
+            found[0] = b;
+            found[1] = before;
+          }
+        }
       }
     }
-    carry += round;
+    if (look == 0) {
+      total = carry;
+      share = share_of(total, gridDim.x, p.min_share);
+      at = blockIdx.x * share;
+    }
   }
   if (keep && tid == 0) p.starts[p.batch] = total;
   __syncthreads();
-  return {total, found[1], (int)found[0]};
+  return {total, found[1], share, (int)found[0]};
 }
 
 // ------------------------------------------------------------------------------------------
@@ -342,11 +352,10 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   } else {
     const Start start = find_start<kUnit>(p, reinterpret_cast<int64_t*>(smem));
     __syncthreads();  // (its scratch is about to be q's place)
-    const int64_t all = start.total * per_sequence, share = share_of(all, gridDim.x, p.min_share);
-    at = share_begin = (int64_t)blockIdx.x * share;
-    end = min(at + share, all);
+    at = share_begin = (int64_t)blockIdx.x * start.share;
+    end = min(at + start.share, start.total);
     b = start.b;
-    before = start.before * per_sequence;
+    before = start.before;
   }
   uint8_t* const ring = smem + Shape::kRing + warp * Shape::kWarpBytes;
   const uint32_t ring_at = smem_u32(ring);
@@ -375,7 +384,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         length = __ldg(p.lengths + ++b);
         keys = keys_of<kUnit>(p, length);
       }
-      item = (int)((at - before) / keys.cost(p));
+      item = (int)quotient(at - before, keys.cost(p));
       const int64_t first = before + (int64_t)item * keys.cost(p) + p.item_cost;  // of its units
       u0 = (int)max(at - first, (int64_t)0);
       u1 = (int)min((int64_t)keys.units, end - first);
@@ -448,11 +457,10 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   };
 
   while (next_item()) {
-    start_item();
     const int head = item / p.row_tiles, row0 = item % p.row_tiles * kRows;
     const int n_rows = min(kRows, p.q_len * heads - row0);
 
-    // ---- q as fragments: kLanes lanes (a power of two that holds the row's width / 8) a row ----
+    // ---- q's rows on their way: kLanes lanes (a power of two that holds the row's width / 8) a row ----
     // Row r of the tile is query (first_row + r) / heads behind first_query (r and heads are small: the quotient by a product
     // is exact), q head (first_row + r) % heads of the kv head.
     const int first_query = row0 / heads, first_row = row0 - first_query * heads;
@@ -460,12 +468,30 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     auto query_of = [&](int r) { return (int)(((float)(first_row + r) + 0.5f) * per_head); };
     constexpr int kLanes = Shape::kK <= 64 ? 8 : Shape::kK <= 128 ? 16 : 32, kAtOnce = 32 / kLanes;
     const int piece = lane % kLanes;
-    for (int r = warp * kAtOnce + lane / kLanes; r < kRows; r += warps * kAtOnce) {
-      float x[8] = {};
+    constexpr int kPasses = (kRows + kWarps * kAtOnce - 1) / (kWarps * kAtOnce);  // (at most)
+    uint4 raw[kPasses];
+#pragma unroll
+    for (int pass = 0; pass < kPasses; ++pass) {
+      const int r = (pass * warps + warp) * kAtOnce + lane / kLanes;
+      raw[pass] = make_uint4(0, 0, 0, 0);
       if (r < n_rows && piece * 8 < p.head_dim) {
         const int i = query_of(r), h = head * heads + first_row + r - i * heads;
-        load8(p.q, p.dtype, b * p.q_stride_b + h * p.q_stride_h + (first_query + i) * p.q_stride_s + piece * 8, x);
+        raw[pass] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.q_stride_b + h * p.q_stride_h +
+                                                         (first_query + i) * p.q_stride_s + piece * 8));
       }
+    }
+    start_item();
+
+    // ---- and as fragments ----
+#pragma unroll
+    for (int pass = 0; pass < kPasses; ++pass) {
+      const int r = (pass * warps + warp) * kAtOnce + lane / kLanes;
+      if (pass * warps * kAtOnce >= kRows) break;  // (all warps alike)
+      float x[8];
+      unpack16(p.dtype, raw[pass].x, x[0], x[1]);
+      unpack16(p.dtype, raw[pass].y, x[2], x[3]);
+      unpack16(p.dtype, raw[pass].z, x[4], x[5]);
+      unpack16(p.dtype, raw[pass].w, x[6], x[7]);
       float top = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
@@ -486,7 +512,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&pair), __float2half2_rn(0.0625f));
         return *reinterpret_cast<const uint32_t*>(&y);
       };
-      if (piece * 8 < Shape::kK) {
+      if (r < kRows && piece * 8 < Shape::kK) {
         // For each 32 channels, block of rows and lane of the MMA: its part of both steps.
         uint4* const frag = reinterpret_cast<uint4*>(smem) + ((piece >> 2) * kN + (r >> 3)) * 32 + (r & 7) * 4;
         if (kInt4) {  // a lane's eight channels are one word of codes, column piece % 4
@@ -502,10 +528,10 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         constexpr int kGroupLanes = Shape::kPerGroupK * 4;
 #pragma unroll
         for (int d = 1; d < kGroupLanes; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        if (piece % kGroupLanes == 0 && piece * 8 < Shape::kK)
+        if (r < kRows && piece % kGroupLanes == 0 && piece * 8 < Shape::kK)
           q_sums[piece / kGroupLanes * kRows + r] = sum * 0x1p-24f;  // in the units of the products of codes
       }
-      if (piece == 0) factors[r] = fmaxf(fabsf(p.scale) * down * (kInt4 ? 0x1p24f : 1.f) * (p.soft_cap > 0.f ? 1.f : kLog2e), 1e-37f);
+      if (r < kRows && piece == 0) factors[r] = fmaxf(fabsf(p.scale) * down * (kInt4 ? 0x1p24f : 1.f) * (p.soft_cap > 0.f ? 1.f : kLog2e), 1e-37f);
     }
     __syncthreads();
 
@@ -914,13 +940,12 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const _
   __shared__ float sums[kMostSlices][kV];
   __shared__ float stats[2][kMostSlices];
   grid_dependency_wait();
-  const int per_sequence = p.kv_heads * p.row_tiles;
   const int lot = threadIdx.x / kEach, d = threadIdx.x % kEach * 8;
-  const int64_t share = share_of(p.starts[p.batch] * per_sequence, ctas, p.min_share);
+  const int64_t share = share_of(p.starts[p.batch], ctas, p.min_share);
   for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
-    const int64_t before = p.starts[b], cost = p.starts[b + 1] - before;
-    const int64_t first = before * per_sequence + blockIdx.x * cost + p.item_cost;  // unit of this item
-    const int64_t c0 = first / share, c1 = cost > 0 ? (first + cost - p.item_cost - 1) / share : c0 - 1;
+    const int64_t before = p.starts[b], cost = quotient(p.starts[b + 1] - before, p.kv_heads * p.row_tiles);
+    const int64_t first = before + blockIdx.x * cost + p.item_cost;  // unit of this item
+    const int64_t c0 = quotient(first, share), c1 = cost > 0 ? quotient(first + cost - p.item_cost - 1, share) : c0 - 1;
     if (c0 == c1) continue;  // written already
     const int head = blockIdx.x / p.row_tiles, row0 = blockIdx.x % p.row_tiles * kRows;
     const int n_rows = min(kRows, p.q_len * p.heads_per_kv - row0);
