@@ -169,13 +169,14 @@ def _check_attend(store, *, q_heads, t=1, window=None, soft_cap=None, sinks=None
     moved = kv_cache_ref.products(store.v[b, :, :n], store.fmt, store.group)
     ref, lse, top, size, moved = kv_cache_ref.attend(q[b].double(), k, v, scale=scale, window=window, soft_cap=soft_cap, sinks=sinks,
                                                      seen=None if seen is None else seen[b, :n], weights=moved)
-    # Rounding: of P * scale to f16, 2^-11 of each term (plus a little for sums in 32 bits: 2^-18); of logits, 2^-24 of each
+    # Rounding: of P * scale to f16, 2^-11 of each term, or to two of them for f16 outputs, 2^-22 (plus a little for sums in 32
+    # bits: 2^-18); of logits, 2^-24 of each
     # of some hundred partial sums of size |q| |k| scale, which moves each p, and with it o, by up to twice that in all; of
     # o to its type.
     logits = (q[b].double().norm(dim=-1).max() * (k.norm(dim=-1).max() if n else 0.0) * abs(scale)).clamp_min(1.0)
     slack = 2.0 ** -18 * logits
     err = (o[b].cpu().double() - ref).abs()
-    before = (ROUNDOFF[torch.float16] + 2.0 ** -18) * moved + 2 * slack * size + 1e-9
+    before = ((ROUNDOFF[torch.float16] if dtype == torch.bfloat16 else 2.0 ** -22) + 2.0 ** -18) * moved + 2 * slack * size + 1e-9
     least = 2.0 ** -25 if dtype == torch.float16 else 0.0  # half a step of f16's subnormals
     bound = before + ROUNDOFF[dtype] * (ref.abs() + before) + least
     assert (err <= bound).all(), (b, n, float(err.max()), float((err / bound).max()))
@@ -206,6 +207,18 @@ def test_rows_shared_by_many_ctas_and_ctas_with_many_rows(page, fmt, lengths):
   first = _check_attend(store, q_heads=4)
   again = _check_attend(store, q_heads=4)
   assert torch.equal(first, again)
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("d,d_v", [(64, 64), (96, 96), (192, 128), (256, 256)])
+@pytest.mark.parametrize("q_heads,t", [(2, 1), (16, 1), (10, 4)])
+def test_f16_outputs(fmt, group, d, d_v, q_heads, t):
+  try:
+    store = Store([33, 700], d=d, d_v=d_v, fmt=fmt, group=group, dtype=torch.float16)
+  except ValueError:
+    assert group in (64, 128)
+    return
+  _check_attend(store, q_heads=q_heads, t=t, dtype=torch.float16)
 
 
 @pytest.mark.parametrize("fmt", ["int4", "e4m3"])

@@ -13,24 +13,38 @@
 //   * q is scaled by a power of two for each row so that its largest entry is near 2^14: bf16 and f16 values lose at most
 //     bits that are 2^-24 of that entry.
 //   * P * scale is scaled by a power of two that follows the largest scale seen (`top`), below 2^14: 11 bits of it are kept.
+//     That is enough for outputs of bf16 (1.73e-3 of the norm from 64 bits where rounding the output alone costs 1.64e-3).  For
+//     f16 what is left of it goes through a second product: 6.0e-4 without (int4, 5111 keys; its codes are all positive, so that
+//     more is lost than of e4m3, 2.8e-4), 2.4e-4 with it (2.1e-4), where rounding the output costs 2.0e-4, for 148 -> 164 us
+//     (32 sequences of 8192 .. 32768, 32 / 8 heads of 128).
 // Softmax statistics are of one pass over the keys, with a running maximum and sum for each row.
-//
-// Bound by: HBM, 64 + 8 bytes a token and head and side (int4, head dim 128, groups of 64); at 6.5 TB/s an SM gets 46 codes
-// a cycle, so what counts beside the bytes in flight is the number of instructions for a code.
 //
 // Split: the keys of all (sequence, kv head, row tile) items, one after the other in units of kUnit tokens, are cut into
 // equal shares for the CTAs, wherever that falls in a sequence.  A share is found on the device from the lengths: the host
 // never needs them, and the launch can be captured in a graph.  The warps of a CTA take the units of its share of an
 // item in turn, each with a ring of its own in shared memory (cp.async; no barrier between warps while keys stream), and
-// join their sums at the end of the item.  An item that more than one CTA has worked on is joined by a second kernel, from
-// sums in the workspace, in the order of the CTAs: results do not depend on who comes first.
+// put their sums together at the end of the item.  An item that more than one CTA has worked on is joined by a second kernel,
+// from sums in the workspace, in the order of the CTAs: results do not depend on who comes first.  Where sequences cannot be long
+// every item is one CTA's, and there is one launch.
+//
+// Bound by: HBM asks for 64 + 8 bytes a token, head and side (int4, head dim 128, groups of 64).  At 6.5 TB/s an SM gets 46 codes
+// a cycle, so that a warp may spend 2.8 instructions on 32 of them; the kernel spends 2.1 (535 on a unit of 32 tokens, keys and
+// values, eight rows; 160 of them unpack), and issues 2.3 to 2.5 a cycle of the 4 that an SM could.  Instructions are what bounds
+// it: without the products the copies alone take 121 of 148 us.  Measured, 32 / 8 heads of 128, int4: 32 sequences of 8192 .. 32768
+// 148 us, 5.1 TB/s of the 6.5 that a plain copy reaches; one of 131072 41 us, 64 of 200 .. 4096 51 us, 3.7 and 3.5 TB/s.  About
+// 9 us of each call are the two launches and the chains of loads at their beginnings (lengths, pages, codes; parts).  e4m3 rows are
+// unpacked by conversions and ask for twice the bytes: 48 sequences of 0 .. 13025 115 us, 5.9 TB/s.
+// Rows of more than one block of eight spend 190 instructions more a block on a unit, and leave room for fewer warps.
 #include <atomic>
 
 #include "cache_common.cuh"
 
 namespace sb {
 
-constexpr int kWarps = 4, kMostWarps = 8;  // of a CTA; kMostWarps where there are few items and each is one CTA's
+// Warps of a CTA; kMostWarps where every item is one CTA's and there are fewer than two for an SM (us, 4 : 8 warps, up to 1024
+// tokens, 8 items 12.5 : 10.6, 256 items 14.6 : 14.6, 1024 items 35.6 : 44.3).  Shares: four CTAs of 4 warps on an SM and two of 8
+// are alike where sequences are long, short ones want the smaller CTAs (64 x 200 .. 4096: 53.6 : 56.3).
+constexpr int kWarps = 4, kMostWarps = 8;
 
 struct AttendParams {
   const uint8_t* k_codes;
@@ -72,7 +86,10 @@ __device__ __forceinline__ void ldmatrix_x2(uint32_t addr, uint32_t& a, uint32_t
   asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+               : "r"(addr)
+               : "memory");
 }
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -205,8 +222,12 @@ constexpr uint32_t kLeastTop = 87u << 23;  // 2^-40
 // shares
 // ------------------------------------------------------------------------------------------
 // What a CTA spends on an item beside its units, in tokens: shares are equal in the sum of both.  (Looking up the item, q as
-// fragments, the first keys' latency, the warps' sums together.)
+// fragments, the first keys' latency, the warps' sums together: some thousand cycles.  us with 0, 320, 640 and 960: 64 x 200 ..
+// 4096 tokens 85, 51.8, 52.3, 54.4; 12 x 0 .. 10000, head dim 256, 28.6, 22.5, 24.6, 28.9.)
 constexpr int kItemTokens = 320;
+// Every item is one CTA's where queries see at most kWholeTokens, or twice as many and there are kWholeItems items at least (us,
+// whole : shares and a second launch; 1024 tokens, 8 items 10.6 : 12.1, 256 items 14.6 : 22.0; 2048 tokens, 8 items 14.6 : 12.5,
+// 64 items 14.6 : 15.3, 256 items 23.1 : 27.7, 1024 items 57.8 : 57.3; 4096 tokens, 64 items 22.9 : 17.3).
 constexpr int kWholeTokens = 1024, kWholeItems = 64;
 
 struct Keys {  // of a sequence: tokens [lo, hi) in whole units from lo, which is a multiple of kUnit
@@ -403,8 +424,9 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   auto look_up = [&](int turn) -> uint32_t {
     const int u = u0 + warp + (turn + lane / kTiles) * warps, token = keys.lo + u * kUnit + lane % kTiles * 16;
     const int page = u < u1 && token < keys.hi ? __ldg(p.page_table + b * p.table_stride + (token >> p.page_shift)) : -1;
-    return page >= 0 && page < p.n_pages ? ((uint32_t)(page * p.kv_heads + item / p.row_tiles) << (p.page_shift - 4)) + ((token & (p.page_size - 1)) >> 4)
-                                         : kNowhere;
+    if (page < 0 || page >= p.n_pages) return kNowhere;
+    const uint32_t first = (uint32_t)(page * p.kv_heads + item / p.row_tiles) << (p.page_shift - 4);
+    return first + ((token & (p.page_size - 1)) >> 4);
   };
   uint32_t places, next_places;
   uint32_t absent;  // a bit for each tile of the batch that has no page
@@ -439,7 +461,8 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
           copy_tile(place, to, i);
         } else if (!kInt4) {
           // P is 0 there, but 0 times what lay there before need not be (codes of four bits are numbers always)
-          for (int j = lane; j < Shape::kRowV; j += 32) cp_async16_zeros(to + kUnit * Shape::kRowK + i * 16 * Shape::kRowV + j * 16, p.v_codes);
+          const uint32_t values = to + kUnit * Shape::kRowK + i * 16 * Shape::kRowV;
+          for (int j = lane; j < Shape::kRowV; j += 32) cp_async16_zeros(values + j * 16, p.v_codes);
         }
       }
     }
@@ -531,7 +554,9 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         if (r < kRows && piece % kGroupLanes == 0 && piece * 8 < Shape::kK)
           q_sums[piece / kGroupLanes * kRows + r] = sum * 0x1p-24f;  // in the units of the products of codes
       }
-      if (r < kRows && piece == 0) factors[r] = fmaxf(fabsf(p.scale) * down * (kInt4 ? 0x1p24f : 1.f) * (p.soft_cap > 0.f ? 1.f : kLog2e), 1e-37f);
+      // (not 0, so that logits of -inf keep being that)
+      if (r < kRows && piece == 0)
+        factors[r] = fmaxf(fabsf(p.scale) * down * (kInt4 ? 0x1p24f : 1.f) * (p.soft_cap > 0.f ? 1.f : kLog2e), 1e-37f);
     }
     __syncthreads();
 
@@ -558,8 +583,9 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     const uint4* const frags = reinterpret_cast<const uint4*>(smem) + lane;
     // where a lane's rows of matrices begin: K, the next tile's in the upper half of the warp; V, the next piece's
     const uint32_t lane_k = Pieces<Shape::kRowK>::row_at(kTiles > 1 ? lane : lane & 15);
-    const uint32_t lane_v = kUnit * Shape::kRowK + Pieces<Shape::kRowV>::at(Pieces<Shape::kRowV>::row_at(lane & 15), Pieces<Shape::kRowV>::kTurn > 0 ? lane >> 4 : 0) +
-                            (Pieces<Shape::kRowV>::kTurn > 0 ? 0 : (lane >> 4) * 16);
+    using PiecesV = Pieces<Shape::kRowV>;
+    const uint32_t lane_v = kUnit * Shape::kRowK + (PiecesV::kTurn > 0 ? PiecesV::at(PiecesV::row_at(lane & 15), lane >> 4)
+                                                                       : PiecesV::row_at(lane & 15) + (lane >> 4) * 16);
     int stage = 0, turn = 0;
     for (int u = u0 + warp; u < u1; u += warps, ++turn) {
       cp_async_wait<kAhead - 1>();
@@ -686,7 +712,8 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
               const int token = token0 + i * 16 + (j >> 1) * 8 + g;
-              const bool keep = !(none >> i & 1) && token < keys.hi && token <= position && (p.window < 0 || token >= position - p.window);
+              const bool held = !(none >> i & 1) && token < keys.hi;
+              const bool keep = held && token <= position && (p.window < 0 || token >= position - p.window);
               if (keep)
                 seen |= 1u << ((i * kN + nb) * 4 + j);
               else
@@ -773,7 +800,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
           }
 
       // ---- O ----
-      auto accumulate = [&](auto masked) {
+      auto accumulate = [&](auto masked, auto fine) {
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
           uint32_t pairs[2][kGroupsV], words[4];
@@ -788,6 +815,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
 #pragma unroll
           for (int group = 0; group < kGroupsV; ++group) {
             uint32_t pf[kN][2];  // P * scale as the MMAs' second operand
+            uint32_t rest[kN][2];  // fine: what that leaves of it
             float scale[2], zero[2];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -803,8 +831,15 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
                 x[j] = dead ? 0.f : s[i][nb][j] * scale[j >> 1];  // (whatever lies there, NaN too)
                 if (kInt4 && !dead) zeros[group][nb][j & 1] = fmaf(s[i][nb][j], zero[j >> 1], zeros[group][nb][j & 1]);
               }
-              pf[nb][0] = movmatrix(pack_f16(x[0], x[1]));
-              pf[nb][1] = movmatrix(pack_f16(x[2], x[3]));
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const uint32_t pair = pack_f16(x[half * 2], x[half * 2 + 1]);
+                pf[nb][half] = movmatrix(pair);
+                if (decltype(fine)::value) {
+                  const float2 kept = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+                  rest[nb][half] = movmatrix(pack_f16(x[half * 2] - kept.x, x[half * 2 + 1] - kept.y));
+                }
+              }
             }
 #pragma unroll
             for (int cc = 0; cc < Shape::kPerGroupV; ++cc) {
@@ -827,21 +862,34 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
                 for (int nb = 0; nb < kN; ++nb) {
                   mma_f16(o[c][0][nb], a, pf[nb][0], pf[nb][1]);
                   mma_f16(o[c][1][nb], a2, pf[nb][0], pf[nb][1]);
+                  if (decltype(fine)::value) {
+                    mma_f16(o[c][0][nb], a, rest[nb][0], rest[nb][1]);
+                    mma_f16(o[c][1][nb], a2, rest[nb][0], rest[nb][1]);
+                  }
                 }
               } else {
                 const uint32_t x0 = __byte_perm(w0, 0, 0x3120), x1 = __byte_perm(w1, 0, 0x3120);
                 const uint32_t a[4] = {e4m3x2_to_f16x2(x0), e4m3x2_to_f16x2(x0 >> 16), e4m3x2_to_f16x2(x1), e4m3x2_to_f16x2(x1 >> 16)};
 #pragma unroll
-                for (int nb = 0; nb < kN; ++nb) mma_f16(o[c][0][nb], a, pf[nb][0], pf[nb][1]);
+                for (int nb = 0; nb < kN; ++nb) {
+                  mma_f16(o[c][0][nb], a, pf[nb][0], pf[nb][1]);
+                  if (decltype(fine)::value) mma_f16(o[c][0][nb], a, rest[nb][0], rest[nb][1]);
+                }
               }
             }
           }
         }
       };
-      if (whole)
-        accumulate(std::false_type{});
-      else
-        accumulate(std::true_type{});
+      if (p.dtype == SPLASH_F16) {
+        if (whole)
+          accumulate(std::false_type{}, std::true_type{});
+        else
+          accumulate(std::true_type{}, std::true_type{});
+      } else if (whole) {
+        accumulate(std::false_type{}, std::false_type{});
+      } else {
+        accumulate(std::true_type{}, std::false_type{});
+      }
       __syncwarp();
     }
     cp_async_wait<0>();  // (nothing is in flight that anyone waits for; the place of the stages is about to be written)
@@ -900,7 +948,8 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
 #pragma unroll 4
       for (int w = 0; w < active; ++w) {
         const float weight = ex2(warp_base[w * kRows + r] - most);
-        const float4* const from = reinterpret_cast<const float4*>(smem + Shape::kRing + w * Shape::kWarpBytes + (r * Shape::kV + d) * 4);
+        const uint8_t* const sums = smem + Shape::kRing + w * Shape::kWarpBytes;
+        const float4* const from = reinterpret_cast<const float4*>(sums + (r * Shape::kV + d) * 4);
         const float4 lo = from[0], hi = from[1];
         const float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -1037,7 +1086,8 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   if (cudaGetDevice(&device) != cudaSuccess) return SPLASH_ERR_CUDA;
   const uint64_t bit = 1ull << (device & 63);
   if (device > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem(kMostWarps)) != cudaSuccess) return SPLASH_ERR_CUDA;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem(kMostWarps)) != cudaSuccess)
+      return SPLASH_ERR_CUDA;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const int64_t items = (int64_t)p.kv_heads * p.row_tiles * p.batch;
@@ -1056,7 +1106,8 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   attribute.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, cache_attend_join_kernel<Shape::kRows, Shape::kV>, p, ctas) == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
+  const cudaError_t launched = cudaLaunchKernelEx(&config, cache_attend_join_kernel<Shape::kRows, Shape::kV>, p, ctas);
+  return launched == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
 }
 
 // CTAs that the GPU holds at a time

