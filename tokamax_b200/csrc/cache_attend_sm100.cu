@@ -980,8 +980,11 @@ constexpr int kJoinThreads = 256;
 // blockIdx.x: row tile of an item (fastest) and head; y: sequence.  A thread has eight channels of a row; a row's parts are
 // dealt to as many threads as there are parts for, so that a block takes several rows at a time where they are few.  z: the
 // rows that a block takes are every gridDim.z-th such lot.
-template <int kRows, int kV>
-__global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const __grid_constant__ AttendParams p, int ctas) {
+// kAhead: parts whose loads a thread has in flight together, which registers have to hold: four where there are few items, of
+// many parts each, two and twice the blocks on an SM otherwise (us of a whole call, four : two; 8 items of 74 parts 41.3 : 42.7, 24
+// items of some 25 20.7 : 21.6; 128 items of some 5 37.2 : 34.0, 512 of one or two 50.7 : 48.5).
+template <int kRows, int kV, int kAhead>
+__global__ void __launch_bounds__(kJoinThreads, kAhead > 2 ? 2 : 4) cache_attend_join_kernel(const __grid_constant__ AttendParams p, int ctas) {
   constexpr int kEach = kV / 8, kLanes = kJoinThreads / kEach;  // threads of a row's channels; how many such lots
   constexpr int kMostSlices = kLanes >= 16 ? 16 : 8;
   static_assert(kLanes >= 8);
@@ -1006,7 +1009,6 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const _
       float most = kNoMaximum, sum = 0.f, x[8] = {};
       const bool mine = lot < kMostSlices && r < n_rows;
       if (mine) {
-        constexpr int kAhead = 4;  // parts whose loads are in flight together
         for (int64_t c = c0 + slice; c <= c1; c += slices * kAhead) {
           float m[kAhead], l[kAhead];
           float4 lo[kAhead], hi[kAhead];
@@ -1096,9 +1098,11 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   if (cudaGetLastError() != cudaSuccess) return SPLASH_ERR_CUDA;
   if (p.whole) return SPLASH_OK;
   cudaLaunchConfig_t config{};
-  // (as many blocks of an item as its rows and the GPU have room for: where items are few, each has many parts)
+  // (as many blocks of an item as its rows and the GPU have room for, where items are few)
+  const int rows = p.q_len * p.heads_per_kv < Shape::kRows ? p.q_len * p.heads_per_kv : Shape::kRows;
+  const bool few = items < kSms / 2;
   config.gridDim = dim3((unsigned)(p.kv_heads * p.row_tiles), (unsigned)(p.batch < 65535 ? p.batch : 65535),
-                        (unsigned)(items >= 8 * kSms ? 1 : items * Shape::kRows <= 8 * kSms ? Shape::kRows : 8 * kSms / items));
+                        (unsigned)(items >= 2 * kSms ? 1 : items * rows <= 8 * kSms ? rows : 8 * kSms / items));
   config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
   cudaLaunchAttribute attribute{};
@@ -1106,7 +1110,8 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   attribute.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  const cudaError_t launched = cudaLaunchKernelEx(&config, cache_attend_join_kernel<Shape::kRows, Shape::kV>, p, ctas);
+  const auto join = few ? cache_attend_join_kernel<Shape::kRows, Shape::kV, 4> : cache_attend_join_kernel<Shape::kRows, Shape::kV, 2>;
+  const cudaError_t launched = cudaLaunchKernelEx(&config, join, p, ctas);
   return launched == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
 }
 
