@@ -498,7 +498,8 @@ int splash_cache_append(const SplashCacheAppendArgs* args, void* cuda_stream);
 /* Writes the first lengths[b] tokens of the sequences to k [batch, kv_heads, max_len, head_dim] and v [.., head_dim_v]
  * (one type of bf16, f16, f32; values are rounded to it once); zeros behind them.  page_table [batch, n_table] int32
  * (row stride table_stride): the page of tokens i * page_size ..; tokens on a page outside 0 .. n_pages - 1, and
- * those that the table does not reach, read as zeros.  lengths [batch] int32 on the device. */
+ * those that the table does not reach, read as zeros.  lengths [batch] int32 on the device.  max_len and (for
+ * splash_cache_attend) the tokens that a row of the table has room for: 2^30 at most. */
 typedef struct SplashCacheReadArgs {
   SplashKvCache cache;
   SplashTensor k, v;

@@ -93,6 +93,7 @@ CACHE_FAULTS = [("cache.k_codes", None, -1), ("cache.v_scales", 4104, -1), ("cac
     ("SplashCacheAppendArgs", "k.data", 4100, -1), ("SplashCacheAppendArgs", "slot_stride", -1, -1),
     ("SplashCacheReadArgs", "page_table", None, -1), ("SplashCacheReadArgs", "n_table", 0, -1), ("SplashCacheReadArgs", "k.size.0", 2, -1),
     ("SplashCacheAttendArgs", "q.dtype", 1, -2), ("SplashCacheAttendArgs", "q.size.1", 3, -1), ("SplashCacheAttendArgs", "lengths", None, -1),
+    ("SplashCacheAttendArgs", "n_table", (1 << 26) + 1, -7), ("SplashCacheReadArgs", "k.size.0", 0, -1),
     ("SplashCacheAttendArgs", "soft_cap", -1.0, -1), ("SplashCacheAttendArgs", "soft_cap", float("nan"), -1),
     ("SplashCacheAttendArgs", "o.size.3", 56, -1)])
 def test_c_entry_points_refuse_before_they_touch_the_gpu(kind, path, value, status):

@@ -230,7 +230,7 @@ def test_more_sequences_than_a_cta_has_threads(fmt, most):
 
 
 @pytest.mark.parametrize("fmt", ["int4", "e4m3"])
-@pytest.mark.parametrize("window", [0, 1, 15, 100, 5000])
+@pytest.mark.parametrize("window", [0, 1, 15, 100, 5000, 2 ** 31 - 1])
 @pytest.mark.parametrize("t", [1, 9])
 def test_window(fmt, window, t):
   store = Store([1, 8, 9, 100, 1000, 1300], d=64, fmt=fmt, group=32 if fmt == "int4" else None)

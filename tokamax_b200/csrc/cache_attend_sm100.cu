@@ -139,7 +139,6 @@ struct AttendShape {
   static constexpr int kPerGroupK = kChunksK / kGroupsK, kPerGroupV = kChunksV / kGroupsV;
   static constexpr int kScaleK = cache_scale_bytes(kFormat, kK, kG_), kScaleV = cache_scale_bytes(kFormat, kV, kG_);
   static constexpr int kStageBytes = (kUnit * (kRowK + kRowV + kScaleK + kScaleV) + 127) / 128 * 128;
-  static constexpr int kStages = 2;
   static constexpr int kRegisters = kV * kN / 4 + 90;  // sums, and about what else a thread holds
   static constexpr int kResident = 65536 / (kWarps * 32 * (kRegisters < 128 ? 128 : kRegisters));  // CTAs of an SM
   static constexpr int kMostRegisters = kResident >= 4 ? 128 : kResident == 3 ? 168 : 255;
@@ -149,8 +148,8 @@ struct AttendShape {
   static constexpr int kFactors = kQSums + kGroupsK * kRows * 4;   // [kRows] what S is multiplied by
   static constexpr int kStats = kFactors + kRows * 4;              // [3][kMostWarps][kRows] of the warps, see there
   static constexpr int kRing = (kStats + 3 * kMostWarps * kRows * 4 + 127) / 128 * 128;
-  // of a warp: its stages, and in their place its sums [kRows][kV] once they have run dry
-  static constexpr int kWarpBytes = kStages * kStageBytes > kRows * kV * 4 ? kStages * kStageBytes : kRows * kV * 4;
+  // of a warp: its two stages, and in their place its sums [kRows][kV] once they have run dry
+  static constexpr int kWarpBytes = 2 * kStageBytes > kRows * kV * 4 ? 2 * kStageBytes : kRows * kV * 4;
   static constexpr int smem(int warps) { return kRing + warps * kWarpBytes; }
 };
 
@@ -380,7 +379,6 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   }
   uint8_t* const ring = smem + Shape::kRing + warp * Shape::kWarpBytes;
   const uint32_t ring_at = smem_u32(ring);
-  constexpr int stage_step = Shape::kStageBytes;
   const int heads = p.heads_per_kv;
 
   // The item that is worked on (or whose keys are on their way): b, item = head * row_tiles + row tile, units u0 .. u1 - 1.
@@ -450,7 +448,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       next_places = look_up(turn + kTurns);
     }
     const uint32_t missing = absent >> first & ((1u << kTiles) - 1);
-    const uint32_t to = ring_at + stage * stage_step;
+    const uint32_t to = ring_at + stage * Shape::kStageBytes;
     if (missing == 0) {
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) copy_tile(__shfl_sync(~0u, places, first + i), to, i);
@@ -469,14 +467,12 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     cp_async_commit();
     return missing;
   };
-  constexpr int kAhead = Shape::kStages - 1;  // units on their way while one is worked on
-  static_assert(kAhead == 1);
-  uint32_t missing[kAhead];
+  uint32_t next_missing = 0;  // of the unit that is on its way
   auto start_item = [&]() {
     places = look_up(0);
     next_places = look_up(kTurns);
     absent = __ballot_sync(~0u, places == kNowhere);
-    missing[0] = fetch(0, 0);
+    next_missing = fetch(0, 0);
   };
 
   while (next_item()) {
@@ -586,18 +582,16 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     using PiecesV = Pieces<Shape::kRowV>;
     const uint32_t lane_v = kUnit * Shape::kRowK + (PiecesV::kTurn > 0 ? PiecesV::at(PiecesV::row_at(lane & 15), lane >> 4)
                                                                        : PiecesV::row_at(lane & 15) + (lane >> 4) * 16);
-    int stage = 0, turn = 0;
+    int turn = 0;
     for (int u = u0 + warp; u < u1; u += warps, ++turn) {
-      cp_async_wait<kAhead - 1>();
+      const int stage = turn & 1;
+      const uint32_t none = next_missing;
+      cp_async_wait<0>();
       __syncwarp();
-      const uint32_t none = missing[0];
-#pragma unroll
-      for (int i = 0; i + 1 < kAhead; ++i) missing[i] = missing[i + 1];
-      missing[kAhead - 1] = fetch(turn + kAhead, stage == 0 ? kAhead : stage - 1);
-      const uint32_t from_k = ring_at + stage * stage_step + lane_k, from_v = ring_at + stage * stage_step + lane_v;
-      const uint8_t* const scales_k = ring + stage * stage_step + kUnit * (Shape::kRowK + Shape::kRowV);
+      next_missing = fetch(turn + 1, stage ^ 1);
+      const uint32_t from_k = ring_at + stage * Shape::kStageBytes + lane_k, from_v = ring_at + stage * Shape::kStageBytes + lane_v;
+      const uint8_t* const scales_k = ring + stage * Shape::kStageBytes + kUnit * (Shape::kRowK + Shape::kRowV);
       const uint8_t* const scales_v = scales_k + kUnit * Shape::kScaleK;
-      stage = stage == kAhead ? 0 : stage + 1;
 
       // ---- S ----
       float s[kTiles][kN][4];
@@ -1147,7 +1141,7 @@ static int with_shape(const SplashCacheAttendArgs& a, Fn&& fn) {
     if constexpr (kV <= 128) {
       if (rows > 16 && rows <= 24) return fn(AttendShape<kF, kK, kV, kG, 3>{});
     }
-    const bool by_eight = rows <= 8 || (kV > 128 && a.q.size[0] * reach_of(a) * c.kv_heads < kWideTokens);
+    const bool by_eight = rows <= 8 || (kV > 128 && reach_of(a) < kWideTokens / (a.q.size[0] * c.kv_heads));
     return by_eight ? fn(AttendShape<kF, kK, kV, kG, 1>{}) : fn(AttendShape<kF, kK, kV, kG, 2>{});
   };
   auto wide = [&](auto k, auto v) {
@@ -1185,6 +1179,7 @@ static int check_attend(const SplashCacheAttendArgs& a) {
   if (a.page_table == nullptr || a.lengths == nullptr || a.n_table <= 0 || a.table_stride < 0) return SPLASH_ERR_INVALID_ARGUMENT;
   if (!(a.soft_cap >= 0.f)) return SPLASH_ERR_INVALID_ARGUMENT;
   if (a.q.size[0] > (1 << 24) || a.q.size[1] > (1 << 20) || a.q.size[2] > (1 << 20) || a.q.size[1] * a.q.size[2] > (1 << 26) ||
+      (int64_t)a.n_table * c.page_size > (1 << 30) ||
       c.n_pages * c.kv_heads > 0x7fffffffll / (c.page_size / 16))  // (tiles of 16 tokens are counted in 32 bits)
     return SPLASH_ERR_TOO_LARGE;
   return SPLASH_OK;
@@ -1236,7 +1231,7 @@ static int cache_attend(const SplashCacheAttendArgs& a, cudaStream_t stream) {
   p.dtype = a.q.dtype;
   p.head_dim = c.head_dim;
   p.head_dim_v = c.head_dim_v;
-  p.window = a.window < 0 ? -1 : a.window;
+  p.window = a.window < 0 ? -1 : a.window < (1 << 30) ? a.window : 1 << 30;  // (tables reach no further)
   return with_shape(a, [&](auto shape) -> int {
     using Shape = decltype(shape);
     AttendParams own = p;
