@@ -221,9 +221,10 @@ constexpr uint32_t kLeastTop = 87u << 23;  // 2^-40
 // shares
 // ------------------------------------------------------------------------------------------
 // What a CTA spends on an item beside its units, in tokens: shares are equal in the sum of both.  (Looking up the item, q as
-// fragments, the first keys' latency, the warps' sums together: some thousand cycles.  us with 0, 320, 640 and 960: 64 x 200 ..
-// 4096 tokens 85, 51.8, 52.3, 54.4; 12 x 0 .. 10000, head dim 256, 28.6, 22.5, 24.6, 28.9.)
-constexpr int kItemTokens = 320;
+// fragments, the first keys' latency, the warps' sums together: some thousand cycles, more with more rows.  us with 160, 240, 320 and
+// 480; eight rows: 64 x 200 .. 4096 tokens 51.4, 48.7, 47.2, 48.1, 32 x 8192 .. 32768 153.2, 153.1, 153.0, 156.3; 24 rows, e4m3: 16 x 1000
+// .. 8192 54.9, 53.4, 51.9, 49.2, and with 640 49.3.)
+__host__ __device__ constexpr int item_tokens(int blocks) { return blocks == 1 ? 320 : 480; }
 // Every item is one CTA's where queries see at most kWholeTokens, or twice as many and there are kWholeItems items at least (us,
 // whole : shares and a second launch; 1024 tokens, 8 items 10.6 : 12.1, 256 items 14.6 : 22.0; 2048 tokens, 8 items 14.6 : 12.5,
 // 64 items 14.6 : 15.3, 256 items 23.1 : 27.7, 1024 items 57.8 : 57.3; 4096 tokens, 64 items 22.9 : 17.3).
@@ -1245,7 +1246,7 @@ static int cache_attend(const SplashCacheAttendArgs& a, cudaStream_t stream) {
       own.starts = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(a.workspace) + parts);
     }
     own.row_tiles = (p.q_len * p.heads_per_kv + Shape::kRows - 1) / Shape::kRows;
-    own.item_cost = kItemTokens / Shape::kUnit;
+    own.item_cost = item_tokens(Shape::kN) / Shape::kUnit;
     own.min_share = kWarps;
     return launch<Shape>(own, resident<Shape>(), stream);
   });
