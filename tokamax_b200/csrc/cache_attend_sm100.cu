@@ -28,12 +28,12 @@
 // every item is one CTA's, and there is one launch.
 //
 // Bound by: HBM asks for 64 + 8 bytes a token, head and side (int4, head dim 128, groups of 64).  At 6.5 TB/s an SM gets 46 codes
-// a cycle, so that a warp may spend 2.8 instructions on 32 of them; the kernel spends 2.1 (535 on a unit of 32 tokens, keys and
+// a cycle, so that a warp may spend 2.8 instructions on 32 of them; the kernel spends 2.1 (some 525 on a unit of 32 tokens, keys and
 // values, eight rows; 160 of them unpack), and issues 2.3 to 2.5 a cycle of the 4 that an SM could.  Instructions are what bounds
-// it: without the products the copies alone take 121 of 148 us.  Measured, 32 / 8 heads of 128, int4: 32 sequences of 8192 .. 32768
-// 148 us, 5.1 TB/s of the 6.5 that a plain copy reaches; one of 131072 41 us, 64 of 200 .. 4096 51 us, 3.7 and 3.5 TB/s.  About
+// it: without the products the copies alone take 121 us of the first case.  Measured, 32 / 8 heads of 128, int4: 32 sequences of
+// 8192 .. 32768 144 us, 5.2 TB/s of the 6.5 that a plain copy reaches; one of 131072 41 us, 64 of 200 .. 4096 47 us, 3.7 and 3.8 TB/s.  About
 // 9 us of each call are the two launches and the chains of loads at their beginnings (lengths, pages, codes; parts).  e4m3 rows are
-// unpacked by conversions and ask for twice the bytes: 48 sequences of 0 .. 13025 115 us, 5.9 TB/s.
+// unpacked by conversions and ask for twice the bytes: 48 sequences of 0 .. 13025 113 us, 6.0 TB/s.
 // Rows of more than one block of eight spend 190 instructions more a block on a unit, and leave room for fewer warps.
 #include <atomic>
 
