@@ -14,9 +14,11 @@
 //     bits that are 2^-24 of that entry.
 //   * P * scale is scaled by a power of two that follows the largest scale seen (`top`), below 2^14: 11 bits of it are kept.
 //     That is enough for outputs of bf16 (1.73e-3 of the norm from 64 bits where rounding the output alone costs 1.64e-3).  For
-//     f16 what is left of it goes through a second product: 6.0e-4 without (int4, 5111 keys; its codes are all positive, so that
-//     more is lost than of e4m3, 2.8e-4), 2.4e-4 with it (2.1e-4), where rounding the output costs 2.0e-4, for 148 -> 164 us
-//     (32 sequences of 8192 .. 32768, 32 / 8 heads of 128).
+//     f16 what is left of it goes through a second product, and int4's codes are taken less 8, with 8 scale_g in the zeros: sums
+//     of codes, all positive, are far larger than what comes out of long and even rows, and their own rounding in 32 bits shows.
+//     f16, int4, 5111 and 60000 keys: 6.0e-4 without either, 2.4e-4 and 4.7e-4 with the second product, 2.0e-4 and 2.2e-4
+//     with both, where rounding the output costs 2.0e-4 (e4m3: 2.8e-4, 2.1e-4 with the second product); 144, 160 and
+//     172 us (32 sequences of 8192 .. 32768, 32 / 8 heads of 128).
 // Softmax statistics are of one pass over the keys, with a running maximum and sum for each row.
 //
 // Split: the keys of all (sequence, kv head, row tile) items, one after the other in units of kUnit tokens, are cut into
@@ -109,6 +111,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Codes (odd: 16 times what they are) as they stand in a pair of halves, less 8: exact.
+__device__ __forceinline__ uint32_t less_eight(uint32_t pair, bool odd) {
+  const uint32_t eights = odd ? 0x80808080u : 0x80088008u;  // -8 * 2^-24 (times 16)
+  const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&pair), *reinterpret_cast<const __half2*>(&eights));
+  return *reinterpret_cast<const uint32_t*>(&x);
 }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -816,6 +824,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
             for (int half = 0; half < 2; ++half) {
               scale[half] = __uint_as_float(pairs[half][group] & 0xffff0000u);
               zero[half] = bf16_bits_to_float(pairs[half][group]);
+              if (decltype(fine)::value) zero[half] = fmaf(scale[half], 8.f, zero[half]);  // of codes less 8
             }
 #pragma unroll
             for (int nb = 0; nb < kN; ++nb) {
@@ -849,10 +858,17 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
               }
               uint32_t w0 = words[c % 2 * 2], w1 = words[c % 2 * 2 + 1];
               if constexpr (kInt4) {
-                const uint32_t a[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+                uint32_t a[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
                 w0 >>= 8;
                 w1 >>= 8;
-                const uint32_t a2[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+                uint32_t a2[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+                if (decltype(fine)::value) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    a[k] = less_eight(a[k], k & 1);
+                    a2[k] = less_eight(a2[k], k & 1);
+                  }
+                }
 #pragma unroll
                 for (int nb = 0; nb < kN; ++nb) {
                   mma_f16(o[c][0][nb], a, pf[nb][0], pf[nb][1]);
