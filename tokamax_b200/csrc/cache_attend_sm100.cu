@@ -233,10 +233,11 @@ constexpr uint32_t kLeastTop = 87u << 23;  // 2^-40
 // 480; eight rows: 64 x 200 .. 4096 tokens 51.4, 48.7, 47.2, 48.1, 32 x 8192 .. 32768 153.2, 153.1, 153.0, 156.3; 24 rows, e4m3: 16 x 1000
 // .. 8192 54.9, 53.4, 51.9, 49.2, and with 640 49.3.)
 __host__ __device__ constexpr int item_tokens(int blocks) { return blocks == 1 ? 320 : 480; }
-// Every item is one CTA's where queries see at most kWholeTokens, or twice as many and there are kWholeItems items at least (us,
-// whole : shares and a second launch; 1024 tokens, 8 items 10.6 : 12.1, 256 items 14.6 : 22.0; 2048 tokens, 8 items 14.6 : 12.5,
-// 64 items 14.6 : 15.3, 256 items 23.1 : 27.7, 1024 items 57.8 : 57.3; 4096 tokens, 64 items 22.9 : 17.3).
-constexpr int kWholeTokens = 1024, kWholeItems = 64;
+// Every item is one CTA's where queries see at most kWholeTokens, or twice as many and there are kWholeItems .. kMostWholeItems - 1
+// items (us, whole : shares and a second launch; 1024 tokens, 8 items 10.5 : 11.5, 256 items 14.6 : 18.8, 1024 items 35.0 : 37.9;
+// 2048 tokens, 8 items 14.6 : 11.6, 64 items 14.9 : 14.7, 256 items 22.6 : 24.9, 1024 items 57.4 : 52.8; 3000 tokens, 256 items
+// 28.3 : 27.6).
+constexpr int kWholeTokens = 1024, kWholeItems = 64, kMostWholeItems = 4 * kSms;
 
 struct Keys {  // of a sequence: tokens [lo, hi) in whole units from lo, which is a multiple of kUnit
   int lo, hi, units;
@@ -1207,7 +1208,8 @@ template <typename Shape>
 static bool is_whole(const SplashCacheAttendArgs& a) {
   const int64_t tiles = (a.q.size[2] * (a.q.size[1] / a.cache.kv_heads) + Shape::kRows - 1) / Shape::kRows;
   const int64_t items = a.q.size[0] * a.cache.kv_heads * tiles;
-  return reach_of(a) <= (items < kWholeItems ? kWholeTokens : 2 * kWholeTokens) && items <= INT32_MAX;
+  const bool some = items >= kWholeItems && items < kMostWholeItems;
+  return reach_of(a) <= (some ? 2 * kWholeTokens : kWholeTokens) && items <= INT32_MAX;
 }
 
 template <typename Shape>
