@@ -87,6 +87,23 @@ def test_f32_rows_are_held_to_within_half_a_step():
         assert ((got.cpu().double() - x.double()).abs() <= bound).all()
 
 
+def test_f32_rows_of_extreme_sizes():
+  """Ranges beyond 32 bits are NaN; rows of subnormal scales, which divide by other means, hold what they can."""
+  x = torch.zeros(1, 1, 4, 64)
+  x[0, 0, 0, :2] = torch.tensor([3e38, -3e38])
+  x[0, 0, 1] = torch.arange(64) * 1e-30
+  x[0, 0, 2] = torch.arange(64) * 1e-38
+  x[0, 0, 3] = torch.arange(64) * 1e30
+  store = Store([4], heads=1, d=64, group=64, dtype=torch.float32, keys=lambda _: x, values=lambda _: x)
+  k, _ = kv_cache.read(store.cache, store.table, store.lengths, 4, dtype=torch.float32)
+  got = k[0, 0].cpu().double()
+  assert got[0].isnan().all()
+  for row, size in ((1, 1e-30), (2, 1e-38), (3, 1e30)):
+    # half a step of 63 / 15, and a scale of 8 bits (7 below 2^-126, where steps of bf16 are 2^-133)
+    step = 63 * size / 15
+    assert ((got[row] - x[0, 0, row].double()).abs() <= step / 2 + 15 * (step * 2.0 ** -8 + 2.0 ** -134)).all(), row
+
+
 def test_tokens_of_a_projection_are_written_through_their_strides():
   store = Store([40, 23], heads=2, d=64, group=64)
   fresh = Store([40, 23], heads=2, d=64, group=64, seed=1)

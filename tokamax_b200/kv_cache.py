@@ -108,7 +108,8 @@ def slots_of(cache: KVCache, page_table: torch.Tensor, positions: torch.Tensor) 
 
 
 def append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
-  """Quantises ``k [B, kv_heads, T, D]`` and ``v`` (bf16, f16 or f32) into the slots ``[B, T]`` (int32 or int64).
+  """Quantises ``k [B, kv_heads, T, D]`` and ``v`` (bf16, f16 or f32) into the slots ``[B, T]`` (int32 or int64).  A group (row)
+  with a value that is not finite reads back as NaN.
 
   A slot outside the cache (-1 for padding) means that the token is not kept.  k and v are read through their strides: the
   ``[B, T, H, D]`` of a projection, transposed, is not copied.  No two tokens of a call may have the same slot."""
