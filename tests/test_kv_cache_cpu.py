@@ -39,6 +39,17 @@ def test_slots():
   assert slots.tolist() == [[112, 127, 32, -1, -1], [63, -1, 143, 5, 128]]
 
 
+def test_positions_behind_the_page_table_have_no_slot():
+  cache = kv_cache.make_kv_cache(9, 16, 1, 64, device="cpu")
+  table = torch.tensor([[7, 2], [0, -1]], dtype=torch.int32)
+  slots = kv_cache.slots_of(cache, table, torch.tensor([[31, 32, 48, 2 ** 31 - 1], [15, 16, 33, -1]], dtype=torch.int32))
+  assert slots.tolist() == [[47, -1, -1, -1], [15, -1, -1, -1]]
+  far = kv_cache.slots_of(cache, table, torch.tensor([[2 ** 62], [0]]))
+  assert far.dtype == torch.int64 and far.tolist() == [[-1], [0]]
+  assert kv_cache.slots_of(cache, table[:, :0], torch.tensor([[0, -1], [5, 40]])).tolist() == [[-1, -1], [-1, -1]]
+  assert kv_cache.slots_of(cache, table, torch.zeros(2, 0, dtype=torch.int32)).shape == (2, 0)
+
+
 def test_a_cache_on_the_cpu_has_no_operators():
   cache = kv_cache.make_kv_cache(2, 16, 1, 64, device="cpu")
   x = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16)

@@ -99,12 +99,17 @@ def make_kv_cache(n_pages: int, page_size: int, kv_heads: int, head_dim: int, he
 
 
 def slots_of(cache: KVCache, page_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
-  """Slots (int64) of the tokens at ``positions [B, T]`` of the sequences of ``page_table [B, pages]``; a negative position has
-  none (-1).  They are the same for every layer of a model: worked out once a step."""
+  """Slots (int64) of the tokens at ``positions [B, T]`` of the sequences of ``page_table [B, pages]``; a negative position, one
+  behind the table and one on a page that the table has as -1 have none (-1: :func:`append` does not keep the token).  They are the
+  same for every layer of a model: worked out once a step."""
+  n_table = page_table.shape[1]
+  if n_table == 0:
+    return torch.full(positions.shape, -1, dtype=torch.int64, device=positions.device)
   where = positions.clamp_min(0).long()
-  page = page_table.long().gather(1, where // cache.page_size)
+  index = where // cache.page_size
+  page = page_table.long().gather(1, index.clamp_max(n_table - 1))
   slots = page * cache.page_size + where % cache.page_size
-  return torch.where((positions >= 0) & (page >= 0), slots, -1)
+  return torch.where((positions >= 0) & (index < n_table) & (page >= 0), slots, -1)
 
 
 def append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
