@@ -463,6 +463,7 @@ int splash_bwd_static_scratch(const SplashBwdArgs* args, void* cuda_stream);
  *         clamped to 0 .. 15 (0 where scale is 0), all of it in 32 bits, ties to even
  *   e4m3: value = scale * code, scale = bf16(amax / 448), code = e4m3(x / scale), saturating
  * A group (row) with a value that is not finite, or whose range is not, is held, and read back, as NaN.
+ * The arrays need not be zeroed: what was never written has no part in attention as long as no query sees it.
  * ---------------------------------------------------------------------------------------- */
 typedef enum SplashCacheFormat { SPLASH_CACHE_INT4 = 0, SPLASH_CACHE_E4M3 = 1 } SplashCacheFormat;
 

@@ -1,10 +1,12 @@
 """The quantised key / value cache against its definition in 64 bits: rows written and read back, attention over them."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
 from oracle import kv_cache_ref
+from tokamax_b200 import _native
 from tokamax_b200 import kv_cache
 
 pytestmark = pytest.mark.gpu
@@ -417,3 +419,67 @@ def test_refusals():
       bad()
   with torch.no_grad():
     kv_cache.attend(cache, q.clone().requires_grad_(True), table, lengths)
+
+
+# ----------------------------------------------------------------------------------------------
+# both ways through attention: every item one CTA's, and shares that a second launch joins
+# ----------------------------------------------------------------------------------------------
+def _workspace_bytes(store, q_heads, t, table, window=None):
+  """What splash_cache_attend asks for on these sizes: 0 where every item is one CTA's."""
+  a = _native.SplashCacheAttendArgs()
+  c, cache = a.cache, store.cache
+  c.k_codes, c.k_scales, c.v_codes, c.v_scales = (x.data_ptr() for x in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales))
+  c.n_pages, c.format, c.page_size, c.kv_heads = cache.n_pages, kv_cache.FORMATS[cache.fmt], cache.page_size, cache.kv_heads
+  c.group, c.head_dim, c.head_dim_v = cache.group_size or 0, cache.head_dim, cache.head_dim_v
+  widths = (C.c_int32 * 2)()
+  at = C.addressof(widths)
+  _native.lib().splash_cache_row_widths(cache.head_dim, cache.head_dim_v, C.cast(at, C.POINTER(C.c_int32)), C.cast(at + 4, C.POINTER(C.c_int32)))
+  c.row_k, c.row_v = widths
+  for x, d in ((a.q, cache.head_dim), (a.o, cache.head_dim_v)):
+    x.data, x.dtype = cache.k_codes.data_ptr(), 0
+    for i, (n, s) in enumerate(zip((len(store.lengths_list), q_heads, t, d), (q_heads * t * d, t * d, d, 1))):
+      x.size[i], x.stride[i] = n, s
+  a.page_table, a.table_stride, a.n_table, a.lengths = table.data_ptr(), table.shape[1], table.shape[1], store.lengths.data_ptr()
+  a.window = -1 if window is None else window
+  return _native.lib().splash_cache_attend_workspace_bytes(C.byref(a))
+
+
+def _table_of(store, shares, q_heads, t, window=None):
+  """The store's page table as it is, or wide enough for shares (its sequences are as they were)."""
+  table = store.table
+  if shares:
+    table = torch.full((table.shape[0], 8192 // store.page), -1, dtype=torch.int32, device=DEV)
+    table[:, :store.table.shape[1]] = store.table
+  assert (_workspace_bytes(store, q_heads, t, table, window) > 0) == shares
+  return table
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("d,d_v", [(64, 64), (128, 128), (192, 128), (256, 256)])
+@pytest.mark.parametrize("q_heads,t", [(2, 1), (16, 1), (10, 4)])
+@pytest.mark.parametrize("shares", [False, True])
+def test_arrays_that_were_never_written(fmt, group, d, d_v, q_heads, t, shares):
+  """NaN (0x7f and 0xff of e4m3) in the codes wherever nothing was written: behind the ends of sequences, on other pages, and in place of
+  tokens that stand before every window."""
+  lengths = [1, 50, 77, 0, 700]
+  try:
+    store = Store(lengths, d=d, d_v=d_v, fmt=fmt, group=group, spare=2, page=64)
+  except ValueError:
+    assert group in (64, 128)
+    return
+  for window in (None, 20):
+    table = _table_of(store, shares and window is None, q_heads, t, window)  # (a window's items are one CTA's)
+    want = _check_attend(store, q_heads=q_heads, t=t, table=table, window=window)
+    arrays = (store.cache.k_codes, store.cache.v_codes)
+    before = [x.clone() for x in arrays]
+    for x in arrays:
+      x.fill_(0x7f)
+      x.view(-1)[1::2] = 0xff
+    slots = store.slots.clone()
+    if window is not None:  # what no query sees was never written either
+      for b, n in enumerate(lengths):
+        slots[b, :max(n - t - window, 0)] = -1
+    kv_cache.append(store.cache, store.k.to(DEV), store.v.to(DEV), slots)
+    assert torch.equal(want, _check_attend(store, q_heads=q_heads, t=t, table=table, window=window))
+    for x, y in zip(arrays, before):
+      x.copy_(y)

@@ -76,9 +76,6 @@ struct AttendParams {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async16_zeros(uint32_t dst, const void* somewhere) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, 0;" ::"r"(dst), "l"(somewhere) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -465,13 +462,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     } else if (u0 + warp + turn * warps < u1) {
       for (int i = 0; i < kTiles; ++i) {
         const uint32_t place = __shfl_sync(~0u, places, first + i);
-        if (!(missing >> i & 1)) {
-          copy_tile(place, to, i);
-        } else if (!kInt4) {
-          // P is 0 there, but 0 times what lay there before need not be (codes of four bits are numbers always)
-          const uint32_t values = to + kUnit * Shape::kRowK + i * 16 * Shape::kRowV;
-          for (int j = lane; j < Shape::kRowV; j += 32) cp_async16_zeros(values + j * 16, p.v_codes);
-        }
+        if (!(missing >> i & 1)) copy_tile(place, to, i);
       }
     }
     cp_async_commit();
@@ -706,6 +697,12 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       const int token0 = keys.lo + u * kUnit;
       const bool whole = none == 0 && u >= whole_lo && u < whole_hi;
       uint32_t seen = ~0u;  // a bit for each of s, where not whole: tile, block, element
+      // Of a unit's tokens, what no row sees (behind the end, without a page, before every window) may be anything, never written
+      // maybe.
+      auto some_row_sees = [&](int token) {
+        const int at = token0 + token, position = position0 + query_of(n_rows - 1);
+        return at < keys.hi && at <= position && (p.window < 0 || at >= position0 - p.window) && !(none >> (token >> 4) & 1);
+      };
       if (!whole) {
         seen = 0;
 #pragma unroll
@@ -726,6 +723,17 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
           }
       }
       static_assert(kTiles * kN * 4 <= 32);
+      if (!kInt4 && !whole) {
+        // V's codes of tokens that no row sees become 0: P is 0 there, but 0 times whatever lies there need not be.  (Codes of four
+        // bits are numbers always.)
+        constexpr int kEach = Shape::kRowV / 16;
+        uint4* const values = reinterpret_cast<uint4*>(ring + stage * Shape::kStageBytes + kUnit * Shape::kRowK);
+        for (int j = lane; j < kUnit * kEach; j += 32) {  // (a row's pieces are turned within the row)
+          const int token = j / kEach;
+          if (!some_row_sees(token)) values[j] = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+      }
 
       // ---- the maximum that P is taken against: raised where a logit passes it by more than kSlack ----
       bool grows = false;
