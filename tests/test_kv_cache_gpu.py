@@ -459,8 +459,8 @@ def _table_of(store, shares, q_heads, t, window=None):
 @pytest.mark.parametrize("q_heads,t", [(2, 1), (16, 1), (10, 4)])
 @pytest.mark.parametrize("shares", [False, True])
 def test_arrays_that_were_never_written(fmt, group, d, d_v, q_heads, t, shares):
-  """NaN (0x7f and 0xff of e4m3) in the codes wherever nothing was written: behind the ends of sequences, on other pages, and in place of
-  tokens that stand before every window."""
+  """NaN wherever nothing was written, codes (0x7f and 0xff of e4m3) and scales: behind the ends of sequences, on other pages, and in
+  place of tokens that stand before every window."""
   lengths = [1, 50, 77, 0, 700]
   try:
     store = Store(lengths, d=d, d_v=d_v, fmt=fmt, group=group, spare=2, page=64)
@@ -470,11 +470,13 @@ def test_arrays_that_were_never_written(fmt, group, d, d_v, q_heads, t, shares):
   for window in (None, 20):
     table = _table_of(store, shares and window is None, q_heads, t, window)  # (a window's items are one CTA's)
     want = _check_attend(store, q_heads=q_heads, t=t, table=table, window=window)
-    arrays = (store.cache.k_codes, store.cache.v_codes)
+    arrays = (store.cache.k_codes, store.cache.v_codes, store.cache.k_scales.view(torch.int16), store.cache.v_scales.view(torch.int16))
     before = [x.clone() for x in arrays]
-    for x in arrays:
+    for x in arrays[:2]:
       x.fill_(0x7f)
       x.view(-1)[1::2] = 0xff
+    for x in arrays[2:]:
+      x.fill_(0x7fff)
     slots = store.slots.clone()
     if window is not None:  # what no query sees was never written either
       for b, n in enumerate(lengths):

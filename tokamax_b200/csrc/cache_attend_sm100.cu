@@ -698,7 +698,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       const bool whole = none == 0 && u >= whole_lo && u < whole_hi;
       uint32_t seen = ~0u;  // a bit for each of s, where not whole: tile, block, element
       // Of a unit's tokens, what no row sees (behind the end, without a page, before every window) may be anything, never written
-      // maybe.
+      // maybe: it must not have a say in when sums are rescaled either, or last bits would hang on it.
       auto some_row_sees = [&](int token) {
         const int at = token0 + token, position = position0 + query_of(n_rows - 1);
         return at < keys.hi && at <= position && (p.window < 0 || at >= position0 - p.window) && !(none >> (token >> 4) & 1);
@@ -758,22 +758,22 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
           load_words<kGroupsV>(own_top[i / 32], reinterpret_cast<const uint32_t*>(scales_v) + token * kGroupsV);
         else
           own_top[i / 32][0] = (uint32_t)reinterpret_cast<const uint16_t*>(scales_v)[token] << 16;
+        if (!whole && !some_row_sees(token)) {
+#pragma unroll
+          for (int group = 0; group < kGroupsV; ++group) own_top[i / 32][group] = 0;
+        }
 #pragma unroll
         for (int group = 0; group < kGroupsV; ++group) grows = grows || own_top[i / 32][group] >= top + (1u << 23);
       }
       if (__any_sync(~0u, grows)) {
         uint32_t largest = 0;
 #pragma unroll
-        for (int i = 0; i < kUnit; i += 32) {
-          const int token = kUnit < 32 ? lane & (kUnit - 1) : i + lane;
-          if (whole || (!(none >> (token >> 4) & 1) && token0 + token < keys.hi)) {
+        for (int i = 0; i < kUnit; i += 32)
 #pragma unroll
-            for (int group = 0; group < kGroupsV; ++group) {
-              const uint32_t x = own_top[i / 32][group];
-              largest = max(largest, x < 0x7f800000u ? x : 0u);  // (not NaN)
-            }
+          for (int group = 0; group < kGroupsV; ++group) {
+            const uint32_t x = own_top[i / 32][group];
+            largest = max(largest, x < 0x7f800000u ? x : 0u);  // (not NaN)
           }
-        }
         largest = max(__reduce_max_sync(~0u, largest) & 0x7f800000u, top);
         const float rise = __uint_as_float((uint32_t)max(127 - (int)((largest - top) >> 23), 0) << 23);
         top = largest;
