@@ -106,6 +106,23 @@ def test_f32_rows_of_extreme_sizes():
     assert ((got[row] - x[0, 0, row].double()).abs() <= step / 2 + 15 * (step * 2.0 ** -8 + 2.0 ** -134)).all(), row
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_int4_rows_of_subnormal_scales(dtype):
+  """Scales of few bits: codes are clamped to 0 .. 15, and a channel's has no part in its neighbours'."""
+  tops = [1, 7, 8, 15, 22, 23, 100, 217, 240, 255]
+  x = torch.zeros(1, 1, 2 * len(tops), 64)
+  for i, top in enumerate(tops):
+    for row, least in ((2 * i, 0), (2 * i + 1, -3)):
+      x[0, 0, row] = least + torch.arange(64) % (top + 1)
+      x[0, 0, row, 5::7] = least + top
+      x[0, 0, row, 32:] += 9  # (of another group: the same range)
+  x = (x.double() * 2.0 ** -133).to(dtype)
+  assert x.double().mul(2.0 ** 133).frac().abs().max() == 0 and x.double().max() > 255 * 2.0 ** -133
+  store = Store([x.shape[2]], heads=1, d=64, group=32, dtype=dtype, keys=lambda _: x, values=lambda _: x)
+  k, _ = kv_cache.read(store.cache, store.table, store.lengths, x.shape[2], dtype=torch.float32)
+  assert torch.equal(k[0].cpu().double(), store.held(0)[0])
+
+
 def test_tokens_of_a_projection_are_written_through_their_strides():
   store = Store([40, 23], heads=2, d=64, group=64)
   fresh = Store([40, 23], heads=2, d=64, group=64, seed=1)

@@ -192,8 +192,9 @@ __device__ __forceinline__ void store_row(const AppendParams& p, const RowSide& 
       const bool plain = scale <= kLeastDivisor;
       auto quotient = [&](float v) {
         const float d = v - zero, t = plain ? d / scale : divide(d, scale, inverse);
-        // (bf16: zero is the least value itself and the quotient within 0 .. 15.06)
-        return kDType == SPLASH_BF16 ? t : fminf(fmaxf(t, 0.f), 15.f);
+        // (bf16: zero is the least value itself, and a scale of eight bits leaves the quotient within 0 .. 15.06.  A subnormal scale
+        // has fewer: 22 for a range of 22 times the least bf16.)
+        return kDType == SPLASH_BF16 && !plain ? t : fminf(fmaxf(t, 0.f), 15.f);
       };
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
