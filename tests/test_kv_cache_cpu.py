@@ -60,6 +60,24 @@ def test_a_cache_on_the_cpu_has_no_operators():
       call()
 
 
+def _calls(cache):
+  """A call of each operator, by its floating operands."""
+  i = torch.zeros(1, dtype=torch.int32)
+  return {"append": (lambda k, v: kv_cache.append(cache, k, v, i[None]), 2), "read": (lambda x: kv_cache.read(cache, i[None], i + 1, 4)[0] + x.sum(), 1),
+          "attend": (lambda q: kv_cache.attend(cache, q, i[None], i + 1), 1)}
+
+
+@pytest.mark.parametrize("name", ["append", "read", "attend"])
+def test_calls_are_not_recorded(name):
+  """A graph of torch.jit.trace would give back memory that nothing wrote."""
+  call, n = _calls(kv_cache.make_kv_cache(2, 16, 1, 64, device="cpu"))[name]
+  operands = tuple(torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16) for _ in range(n))
+  with pytest.raises(NotImplementedError, match="recorded"):
+    torch.jit.trace(call, operands, check_trace=False)
+  with pytest.raises(RuntimeError, match="CUDA"):  # (and nothing of it is left over)
+    call(*operands)
+
+
 def _args(kind):
   """Arguments that pass every check up to the missing device; addresses that nobody reads."""
   a = getattr(_native, kind)()

@@ -438,6 +438,21 @@ def test_refusals():
     kv_cache.attend(cache, q.clone().requires_grad_(True), table, lengths)
 
 
+def test_compiled_calls_give_the_same_and_traced_ones_are_refused():
+  store = Store([70, 31], d=64)
+  q = torch.randn(2, 4, 1, 64, device=DEV, dtype=torch.bfloat16)
+
+  def step(q, k):
+    kv_cache.append(store.cache, k, k, store.slots[:, :1])
+    return kv_cache.attend(store.cache, q, store.table, store.lengths, logits_scale=0.1) * 2.0
+
+  want = step(q, q[:, :2])
+  kv_cache.append(store.cache, store.k[:, :, :1].to(DEV), store.v[:, :, :1].to(DEV), store.slots[:, :1])
+  assert torch.equal(torch.compile(step, backend="eager")(q, q[:, :2]), want)
+  with pytest.raises(NotImplementedError, match="recorded"):
+    torch.jit.trace(step, (q, q[:, :2]), check_trace=False)
+
+
 # ----------------------------------------------------------------------------------------------
 # both ways through attention: every item one CTA's, and shares that a second launch joins
 # ----------------------------------------------------------------------------------------------

@@ -7,6 +7,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -322,6 +323,11 @@ void require_no_grad(const at::Tensor& t, const char* name) {
                               " requires a gradient: the cache's operators have none (call them under torch.no_grad())");
 }
 
+// A recorded graph would hold what allocates the results and not the launch that writes them.
+void require_not_traced() {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "the cache's operators cannot be recorded by torch.jit.trace");
+}
+
 SplashTensor describe_row_tensor(const at::Tensor& t, const char* name, bool f32_too) {
   SplashTensor d{};
   const auto type = t.scalar_type();
@@ -350,6 +356,7 @@ int on_stream_of(const at::Tensor& t, Fn&& call) {
 
 void cache_append(const KvCache& cache, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& slots_in) {
   const SplashKvCache& c = cache.desc;
+  require_not_traced();
   TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.dim() == 4 && slots_in.dim() == 2, "expected k and v of [B, H, T, D] and slots of [B, T]");
   TORCH_CHECK_VALUE(k_in.size(1) == c.kv_heads && k_in.size(3) == c.head_dim && v_in.size(3) == c.head_dim_v, "k ", k_in.sizes(), " / v ",
                     v_in.sizes(), " do not match a cache of ", c.kv_heads, " heads of ", c.head_dim, " / ", c.head_dim_v, " channels");
@@ -397,6 +404,7 @@ at::Tensor set_pages(Args& a, const KvCache& cache, const at::Tensor& table_in, 
 std::tuple<at::Tensor, at::Tensor> cache_read(const KvCache& cache, const at::Tensor& table_in, const at::Tensor& lengths, int64_t max_len,
                                               at::ScalarType type) {
   const SplashKvCache& c = cache.desc;
+  require_not_traced();
   SplashCacheReadArgs a{};
   const at::Tensor table = set_pages(a, cache, table_in, lengths);
   TORCH_CHECK_VALUE(max_len >= 0, "max_len is not negative, got ", max_len);
@@ -414,6 +422,7 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
                                                   const at::Tensor& lengths, double scale, std::optional<int64_t> window,
                                                   std::optional<double> soft_cap, const Maybe& sinks_in, double mask_value, bool residuals) {
   const SplashKvCache& c = cache.desc;
+  require_not_traced();
   TORCH_CHECK_VALUE(q_in.dim() == 4 && q_in.size(3) == c.head_dim && q_in.size(1) % c.kv_heads == 0, "q ", q_in.sizes(),
                     " does not match a cache of ", c.kv_heads, " heads of ", c.head_dim, " channels: expected [B, heads, T, D]");
   SplashCacheAttendArgs a{};
