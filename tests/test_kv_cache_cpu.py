@@ -4,6 +4,7 @@ import re
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from oracle import kv_cache_ref
 from tokamax_b200 import _native
@@ -76,6 +77,32 @@ def test_calls_are_not_recorded(name):
     torch.jit.trace(call, operands, check_trace=False)
   with pytest.raises(RuntimeError, match="CUDA"):  # (and nothing of it is left over)
     call(*operands)
+
+
+@pytest.mark.parametrize("name,which", [("append", 0), ("append", 1), ("attend", 0)])
+def test_operands_with_a_derivative_are_refused(name, which):
+  """A gradient or a tangent of forward mode would be lost without a word."""
+  call, n = _calls(kv_cache.make_kv_cache(2, 16, 1, 64, device="cpu"))[name]
+  operands = [torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16) for _ in range(n)]
+  plain = operands[which]
+  operands[which] = plain.clone().requires_grad_(True)
+  with pytest.raises(NotImplementedError, match="gradient"):
+    call(*operands)
+  with forward_ad.dual_level():
+    operands[which] = forward_ad.make_dual(plain, torch.ones_like(plain))
+    with pytest.raises(NotImplementedError, match="tangent"):
+      call(*operands)
+    with torch.inference_mode(), pytest.raises(RuntimeError, match="CUDA"):  # (which takes no derivatives of either kind)
+      call(*operands)
+
+
+def test_sinks_with_a_derivative_are_refused():
+  cache = kv_cache.make_kv_cache(2, 16, 1, 64, device="cpu")
+  q, i, sinks = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32), torch.zeros(1)
+  with pytest.raises(NotImplementedError, match="sinks requires"):
+    kv_cache.attend(cache, q, i[None], i, sinks=sinks.clone().requires_grad_(True))
+  with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="sinks has a tangent"):
+    kv_cache.attend(cache, q, i[None], i, sinks=forward_ad.make_dual(sinks, torch.ones(1)))
 
 
 def _args(kind):

@@ -10,6 +10,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -321,6 +322,8 @@ void require_on_gpu(const at::Tensor& t, const KvCache& cache, const char* name)
 void require_no_grad(const at::Tensor& t, const char* name) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(t.requires_grad() && at::GradMode::is_enabled()), name,
                               " requires a gradient: the cache's operators have none (call them under torch.no_grad())");
+  TORCH_CHECK_NOT_IMPLEMENTED(!(t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()), name,
+                              " has a tangent of forward mode: the cache's operators have none");
 }
 
 // A recorded graph would hold what allocates the results and not the launch that writes them.
@@ -365,11 +368,11 @@ void cache_append(const KvCache& cache, const at::Tensor& k_in, const at::Tensor
   TORCH_CHECK_VALUE(k_in.scalar_type() == v_in.scalar_type(), "k and v have one type, got ", k_in.scalar_type(), " and ", v_in.scalar_type());
   const auto type = slots_in.scalar_type();
   TORCH_CHECK_VALUE(type == at::kInt || type == at::kLong, "slots are int32 or int64, got ", type);
+  require_no_grad(k_in, "k");
+  require_no_grad(v_in, "v");
   require_on_gpu(k_in, cache, "k");
   require_on_gpu(v_in, cache, "v");
   require_on_gpu(slots_in, cache, "slots");
-  require_no_grad(k_in, "k");
-  require_no_grad(v_in, "v");
   SplashCacheAppendArgs a{};
   a.cache = c;
   if (slots_in.numel() == 0) return;
@@ -423,6 +426,8 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
                                                   std::optional<double> soft_cap, const Maybe& sinks_in, double mask_value, bool residuals) {
   const SplashKvCache& c = cache.desc;
   require_not_traced();
+  require_no_grad(q_in, "q");
+  if (sinks_in.has_value()) require_no_grad(*sinks_in, "sinks");
   TORCH_CHECK_VALUE(q_in.dim() == 4 && q_in.size(3) == c.head_dim && q_in.size(1) % c.kv_heads == 0, "q ", q_in.sizes(),
                     " does not match a cache of ", c.kv_heads, " heads of ", c.head_dim, " channels: expected [B, heads, T, D]");
   SplashCacheAttendArgs a{};
@@ -431,13 +436,11 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
   TORCH_CHECK_VALUE(!window.has_value() || (*window >= 0 && *window <= INT32_MAX), "local_window_size is not negative");
   TORCH_CHECK_VALUE(!soft_cap.has_value() || *soft_cap > 0, "logits_soft_cap is positive");
   require_on_gpu(q_in, cache, "q");
-  require_no_grad(q_in, "q");
   const int64_t b = q_in.size(0), heads = q_in.size(1), t = q_in.size(2);
   Maybe sinks;
   if (sinks_in.has_value()) {
     TORCH_CHECK_VALUE(sinks_in->dim() == 1 && sinks_in->size(0) == heads, "sinks ", sinks_in->sizes(), " for ", heads, " q heads");
     require_on_gpu(*sinks_in, cache, "sinks");
-    require_no_grad(*sinks_in, "sinks");
     sinks = sinks_in->to(at::kFloat).contiguous();
     a.sinks = static_cast<const float*>(sinks->data_ptr());
   }

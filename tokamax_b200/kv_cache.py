@@ -16,8 +16,8 @@ Formats:
 Tokens lie in pages of ``page_size`` tokens.  A token's place is its slot, ``page * page_size + offset``; a sequence's pages
 are a row of the page table.  Whoever owns the cache hands pages out; :func:`slots_of` turns positions into slots.
 
-The operators serve inference: operands that require a gradient are refused, and so are calls under ``torch.jit.trace``, whose graph
-would not hold the launches.
+The operators serve inference: operands that require a gradient or have a tangent of forward mode are refused, and so are calls
+under ``torch.jit.trace``, whose graph would not hold the launches.
 """
 from __future__ import annotations
 
