@@ -283,6 +283,16 @@ def test_soft_cap_and_sinks(fmt, dtype):
   _check_attend(store, q_heads=6, t=2, soft_cap=30.0, sinks=sinks, window=64, dtype=dtype)
 
 
+@pytest.mark.parametrize("fmt", ["int4", "e4m3"])
+@pytest.mark.parametrize("soft_cap", [0.5, 50.0, 1000.0, 1e5])
+@pytest.mark.parametrize("q_heads,t", [(4, 1), (8, 4), (10, 4)])
+def test_soft_caps_far_above_and_below_the_logits(fmt, soft_cap, q_heads, t):
+  """tanh's error is 1.1e-7 of itself up to 1/2 and 1.7e-7 beyond, so that a logit's is 4e-7 of the logit at most: well inside what
+  _check_attend allows for its products, at any cap."""
+  store = Store([1, 65, 700, 1300], d=128, fmt=fmt, group=64 if fmt == "int4" else None, page=64)
+  _check_attend(store, q_heads=q_heads, t=t, soft_cap=soft_cap)
+
+
 def test_sizes_of_scales_and_queries():
   """Tokens whose values differ by powers of ten, queries that are large, small and zero."""
   for fmt, group in FORMATS:

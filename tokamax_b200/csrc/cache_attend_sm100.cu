@@ -681,16 +681,20 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
             }
           }
       }
-      if (p.soft_cap > 0.f) {  // cap * tanh(x / cap) in units of log2, tanh y = 1 - 2 / (exp(2 y) + 1)
-        const float inside = 2.f * kLog2e / p.soft_cap, outside = p.soft_cap * kLog2e;
+      if (p.soft_cap > 0.f) {  // cap * tanh(x / cap) in units of log2
+        const float inside = 1.f / p.soft_cap, outside = p.soft_cap * kLog2e;
 #pragma unroll
-        for (int nb = 0; nb < kN; ++nb)
+        for (int nb = 0; nb < kN; ++nb) {
+          const float2 f = *reinterpret_cast<const float2*>(factors + nb * 8 + t4 * 2);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float f = factors[nb * 8 + t4 * 2 + (j & 1)] * inside;
+          for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i) s[i][nb][j] = outside - __fdividef(2.f * outside, ex2(s[i][nb][j] * f) + 1.f);
-          }
+            for (int j = 0; j < 4; j += 2) {
+              const float2 t = tanh_each(make_float2(s[i][nb][j] * f.x * inside, s[i][nb][j + 1] * f.y * inside));
+              s[i][nb][j] = t.x * outside;
+              s[i][nb][j + 1] = t.y * outside;
+            }
+        }
       }
 
       // ---- what is seen ----
