@@ -159,6 +159,12 @@ def test_c_entry_points_refuse_before_they_touch_the_gpu(kind, path, value, stat
   assert getattr(_native.lib(), fn)(None, None) == -1
 
 
+def test_a_scale_that_is_no_number():
+  a = _spoilt("SplashCacheAttendArgs", "scale", float("nan"))
+  assert _native.lib().splash_cache_attend(C.byref(a), None) == -1
+  assert _native.lib().splash_cache_attend_workspace_bytes(C.byref(a)) == 0
+
+
 def test_workspace():
   lib = _native.lib()
   short = _args("SplashCacheAttendArgs")  # two pages: every item is one CTA's

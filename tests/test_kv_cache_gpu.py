@@ -448,6 +448,15 @@ def test_refusals():
     kv_cache.attend(cache, q.clone().requires_grad_(True), table, lengths)
 
 
+def test_scales_and_caps_that_are_no_numbers_are_refused():
+  """A scale of NaN passed for one of nothing, a cap below the least of 32 bits for none."""
+  store = Store([20], d=64)
+  q = torch.zeros(1, 2, 1, 64, device=DEV, dtype=torch.bfloat16)
+  for kw in (dict(logits_scale=math.nan), dict(logits_soft_cap=1e-50), dict(logits_soft_cap=math.nan), dict(logits_soft_cap=-1.0)):
+    with pytest.raises(ValueError):
+      kv_cache.attend(store.cache, q, store.table, store.lengths, **kw)
+
+
 def test_compiled_calls_give_the_same_and_traced_ones_are_refused():
   store = Store([70, 31], d=64)
   q = torch.randn(2, 4, 1, 64, device=DEV, dtype=torch.bfloat16)

@@ -1207,7 +1207,7 @@ static int check_attend(const SplashCacheAttendArgs& a) {
     if (a.q.size[i] != a.o.size[i]) return SPLASH_ERR_INVALID_ARGUMENT;
   if (a.q.size[3] != c.head_dim || a.o.size[3] != c.head_dim_v || a.q.size[1] % c.kv_heads != 0) return SPLASH_ERR_INVALID_ARGUMENT;
   if (a.page_table == nullptr || a.lengths == nullptr || a.n_table <= 0 || a.table_stride < 0) return SPLASH_ERR_INVALID_ARGUMENT;
-  if (!(a.soft_cap >= 0.f)) return SPLASH_ERR_INVALID_ARGUMENT;
+  if (!(a.soft_cap >= 0.f) || a.scale != a.scale) return SPLASH_ERR_INVALID_ARGUMENT;  // (not NaN)
   if (a.q.size[0] > (1 << 24) || a.q.size[1] > (1 << 20) || a.q.size[2] > (1 << 20) || a.q.size[1] * a.q.size[2] > (1 << 26) ||
       (int64_t)a.n_table * c.page_size > (1 << 30) ||
       c.n_pages * c.kv_heads > 0x7fffffffll / (c.page_size / 16))  // (tiles of 16 tokens are counted in 32 bits)

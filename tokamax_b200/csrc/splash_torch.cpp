@@ -14,6 +14,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <cmath>
 #include <memory>
 #include <optional>
 #include <tuple>
@@ -434,7 +435,8 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
   const at::Tensor table = set_pages(a, cache, table_in, lengths);
   TORCH_CHECK_VALUE(q_in.size(0) == lengths.size(0), "q of ", q_in.size(0), " sequences, lengths of ", lengths.size(0));
   TORCH_CHECK_VALUE(!window.has_value() || (*window >= 0 && *window <= INT32_MAX), "local_window_size is not negative");
-  TORCH_CHECK_VALUE(!soft_cap.has_value() || *soft_cap > 0, "logits_soft_cap is positive");
+  TORCH_CHECK_VALUE(!soft_cap.has_value() || (float)*soft_cap > 0, "logits_soft_cap is positive (in 32 bits), got ", *soft_cap);
+  TORCH_CHECK_VALUE(!std::isnan(scale), "logits_scale is NaN");
   require_on_gpu(q_in, cache, "q");
   const int64_t b = q_in.size(0), heads = q_in.size(1), t = q_in.size(2);
   Maybe sinks;
