@@ -123,6 +123,28 @@ def test_int4_rows_of_subnormal_scales(dtype):
   assert torch.equal(k[0].cpu().double(), store.held(0)[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_values_beside_a_tie_are_rounded_once(dtype):
+  """scale * code half way between two values of the type, and a zero far below: rounding to 32 bits first loses the zero, and the
+  tie then goes to the even one."""
+  x = torch.zeros(1, 1, 8, 64)
+  for row, (scale, least) in enumerate([(255.0, 2.0 ** -30), (255.0, -2.0 ** -30), (129.0, 2.0 ** -25), (129.0, -2.0 ** -25), (1.9921875, 2.0 ** -38),
+                                        (1.9921875, -2.0 ** -38), (131.0, -2.0 ** -38), (253.0, 2.0 ** -38)]):
+    x[0, 0, row] = torch.arange(64) % 16 * scale
+    x[0, 0, row, ::16] = least
+  store = Store([8], heads=1, d=64, group=64, dtype=torch.float32, keys=lambda _: x, values=lambda _: -x)
+  k, v = kv_cache.read(store.cache, store.table, store.lengths, 8, dtype=dtype)
+  twice = False
+  for got, ref in zip((k[0], v[0]), store.held(0)):
+    # rounded to odd in 32 bits, then to the type: once in all
+    near = ref.float()
+    other = torch.nextafter(near, torch.where(ref > near.double(), math.inf, -math.inf))
+    odd = torch.where((near.double() == ref) | (near.view(torch.int32) & 1 == 1), near, other)
+    assert torch.equal(got.cpu(), odd.to(dtype))
+    twice = twice or not torch.equal(odd.to(dtype), near.to(dtype))
+  assert twice
+
+
 def test_tokens_of_a_projection_are_written_through_their_strides():
   store = Store([40, 23], heads=2, d=64, group=64)
   fresh = Store([40, 23], heads=2, d=64, group=64, seed=1)
