@@ -177,6 +177,30 @@ def test_slots_outside_the_cache_are_not_kept():
     assert torch.equal(a, t)
 
 
+@pytest.mark.parametrize("fmt,dtype", [("int4", torch.bfloat16), ("e4m3", torch.float32)])
+def test_more_sequences_than_a_grid_has_blocks(fmt, dtype):
+  """Written, read and attended to: 70000 sequences of 0 .. 2 tokens, two of a page each."""
+  batch, d = 70000, 64
+  g = torch.Generator(device=DEV).manual_seed(0)
+  cache = kv_cache.make_kv_cache(batch // 2, 16, 1, d, fmt=fmt, device=DEV)
+  lengths = (torch.arange(batch, device=DEV) % 3).int()
+  table = (torch.arange(batch, device=DEV) // 2 % (batch // 2)).int()[:, None]
+  k = torch.randn(batch, 1, 2, d, generator=g, device=DEV).to(torch.bfloat16)
+  k[1::2] = k[::2]  # (the two sequences of a page are one)
+  positions = torch.arange(2, device=DEV)[None].expand(batch, -1).clone()
+  positions[1::2] = -1
+  kv_cache.append(cache, k, k, kv_cache.slots_of(cache, table, positions))
+  got, _ = kv_cache.read(cache, table, lengths, 2, dtype=dtype)
+  want = kv_cache_ref.held(k, fmt, cache.group_size).to(DEV)
+  want[lengths < 2, :, 1] = 0
+  want[lengths < 1] = 0
+  assert torch.equal(got, want.float().to(dtype))
+  o = kv_cache.attend(cache, k[:, :, :1], table, lengths, logits_scale=0.0)
+  mean = torch.where(lengths > 1, 0.5, 1.0)[:, None, None] * want.sum(2)  # a scale of 0: all keys alike
+  # a term is rounded by 2^-12 of a product (P * scale), which is a group's range at most, and the sum by 2^-9 of it
+  assert ((o[:, :, 0].double() - mean).abs() <= 2.0 ** -8 * want.abs().amax((1, 2, 3))[:, None, None]).all()
+
+
 def test_pages_outside_the_cache_read_as_zeros_and_are_not_seen():
   store = Store([70, 64, 100], heads=2, d=64, spare=3)
   table = store.table.clone()

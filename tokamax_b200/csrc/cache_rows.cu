@@ -476,17 +476,26 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_kernel(const __grid_co
   }
 }
 
+constexpr int64_t kMostSequences = 32767;  // of a launch: two blocks each in a grid's last dimension
+
 template <int kFormat, int kTeam>
-static int launch_read(const ReadParams& p, int dtype, int batch, cudaStream_t stream) {
+static int launch_read(ReadParams p, int dtype, int64_t batch, cudaStream_t stream) {
   constexpr int kTokens = kRowThreads / kTeam * kReadEach;
-  const dim3 grid((unsigned)((p.max_len + kTokens - 1) / kTokens), (unsigned)p.kv_heads, (unsigned)batch * 2);
-  if (dtype == SPLASH_BF16)
-    cache_read_kernel<kFormat, kTeam, SPLASH_BF16><<<grid, kRowThreads, 0, stream>>>(p);
-  else if (dtype == SPLASH_F16)
-    cache_read_kernel<kFormat, kTeam, SPLASH_F16><<<grid, kRowThreads, 0, stream>>>(p);
-  else
-    cache_read_kernel<kFormat, kTeam, SPLASH_F32><<<grid, kRowThreads, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
+  for (; batch > 0; batch -= kMostSequences) {
+    const int64_t some = batch < kMostSequences ? batch : kMostSequences;
+    const dim3 grid((unsigned)((p.max_len + kTokens - 1) / kTokens), (unsigned)p.kv_heads, (unsigned)some * 2);
+    if (dtype == SPLASH_BF16)
+      cache_read_kernel<kFormat, kTeam, SPLASH_BF16><<<grid, kRowThreads, 0, stream>>>(p);
+    else if (dtype == SPLASH_F16)
+      cache_read_kernel<kFormat, kTeam, SPLASH_F16><<<grid, kRowThreads, 0, stream>>>(p);
+    else
+      cache_read_kernel<kFormat, kTeam, SPLASH_F32><<<grid, kRowThreads, 0, stream>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return SPLASH_ERR_CUDA;
+    p.page_table += some * p.table_stride;
+    p.lengths += some;
+    for (RowSide& side : p.side) side.data = static_cast<uint8_t*>(side.data) + some * side.stride_b * (dtype == SPLASH_F32 ? 4 : 2);
+  }
+  return SPLASH_OK;
 }
 
 static int cache_read(const SplashCacheReadArgs& a, cudaStream_t stream) {
@@ -499,7 +508,7 @@ static int cache_read(const SplashCacheReadArgs& a, cudaStream_t stream) {
   for (int i = 0; i < 3; ++i)
     if (a.k.size[i] != a.v.size[i]) return SPLASH_ERR_INVALID_ARGUMENT;
   if (a.k.size[1] != c.kv_heads || a.k.size[3] != c.head_dim || a.v.size[3] != c.head_dim_v) return SPLASH_ERR_INVALID_ARGUMENT;
-  if (a.k.size[2] > (1ll << 30) || a.k.size[0] > 32767) return SPLASH_ERR_TOO_LARGE;
+  if (a.k.size[2] > (1ll << 30) || a.k.size[0] > 0x7fffffffll) return SPLASH_ERR_TOO_LARGE;
   ReadParams p{};
   p.side[0] = side_of(a.k, c.k_codes, c.k_scales, c.row_k);
   p.side[1] = side_of(a.v, c.v_codes, c.v_scales, c.row_v);
@@ -515,8 +524,8 @@ static int cache_read(const SplashCacheReadArgs& a, cudaStream_t stream) {
   p.group_shift = log2_of(c.group);
   return with_team(c, [&](auto team) -> int {
     constexpr int kTeam = decltype(team)::value;
-    return c.format == SPLASH_CACHE_INT4 ? launch_read<SPLASH_CACHE_INT4, kTeam>(p, a.k.dtype, (int)a.k.size[0], stream)
-                                         : launch_read<SPLASH_CACHE_E4M3, kTeam>(p, a.k.dtype, (int)a.k.size[0], stream);
+    return c.format == SPLASH_CACHE_INT4 ? launch_read<SPLASH_CACHE_INT4, kTeam>(p, a.k.dtype, a.k.size[0], stream)
+                                         : launch_read<SPLASH_CACHE_E4M3, kTeam>(p, a.k.dtype, a.k.size[0], stream);
   });
 }
 
