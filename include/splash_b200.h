@@ -517,6 +517,8 @@ int splash_cache_read(const SplashCacheReadArgs* args, void* cuda_stream);
  * window >= 0 also j >= position - window, except those on pages outside the cache or that the table does not reach.  q head h reads kv head
  * h / (q_heads / kv_heads).  soft_cap, sinks, logsumexp, max_logits, mask_value: as for splash_fwd.  A row that sees
  * nothing is zeros, its logsumexp and max_logits the mask value (with a sink: the sink's logit).
+ * Products and softmax statistics are of 32 bits; the weights times the scales of V are f16, two of them for f16 outputs: 11 bits (22),
+ * down to 2^-22 of a row's largest.
  * The grid, and with it the order of sums, follows from sizes and lengths alone: results repeat bit for bit. */
 typedef struct SplashCacheAttendArgs {
   SplashKvCache cache;

@@ -582,3 +582,34 @@ def test_arrays_that_were_never_written(fmt, group, d, d_v, q_heads, t, shares):
     assert torch.equal(want, _check_attend(store, q_heads=q_heads, t=t, table=table, window=window))
     for x, y in zip(arrays, before):
       x.copy_(y)
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("q_heads", [2, 16, 20])
+@pytest.mark.parametrize("shares", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_huge_values_of_keys_without_weight(fmt, group, q_heads, shares, dtype):
+  """Values 2^12 .. 2^40 times the others', at keys that no row, or every second row only, gives any weight: the rows' outputs are held
+  as if those keys were not there (what _check_attend allows for is weighted by P)."""
+  d, n = 128, 900
+  g = torch.Generator().manual_seed(5)  # the queries that _check_attend will take
+  q = (torch.randn(1, 1, q_heads, d, generator=g) * 1.5).to(dtype)[0, 0].double()
+  none, half = torch.full((q_heads,), -60.0, dtype=torch.float64), torch.full((q_heads,), -60.0, dtype=torch.float64)
+  half[::2] = 60.0
+  # (position, logits of the rows, size of the values)
+  cases = [[(3, none, 30)], [(450, none, 40), (451, none, 12)], [(899, none, 20)], [(5, none + 60, 30), (700, none + 130, 0)]]
+  if dtype == torch.bfloat16:
+    cases += [[(40, half, 30)], [(640, half, 13), (100, none, 40)]]
+  for case in cases:
+    def keys(k, case=case):
+      for at, logits, _ in case:
+        k[0, 0, at] = (torch.linalg.lstsq(q, logits[:, None] * d ** 0.5).solution[:, 0]).float()
+      return k
+
+    def values(v, case=case):
+      for at, _, size in case:
+        v[0, 0, at] *= 2.0 ** size
+      return v
+
+    store = Store([n], heads=1, d=d, fmt=fmt, group=group, page=64, keys=keys, values=values)
+    _check_attend(store, q_heads=q_heads, dtype=dtype, table=_table_of(store, shares, q_heads, 1))

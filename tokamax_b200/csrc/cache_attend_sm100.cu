@@ -12,7 +12,10 @@
 //     shift; the 2^24 and the 16 are powers of two that go into the row's factor, q and the result.
 //   * q is scaled by a power of two for each row so that its largest entry is near 2^14: bf16 and f16 values lose at most
 //     bits that are 2^-24 of that entry.
-//   * P * scale is scaled by a power of two that follows the largest scale seen (`top`), below 2^14: 11 bits of it are kept.
+//   * P * scale is scaled by a power of two for each row, below 2^14: 11 bits of it are kept, though nothing below 2^-22 of the row's
+//     largest (a row's largest stands at 2^-3 at least, and f16 ends at 2^-25).  The power follows the largest scale seen, or the
+//     row's largest P * scale where that is far less: values of a key without weight, however large, cost the others nothing.  What
+//     remains: where the scales of one row's groups of channels are 2^11 apart and more, the smaller group keeps fewer bits than 11.
 //     That is enough for outputs of bf16 (1.73e-3 of the norm from 64 bits where rounding the output alone costs 1.64e-3).  For
 //     f16 what is left of it goes through a second product, and int4's codes are taken less 8, with 8 scale_g in the zeros: sums
 //     of codes, all positive, are far larger than what comes out of long and even rows, and their own rounding in 32 bits shows.
@@ -219,8 +222,9 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[kCount], const uint32_t
 
 constexpr float kNoMaximum = -1.0e30f;  // of a row that has seen no key yet: finite, so that differences are
 constexpr float kSlack = 8.f;           // how far (in units of log2) logits may pass the maximum that P is taken against
-constexpr int kUnitLog2 = 5;            // P * scale is below 2^(kSlack + 1 + kUnitLog2) = 2^14
+constexpr float kUnitLog2 = 5.f;        // P * scale is below 2^(kSlack + 1 + kUnitLog2) = 2^14
 constexpr uint32_t kLeastTop = 87u << 23;  // 2^-40
+constexpr float kLeastTopLog2 = -40.f, kSpare = 8.f, kRoom = 6.f;
 
 // ------------------------------------------------------------------------------------------
 // shares
@@ -561,9 +565,11 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     float m[kN][2], base[kN][2], l[kN][2], factor[kN][2], highest[kN][2];  // highest: of this lane's logits
     float o[Shape::kChunksV][kSteps][kN][4] = {};
     float zeros[kGroupsV][kN][2] = {};
-    // The largest scale of V seen, as bits, rounded down to a power of two (2^-40 at least).  P is taken in units of `unit` =
-    // 2^kUnitLog2 / top throughout: in l, the zeros' sums and O.
-    uint32_t top = kLeastTop;
+    // Each row's P is taken in units of a power of two throughout (in l, the zeros' sums and O; `base` has it), 2^kUnitLog2 over the
+    // row's top: the largest scale of V seen, or 2^kRoom times the largest P * scale of the row where that is less by 2^kSpare,
+    // which a key of huge values and no weight would otherwise leave few bits of.  As bits, rounded down to powers of two (2^-40 at
+    // least): the least of the rows' tops, and the largest scale seen.
+    uint32_t top = kLeastTop, largest_seen = kLeastTop;
 #pragma unroll
     for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
@@ -753,7 +759,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
           highest[nb][j] = fmaxf(highest[nb][j], most[nb][j]);
           grows = grows || most[nb][j] > m[nb][j] + kSlack;
         }
-      // ---- and the power of two that P * scale is taken in: lowered where a scale passes `top` by a factor of two ----
+      // ---- and the power of two that P * scale is taken in: seen to where a scale passes `top` by a factor of two ----
       uint32_t own_top[(kUnit + 31) / 32][kGroupsV];  // a lane a token
 #pragma unroll
       for (int i = 0; i < kUnit; i += 32) {
@@ -770,29 +776,55 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         for (int group = 0; group < kGroupsV; ++group) grows = grows || own_top[i / 32][group] >= top + (1u << 23);
       }
       if (__any_sync(~0u, grows)) {
+        auto largest_of = [](const uint32_t (&scales)[kGroupsV]) {  // of a token, as bits (not NaN)
+          uint32_t x = 0;
+#pragma unroll
+          for (int group = 0; group < kGroupsV; ++group) x = max(x, scales[group] < 0x7f800000u ? scales[group] : 0u);
+          return x;
+        };
         uint32_t largest = 0;
 #pragma unroll
-        for (int i = 0; i < kUnit; i += 32)
+        for (int i = 0; i < kUnit; i += 32) {
+          const uint32_t own = largest_of(own_top[i / 32]);
+          largest = max(largest, own);
+        }
+        largest_seen = max(__reduce_max_sync(~0u, largest) & 0x7f800000u, largest_seen);
+        const float largest_log2 = (float)((int)(largest_seen >> 23) - 127);
+        float scale_log2[kTiles][2];  // of the tokens of s, rounded down
 #pragma unroll
-          for (int group = 0; group < kGroupsV; ++group) {
-            const uint32_t x = own_top[i / 32][group];
-            largest = max(largest, x < 0x7f800000u ? x : 0u);  // (not NaN)
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int token = i * 16 + half * 8 + g;
+            uint32_t own[kGroupsV];
+            if constexpr (kInt4)
+              load_words<kGroupsV>(own, reinterpret_cast<const uint32_t*>(scales_v) + token * kGroupsV);
+            else
+              own[0] = (uint32_t)reinterpret_cast<const uint16_t*>(scales_v)[token] << 16;
+            scale_log2[i][half] = (float)((int)(largest_of(own) >> 23) - 127);
           }
-        largest = max(__reduce_max_sync(~0u, largest) & 0x7f800000u, top);
-        const float rise = __uint_as_float((uint32_t)max(127 - (int)((largest - top) >> 23), 0) << 23);
-        top = largest;
-        const float unit_log2 = (float)(kUnitLog2 + 127 - (int)(top >> 23));
+        float least_log2 = largest_log2;
 #pragma unroll
         for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float x = fmaxf(m[nb][j], most[nb][j]);
-            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
-            const float alpha = ex2(m[nb][j] - x) * rise;
+            float x = fmaxf(m[nb][j], most[nb][j]), w = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) w = fmaxf(w, fmaf(s[i][nb][half * 2 + j], factor[nb][j], scale_log2[i][half]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+              x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+              w = fmaxf(w, __shfl_xor_sync(~0u, w, d));
+            }
+            // of these keys, and of those before (whose unit `base` holds)
+            float top_log2 = max3(w - x, base[nb][j] + kUnitLog2 - x, kLeastTopLog2);
+            top_log2 = largest_log2 - top_log2 > kSpare ? top_log2 + kRoom : largest_log2;
+            if (x > kNoMaximum) least_log2 = fminf(least_log2, top_log2);
+            const float taken = x - kUnitLog2 + top_log2, alpha = ex2(base[nb][j] - taken);
             m[nb][j] = x;
-            base[nb][j] = x - unit_log2;
+            base[nb][j] = taken;
             l[nb][j] *= alpha;
 #pragma unroll
             for (int c = 0; c < Shape::kChunksV; ++c)
@@ -804,6 +836,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
 #pragma unroll
             for (int c = 0; c < kGroupsV; ++c) zeros[c][nb][j] *= alpha;
           }
+        top = (uint32_t)(__reduce_min_sync(~0u, (int)floorf(least_log2)) + 127) << 23;
       }
 #pragma unroll
       for (int nb = 0; nb < kN; ++nb)
