@@ -613,3 +613,89 @@ def test_huge_values_of_keys_without_weight(fmt, group, q_heads, shares, dtype):
 
     store = Store([n], heads=1, d=d, fmt=fmt, group=group, page=64, keys=keys, values=values)
     _check_attend(store, q_heads=q_heads, dtype=dtype, table=_table_of(store, shares, q_heads, 1))
+
+
+def test_streams_and_graphs_of_shares():
+  """As test_streams_and_graphs, where items are cut into shares: two launches and a workspace."""
+  store = Store([5000, 3100, 40], d=128, group=64, page=64)
+  assert _workspace_bytes(store, 4, 1, store.table) > 0
+  q = torch.randn(3, 4, 1, 128, device=DEV, dtype=torch.bfloat16)
+  call = lambda: kv_cache.attend(store.cache, q, store.table, store.lengths, logits_scale=0.1, save_residuals=True)  # noqa: E731
+  same = lambda a, b: torch.equal(a[0], b[0]) and all(torch.equal(a[1][x], b[1][x]) for x in a[1])  # noqa: E731
+  want = call()
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    outs = [call() for _ in range(20)]
+  mine = [call() for _ in range(20)]  # two streams at a time: each call has a workspace of its own
+  side.synchronize()
+  assert all(same(o, want) for o in outs + mine)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    kv_cache.append(store.cache, q[:, :2], q[:, :2], store.slots[:, :1])
+    first = call()
+    second = call()  # (in the place of the first one's workspace, maybe)
+  for lengths in ([17, 0, 40], [5000, 1, 39], [0, 0, 0], [4999, 3100, 40]):
+    store.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))  # lengths change between replays, and with them the shares
+    graph.replay()
+    kv_cache.append(store.cache, q[:, :2], q[:, :2], store.slots[:, :1])
+    want = call()
+    assert same(first, want) and same(second, want)
+    for b, n in enumerate(lengths):
+      assert bool(want[0][b].any()) == (n > 0)
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("d,d_v", [(64, 64), (96, 96), (192, 128), (256, 256)])
+@pytest.mark.parametrize("q_heads,t", [(2, 1), (16, 1), (10, 4)])
+def test_f16_outputs_of_shares(fmt, group, d, d_v, q_heads, t):
+  try:
+    store = Store([33, 2700, 0, 1], d=d, d_v=d_v, fmt=fmt, group=group, page=64, dtype=torch.float16)
+  except ValueError:
+    assert group in (64, 128)
+    return
+  _check_attend(store, q_heads=q_heads, t=t, dtype=torch.float16, table=_table_of(store, True, q_heads, t))
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+def test_pages_and_lengths_outside_of_shares(fmt, group):
+  """Pages that are none in the middle of long sequences, lengths beyond the table and below zero."""
+  store = Store([3000, 640, 1000], d=128, fmt=fmt, group=group, page=16, spare=3)
+  table = _table_of(store, True, 4, 3)
+  seen = torch.ones(3, 3000, dtype=torch.bool)
+  for b, pages in enumerate((range(3, 60), (0, 5, 39), range(0, 63))):
+    for i, at in enumerate(pages):
+      table[b, at] = (-1, store.cache.n_pages, 2 ** 31 - 1, -5)[i % 4]
+      seen[b, at * 16:at * 16 + 16] = False
+  seen[1, 640:], seen[2, 1000:] = True, True  # (behind the end: not looked at)
+  _check_attend(store, q_heads=4, t=3, seen=seen, table=table)
+  q = torch.randn(3, 4, 1, 128, device=DEV, dtype=torch.bfloat16)
+  call = lambda lengths, table: kv_cache.attend(store.cache, q, table, lengths, logits_scale=0.1)  # noqa: E731
+  short = store.table[:, :128].contiguous()  # 2048 tokens: the first sequence is longer
+  assert _workspace_bytes(store, 4, 1, short) > 0
+  lengths = torch.tensor([3000, -7, 2 ** 31 - 1], dtype=torch.int32, device=DEV)
+  o = call(lengths, short)
+  full = call(torch.tensor([2048, 0, 2048], dtype=torch.int32, device=DEV), short)  # (the same shares)
+  assert torch.equal(o, full) and not o[1].any() and o[0].any() and o[2].any()
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+def test_what_is_not_seen_has_no_part_in_shares(fmt, group):
+  """As test_what_lies_in_places_that_are_not_seen, with NaN in the middle of what a window leaves out of long sequences."""
+  store = Store([4100, 3000], d=128, fmt=fmt, group=group, page=64)
+  table = _table_of(store, True, 4, 2, 2500)
+  call = lambda: _check_attend(store, q_heads=4, t=2, window=2500, table=table)  # noqa: E731
+  clean = call()
+  bad = torch.full((1, 2, 1, 128), math.nan, device=DEV)
+  for at in (5, 1000, 1596):  # query 0 stands at 4098 and sees 1598 ..
+    kv_cache.append(store.cache, bad, bad, store.slots[:1, at:at + 1])
+  assert torch.equal(clean, call())
+  kv_cache.append(store.cache, bad, bad, store.slots[:1, 1598:1599])  # seen by query 0 alone
+  o = _attend_of(store, 4, 2, 2500, table)
+  assert o[0, :, 0].isnan().all() and not o[0, :, 1].isnan().any() and torch.equal(o[1], clean[1])
+
+
+def _attend_of(store, q_heads, t, window, table):
+  g = torch.Generator().manual_seed(5)
+  q = (torch.randn(len(store.lengths_list), t, q_heads, store.d, generator=g) * 1.5).to(torch.bfloat16).transpose(1, 2)
+  return kv_cache.attend(store.cache, q.to(DEV), table, store.lengths, logits_scale=store.d ** -0.5, local_window_size=window)
