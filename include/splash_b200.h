@@ -518,7 +518,7 @@ int splash_cache_read(const SplashCacheReadArgs* args, void* cuda_stream);
  * h / (q_heads / kv_heads).  soft_cap, sinks, logsumexp, max_logits, mask_value: as for splash_fwd.  A row that sees
  * nothing is zeros, its logsumexp and max_logits the mask value (with a sink: the sink's logit).
  * Products and softmax statistics are of 32 bits; the weights times the scales of V are f16, two of them for f16 outputs: 11 bits (22),
- * down to 2^-22 of a row's largest.
+ * down to 2^-22 of a row's largest.  Logits are of up to 2^26 in size (32 bits hold those to 4): beyond, weights may overflow.
  * The grid, and with it the order of sums, follows from sizes and lengths alone: results repeat bit for bit. */
 typedef struct SplashCacheAttendArgs {
   SplashKvCache cache;

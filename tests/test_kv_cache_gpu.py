@@ -584,6 +584,35 @@ def test_arrays_that_were_never_written(fmt, group, d, d_v, q_heads, t, shares):
       x.copy_(y)
 
 
+@pytest.mark.parametrize("shares", [False, True])
+@pytest.mark.parametrize("size", [0, 10, 17, 18, 19, 20])
+def test_logits_that_32_bits_hold_to_eight(size, shares):
+  """Logits of 63 * 2^size that rise every 64 keys (in units of log2; at 2^26 by 8 now and then).  All keys' values are the same, and so
+  is o, whatever the weights that are left."""
+  n, d = 4096, 64
+  c, q0 = 2.0 ** (size // 2), 2.0 ** (size - size // 2)
+  q = torch.full((1, 2, 1, d), q0)
+  q[..., 63] = 2.0 ** -4
+  for gain in (1.0, 2.0, 4.0, 8.0, 16.0):
+    for step in (0.75, 4.0, 7.0):
+      def keys(k, step=step):
+        k[0, 0] = c
+        k[0, 0, :, 63] += torch.arange(n) // 64 * step * math.log(2.0) / q[0, 0, 0, 63]
+        return k
+
+      def values(v, gain=gain):
+        v[0, 0] = v[0, 0, :1] * gain
+        return v
+
+      store = Store([n], heads=1, d=d, group=32, page=64, dtype=torch.float32, keys=keys, values=values)
+      window = None if shares else 1000  # (an item is one CTA's where windows are short)
+      o = kv_cache.attend(store.cache, q.to(DEV).to(torch.bfloat16), _table_of(store, shares, 2, 1, window), store.lengths, logits_scale=1.0,
+                          local_window_size=window)
+      want = store.held(0)[1][:, :1]
+      # P * scale and the output are rounded; products are up to the group's range
+      assert ((o[0].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -11 * (want.amax() - want.amin())).all(), (gain, step)
+
+
 @pytest.mark.parametrize("fmt,group", FORMATS)
 @pytest.mark.parametrize("q_heads", [2, 16, 20])
 @pytest.mark.parametrize("shares", [False, True])

@@ -562,7 +562,8 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     __syncthreads();
 
     // ---- this lane's columns: rows nb * 8 + t4 * 2 and the next ----
-    float m[kN][2], base[kN][2], l[kN][2], factor[kN][2], highest[kN][2];  // highest: of this lane's logits
+    // highest: of this lane's logits; limit: what they may reach before the maximum is raised
+    float limit[kN][2], base[kN][2], l[kN][2], factor[kN][2], highest[kN][2];
     float o[Shape::kChunksV][kSteps][kN][4] = {};
     float zeros[kGroupsV][kN][2] = {};
     // Each row's P is taken in units of a power of two throughout (in l, the zeros' sums and O; `base` has it), 2^kUnitLog2 over the
@@ -574,7 +575,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        m[nb][j] = base[nb][j] = highest[nb][j] = kNoMaximum;
+        limit[nb][j] = base[nb][j] = highest[nb][j] = kNoMaximum;
         l[nb][j] = 0.f;
         factor[nb][j] = p.soft_cap > 0.f ? 1.f : factors[nb * 8 + t4 * 2 + j];
       }
@@ -745,9 +746,8 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         __syncwarp();
       }
 
-      // ---- the maximum that P is taken against: raised where a logit passes it by more than kSlack ----
+      // ---- the maximum that P is taken against: raised where a logit passes its limit, kSlack above it ----
       bool grows = false;
-      float most[kN][2];
 #pragma unroll
       for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
@@ -755,9 +755,9 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
           float x = fmaxf(s[0][nb][j], s[0][nb][2 + j]);
 #pragma unroll
           for (int i = 1; i < kTiles; ++i) x = max3(x, s[i][nb][j], s[i][nb][2 + j]);
-          most[nb][j] = x * factor[nb][j];
-          highest[nb][j] = fmaxf(highest[nb][j], most[nb][j]);
-          grows = grows || most[nb][j] > m[nb][j] + kSlack;
+          const float most = x * factor[nb][j];
+          highest[nb][j] = fmaxf(highest[nb][j], most);
+          grows = grows || most > limit[nb][j];
         }
       // ---- and the power of two that P * scale is taken in: seen to where a scale passes `top` by a factor of two ----
       uint32_t own_top[(kUnit + 31) / 32][kGroupsV];  // a lane a token
@@ -808,7 +808,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float x = fmaxf(m[nb][j], most[nb][j]), w = -INFINITY;
+            float x = highest[nb][j], w = -INFINITY;
 #pragma unroll
             for (int i = 0; i < kTiles; ++i)
 #pragma unroll
@@ -823,7 +823,10 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
             top_log2 = largest_log2 - top_log2 > kSpare ? top_log2 + kRoom : largest_log2;
             if (x > kNoMaximum) least_log2 = fminf(least_log2, top_log2);
             const float taken = x - kUnitLog2 + top_log2, alpha = ex2(base[nb][j] - taken);
-            m[nb][j] = x;
+            // Logits of 2^20 and more are 2^-3 apart and more, from 2^26 on as far as kSlack: no room between one and the next.  (`base`
+            // is rounded as they are, and with it what P is taken in: up to some 2^27 f16 has room for that.  P from logits rounded
+            // as the maximum is, which goes further, costs 1 to 3 %.)
+            limit[nb][j] = fabsf(x) < 0x1p20f ? x + kSlack : x;
             base[nb][j] = taken;
             l[nb][j] *= alpha;
 #pragma unroll
