@@ -69,7 +69,7 @@ struct AttendParams {
   int64_t q_stride_b, q_stride_h, q_stride_s, o_stride_b, o_stride_h, o_stride_s, table_stride, n_pages;
   float scale, soft_cap, mask_value;
   int32_t batch, q_heads, kv_heads, heads_per_kv, q_len, row_tiles, n_table, page_size, page_shift, dtype;
-  int32_t head_dim, head_dim_v, window, item_cost, min_share;  // item_cost, min_share: in units
+  int32_t head_dim, head_dim_v, window, item_cost;  // item_cost: in units
   bool whole;  // every item is one CTA's
 };
 
@@ -129,6 +129,7 @@ template <int kFormat_, int kK_, int kV_, int kG_, int kN_>
 struct AttendShape {
   static constexpr int kFormat = kFormat_, kK = kK_, kV = kV_, kN = kN_;
   static constexpr bool kInt4 = kFormat == SPLASH_CACHE_INT4;
+  static_assert(kN >= 1 && kN <= 3);
   static constexpr int kRows = 8 * kN;
   static constexpr int kRowK = cache_row_bytes(kFormat, kK), kRowV = cache_row_bytes(kFormat, kV);
   // Tokens of a unit.  A warp has a unit in flight while it works on another: about 4 KB (a quarter more or less with what 16
@@ -136,7 +137,7 @@ struct AttendShape {
   // a unit may be 8 KB (e4m3, head dim 128, 24 rows, 16 sequences of 1000 .. 8192 tokens: 63 -> 60 us), unless the logits
   // of 32 tokens do not fit beside the sums (int4, whose scales take registers too).
   static constexpr int kRowBytes = kRowK + kRowV;
-  static constexpr int kUnit = kN > 2   ? (kInt4 ? (kRowBytes <= 64 && kN == 3 ? 32 : 16) : kRowBytes <= 256 ? 32 : 16)
+  static constexpr int kUnit = kN > 2   ? (kInt4 ? (kRowBytes <= 64 ? 32 : 16) : kRowBytes <= 256 ? 32 : 16)
                                : kN == 2 ? (kRowBytes <= (kInt4 ? 128 : 256) ? 32 : 16)
                                          : (kRowBytes <= 64 ? 64 : kRowBytes <= 128 ? 32 : 16);
   static constexpr int kTiles = kUnit / 16;
@@ -259,9 +260,9 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return (a | b) >> 32 == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
-__device__ __forceinline__ int64_t share_of(int64_t total, int ctas, int min_share) {
+__device__ __forceinline__ int64_t share_of(int64_t total, int ctas) {  // a unit for each warp at least
   const int64_t share = quotient(total + ctas - 1, ctas);
-  return share > min_share ? share : min_share;
+  return share > kWarps ? share : kWarps;
 }
 
 struct Start {  // where a CTA's share begins
@@ -305,7 +306,7 @@ __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
       if (look == 1) {
         if (once) {
           total = carry;
-          share = share_of(total, gridDim.x, p.min_share);
+          share = share_of(total, gridDim.x);
           at = blockIdx.x * share;
         }
         if (b < p.batch) {
@@ -319,7 +320,7 @@ __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
     }
     if (look == 0) {
       total = carry;
-      share = share_of(total, gridDim.x, p.min_share);
+      share = share_of(total, gridDim.x);
       at = blockIdx.x * share;
     }
   }
@@ -1053,7 +1054,7 @@ __global__ void __launch_bounds__(kJoinThreads, kAhead > 2 ? 2 : 4) cache_attend
   __shared__ float stats[2][kMostSlices];
   grid_dependency_wait();
   const int lot = threadIdx.x / kEach, d = threadIdx.x % kEach * 8;
-  const int64_t share = share_of(p.starts[p.batch], ctas, p.min_share);
+  const int64_t share = share_of(p.starts[p.batch], ctas);
   for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
     const int64_t before = p.starts[b], cost = quotient(p.starts[b + 1] - before, p.kv_heads * p.row_tiles);
     const int64_t first = before + blockIdx.x * cost + p.item_cost;  // unit of this item
@@ -1313,7 +1314,6 @@ static int cache_attend(const SplashCacheAttendArgs& a, cudaStream_t stream) {
     }
     own.row_tiles = (p.q_len * p.heads_per_kv + Shape::kRows - 1) / Shape::kRows;
     own.item_cost = item_tokens(Shape::kN) / Shape::kUnit;
-    own.min_share = kWarps;
     return launch<Shape>(own, resident<Shape>(), stream);
   });
 }

@@ -33,19 +33,6 @@ __device__ __forceinline__ void unpack16(int dtype, uint32_t w, float& lo, float
   }
 }
 
-// Eight values of one of the three element types from 16-byte aligned memory, and back.
-__device__ __forceinline__ void load8(const void* base, int dtype, int64_t at, float (&x)[8]) {
-  if (dtype == SPLASH_F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
-    const float4 a = __ldg(p), b = __ldg(p + 1);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    return;
-  }
-  const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
-  const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) unpack16(dtype, words[i], x[2 * i], x[2 * i + 1]);
-}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -53,6 +40,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ uint32_t pack16(int dtype, float lo, float hi) {
   return dtype == SPLASH_BF16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
 }
+// Eight values of one of the three element types to 16-byte aligned memory.
 __device__ __forceinline__ void store8(void* base, int dtype, int64_t at, const float (&x)[8]) {
   if (dtype == SPLASH_F32) {
     float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + at);
