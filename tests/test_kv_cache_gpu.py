@@ -724,6 +724,26 @@ def test_what_is_not_seen_has_no_part_in_shares(fmt, group):
   assert o[0, :, 0].isnan().all() and not o[0, :, 1].isnan().any() and torch.equal(o[1], clean[1])
 
 
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,batch", [(131072, 300), (1900, 6000)])
+def test_errors_do_not_grow_with_the_call(fmt, group, dtype, n, batch):
+  """Even rows of many keys, whose outputs are far smaller than the values, in a call so large that a warp adds up thousands of them.
+  Rounding P * scale is 0.35e-3 of an output's norm (int4, bf16; codes are 2.7 times the deviation of a group's values), a sum
+  of products that loses 2^-25 at each of 64 steps (1024 tokens) some 5e-6 of the values, 0.5e-3 of outputs over 131072 keys: beside the
+  1.65e-3 of rounding the output itself (f16: an eighth of all three), half as much again is allowed."""
+  store = Store([n], heads=1, d=128, fmt=fmt, group=group, page=256, values=lambda v: v / v.norm(dim=-1, keepdim=True) * 128 ** 0.5)
+  g = torch.Generator().manual_seed(3)
+  q = torch.randn(1, 4, 1, 128, generator=g).to(dtype)
+  k, v = store.held(0)
+  p = torch.softmax(k[0] @ q[0, :, 0].double().T * 128 ** -0.5, 0)
+  want = p.T @ v[0]
+  o = kv_cache.attend(store.cache, q.to(DEV).expand(batch, -1, -1, -1), store.table.expand(batch, -1), store.lengths.repeat(batch),
+                      logits_scale=128 ** -0.5)
+  error = (o[:, :, 0].cpu().double() - want).norm(dim=(1, 2)).max()
+  assert error <= 1.5 * (want.to(dtype).double() - want).norm(), float(error / want.norm())
+
+
 def _attend_of(store, q_heads, t, window, table):
   g = torch.Generator().manual_seed(5)
   q = (torch.randn(len(store.lengths_list), t, q_heads, store.d, generator=g) * 1.5).to(torch.bfloat16).transpose(1, 2)

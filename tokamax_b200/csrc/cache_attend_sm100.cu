@@ -22,6 +22,7 @@
 //     f16, int4, 5111 and 60000 keys: 6.0e-4 without either, 2.4e-4 and 4.7e-4 with the second product, 2.0e-4 and 2.2e-4
 //     with both, where rounding the output costs 2.0e-4 (e4m3: 2.8e-4, 2.1e-4 with the second product); 144, 160 and
 //     172 us (32 sequences of 8192 .. 32768, 32 / 8 heads of 128).
+//   * sums of int4 codes are levelled every kLevelTokens tokens of a warp, see there: their error does not grow with the call.
 // Softmax statistics are of one pass over the keys, with a running maximum and sum for each row.
 //
 // Split: the keys of all (sequence, kv head, row tile) items, one after the other in units of kUnit tokens, are cut into
@@ -224,6 +225,10 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[kCount], const uint32_t
 constexpr float kNoMaximum = -1.0e30f;  // of a row that has seen no key yet: finite, so that differences are
 constexpr float kSlack = 8.f;           // how far (in units of log2) logits may pass the maximum that P is taken against
 constexpr float kUnitLog2 = 5.f;        // P * scale is below 2^(kSlack + 1 + kUnitLog2) = 2^14
+// Tokens of a warp after which the sums of int4 codes are levelled (bf16, 32 / 8 heads of 128, us with 512, 768, 1024 and never: 32 x
+// 8192 .. 32768 tokens 151.7, 150.7, 150.0, 147.5; one of 131072, 41.6, 41.7, 41.4, 41.4; relative error of outputs over even rows of
+// 131072 and 2^20 tokens, in calls of 1.3e8 and 1e8 of them: 512 1.8e-3 and 2.8e-3, 1024 1.9e-3 and 3.4e-3, never 4.5e-2 and 0.16).
+constexpr int kLevelTokens = 1024;
 constexpr uint32_t kLeastTop = 87u << 23;  // 2^-40
 constexpr float kLeastTopLog2 = -40.f, kSpare = 8.f, kRoom = 6.f;
 
@@ -748,7 +753,9 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       }
 
       // ---- the maximum that P is taken against: raised where a logit passes its limit, kSlack above it ----
-      bool grows = false;
+      constexpr int kLevel = kLevelTokens / kUnit;
+      const bool level = kInt4 && turn % kLevel == kLevel - 1;
+      bool grows = level;
 #pragma unroll
       for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
@@ -840,6 +847,34 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
 #pragma unroll
             for (int c = 0; c < kGroupsV; ++c) zeros[c][nb][j] *= alpha;
           }
+        // The mean of a group's sums goes to its zeros from time to time: products of codes are positive, and a sum that MMAs add
+        // up loses the bits that it cuts off at every step.
+        if (level) {
+#pragma unroll
+          for (int group = 0; group < kGroupsV; ++group)
+#pragma unroll
+            for (int nb = 0; nb < kN; ++nb)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                constexpr int kPer = Shape::kPerGroupV;
+                float mean = 0.f;
+#pragma unroll
+                for (int c = group * kPer; c < (group + 1) * kPer; ++c)
+#pragma unroll
+                  for (int k = 0; k < kSteps; ++k) mean += fmaf(o[c][k][nb][2 + j], 0.0625f, o[c][k][nb][j]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) mean += __shfl_xor_sync(~0u, mean, d);
+                mean *= 1.f / (kPer * 32);
+#pragma unroll
+                for (int c = group * kPer; c < (group + 1) * kPer; ++c)
+#pragma unroll
+                  for (int k = 0; k < kSteps; ++k) {
+                    o[c][k][nb][j] -= mean;
+                    o[c][k][nb][2 + j] = fmaf(mean, -16.f, o[c][k][nb][2 + j]);
+                  }
+                zeros[group][nb][j] = fmaf(mean, 0x1p21f, zeros[group][nb][j]);  // (2^24, for eight lanes together)
+              }
+        }
         top = (uint32_t)(__reduce_min_sync(~0u, (int)floorf(least_log2)) + 127) << 23;
       }
 #pragma unroll
