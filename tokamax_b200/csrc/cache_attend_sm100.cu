@@ -20,8 +20,8 @@
 //     f16 what is left of it goes through a second product, and int4's codes are taken less 8, with 8 scale_g in the zeros: sums
 //     of codes, all positive, are far larger than what comes out of long and even rows, and their own rounding in 32 bits shows.
 //     f16, int4, 5111 and 60000 keys: 6.0e-4 without either, 2.4e-4 and 4.7e-4 with the second product, 2.0e-4 and 2.2e-4
-//     with both, where rounding the output costs 2.0e-4 (e4m3: 2.8e-4, 2.1e-4 with the second product); 144, 160 and
-//     172 us (32 sequences of 8192 .. 32768, 32 / 8 heads of 128).
+//     with both, where rounding the output costs 2.0e-4 (e4m3: 2.8e-4, 2.1e-4 with the second product).  It costs a
+//     sixth: 32 sequences of 8192 .. 32768, 32 / 8 heads of 128, bf16 150 us, f16 176.
 //   * sums of int4 codes are levelled every kLevelTokens tokens of a warp, see there: their error does not grow with the call.
 // Softmax statistics are of one pass over the keys, with a running maximum and sum for each row.
 //
@@ -33,14 +33,19 @@
 // from sums in the workspace, in the order of the CTAs: results do not depend on who comes first.  Where sequences cannot be long
 // every item is one CTA's, and there is one launch.
 //
-// Bound by: HBM asks for 64 + 8 bytes a token, head and side (int4, head dim 128, groups of 64).  At 6.5 TB/s an SM gets 46 codes
-// a cycle, so that a warp may spend 2.8 instructions on 32 of them; the kernel spends 2.1 (some 525 on a unit of 32 tokens, keys and
-// values, eight rows; 160 of them unpack), and issues 2.3 to 2.5 a cycle of the 4 that an SM could.  Instructions are what bounds
-// it: without the products the copies alone take 121 us of the first case.  Measured, 32 / 8 heads of 128, int4: 32 sequences of
-// 8192 .. 32768 144 us, 5.2 TB/s of the 6.5 that a plain copy reaches; one of 131072 41 us, 64 of 200 .. 4096 47 us, 3.7 and 3.8 TB/s.  About
-// 9 us of each call are the two launches and the chains of loads at their beginnings (lengths, pages, codes; parts).  e4m3 rows are
-// unpacked by conversions and ask for twice the bytes: 48 sequences of 0 .. 13025 113 us, 6.0 TB/s.
-// Rows of more than one block of eight spend 190 instructions more a block on a unit, and leave room for fewer warps.
+// Bound by: no one thing.  HBM asks for 64 + 8 bytes a token, head and side (int4, head dim 128, groups of 64), 46 codes a cycle and SM at
+// 6.5 TB/s; a warp spends some 545 instructions on a unit of 32 tokens (keys and values, eight rows; 160 of them unpack), 2.2 for
+// 32 codes, and an SM issues 2.2 a cycle of the 4 that it could, its 14 warps waiting for their own last instruction most often.  The
+// copies alone, with the products left out, take most of the time as well (us of a call, whole : copies alone; 32 / 8 heads of 128,
+// int4): 32 sequences of 8192 .. 32768 149.9 : 119.9, one of 131072 41.4 : 35.0, 64 of 200 .. 4096 48.8 : 38.0: copies, first loads
+// and launches bound a call as much as its instructions do, and warps that wait at one of them do not get on with the other.
+// Throughput 4.9, 3.6 and 3.4 TB/s of the 6.5 that a plain copy reaches.  About 9 us of each call are the two launches and the chains of
+// loads at their beginnings (lengths, pages, codes; parts).  e4m3 rows are unpacked by conversions and ask for twice the bytes: 48
+// sequences of 0 .. 13025 109 us, 6.2 TB/s.
+// Rows of more than one block of eight spend 190 instructions more a block on a unit, and leave room for fewer warps.  Registers: the
+// element type is a value at run time, so a kernel holds four forms of the product with P (masked or not, f16's second product or
+// not); 32 of the 50 kernels spill, up to 204 bytes a thread (most where groups of 32 keep many scales), in the forms that are timed
+// here 0 (8 rows, head dim 128, groups of 64) to 28.
 #include <atomic>
 
 #include "cache_common.cuh"
@@ -236,9 +241,15 @@ constexpr float kLeastTopLog2 = -40.f, kSpare = 8.f, kRoom = 6.f;
 // shares
 // ------------------------------------------------------------------------------------------
 // What a CTA spends on an item beside its units, in tokens: shares are equal in the sum of both.  (Looking up the item, q as
-// fragments, the first keys' latency, the warps' sums together: some thousand cycles, more with more rows.  us with 160, 240, 320 and
-// 480; eight rows: 64 x 200 .. 4096 tokens 51.4, 48.7, 47.2, 48.1, 32 x 8192 .. 32768 153.2, 153.1, 153.0, 156.3; 24 rows, e4m3: 16 x 1000
-// .. 8192 54.9, 53.4, 51.9, 49.2, and with 640 49.3.)
+// fragments, the first keys' latency, the warps' sums together: some thousand cycles, more with more rows.)  us with 160, 320, 480, 640 and
+// 960 tokens, int4 | e4m3:
+//   8 rows of 128    64 x 200 .. 4096, 8 kv heads      53.6 49.6 50.5 50.6 52.8 | 60.4 60.1 61.0 62.1 65.2
+//   8 rows of 256    24 x 300 .. 9000, 4               37.9 37.9 38.3 39.3 40.4 | 45.6 46.2 46.0 45.9 45.8
+//   16 rows of 64    24 x 300 .. 8000, 4               29.2 27.3 27.1 27.1 27.8 | 29.1 27.3 27.0 27.0 28.1
+//   16 rows of 128   32 x 200 .. 6000, 4               37.5 34.7 34.2 34.2 36.3 | 39.4 36.1 34.9 35.0 36.1
+//   16 of 192 / 128  24 x 300 .. 9000, 4               43.8 41.4 42.0 42.8 44.4 | 46.5 43.4 43.4 44.2 45.6
+//   16 rows of 256   32 x 8000 .. 30000, 2             124.2 121.2 120.5 121.1 122.4 | 119.9 117.1 118.4 119.4 119.9
+//   20 rows of 128   16 x 1000 .. 8192, 8              64.6 59.9 59.9 60.1 62.2 | 54.9 52.6 49.7 49.8 51.6
 __host__ __device__ constexpr int item_tokens(int blocks) { return blocks == 1 ? 320 : 480; }
 // Every item is one CTA's where queries see at most kWholeTokens, or twice as many and there are kWholeItems .. kMostWholeItems - 1
 // items (us, whole : shares and a second launch; 1024 tokens, 8 items 10.5 : 11.5, 256 items 14.6 : 18.8, 1024 items 35.0 : 37.9;
