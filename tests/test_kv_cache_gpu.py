@@ -724,6 +724,21 @@ def test_what_is_not_seen_has_no_part_in_shares(fmt, group):
   assert o[0, :, 0].isnan().all() and not o[0, :, 1].isnan().any() and torch.equal(o[1], clean[1])
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("q_heads", [2, 16, 20])
+def test_f16_outputs_of_values_that_cancel(group, q_heads):
+  """One key has nearly all the weight, and its values are next to nothing beside a group's zero and products, which cancel."""
+  def values(v):
+    v[..., ::3] = v[..., ::3] * 1e-3
+    return v
+
+  for seed in range(6):
+    for lengths in ([1, 2, 3, 22], [40, 7, 300, 5]):
+      store = Store(lengths, d=128, fmt="int4", group=group, dtype=torch.float16, seed=seed, values=values)
+      _check_attend(store, q_heads=q_heads, dtype=torch.float16, q_scale=4.0, seed=seed)
+      _check_attend(store, q_heads=q_heads, t=2, dtype=torch.float16, q_scale=12.0, seed=seed)
+
+
 @pytest.mark.parametrize("fmt,group", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n,batch", [(131072, 300), (1900, 6000)])

@@ -21,7 +21,8 @@
 //     of codes, all positive, are far larger than what comes out of long and even rows, and their own rounding in 32 bits shows.
 //     f16, int4, 5111 and 60000 keys: 6.0e-4 without either, 2.4e-4 and 4.7e-4 with the second product, 2.0e-4 and 2.2e-4
 //     with both, where rounding the output costs 2.0e-4 (e4m3: 2.8e-4, 2.1e-4 with the second product).  It costs a
-//     sixth: 32 sequences of 8192 .. 32768, 32 / 8 heads of 128, bf16 150 us, f16 176.
+//     sixth: 32 sequences of 8192 .. 32768, 32 / 8 heads of 128, bf16 150 us, f16 179.  Codes less 8 are not left as subnormals: MMAs
+//     line up products by the exponents that their factors are written with, and cut off up to 2^-15 of a product of a subnormal.
 //   * sums of int4 codes are levelled every kLevelTokens tokens of a warp, see there: their error does not grow with the call.
 // Softmax statistics are of one pass over the keys, with a running maximum and sum for each row.
 //
@@ -118,10 +119,16 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Codes (odd: 16 times what they are) as they stand in a pair of halves, less 8: exact.
-__device__ __forceinline__ uint32_t less_eight(uint32_t pair, bool odd) {
-  const uint32_t eights = odd ? 0x80808080u : 0x80088008u;  // -8 * 2^-24 (times 16)
-  const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&pair), *reinterpret_cast<const __half2*>(&eights));
+// A word's codes 0 and 4 (odd: 1 and 5) less 8, as a pair of halves that are no subnormals: 1024 + code and 64 + code have a code in
+// just the bits where it stands.  Exact.  (The mask and the exponent in one instruction, which the compiler does not find: f16, 32 x
+// 8192 .. 32768 tokens 194 -> 179 us.)
+__device__ __forceinline__ uint32_t less_eight(uint32_t word, bool odd) {
+  uint32_t pair;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;"  // (a & b) | c
+      : "=r"(pair)
+      : "r"(word), "r"(odd ? 0x00f000f0u : 0x000f000fu), "r"(odd ? 0x54005400u : 0x64006400u));
+  const uint32_t less = odd ? 0xd480d480u : 0xe408e408u;  // -72, -1032
+  const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&pair), *reinterpret_cast<const __half2*>(&less));
   return *reinterpret_cast<const uint32_t*>(&x);
 }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -235,6 +242,7 @@ constexpr float kUnitLog2 = 5.f;        // P * scale is below 2^(kSlack + 1 + kU
 // 131072 and 2^20 tokens, in calls of 1.3e8 and 1e8 of them: 512 1.8e-3 and 2.8e-3, 1024 1.9e-3 and 3.4e-3, never 4.5e-2 and 0.16).
 constexpr int kLevelTokens = 1024;
 constexpr uint32_t kLeastTop = 87u << 23;  // 2^-40
+constexpr float kCodeUnit = 0x1p24f;  // a code in the low bits of a half, in units of the number that it is there
 constexpr float kLeastTopLog2 = -40.f, kSpare = 8.f, kRoom = 6.f;
 
 // ------------------------------------------------------------------------------------------
@@ -868,11 +876,12 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 constexpr int kPer = Shape::kPerGroupV;
+                const float odd = p.dtype == SPLASH_F16 ? 1.f : 16.f, unit = p.dtype == SPLASH_F16 ? 1.f : kCodeUnit;
                 float mean = 0.f;
 #pragma unroll
                 for (int c = group * kPer; c < (group + 1) * kPer; ++c)
 #pragma unroll
-                  for (int k = 0; k < kSteps; ++k) mean += fmaf(o[c][k][nb][2 + j], 0.0625f, o[c][k][nb][j]);
+                  for (int k = 0; k < kSteps; ++k) mean += fmaf(o[c][k][nb][2 + j], 1.f / odd, o[c][k][nb][j]);
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) mean += __shfl_xor_sync(~0u, mean, d);
                 mean *= 1.f / (kPer * 32);
@@ -881,9 +890,9 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
 #pragma unroll
                   for (int k = 0; k < kSteps; ++k) {
                     o[c][k][nb][j] -= mean;
-                    o[c][k][nb][2 + j] = fmaf(mean, -16.f, o[c][k][nb][2 + j]);
+                    o[c][k][nb][2 + j] = fmaf(-odd, mean, o[c][k][nb][2 + j]);
                   }
-                zeros[group][nb][j] = fmaf(mean, 0x1p21f, zeros[group][nb][j]);  // (2^24, for eight lanes together)
+                zeros[group][nb][j] = fmaf(mean, unit / 8.f, zeros[group][nb][j]);  // (eight lanes')
               }
         }
         top = (uint32_t)(__reduce_min_sync(~0u, (int)floorf(least_log2)) + 127) << 23;
@@ -954,17 +963,14 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
               }
               uint32_t w0 = words[c % 2 * 2], w1 = words[c % 2 * 2 + 1];
               if constexpr (kInt4) {
-                uint32_t a[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+                auto codes = [](uint32_t word, bool odd) {
+                  if (decltype(fine)::value) return less_eight(word, odd);
+                  return word & (odd ? 0x00f000f0u : 0x000f000fu);
+                };
+                const uint32_t a[4] = {codes(w0, false), codes(w0, true), codes(w1, false), codes(w1, true)};
                 w0 >>= 8;
                 w1 >>= 8;
-                uint32_t a2[4] = {w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
-                if (decltype(fine)::value) {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    a[k] = less_eight(a[k], k & 1);
-                    a2[k] = less_eight(a2[k], k & 1);
-                  }
-                }
+                const uint32_t a2[4] = {codes(w0, false), codes(w0, true), codes(w1, false), codes(w1, true)};
 #pragma unroll
                 for (int nb = 0; nb < kN; ++nb) {
                   mma_f16(o[c][0][nb], a, pf[nb][0], pf[nb][1]);
@@ -1006,6 +1012,8 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     const int active = min(warps, u1 - u0);
     if (warp < active) {
       float* const own = reinterpret_cast<float*>(ring);
+      // of products of int4 codes
+      const float back = p.dtype == SPLASH_F16 ? 1.f : kCodeUnit, back_odd = p.dtype == SPLASH_F16 ? 1.f : kCodeUnit / 16.f;
 #pragma unroll
       for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
@@ -1031,11 +1039,10 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
 #pragma unroll
           for (int c = 0; c < Shape::kChunksV; ++c) {
             if constexpr (kInt4) {
-              constexpr float kBack = 0x1p24f;  // of products of codes
               const float zero = z[c / Shape::kPerGroupV];
               *reinterpret_cast<float4*>(own + r * Shape::kV + c * 32 + g * 4) =
-                  make_float4(fmaf(o[c][0][nb][j], kBack, zero), fmaf(o[c][0][nb][2 + j], kBack * 0.0625f, zero),
-                              fmaf(o[c][1][nb][j], kBack, zero), fmaf(o[c][1][nb][2 + j], kBack * 0.0625f, zero));
+                  make_float4(fmaf(o[c][0][nb][j], back, zero), fmaf(o[c][0][nb][2 + j], back_odd, zero),
+                              fmaf(o[c][1][nb][j], back, zero), fmaf(o[c][1][nb][2 + j], back_odd, zero));
             } else {
               *reinterpret_cast<float2*>(own + r * Shape::kV + c * 16 + g * 2) = make_float2(o[c][0][nb][j], o[c][0][nb][2 + j]);
             }
