@@ -422,6 +422,26 @@ def test_queries_through_their_strides_and_nothing_at_all():
   kv_cache.append(store.cache, q[:, :2, :0], q[:, :2, :0], store.slots[:, :0])
 
 
+@pytest.mark.parametrize("offset", [1, 4, 8])
+def test_contiguous_tensors_that_begin_anywhere(offset):
+  """Their rows lie one behind the other, but not on boundaries of 16 bytes: a copy, which contiguous() alone does not make."""
+  store = Store([90, 31], d=64, group=64)
+  g = torch.Generator(device=DEV).manual_seed(0)
+
+  def shifted(*shape):
+    x = torch.randn(math.prod(shape) + offset, generator=g, device=DEV).to(torch.bfloat16)
+    return x[offset:].view(shape), x[offset:].clone().view(shape)
+
+  (q, q_aligned), (k, k_aligned), (v, v_aligned) = shifted(2, 4, 3, 64), shifted(2, 2, 3, 64), shifted(2, 2, 3, 64)
+  kv_cache.append(store.cache, k_aligned, v_aligned, store.slots[:, :3])
+  want = kv_cache.attend(store.cache, q_aligned, store.table, store.lengths, logits_scale=0.1)
+  store = Store([90, 31], d=64, group=64)
+  kv_cache.append(store.cache, k, v, store.slots[:, :3])
+  assert q.is_contiguous() and torch.equal(kv_cache.attend(store.cache, q, store.table, store.lengths, logits_scale=0.1), want)
+  one = k[:1, :1, :1]  # a token: contiguous, whatever its strides are
+  kv_cache.append(Store([3], heads=1, d=64).cache, one, one, torch.zeros(1, 1, dtype=torch.int32, device=DEV))
+
+
 def test_offsets_beyond_32_bits():
   """Codes of the pages at the end lie more than 2^32 bytes from the first."""
   page, heads, d = 4096, 8, 256

@@ -154,3 +154,18 @@ def test_compiled_calls_give_the_same(native_calls):
   ts = _leaves(q, k, v)
   out = torch.compile(call, backend="eager")(*ts)
   assert all(torch.equal(a, b) for a, b in zip((out, *torch.autograd.grad(out, ts, do)), want))
+
+
+def test_contiguous_operands_that_begin_between_boundaries():
+  """Copied by the call: the kernels read rows from boundaries of 16 bytes."""
+  tensors = _operands(64)
+  kernel = _kernel()
+  results = []
+  for offset in (0, 3):
+    q, k, v, do = (torch.cat([t.new_zeros(offset), t.flatten()])[offset:].view(t.shape) for t in tensors)
+    ts = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    assert all(t.is_contiguous() and (t.data_ptr() % 16 == 0) == (offset == 0) for t in ts)
+    out = kernel(*ts, logits_scale=0.125)
+    results.append((out, *torch.autograd.grad(out, ts, do)))
+  kernel.check_errors()
+  assert all(torch.equal(a, b) for a, b in zip(*results))

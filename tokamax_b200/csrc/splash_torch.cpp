@@ -44,7 +44,9 @@ at::Tensor usable(const at::Tensor& t) {
   TORCH_CHECK(t.dim() == 4, "expected a tensor of rank 4, got rank ", t.dim());
   bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
-  return ok ? t : t.contiguous();
+  if (ok) return t;
+  const at::Tensor copy = t.contiguous();  // (t itself where it is contiguous and begins between two boundaries of 16 bytes)
+  return copy.data_ptr() == t.data_ptr() ? copy.clone(at::MemoryFormat::Contiguous) : copy;
 }
 
 // The kernels follow every address that they are given: each must be one of their own device, that of `q`.
