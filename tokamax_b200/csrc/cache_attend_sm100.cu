@@ -45,8 +45,8 @@
 // sequences of 0 .. 13025 109 us, 6.2 TB/s.
 // Rows of more than one block of eight spend 190 instructions more a block on a unit, and leave room for fewer warps.  Registers: the
 // element type is a value at run time, so a kernel holds four forms of the product with P (masked or not, f16's second product or
-// not); 32 of the 50 kernels spill, up to 204 bytes a thread (most where groups of 32 keep many scales), in the forms that are timed
-// here 0 (8 rows, head dim 128, groups of 64) to 28.
+// not); 34 of the 50 kernels spill, up to 224 bytes a thread (most where groups of 32 keep many scales), the forms that are timed here
+// 0 (e4m3) to 36 (head dim 64 in groups of 32).
 #include <atomic>
 
 #include "cache_common.cuh"

@@ -144,6 +144,9 @@ def attend(cache: KVCache, q: torch.Tensor, page_table: torch.Tensor, lengths: t
   nothing is zeros and its logsumexp and maximum the mask value.  ``save_residuals`` adds ``{"logsumexp", "max_logits"}``
   ``[B, q_heads, T]``.
 
+  Weights times the scales of V are held to 11 bits (22 for f16 outputs), down to 2^-22 of a row's largest; logits may be up to 2^26 in
+  size.  What no query sees, a page's places that were never written among it, has no part.
+
   Made for few rows (T times q heads per kv head up to some tens: the codes are unpacked again for every 16 of them);
   a chunk of a prompt is better off with :func:`read` and a splash kernel.  Nothing is copied to the host: lengths and pages
   may change between the replays of a captured graph."""
