@@ -541,6 +541,90 @@ int splash_cache_attend(const SplashCacheAttendArgs* args, void* cuda_stream);
  * sizes that splash_cache_attend refuses. */
 size_t splash_cache_attend_workspace_bytes(const SplashCacheAttendArgs* args);
 
+/* The same over tables of pages for each kv head and query, which need not be the whole of a sequence (what
+ * splash_cache_choose gives, say): page_table [batch, kv_heads, q_len, n_table] (row stride table_stride, rows one behind the
+ * other) and lengths [batch, kv_heads, q_len].  Query i of the q heads of kv head h sees the first lengths[b, h, i] tokens of its
+ * table.  `window` has to be negative: the tokens' places in the sequence are not known. */
+int splash_cache_attend_tables(const SplashCacheAttendArgs* args, void* cuda_stream);
+size_t splash_cache_attend_tables_workspace_bytes(const SplashCacheAttendArgs* args);
+
+/* Bounds of the keys of whole pages, for splash_cache_choose: of each page and kv head the least and the largest value of each
+ * channel, in 8 bits.
+ *   codes [n_pages, kv_heads, 2, row_k] int8: the least values, then the largest; 0 behind head_dim
+ *   scales [n_pages, kv_heads] fp32
+ * with value = scale * code, scale = amax / 127 over the page's bounds of a head, code = round(x / scale) clamped to -127 .. 127
+ * (0 where scale is 0), all of it in 32 bits, ties to even.  A NaN counts as 0 and an infinity as the largest number.
+ * Written are the bounds of the pages that the newest `newest` tokens of each sequence have made whole: those whose last
+ * token is one of positions lengths[b] - newest .. lengths[b] - 1.  Pages outside the cache are passed over. */
+typedef struct SplashPageBounds {
+  int8_t* codes;                /* 16-byte aligned */
+  float* scales;
+} SplashPageBounds;
+
+typedef struct SplashCacheBoundArgs {
+  SplashKvCache cache;
+  SplashPageBounds bounds;
+  const int32_t* page_table;    /* as for splash_cache_attend */
+  int64_t table_stride;
+  int32_t n_table;
+  int64_t batch;
+  const int32_t* lengths;
+  int64_t newest;
+} SplashCacheBoundArgs;
+int splash_cache_bound(const SplashCacheBoundArgs* args, void* cuda_stream);
+
+/* For each sequence, kv head and query the `count` pages whose bounds allow the largest logits.  q [batch, q_heads, q_len, head_dim],
+ * bf16 or f16; query i of sequence b stands at position lengths[b] - q_len + i (at the end of the table at most), on its own page.
+ * Candidates are the pages up to that one, except those outside the cache.  The `first` first pages of the sequence and the `last`
+ * ones up to the query's own (count >= first + last, last >= 1) are always taken, then those of the largest score, of equal ones the first:
+ *   score = scale(page) * max over the q heads of the kv head of sum over channels c of q_c * (q_c > 0 ? largest_c : least_c)
+ * with q in 8 bits, q_c = round(q / s) clamped to -127 .. 127, s = amax / 127 over the q heads and channels of the query and kv head (NaN and
+ * infinities as for the bounds).  Sums are of whole numbers: the choice does not depend on their order.
+ * tables [batch, kv_heads, q_len, count] int32: the pages taken, as numbers of the pool, in the order of the sequence, then -1;
+ * table_lengths [batch, kv_heads, q_len] int32: the tokens up to the query's position that lie on them.
+ * Bounds of the queries' own pages are not read.  workspace: splash_cache_choose_workspace_bytes, 16-byte aligned; need not be zeroed. */
+typedef struct SplashCacheChooseArgs {
+  SplashKvCache cache;
+  SplashPageBounds bounds;
+  SplashTensor q;
+  const int32_t* page_table;    /* as for splash_cache_attend */
+  int64_t table_stride;
+  int32_t n_table;
+  const int32_t* lengths;
+  int32_t* tables;
+  int32_t* table_lengths;
+  int32_t count, first, last;
+  void* workspace;
+  size_t workspace_bytes;
+} SplashCacheChooseArgs;
+int splash_cache_choose(const SplashCacheChooseArgs* args, void* cuda_stream);
+/* 0 where the scores of a row of the table have room on the chip, and for sizes that splash_cache_choose refuses. */
+size_t splash_cache_choose_workspace_bytes(const SplashCacheChooseArgs* args);
+
+/* ------------------------------------------------------------------------------------------
+ * Rotary positions.  No counterpart in the reference, whose attention takes queries and keys that
+ * have them already.
+ *
+ * Pair i of a row's first `dim` channels, (x[i], x[i + dim / 2]) or, interleaved, (x[2i], x[2i + 1]), is turned by position *
+ * turns[i] and multiplied by `factor`; the other channels are copied:
+ *   y0 = factor * (x0 cos a - x1 sin a), y1 = factor * (x1 cos a + x0 sin a)
+ * turns [dim / 2]: 2^64ths of a whole turn for each token, so that the angle of any position (a 64-bit product, whose overflow
+ * is whole turns) has no error but that of `turns`.  inverse: by the negative angle, which is the gradient's way back.
+ * x and y: up to two tensors each ([batch, heads, tokens, head_dim], one type of bf16, f16, f32; the same sizes but for heads; data
+ * NULL: none), strides multiples of 8 elements; x may be y.  Products and sums are of 32 bits.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct SplashRotateArgs {
+  SplashTensor x[2], y[2];
+  const void* positions;        /* [batch, tokens], row stride position_stride, contiguous tokens */
+  int32_t positions_are_64;     /* 1: int64, 0: int32 */
+  int64_t position_stride;
+  const uint64_t* turns;
+  int32_t dim;                  /* even, 2 .. head_dim */
+  int32_t interleaved, inverse;
+  float factor;
+} SplashRotateArgs;
+int splash_rotate(const SplashRotateArgs* args, void* cuda_stream);
+
 /* Copies the 4-word device error record to host (synchronises the stream) and maps it to a
  * status: SPLASH_OK or SPLASH_ERR_KERNEL_TIMEOUT.  record_out may be NULL. */
 int splash_read_error(const uint32_t* error_record, void* cuda_stream, uint32_t record_out[4]);

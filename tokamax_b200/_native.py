@@ -33,6 +33,8 @@ SOURCES = (
     "exchange.cu",
     "cache_rows.cu",
     "cache_attend_sm100.cu",
+    "cache_pages.cu",
+    "rotary.cu",
     "splash_xla_ffi.cc",  # handlers compile only where xla/ffi/api/ffi.h is on the include path
 )
 
@@ -268,6 +270,53 @@ class SplashCacheAttendArgs(C.Structure):
   ]
 
 
+class SplashPageBounds(C.Structure):
+  _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p)]
+
+
+class SplashCacheBoundArgs(C.Structure):
+  _fields_ = [
+      ("cache", SplashKvCache),
+      ("bounds", SplashPageBounds),
+      ("page_table", C.c_void_p),
+      ("table_stride", C.c_int64),
+      ("n_table", C.c_int32),
+      ("batch", C.c_int64),
+      ("lengths", C.c_void_p),
+      ("newest", C.c_int64),
+  ]
+
+
+class SplashCacheChooseArgs(C.Structure):
+  _fields_ = [
+      ("cache", SplashKvCache),
+      ("bounds", SplashPageBounds),
+      ("q", SplashTensor),
+      ("page_table", C.c_void_p),
+      ("table_stride", C.c_int64),
+      ("n_table", C.c_int32),
+      ("lengths", C.c_void_p),
+      ("tables", C.c_void_p),
+      ("table_lengths", C.c_void_p),
+      ("count", C.c_int32), ("first", C.c_int32), ("last", C.c_int32),
+      ("workspace", C.c_void_p),
+      ("workspace_bytes", C.c_size_t),
+  ]
+
+
+class SplashRotateArgs(C.Structure):
+  _fields_ = [
+      ("x", SplashTensor * 2), ("y", SplashTensor * 2),
+      ("positions", C.c_void_p),
+      ("positions_are_64", C.c_int32),
+      ("position_stride", C.c_int64),
+      ("turns", C.c_void_p),
+      ("dim", C.c_int32),
+      ("interleaved", C.c_int32), ("inverse", C.c_int32),
+      ("factor", C.c_float),
+  ]
+
+
 # name -> (restype, argtypes); every function include/splash_b200.h declares.
 _PROTOTYPES = {
     "splash_maskinfo_build": (C.c_int, [C.POINTER(SplashMaskNode), C.c_int32, C.c_int64, C.c_int64,
@@ -305,6 +354,12 @@ _PROTOTYPES = {
     "splash_cache_read": (C.c_int, [C.POINTER(SplashCacheReadArgs), C.c_void_p]),
     "splash_cache_attend": (C.c_int, [C.POINTER(SplashCacheAttendArgs), C.c_void_p]),
     "splash_cache_attend_workspace_bytes": (C.c_size_t, [C.POINTER(SplashCacheAttendArgs)]),
+    "splash_cache_attend_tables": (C.c_int, [C.POINTER(SplashCacheAttendArgs), C.c_void_p]),
+    "splash_cache_attend_tables_workspace_bytes": (C.c_size_t, [C.POINTER(SplashCacheAttendArgs)]),
+    "splash_cache_bound": (C.c_int, [C.POINTER(SplashCacheBoundArgs), C.c_void_p]),
+    "splash_cache_choose": (C.c_int, [C.POINTER(SplashCacheChooseArgs), C.c_void_p]),
+    "splash_cache_choose_workspace_bytes": (C.c_size_t, [C.POINTER(SplashCacheChooseArgs)]),
+    "splash_rotate": (C.c_int, [C.POINTER(SplashRotateArgs), C.c_void_p]),
     "splash_read_error": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_uint32 * 4)]),
     "splash_probe_bounded_wait": (C.c_int, [C.c_void_p, C.c_int64, C.c_uint32, C.c_void_p]),
     "splash_xla_ffi_compiled": (C.c_int, []),
@@ -426,6 +481,10 @@ def host():
             "splash_fwd_shard", "splash_bwd_shard", "splash_bwd_workspace_bytes", "splash_bwd_fused_workspace_bytes")))
         module.bind_cache_library(*(C.cast(getattr(handle, name), C.c_void_p).value for name in (
             "splash_cache_append", "splash_cache_read", "splash_cache_attend", "splash_cache_attend_workspace_bytes")))
+        module.bind_page_library(*(C.cast(getattr(handle, name), C.c_void_p).value for name in (
+            "splash_cache_attend_tables", "splash_cache_attend_tables_workspace_bytes", "splash_cache_bound", "splash_cache_choose",
+            "splash_cache_choose_workspace_bytes")))
+        module.bind_rotary_library(C.cast(handle.splash_rotate, C.c_void_p).value)
         module.bind_check(check)
         _host = module
   return _host

@@ -75,9 +75,12 @@ struct AttendParams {
   int64_t* starts;  // [batch + 1] where each sequence's items begin, in the measure of shares
   int64_t q_stride_b, q_stride_h, q_stride_s, o_stride_b, o_stride_h, o_stride_s, table_stride, n_pages;
   float scale, soft_cap, mask_value;
-  int32_t batch, q_heads, kv_heads, heads_per_kv, q_len, row_tiles, n_table, page_size, page_shift, dtype;
+  // A page table is of a sequence, or (`by_head`) of a sequence, kv head and query: `batch` counts tables, q_len is 1 then, and
+  // `queries` is what q has of them.  items: kv heads of a table times row tiles.
+  int32_t batch, q_heads, kv_heads, heads_per_kv, q_len, queries, items, row_tiles, n_table, page_size, page_shift, dtype;
   int32_t head_dim, head_dim_v, window, item_cost;  // item_cost: in units
   bool whole;  // every item is one CTA's
+  bool by_head;
 };
 
 // ------------------------------------------------------------------------------------------
@@ -300,7 +303,7 @@ struct Start {  // where a CTA's share begins
 template <int kUnit>
 __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
   constexpr int kThreads = kWarps * 32;
-  const int64_t per_sequence = p.kv_heads * p.row_tiles;
+  const int64_t per_sequence = p.items;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t* const found = scratch + kWarps;
   const bool keep = blockIdx.x == 0;  // this CTA writes down where the sequences start
@@ -363,9 +366,19 @@ __device__ __forceinline__ void add_sink(float sink, float& m, float& l) {
   m = top;
 }
 
+// The sequence, kv head and first query of the rows of an item: table b, kv head times row tiles `item`.
+struct Rows {
+  int b, head, query;
+};
+__device__ __forceinline__ Rows rows_of(const AttendParams& p, int b, int item) {
+  if (!p.by_head) return {b, item / p.row_tiles, 0};
+  const unsigned pair = (unsigned)b / (unsigned)p.queries;
+  return {(int)(pair / (unsigned)p.kv_heads), (int)(pair % (unsigned)p.kv_heads), (int)((unsigned)b % (unsigned)p.queries)};
+}
+
 // Eight channels of a row, from the sums of all its keys.
-__device__ __forceinline__ void finish_row(const AttendParams& p, int b, int head, int row, int d, float (&x)[8], float m, float l) {
-  const int i = row / p.heads_per_kv, h = head * p.heads_per_kv + row % p.heads_per_kv;
+__device__ __forceinline__ void finish_row(const AttendParams& p, const Rows& rows, int row, int d, float (&x)[8], float m, float l) {
+  const int b = rows.b, i = rows.query + row / p.heads_per_kv, h = rows.head * p.heads_per_kv + row % p.heads_per_kv;
   float weight = 1.f;
   if (p.sinks != nullptr) {
     const float own = m;
@@ -377,7 +390,7 @@ __device__ __forceinline__ void finish_row(const AttendParams& p, int b, int hea
   for (int k = 0; k < 8; ++k) x[k] *= weight;
   if (d < p.head_dim_v) store8(p.o, p.dtype, b * p.o_stride_b + h * p.o_stride_h + i * p.o_stride_s + d, x);
   if (d == 0) {
-    const int64_t to = ((int64_t)b * p.q_heads + h) * p.q_len + i;
+    const int64_t to = ((int64_t)b * p.q_heads + h) * p.queries + i;
     if (p.lse != nullptr) p.lse[to] = l == 0.f ? p.mask_value : (m + __log2f(l)) * kLn2;
     if (p.max_logits != nullptr) p.max_logits[to] = l == 0.f ? p.mask_value : m * kLn2;
   }
@@ -399,7 +412,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   const int g = lane >> 2, t4 = lane & 3;
   grid_dependents_launch();  // the joining kernel may come up beside this one; it waits for its end
 
-  const int per_sequence = p.kv_heads * p.row_tiles;
+  const int per_sequence = p.items;
   int64_t at, end, before, share_begin;  // in the measure of shares; before: what lies before sequence b
   int b;
   if (p.whole) {  // items in turn
@@ -418,7 +431,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   const int heads = p.heads_per_kv;
 
   // The item that is worked on (or whose keys are on their way): b, item = head * row_tiles + row tile, units u0 .. u1 - 1.
-  int item = 0, u0 = 0, u1 = 0, length = 0;
+  int item = 0, u0 = 0, u1 = 0, length = 0, head = 0;
   Keys keys{};
   bool is_last = false;  // its first unit is in this share, so that its sums are those of place 1
   auto next_item = [&]() -> bool {
@@ -459,7 +472,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     const int u = u0 + warp + (turn + lane / kTiles) * warps, token = keys.lo + u * kUnit + lane % kTiles * 16;
     const int page = u < u1 && token < keys.hi ? __ldg(p.page_table + b * p.table_stride + (token >> p.page_shift)) : -1;
     if (page < 0 || page >= p.n_pages) return kNowhere;
-    const uint32_t first = (uint32_t)(page * p.kv_heads + item / p.row_tiles) << (p.page_shift - 4);
+    const uint32_t first = (uint32_t)(page * p.kv_heads + head) << (p.page_shift - 4);
     return first + ((token & (p.page_size - 1)) >> 4);
   };
   uint32_t places, next_places;
@@ -506,7 +519,9 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   };
 
   while (next_item()) {
-    const int head = item / p.row_tiles, row0 = item % p.row_tiles * kRows;
+    const Rows rows = rows_of(p, b, item);
+    head = rows.head;
+    const int row0 = item % p.row_tiles * kRows;
     const int n_rows = min(kRows, p.q_len * heads - row0);
 
     // ---- q's rows on their way: kLanes lanes (a power of two that holds the row's width / 8) a row ----
@@ -525,8 +540,8 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       raw[pass] = make_uint4(0, 0, 0, 0);
       if (r < n_rows && piece * 8 < p.head_dim) {
         const int i = query_of(r), h = head * heads + first_row + r - i * heads;
-        raw[pass] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.q_stride_b + h * p.q_stride_h +
-                                                         (first_query + i) * p.q_stride_s + piece * 8));
+        raw[pass] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + rows.b * p.q_stride_b + h * p.q_stride_h +
+                                                         (rows.query + first_query + i) * p.q_stride_s + piece * 8));
       }
     }
     start_item();
@@ -1080,7 +1095,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         }
         continue;
       }
-      finish_row(p, b, head, row0 + r, d, x, most, sum);
+      finish_row(p, rows, row0 + r, d, x, most, sum);
     }
     __syncthreads();  // before q's place, the statistics and the ring are written again
   }
@@ -1109,11 +1124,12 @@ __global__ void __launch_bounds__(kJoinThreads, kAhead > 2 ? 2 : 4) cache_attend
   const int lot = threadIdx.x / kEach, d = threadIdx.x % kEach * 8;
   const int64_t share = share_of(p.starts[p.batch], ctas);
   for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
-    const int64_t before = p.starts[b], cost = quotient(p.starts[b + 1] - before, p.kv_heads * p.row_tiles);
+    const int64_t before = p.starts[b], cost = quotient(p.starts[b + 1] - before, p.items);
     const int64_t first = before + blockIdx.x * cost + p.item_cost;  // unit of this item
     const int64_t c0 = quotient(first, share), c1 = cost > 0 ? quotient(first + cost - p.item_cost - 1, share) : c0 - 1;
     if (c0 == c1) continue;  // written already
-    const int head = blockIdx.x / p.row_tiles, row0 = blockIdx.x % p.row_tiles * kRows;
+    const Rows rows = rows_of(p, b, blockIdx.x);
+    const int row0 = blockIdx.x % p.row_tiles * kRows;
     const int n_rows = min(kRows, p.q_len * p.heads_per_kv - row0);
     int slices = 1;
     while (slices < kMostSlices && slices * 2 <= c1 - c0 + 1) slices *= 2;
@@ -1185,7 +1201,7 @@ __global__ void __launch_bounds__(kJoinThreads, kAhead > 2 ? 2 : 4) cache_attend
         }
         __syncthreads();
       }
-      if (mine && slice == 0) finish_row(p, b, head, row0 + r, d, x, most, sum);
+      if (mine && slice == 0) finish_row(p, rows, row0 + r, d, x, most, sum);
     }
   }
 }
@@ -1206,7 +1222,7 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
       return SPLASH_ERR_CUDA;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int64_t items = (int64_t)p.kv_heads * p.row_tiles * p.batch;
+  const int64_t items = (int64_t)p.items * p.batch;
   const int warps = p.whole && items < 2 * kSms ? kMostWarps : kWarps;
   kernel<<<p.whole && items < ctas ? (int)items : ctas, warps * 32, Shape::smem(warps), stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return SPLASH_ERR_CUDA;
@@ -1215,7 +1231,7 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   // (as many blocks of an item as its rows and the GPU have room for, where items are few)
   const int rows = p.q_len * p.heads_per_kv < Shape::kRows ? p.q_len * p.heads_per_kv : Shape::kRows;
   const bool few = items < kSms / 2;
-  config.gridDim = dim3((unsigned)(p.kv_heads * p.row_tiles), (unsigned)(p.batch < 65535 ? p.batch : 65535),
+  config.gridDim = dim3((unsigned)p.items, (unsigned)(p.batch < 65535 ? p.batch : 65535),
                         (unsigned)(items >= 2 * kSms ? 1 : items * rows <= 8 * kSms ? rows : 8 * kSms / items));
   config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
@@ -1287,7 +1303,19 @@ static int with_shape(const SplashCacheAttendArgs& a, Fn&& fn) {
   }
 }
 
-static int check_attend(const SplashCacheAttendArgs& a) {
+// The sizes of a call with a table for each kv head and query: as many sequences of one query and one kv head.
+static SplashCacheAttendArgs sizes_by_head(const SplashCacheAttendArgs& a) {
+  SplashCacheAttendArgs s = a;
+  for (SplashTensor* t : {&s.q, &s.o}) {
+    t->size[0] *= a.cache.kv_heads * a.q.size[2];
+    t->size[1] /= a.cache.kv_heads;
+    t->size[2] = 1;
+  }
+  s.cache.kv_heads = 1;
+  return s;
+}
+
+static int check_attend(const SplashCacheAttendArgs& a, bool by_head) {
   const SplashKvCache& c = a.cache;
   if (const int status = check_cache(c)) return status;
   for (const SplashTensor* t : {&a.q, &a.o})
@@ -1302,6 +1330,8 @@ static int check_attend(const SplashCacheAttendArgs& a) {
       (int64_t)a.n_table * c.page_size > (1 << 30) ||
       c.n_pages * c.kv_heads > 0x7fffffffll / (c.page_size / 16))  // (tiles of 16 tokens are counted in 32 bits)
     return SPLASH_ERR_TOO_LARGE;
+  if (by_head && a.window >= 0) return SPLASH_ERR_INVALID_ARGUMENT;
+  if (by_head && a.q.size[0] * c.kv_heads * a.q.size[2] > (1 << 24)) return SPLASH_ERR_TOO_LARGE;
   return SPLASH_OK;
 }
 
@@ -1319,9 +1349,10 @@ static size_t parts_bytes() {
   return (size_t)resident<Shape>() * 2 * Shape::kRows * (Shape::kV + 2) * 4;
 }
 
-static int cache_attend(const SplashCacheAttendArgs& a, cudaStream_t stream) {
-  if (const int status = check_attend(a)) return status;
-  const SplashKvCache& c = a.cache;
+static int cache_attend(const SplashCacheAttendArgs& args, bool by_head, cudaStream_t stream) {
+  if (const int status = check_attend(args, by_head)) return status;
+  const SplashCacheAttendArgs a = by_head ? sizes_by_head(args) : args;
+  const SplashKvCache& c = args.cache;
   AttendParams p{};
   p.k_codes = static_cast<const uint8_t*>(c.k_codes);
   p.k_scales = static_cast<const uint8_t*>(c.k_scales);
@@ -1342,10 +1373,12 @@ static int cache_attend(const SplashCacheAttendArgs& a, cudaStream_t stream) {
   p.soft_cap = a.soft_cap;
   p.mask_value = a.mask_value;
   p.batch = (int32_t)a.q.size[0];
-  p.q_heads = (int32_t)a.q.size[1];
+  p.q_heads = (int32_t)args.q.size[1];
   p.kv_heads = c.kv_heads;
   p.heads_per_kv = p.q_heads / c.kv_heads;
   p.q_len = (int32_t)a.q.size[2];
+  p.queries = (int32_t)args.q.size[2];
+  p.by_head = by_head;
   p.n_table = a.n_table;
   p.page_size = c.page_size;
   p.page_shift = log2_of(c.page_size);
@@ -1366,13 +1399,15 @@ static int cache_attend(const SplashCacheAttendArgs& a, cudaStream_t stream) {
       own.starts = reinterpret_cast<int64_t*>(static_cast<uint8_t*>(a.workspace) + parts);
     }
     own.row_tiles = (p.q_len * p.heads_per_kv + Shape::kRows - 1) / Shape::kRows;
+    own.items = a.cache.kv_heads * own.row_tiles;
     own.item_cost = item_tokens(Shape::kN) / Shape::kUnit;
     return launch<Shape>(own, resident<Shape>(), stream);
   });
 }
 
-static size_t cache_attend_workspace(const SplashCacheAttendArgs& a) {
-  if (check_attend(a) != SPLASH_OK) return 0;
+static size_t cache_attend_workspace(const SplashCacheAttendArgs& args, bool by_head) {
+  if (check_attend(args, by_head) != SPLASH_OK) return 0;
+  const SplashCacheAttendArgs a = by_head ? sizes_by_head(args) : args;
   size_t bytes = 0;
   with_shape(a, [&](auto shape) -> int {
     using Shape = decltype(shape);
@@ -1387,11 +1422,19 @@ static size_t cache_attend_workspace(const SplashCacheAttendArgs& a) {
 extern "C" {
 
 int splash_cache_attend(const SplashCacheAttendArgs* args, void* cuda_stream) {
-  return args == nullptr ? SPLASH_ERR_INVALID_ARGUMENT : sb::cache_attend(*args, static_cast<cudaStream_t>(cuda_stream));
+  return args == nullptr ? SPLASH_ERR_INVALID_ARGUMENT : sb::cache_attend(*args, false, static_cast<cudaStream_t>(cuda_stream));
 }
 
 size_t splash_cache_attend_workspace_bytes(const SplashCacheAttendArgs* args) {
-  return args == nullptr ? 0 : sb::cache_attend_workspace(*args);
+  return args == nullptr ? 0 : sb::cache_attend_workspace(*args, false);
+}
+
+int splash_cache_attend_tables(const SplashCacheAttendArgs* args, void* cuda_stream) {
+  return args == nullptr ? SPLASH_ERR_INVALID_ARGUMENT : sb::cache_attend(*args, true, static_cast<cudaStream_t>(cuda_stream));
+}
+
+size_t splash_cache_attend_tables_workspace_bytes(const SplashCacheAttendArgs* args) {
+  return args == nullptr ? 0 : sb::cache_attend_workspace(*args, true);
 }
 
 }  // extern "C"

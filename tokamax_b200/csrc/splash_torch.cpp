@@ -290,6 +290,22 @@ void bind_cache_library(uintptr_t append, uintptr_t read, uintptr_t attend, uint
   cache_lib.attend_workspace_bytes = reinterpret_cast<decltype(cache_lib.attend_workspace_bytes)>(attend_workspace_bytes);
 }
 
+struct PageLibrary {
+  int (*attend)(const SplashCacheAttendArgs*, void*) = nullptr;
+  size_t (*attend_workspace_bytes)(const SplashCacheAttendArgs*) = nullptr;
+  int (*bound)(const SplashCacheBoundArgs*, void*) = nullptr;
+  int (*choose)(const SplashCacheChooseArgs*, void*) = nullptr;
+  size_t (*choose_workspace_bytes)(const SplashCacheChooseArgs*) = nullptr;
+} page_lib;
+
+void bind_page_library(uintptr_t attend, uintptr_t attend_workspace_bytes, uintptr_t bound, uintptr_t choose, uintptr_t choose_workspace_bytes) {
+  page_lib.attend = reinterpret_cast<decltype(page_lib.attend)>(attend);
+  page_lib.attend_workspace_bytes = reinterpret_cast<decltype(page_lib.attend_workspace_bytes)>(attend_workspace_bytes);
+  page_lib.bound = reinterpret_cast<decltype(page_lib.bound)>(bound);
+  page_lib.choose = reinterpret_cast<decltype(page_lib.choose)>(choose);
+  page_lib.choose_workspace_bytes = reinterpret_cast<decltype(page_lib.choose_workspace_bytes)>(choose_workspace_bytes);
+}
+
 // A cache's description, with the tensors that it lies in.
 struct KvCache {
   SplashKvCache desc{};
@@ -334,11 +350,15 @@ void require_not_traced() {
   TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "the cache's operators cannot be recorded by torch.jit.trace");
 }
 
+void require_row_type(at::ScalarType type, const char* name, bool f32_too) {
+  TORCH_CHECK_NOT_IMPLEMENTED(type == at::kBFloat16 || type == at::kHalf || (f32_too && type == at::kFloat), name, ": ", type,
+                              " is not built (bfloat16, float16", f32_too ? ", float32)" : ")");
+}
+
 SplashTensor describe_row_tensor(const at::Tensor& t, const char* name, bool f32_too) {
   SplashTensor d{};
   const auto type = t.scalar_type();
-  TORCH_CHECK_NOT_IMPLEMENTED(type == at::kBFloat16 || type == at::kHalf || (f32_too && type == at::kFloat), name, ": ", type,
-                              " is not built (bfloat16, float16", f32_too ? ", float32)" : ")");
+  require_row_type(type, name, f32_too);
   d.dtype = type == at::kBFloat16 ? SPLASH_BF16 : type == at::kHalf ? SPLASH_F16 : SPLASH_F32;
   d.data = t.data_ptr();
   for (int i = 0; i < 4; ++i) d.size[i] = t.size(i), d.stride[i] = t.stride(i);
@@ -425,7 +445,7 @@ std::tuple<at::Tensor, at::Tensor> cache_read(const KvCache& cache, const at::Te
 }
 
 std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at::Tensor& q_in, const at::Tensor& table_in,
-                                                  const at::Tensor& lengths, double scale, std::optional<int64_t> window,
+                                                  const at::Tensor& lengths_in, double scale, std::optional<int64_t> window,
                                                   std::optional<double> soft_cap, const Maybe& sinks_in, double mask_value, bool residuals) {
   const SplashKvCache& c = cache.desc;
   require_not_traced();
@@ -434,8 +454,20 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
   TORCH_CHECK_VALUE(q_in.dim() == 4 && q_in.size(3) == c.head_dim && q_in.size(1) % c.kv_heads == 0, "q ", q_in.sizes(),
                     " does not match a cache of ", c.kv_heads, " heads of ", c.head_dim, " channels: expected [B, heads, T, D]");
   SplashCacheAttendArgs a{};
-  const at::Tensor table = set_pages(a, cache, table_in, lengths);
-  TORCH_CHECK_VALUE(q_in.size(0) == lengths.size(0), "q of ", q_in.size(0), " sequences, lengths of ", lengths.size(0));
+  const bool by_head = table_in.dim() == 4;  // a table for each kv head and query
+  at::Tensor table, lengths = lengths_in;
+  if (by_head) {
+    TORCH_CHECK_VALUE(lengths.dim() == 3 && table_in.sizes().slice(0, 3) == lengths.sizes() && table_in.size(0) == q_in.size(0) &&
+                          table_in.size(1) == c.kv_heads && table_in.size(2) == q_in.size(2),
+                      "page tables ", table_in.sizes(), " and lengths ", lengths.sizes(), " do not match: expected [B, kv_heads, T, pages] and [B, kv_heads, T]");
+    TORCH_CHECK_VALUE(!window.has_value(), "local_window_size goes by places in the sequence, which tables of chosen pages do not say");
+    const int64_t rows = lengths.numel();
+    lengths = lengths.reshape({rows}).contiguous();
+    table = set_pages(a, cache, table_in.reshape({rows, table_in.size(3)}), lengths);
+  } else {
+    table = set_pages(a, cache, table_in, lengths);
+    TORCH_CHECK_VALUE(q_in.size(0) == lengths.size(0), "q of ", q_in.size(0), " sequences, lengths of ", lengths.size(0));
+  }
   TORCH_CHECK_VALUE(!window.has_value() || (*window >= 0 && *window <= INT32_MAX), "local_window_size is not negative");
   TORCH_CHECK_VALUE(!soft_cap.has_value() || (float)*soft_cap > 0, "logits_soft_cap is positive (in 32 bits), got ", *soft_cap);
   TORCH_CHECK_VALUE(!std::isnan(scale), "logits_scale is NaN");
@@ -465,14 +497,206 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
   a.soft_cap = (float)soft_cap.value_or(0.0);
   a.window = window.has_value() ? (int32_t)*window : -1;
   a.mask_value = (float)mask_value;
-  a.workspace_bytes = cache_lib.attend_workspace_bytes(&a);
+  a.workspace_bytes = (by_head ? page_lib.attend_workspace_bytes : cache_lib.attend_workspace_bytes)(&a);
   at::Tensor workspace;
   if (a.workspace_bytes != 0) {
     workspace = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
     a.workspace = workspace.data_ptr();
   }
-  check_cache_call(on_stream_of(q, [&](void* stream) { return cache_lib.attend(&a, stream); }), "splash_cache_attend");
+  check_cache_call(on_stream_of(q, [&](void* stream) { return (by_head ? page_lib.attend : cache_lib.attend)(&a, stream); }),
+                   by_head ? "splash_cache_attend_tables" : "splash_cache_attend");
   return {o, lse, max_logits};
+}
+
+// The bounds of the keys of a cache's pages, with the tensors that they lie in.
+struct PageBounds {
+  SplashPageBounds desc{};
+  at::Tensor codes, scales;
+
+  PageBounds(at::Tensor codes_in, at::Tensor scales_in) : codes(std::move(codes_in)), scales(std::move(scales_in)) {
+    TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous() && codes.device() == scales.device(),
+                      "the arrays of page bounds are contiguous, on one device");
+    desc.codes = static_cast<int8_t*>(codes.data_ptr());
+    desc.scales = static_cast<float*>(scales.data_ptr());
+  }
+};
+
+void require_bounds_of(const PageBounds& bounds, const KvCache& cache) {
+  const SplashKvCache& c = cache.desc;
+  require_on_gpu(bounds.codes, cache, "the page bounds");
+  TORCH_CHECK_VALUE(bounds.codes.sizes() == at::IntArrayRef({c.n_pages, c.kv_heads, 2, c.row_k}) &&
+                        bounds.scales.sizes() == at::IntArrayRef({c.n_pages, c.kv_heads}),
+                    "page bounds of ", bounds.codes.sizes(), " are not of a cache of ", c.n_pages, " pages, ", c.kv_heads, " heads and rows of ", c.row_k);
+}
+
+void cache_bound(const KvCache& cache, const PageBounds& bounds, const at::Tensor& table_in, const at::Tensor& lengths, int64_t newest) {
+  require_not_traced();
+  SplashCacheBoundArgs a{};
+  const at::Tensor table = set_pages(a, cache, table_in, lengths);
+  require_bounds_of(bounds, cache);
+  TORCH_CHECK_VALUE(newest >= 0, "newest is not negative, got ", newest);
+  a.bounds = bounds.desc;
+  a.batch = lengths.size(0);
+  a.newest = newest;
+  if (a.batch != 0) check_cache_call(on_stream_of(table, [&](void* stream) { return page_lib.bound(&a, stream); }), "splash_cache_bound");
+}
+
+std::tuple<at::Tensor, at::Tensor> cache_choose(const KvCache& cache, const PageBounds& bounds, const at::Tensor& q_in, const at::Tensor& table_in,
+                                                const at::Tensor& lengths, int64_t count, int64_t first, int64_t last) {
+  const SplashKvCache& c = cache.desc;
+  require_not_traced();
+  require_no_grad(q_in, "q");
+  TORCH_CHECK_VALUE(q_in.dim() == 4 && q_in.size(3) == c.head_dim && q_in.size(1) % c.kv_heads == 0 && q_in.size(1) > 0, "q ", q_in.sizes(),
+                    " does not match a cache of ", c.kv_heads, " heads of ", c.head_dim, " channels: expected [B, heads, T, D]");
+  SplashCacheChooseArgs a{};
+  const at::Tensor table = set_pages(a, cache, table_in, lengths);
+  TORCH_CHECK_VALUE(q_in.size(0) == lengths.size(0), "q of ", q_in.size(0), " sequences, lengths of ", lengths.size(0));
+  TORCH_CHECK_VALUE(first >= 0 && last >= 1 && first <= INT32_MAX && last <= INT32_MAX && count <= INT32_MAX && first + last <= count,
+                    "expected first >= 0, last >= 1 and count >= first + last, got first ", first, ", last ", last, ", count ", count);
+  require_bounds_of(bounds, cache);
+  require_on_gpu(q_in, cache, "q");
+  const at::Tensor q = usable(q_in);
+  a.bounds = bounds.desc;
+  a.q = describe_row_tensor(q, "q", false);
+  const auto options = table.options();
+  const at::Tensor tables = at::empty({q.size(0), c.kv_heads, q.size(2), count}, options);
+  const at::Tensor table_lengths = at::empty({q.size(0), c.kv_heads, q.size(2)}, options);
+  if (tables.numel() == 0) return {tables, table_lengths};
+  a.tables = static_cast<int32_t*>(tables.data_ptr());
+  a.table_lengths = static_cast<int32_t*>(table_lengths.data_ptr());
+  a.count = (int32_t)count, a.first = (int32_t)first, a.last = (int32_t)last;
+  a.workspace_bytes = page_lib.choose_workspace_bytes(&a);
+  at::Tensor workspace;
+  if (a.workspace_bytes != 0) {
+    workspace = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
+    a.workspace = workspace.data_ptr();
+  }
+  check_cache_call(on_stream_of(q, [&](void* stream) { return page_lib.choose(&a, stream); }), "splash_cache_choose");
+  return {tables, table_lengths};
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// rotary positions (rotary.py)
+// ------------------------------------------------------------------------------------------------------------------
+int (*rotate_library)(const SplashRotateArgs*, void*) = nullptr;
+
+void bind_rotary_library(uintptr_t rotate) { rotate_library = reinterpret_cast<decltype(rotate_library)>(rotate); }
+
+// What the layers of a model share.
+struct RotaryTable {
+  at::Tensor turns;  // int64 [dim / 2], the bits of unsigned numbers
+  int dim;
+  bool interleaved;
+  double factor;
+};
+
+// x and, where there is one, z, turned by their positions (or back).
+std::tuple<at::Tensor, at::Tensor> rotated(const RotaryTable& table, const at::Tensor& positions, const at::Tensor& x, const Maybe& z, bool inverse) {
+  at::Tensor out[2];
+  SplashRotateArgs a{};
+  at::Tensor in[2];
+  for (int i = 0; i < 2; ++i) {
+    if (i == 1 && !z.has_value()) continue;
+    const at::Tensor& t = i == 0 ? x : *z;
+    in[i] = usable(t);
+    out[i] = at::empty_like(in[i]);  // (in the order of the input's dense strides)
+    if (out[i].numel() == 0) continue;
+    if (usable(out[i]).data_ptr() != out[i].data_ptr()) out[i] = at::empty(in[i].sizes(), in[i].options());
+    a.x[i] = describe_row_tensor(in[i], "rotate", true);
+    a.y[i] = describe_row_tensor(out[i], "rotate", true);
+  }
+  if (a.x[0].data != nullptr || a.x[1].data != nullptr) {
+    a.positions = positions.data_ptr();
+    a.positions_are_64 = positions.scalar_type() == at::kLong;
+    a.position_stride = positions.size(0) == 1 ? 0 : positions.stride(0);
+    a.turns = static_cast<const uint64_t*>(table.turns.data_ptr());
+    a.dim = table.dim;
+    a.interleaved = table.interleaved;
+    a.inverse = inverse;
+    a.factor = (float)table.factor;
+    const int status = on_stream_of(x, [&](void* stream) { return rotate_library(&a, stream); });
+    if (status != 0) raise_status(status, "splash_rotate");
+  }
+  return {out[0], out[1]};
+}
+
+struct RotaryCall : torch::CustomClassHolder {
+  std::shared_ptr<const RotaryTable> table;
+  bool inverse;
+};
+
+// Its own gradient, the other way round: it can be differentiated any number of times.
+struct Rotation : torch::autograd::Function<Rotation> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& positions, const at::Tensor& x, const Maybe& z,
+                               const c10::intrusive_ptr<RotaryCall>& call) {
+    auto [y, w] = rotated(*call->table, positions, x, z, call->inverse);
+    ctx->save_for_backward({positions});
+    ctx->saved_data["call"] = c10::IValue::make_capsule(call);
+    ctx->set_materialize_grads(false);
+    return z.has_value() ? variable_list{y, w} : variable_list{y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const at::Tensor positions = ctx->get_saved_variables()[0];
+    const auto call = c10::static_intrusive_pointer_cast<RotaryCall>(ctx->saved_data["call"].toCapsule());
+    auto back = c10::make_intrusive<RotaryCall>();
+    back->table = call->table;
+    back->inverse = !call->inverse;
+    at::Tensor found[2];
+    const at::Tensor dy = ctx->needs_input_grad(1) ? grads[0] : at::Tensor();
+    const at::Tensor dw = grads.size() > 1 && ctx->needs_input_grad(2) ? grads[1] : at::Tensor();
+    if (dy.defined() || dw.defined()) {
+      const variable_list out = Rotation::apply(positions, dy.defined() ? dy : dw, dy.defined() && dw.defined() ? Maybe(dw) : Maybe(), back);
+      if (dy.defined()) found[0] = out[0];
+      if (dw.defined()) found[1] = out[dy.defined() ? 1 : 0];
+    }
+    return {at::Tensor(), found[0], found[1], at::Tensor()};
+  }
+};
+
+std::tuple<at::Tensor, Maybe> rotate(const std::shared_ptr<RotaryTable>& table, const at::Tensor& positions_in, const at::Tensor& q, const Maybe& k) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "rotate cannot be recorded by torch.jit.trace");
+  const auto type = positions_in.scalar_type();
+  TORCH_CHECK_VALUE(type == at::kInt || type == at::kLong, "positions are int32 or int64, got ", type);
+  TORCH_CHECK_VALUE(q.dim() == 4 && (positions_in.dim() == 1 || positions_in.dim() == 2), "expected q and k of [B, heads, T, D] and positions of [B, T] or [T]");
+  at::Tensor positions = positions_in.dim() == 1 ? positions_in.unsqueeze(0) : positions_in;
+  TORCH_CHECK_VALUE((positions.size(0) == 1 || positions.size(0) == q.size(0)) && positions.size(1) == q.size(2), "positions ", positions_in.sizes(),
+                    " do not match q ", q.sizes());
+  const at::Tensor* const both[2] = {&q, k.has_value() ? &*k : nullptr};
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor* const t = both[i];
+    if (t == nullptr) continue;
+    const char* const name = i == 0 ? "q" : "k";
+    TORCH_CHECK_VALUE(t->dim() == 4 && t->size(0) == q.size(0) && t->size(2) == q.size(2) && t->size(3) == q.size(3), "k ", t->sizes(),
+                      " does not match q ", q.sizes());
+    TORCH_CHECK_VALUE(t->scalar_type() == q.scalar_type(), "q and k have one type, got ", q.scalar_type(), " and ", t->scalar_type());
+    TORCH_CHECK_NOT_IMPLEMENTED(!(t->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()), name,
+                                " has a tangent of forward mode: rotate has none");
+    require_row_type(t->scalar_type(), name, true);
+  }
+  TORCH_CHECK_VALUE(q.size(3) % 8 == 0 && table->dim <= q.size(3), "rows of ", q.size(3), " channels: expected a multiple of 8, ", table->dim, " at least");
+  TORCH_CHECK_NOT_IMPLEMENTED(q.size(3) <= 256, "rows of ", q.size(3), " channels are not built (256 at most)");
+  for (int i = 0; i < 2; ++i) {
+    if (both[i] == nullptr) continue;
+    const at::Device device = both[i]->device();
+    TORCH_CHECK(device.is_cuda(), i == 0 ? "q" : "k", " is on ", device, ": the kernels need a CUDA device");
+    TORCH_CHECK_VALUE(device == table->turns.device(), i == 0 ? "q" : "k", " is on ", device, ", the rotary table on ", table->turns.device());
+  }
+  TORCH_CHECK_VALUE(positions.device() == q.device(), "positions are on ", positions.device(), ", q on ", q.device());
+  if (positions.size(1) > 1 && positions.stride(1) != 1) positions = positions.contiguous();
+  if (!(at::GradMode::is_enabled() && (q.requires_grad() || (k.has_value() && k->requires_grad())))) {
+    const auto [y, w] = rotated(*table, positions, q, k, false);
+    return {y, k.has_value() ? Maybe(w) : Maybe()};
+  }
+  auto call = c10::make_intrusive<RotaryCall>();
+  call->table = table;
+  call->inverse = false;
+  variable_list out;
+  {
+    const WithoutGil release;
+    out = Rotation::apply(positions, q, k, call);
+  }
+  return {out[0], k.has_value() ? Maybe(out[1]) : Maybe()};
 }
 
 }  // namespace
@@ -482,6 +706,13 @@ PYBIND11_MODULE(_splash_torch, m) {
   m.def("bind_cache_library", &bind_cache_library);
   pybind11::class_<KvCache>(m, "KvCache")
       .def(pybind11::init<at::Tensor, at::Tensor, at::Tensor, at::Tensor, int, int, int, int, int, int>());
+  m.def("bind_page_library", &bind_page_library);
+  m.def("bind_rotary_library", &bind_rotary_library);
+  pybind11::class_<PageBounds>(m, "PageBounds").def(pybind11::init<at::Tensor, at::Tensor>());
+  m.def("cache_bound", torch::wrap_pybind_function(cache_bound));
+  m.def("cache_choose", torch::wrap_pybind_function(cache_choose));
+  pybind11::class_<RotaryTable, std::shared_ptr<RotaryTable>>(m, "RotaryTable").def(pybind11::init<at::Tensor, int, bool, double>());
+  m.def("rotate", torch::wrap_pybind_function(rotate));
   m.def("cache_append", torch::wrap_pybind_function(cache_append));
   m.def("cache_read", torch::wrap_pybind_function(cache_read));
   m.def("cache_attend", torch::wrap_pybind_function(cache_attend));

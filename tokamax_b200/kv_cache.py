@@ -13,6 +13,9 @@ Formats:
               ``value = zero + scale * code``, ``zero`` the least value of the group, ``scale`` a fifteenth of its range
   ``"e4m3"``  e4m3 values with a bf16 scale for the row, ``scale = amax / 448``
 
+Long contexts need not be attended to as a whole: :func:`bound_pages` keeps bounds of the keys of each page, :func:`choose_pages`
+the pages for each kv head and query whose bounds allow the largest logits, and :func:`attend` goes over those alone.
+
 Tokens lie in pages of ``page_size`` tokens.  A token's place is its slot, ``page * page_size + offset``; a sequence's pages
 are a row of the page table.  Whoever owns the cache hands pages out; :func:`slots_of` turns positions into slots.
 
@@ -133,6 +136,59 @@ def read(cache: KVCache, page_table: torch.Tensor, lengths: torch.Tensor, max_le
   return _native.host().cache_read(cache.native, page_table, lengths, max_len, dtype)
 
 
+@dataclasses.dataclass(frozen=True, eq=False)
+class PageBounds:
+  """The least and the largest key of each channel of a cache's pages, in 8 bits; made by :func:`make_page_bounds`.
+
+  ``codes`` is int8 ``[n_pages, kv_heads, 2, bytes of a row]`` (the least values, then the largest), ``scales`` float32
+  ``[n_pages, kv_heads]``: ``value = scale * code``."""
+  codes: torch.Tensor
+  scales: torch.Tensor
+  head_dim: int
+  native: object = dataclasses.field(repr=False)
+
+  def values(self) -> torch.Tensor:
+    """The bounds that the codes stand for, float32 ``[n_pages, kv_heads, 2, head_dim]``."""
+    return self.codes[..., :self.head_dim] * self.scales[:, :, None, None]
+
+
+def make_page_bounds(cache: KVCache) -> PageBounds:
+  """Bounds for the pages of ``cache``, all of them 0; :func:`bound_pages` writes them as pages fill."""
+  codes = torch.zeros((*cache.k_codes.shape[:2], 2, _row_k(cache)), dtype=torch.int8, device=cache.device)
+  scales = torch.zeros(cache.k_codes.shape[:2], dtype=torch.float32, device=cache.device)
+  return PageBounds(codes, scales, cache.head_dim, _native.host().PageBounds(codes, scales))
+
+
+def _row_k(cache: KVCache) -> int:
+  return cache.k_codes.shape[3] * (2 if cache.fmt == "int4" else 1)
+
+
+def bound_pages(cache: KVCache, bounds: PageBounds, page_table: torch.Tensor, lengths: torch.Tensor, newest: int) -> None:
+  """Writes the bounds of the pages that the newest ``newest`` tokens of every sequence have made whole (called after
+  :func:`append`, with as many tokens as that has brought the longest growth of a sequence; more do no harm).
+
+  ``lengths [B]`` counts the tokens in the cache, the new ones among them.  A page that is still filling needs no bounds: it is
+  the newest tokens' own, which :func:`choose_pages` always takes.  What the bounds are of is read back from the cache, so that they
+  are the same whatever calls its tokens came in; a page that is taken for another sequence gets its own as it fills."""
+  _native.host().cache_bound(cache.native, bounds.native, page_table, lengths, newest)
+
+
+def choose_pages(cache: KVCache, bounds: PageBounds, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, count: int, *,
+                 first: int = 1, last: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
+  """For every kv head and each of the newest T tokens the ``count`` pages whose keys' bounds allow the largest logits.
+
+  ``q [B, q_heads, T, D]`` (bf16 or f16), ``page_table [B, pages]`` and ``lengths [B]`` as for :func:`attend`: query i stands at
+  position ``lengths[b] - T + i`` and may go over the pages up to its own.  Its ``last`` newest pages (its own among them) and
+  the sequence's ``first`` ones are always taken, the others by their score: the largest, over the q heads of the kv head, of
+  ``sum_c q_c (largest_c if q_c > 0 else least_c)``, of equal ones the first.  q is held in 8 bits for it, as the bounds are, and
+  scores are whole numbers times a page's scale: the choice does not depend on any order of summation.  (For a positive ``logits_scale``.)
+
+  Returns ``tables [B, kv_heads, T, count]``, the pages taken in the order of the sequence, then -1, and ``lengths [B, kv_heads, T]``, the
+  tokens on them up to the query's: what :func:`attend` takes in the place of the page table and the lengths.  Sequences of up to
+  ``count`` pages are attended to as a whole.  Pages outside the cache (-1) are not chosen."""
+  return _native.host().cache_choose(cache.native, bounds.native, q, page_table, lengths, count, first, last)
+
+
 def attend(cache: KVCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *, logits_scale: float = 1.0,
            local_window_size: int | None = None, logits_soft_cap: float | None = None, sinks: torch.Tensor | None = None,
            mask_value: float = DEFAULT_MASK_VALUE, save_residuals: bool = False):
@@ -143,6 +199,9 @@ def attend(cache: KVCache, q: torch.Tensor, page_table: torch.Tensor, lengths: t
   are not seen.  ``sinks [q_heads]`` and ``logits_soft_cap`` mean what they mean for the splash kernels.  A row that sees
   nothing is zeros and its logsumexp and maximum the mask value.  ``save_residuals`` adds ``{"logsumexp", "max_logits"}``
   ``[B, q_heads, T]``.
+
+  ``page_table [B, kv_heads, T, pages]`` with ``lengths [B, kv_heads, T]`` (from :func:`choose_pages`, say) gives every kv head and
+  query pages of its own: the query sees the first ``lengths`` tokens on them.  Such a call takes no ``local_window_size``.
 
   Weights times the scales of V are held to 11 bits (22 for f16 outputs), down to 2^-22 of a row's largest; logits may be up to 2^26 in
   size.  What no query sees, a page's places that were never written among it, has no part.
