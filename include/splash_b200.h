@@ -572,6 +572,8 @@ typedef struct SplashCacheBoundArgs {
   int64_t newest;
 } SplashCacheBoundArgs;
 int splash_cache_bound(const SplashCacheBoundArgs* args, void* cuda_stream);
+/* The bounds that the codes stand for: values fp32 [n_pages, kv_heads, 2, head_dim], 16-byte aligned. */
+int splash_cache_bound_values(const SplashKvCache* cache, const SplashPageBounds* bounds, float* values, void* cuda_stream);
 
 /* For each sequence, kv head and query the `count` pages whose bounds allow the largest logits.  q [batch, q_heads, q_len, head_dim],
  * bf16 or f16; query i of sequence b stands at position lengths[b] - q_len + i (at the end of the table at most), on its own page.

@@ -148,6 +148,15 @@ def test_c_entry_points_refuse_before_they_touch_the_gpu(kind, path, value, stat
   assert getattr(_native.lib(), fn)(None, None) == -1
 
 
+def test_values_of_bounds_are_checked():
+  lib, a = _native.lib(), _args("SplashCacheBoundArgs")
+  assert lib.splash_cache_bound_values(None, C.byref(a.bounds), 4096, None) == lib.splash_cache_bound_values(C.byref(a.cache), None, 4096, None) == -1
+  for values in (None, 4100):
+    assert lib.splash_cache_bound_values(C.byref(a.cache), C.byref(a.bounds), values, None) == -1
+  a.bounds.scales = None
+  assert lib.splash_cache_bound_values(C.byref(a.cache), C.byref(a.bounds), 4096, None) == -1
+
+
 def test_nothing_new_is_nothing_to_do():
   assert _native.lib().splash_cache_bound(C.byref(_spoilt("SplashCacheBoundArgs", "newest", 0)), None) == 0
 

@@ -40,6 +40,7 @@ def _check_bounds(store, before, bounds, newest, lengths=None, table=None):
         c, s = pages_ref.bounds(k[b, :, j * store.page:(j + 1) * store.page])
         codes[page, :, :, :store.d], codes[page, :, :, store.d:], scales[page] = c, 0, s
   assert torch.equal(bounds.scales.cpu(), scales) and torch.equal(bounds.codes.cpu(), codes)
+  assert torch.equal(bounds.values().cpu(), codes[..., :store.d] * scales[:, :, None, None])  # (one product of 32 bits)
 
 
 @pytest.mark.parametrize("fmt,group", FORMATS)

@@ -357,6 +357,7 @@ _PROTOTYPES = {
     "splash_cache_attend_tables": (C.c_int, [C.POINTER(SplashCacheAttendArgs), C.c_void_p]),
     "splash_cache_attend_tables_workspace_bytes": (C.c_size_t, [C.POINTER(SplashCacheAttendArgs)]),
     "splash_cache_bound": (C.c_int, [C.POINTER(SplashCacheBoundArgs), C.c_void_p]),
+    "splash_cache_bound_values": (C.c_int, [C.POINTER(SplashKvCache), C.POINTER(SplashPageBounds), C.c_void_p, C.c_void_p]),
     "splash_cache_choose": (C.c_int, [C.POINTER(SplashCacheChooseArgs), C.c_void_p]),
     "splash_cache_choose_workspace_bytes": (C.c_size_t, [C.POINTER(SplashCacheChooseArgs)]),
     "splash_rotate": (C.c_int, [C.POINTER(SplashRotateArgs), C.c_void_p]),
@@ -482,7 +483,7 @@ def host():
         module.bind_cache_library(*(C.cast(getattr(handle, name), C.c_void_p).value for name in (
             "splash_cache_append", "splash_cache_read", "splash_cache_attend", "splash_cache_attend_workspace_bytes")))
         module.bind_page_library(*(C.cast(getattr(handle, name), C.c_void_p).value for name in (
-            "splash_cache_attend_tables", "splash_cache_attend_tables_workspace_bytes", "splash_cache_bound", "splash_cache_choose",
+            "splash_cache_attend_tables", "splash_cache_attend_tables_workspace_bytes", "splash_cache_bound", "splash_cache_bound_values", "splash_cache_choose",
             "splash_cache_choose_workspace_bytes")))
         module.bind_rotary_library(C.cast(handle.splash_rotate, C.c_void_p).value)
         module.bind_check(check)

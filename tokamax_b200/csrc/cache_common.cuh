@@ -59,6 +59,27 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
   return r;
 }
 
+// a / b, correctly rounded, for `inverse` = 1 / b, correctly rounded: a product, corrected by the remainder that a fused
+// multiply-add leaves (Markstein 1990, "Computation of elementary functions on the IBM RISC System/6000 processor").  It asks for
+// a b whose significand is not all ones, and for no underflow on the way.
+__device__ __forceinline__ float divide(float a, float b, float inverse) {
+  const float q = a * inverse;
+  return fmaf(fmaf(-q, b, a), inverse, q);
+}
+constexpr float kLeastDivisor = 0x1p-80f;  // below it the division of the hardware's own
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
 inline int log2_of(int power_of_two) {
   int n = 0;
   while ((1 << n) < power_of_two) ++n;

@@ -15,9 +15,46 @@ constexpr float kMostCode = 127.f;
 
 // NaN as 0 and infinities as the largest number.
 __device__ __forceinline__ float as_number(float x) { return x != x ? 0.f : fminf(fmaxf(x, -3.4028234663852886e38f), 3.4028234663852886e38f); }
-// round(x / scale) in -127 .. 127
-__device__ __forceinline__ int code_of(float x, float scale) {
-  return scale > 0.f ? (int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -kMostCode), kMostCode) : 0;
+// With NaN where an operand is NaN.
+__device__ __forceinline__ float least_of(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float largest_of(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Quotients by top / 127, rounded to 32 bits, then to whole numbers in -127 .. 127, as bytes.
+struct Coder {
+  float scale, inverse;  // (inverse 0: the hardware's own division)
+  template <int N>
+  __device__ __forceinline__ void operator()(const float (&x)[N], uint32_t (&codes)[(N + 3) / 4]) const {
+    constexpr float kUnits = 12582912.f;  // 1.5 * 2^23: a sum is rounded to whole numbers, and has one in its low bits
+    float sum[(N + 3) / 4 * 4] = {};
+    if (inverse > 0.f) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum[j] = divide(x[j], scale, inverse) + kUnits;
+    } else if (scale > 0.f) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float q;
+        asm volatile("div.rn.f32 %0, %1, %2;" : "=f"(q) : "f"(x[j]), "f"(scale));  // (volatile: not worked out in any case)
+        sum[j] = fminf(fmaxf(q, -kMostCode), kMostCode) + kUnits;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < N; j += 4)
+      codes[j / 4] = __byte_perm(__byte_perm(__float_as_uint(sum[j]), __float_as_uint(sum[j + 1]), 0x0040),
+                                 __byte_perm(__float_as_uint(sum[j + 2]), __float_as_uint(sum[j + 3]), 0x0040), 0x5410);
+  }
+};
+__device__ __forceinline__ Coder coder_of(float top) {
+  const float scale = __fdiv_rn(top, kMostCode);
+  const bool exact = scale > kLeastDivisor && (~__float_as_uint(scale) & 0x7fffffu) != 0;
+  return {scale, exact ? __frcp_rn(scale) : 0.f};
 }
 
 __device__ __forceinline__ bool in_pool(int page, int64_t n_pages) { return page >= 0 && page < n_pages; }
@@ -33,35 +70,38 @@ struct BoundParams {
   const int32_t* page_table;
   const int32_t* lengths;
   int64_t table_stride, n_pages, newest, batch;
-  int32_t n_table, page_size, page_shift, kv_heads, head_dim, row, group_shift;
+  int32_t n_table, page_size, page_shift, kv_heads, head_dim, row, group_shift, slots, split;
 };
 
-constexpr int kBoundThreads = 256;
+constexpr int kBoundThreads = 256, kBoundWarps = kBoundThreads / 32;
+constexpr int kPiece = 16;  // channels of a lane
 
-// Eight channels of a row in 32 bits, from its codes and the scales of their group.
+// Sixteen channels of a row in 32 bits, from their codes and the scales of their group.
 template <int kFormat>
 struct RowPiece {
-  uint32_t w[kFormat == SPLASH_CACHE_INT4 ? 1 : 2];
-  uint32_t scale;
+  static constexpr int kBytes = kFormat == SPLASH_CACHE_INT4 ? kPiece / 2 : kPiece;
+  uint32_t w[kBytes / 4], scale;
   __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales) {
     if constexpr (kFormat == SPLASH_CACHE_INT4) {
-      w[0] = *reinterpret_cast<const uint32_t*>(codes);
-      scale = *reinterpret_cast<const uint32_t*>(scales);
-    } else {
       const uint2 v = *reinterpret_cast<const uint2*>(codes);
       w[0] = v.x, w[1] = v.y;
+      scale = *reinterpret_cast<const uint32_t*>(scales);
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(codes);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
       scale = (uint32_t)*reinterpret_cast<const uint16_t*>(scales) << 16;
     }
   }
-  __device__ __forceinline__ void get(float (&x)[8]) const {
+  __device__ __forceinline__ void get(float (&x)[kPiece]) const {
     const float s = __uint_as_float(scale & 0xffff0000u);
     if constexpr (kFormat == SPLASH_CACHE_INT4) {
+      // (2^23 + code has the code in its low bits; zero and product are 8 and 12 bits, their sum is rounded once)
       const float zero = bf16_bits_to_float(scale);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = fmaf(s, __uint_as_float(w[0] >> 4 * j & 15u | 0x4b000000u) - 8388608.f, zero);
+      for (int j = 0; j < kPiece; ++j) x[j] = fmaf(s, __uint_as_float(w[j / 8] >> 4 * (j % 8) & 15u | 0x4b000000u) - 8388608.f, zero);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < kPiece / 2; ++j) {
         const uint32_t pair = e4m3x2_to_f16x2(w[j / 2] >> (16 * (j & 1)));
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
         x[2 * j] = s * f.x;
@@ -71,71 +111,134 @@ struct RowPiece {
   }
 };
 
-// A block has a page of a sequence and kv head: blockIdx.x the page (from the first that has become whole), y the head, z the
-// sequence.  A team of row / 8 threads has a token's row, eight channels a thread.
-template <int kFormat>
+constexpr int kWarpTokens = 128;
+
+// `split` warps of a block have a page of a sequence and kv head; blockIdx.x: pages (from the first that has become whole) and
+// heads, the heads fastest; y: the sequence.  A team of kTeam lanes (the power of two that holds the row's width / 16) has a
+// token's row.
+template <int kFormat, int kTeam>
 __global__ void __launch_bounds__(kBoundThreads) cache_bound_kernel(const __grid_constant__ BoundParams p) {
-  extern __shared__ float extremes[];  // [2][teams][row]
-  __shared__ float tops[kBoundThreads / 32];
-  const int head = blockIdx.y;
-  const int team_size = p.row / 8, teams = kBoundThreads / team_size;
-  const int team = threadIdx.x / team_size, part = threadIdx.x % team_size;
-  for (int64_t b = blockIdx.z; b < p.batch; b += gridDim.z) {
+  constexpr int kRows = 32 / kTeam;       // of a warp's load
+  constexpr int kAhead = 4;               // loads in flight
+  constexpr int kOwn = kPiece / kRows;    // channels of a lane once the rows are together
+  static_assert(kOwn >= 2);
+  __shared__ float extremes[kBoundWarps][2][32 * kOwn];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % kTeam, team = lane / kTeam;
+  const int share = warp % p.split;  // of the page's tokens
+  const int64_t items = (int64_t)p.slots * p.kv_heads, step = (int64_t)gridDim.x * (kBoundWarps / p.split);
+  const bool real = part * kPiece < p.row;  // (of teams of 96 and 192 channels some lanes have none)
+  for (int64_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
     const int64_t length = min((int64_t)max(__ldg(p.lengths + b), 0), (int64_t)p.n_table << p.page_shift);
-    const int64_t index = (max(length - p.newest, (int64_t)0) >> p.page_shift) + blockIdx.x;
-    if (index >= length >> p.page_shift) continue;
-    const int page = __ldg(p.page_table + b * p.table_stride + index);
-    if (!in_pool(page, p.n_pages)) continue;
-    const uint32_t row0 = ((uint32_t)page * p.kv_heads + head) << p.page_shift;
-    constexpr int kCodeBytes = kFormat == SPLASH_CACHE_INT4 ? 4 : 8;
-    const int row_bytes = team_size * kCodeBytes, scale_bytes = kFormat == SPLASH_CACHE_INT4 ? (p.row >> p.group_shift) * 4 : 2;
-    const uint8_t* const codes = p.codes + (uint64_t)row0 * (unsigned)row_bytes + part * kCodeBytes;
-    const uint8_t* const scales = p.scales + (uint64_t)row0 * (unsigned)scale_bytes + (kFormat == SPLASH_CACHE_INT4 ? (part * 8 >> p.group_shift) * 4 : 0);
-    float least[8], most[8];
+    const int64_t first = max(length - p.newest, (int64_t)0) >> p.page_shift, whole = length >> p.page_shift;
+    for (int64_t item0 = (int64_t)blockIdx.x * (kBoundWarps / p.split); item0 < items; item0 += step) {
+      if (first + item0 / p.kv_heads >= whole) break;  // (all warps of the block alike)
+      const int64_t item = item0 + warp / p.split, index = first + item / p.kv_heads;
+      const int head = (int)(item % p.kv_heads);
+      const int page = item < items && index < whole ? __ldg(p.page_table + b * p.table_stride + index) : -1;
+      const bool mine = in_pool(page, p.n_pages);
+      float lo[kPiece], hi[kPiece];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) least[j] = INFINITY, most[j] = -INFINITY;
-    if (team < teams) {
-#pragma unroll 4
-      for (int t = team; t < p.page_size; t += teams) {
-        RowPiece<kFormat> piece;
-        piece.load(codes + (int64_t)t * row_bytes, scales + (int64_t)t * scale_bytes);
-        float x[8];
-        piece.get(x);
+      for (int j = 0; j < kPiece; ++j) lo[j] = INFINITY, hi[j] = -INFINITY;
+      const uint32_t row0 = ((uint32_t)max(page, 0) * p.kv_heads + head) << p.page_shift;
+      const int row_bytes = kFormat == SPLASH_CACHE_INT4 ? p.row / 2 : p.row, scale_bytes = kFormat == SPLASH_CACHE_INT4 ? (p.row >> p.group_shift) * 4 : 2;
+      const uint8_t* const codes = p.codes + (uint64_t)row0 * (unsigned)row_bytes + part * RowPiece<kFormat>::kBytes;
+      const uint8_t* const scales = p.scales + (uint64_t)row0 * (unsigned)scale_bytes + (kFormat == SPLASH_CACHE_INT4 ? (part * kPiece >> p.group_shift) * 4 : 0);
+      const int own_tokens = p.page_size / p.split, t0 = share * own_tokens + team, t1 = (share + 1) * own_tokens;
+      auto each = [&](auto&& take) {  // of the lane's tokens, kAhead at a time
+        for (int t = t0; t < t1; t += kRows * kAhead) {
+          RowPiece<kFormat> piece[kAhead];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float v = as_number(x[j]);
-          least[j] = fminf(least[j], v);
-          most[j] = fmaxf(most[j], v);
+          for (int i = 0; i < kAhead; ++i) {
+            const int at = t + i * kRows < t1 ? t + i * kRows : t;  // (one of them twice)
+            piece[i].load(codes + (int64_t)at * row_bytes, scales + (int64_t)at * scale_bytes);
+          }
+#pragma unroll
+          for (int i = 0; i < kAhead; i += 2) {
+            float x[kPiece], y[kPiece];
+            piece[i].get(x);
+            piece[i + 1].get(y);
+#pragma unroll
+            for (int j = 0; j < kPiece; ++j) take(j, x[j], y[j]);
+          }
+        }
+      };
+      if (mine && real) {
+        each([&](int j, float x, float y) {
+          lo[j] = least_of(lo[j], x, y);
+          hi[j] = largest_of(hi[j], x, y);
+        });
+        // What is no number or an infinity shows in the extremes: a second look takes it for what it counts as.
+        bool plain = true;
+#pragma unroll
+        for (int j = 0; j < kPiece; ++j) plain = plain && lo[j] > -INFINITY && hi[j] < INFINITY;  // (not where one is NaN)
+        if (!plain) {
+#pragma unroll
+          for (int j = 0; j < kPiece; ++j) lo[j] = INFINITY, hi[j] = -INFINITY;
+          each([&](int j, float x, float y) {
+            lo[j] = least_of(lo[j], as_number(x), as_number(y));
+            hi[j] = largest_of(hi[j], as_number(x), as_number(y));
+          });
         }
       }
-      float* const mine = extremes + team * p.row + part * 8;
+      // The rows of a warp's load together: at each step a lane keeps half of its channels.
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mine[j] = least[j], mine[teams * p.row + j] = most[j];
-    }
-    __syncthreads();
-    // a thread a channel (rows are no wider than a block)
-    float lo = INFINITY, hi = -INFINITY;
-    const bool mine = threadIdx.x < p.head_dim;
-    for (int t = 0; mine && t < teams; ++t) {
-      lo = fminf(lo, extremes[t * p.row + threadIdx.x]);
-      hi = fmaxf(hi, extremes[(teams + t) * p.row + threadIdx.x]);
-    }
-    float top = mine ? fmaxf(fabsf(lo), fabsf(hi)) : 0.f;
+      for (int d = kTeam, n = kPiece / 2; d < 32; d <<= 1, n >>= 1) {
+        const bool upper = lane & d;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
-    __syncthreads();
+        for (int j = 0; j < n; ++j) {
+          const float give_lo = upper ? lo[j] : lo[j + n], give_hi = upper ? hi[j] : hi[j + n];
+          lo[j] = fminf(upper ? lo[j + n] : lo[j], __shfl_xor_sync(~0u, give_lo, d));
+          hi[j] = fmaxf(upper ? hi[j + n] : hi[j], __shfl_xor_sync(~0u, give_hi, d));
+        }
+      }
+      if (p.split > 1) {
 #pragma unroll
-    for (int w = 0; w < kBoundThreads / 32; ++w) top = fmaxf(top, tops[w]);
-    const float scale = __fdiv_rn(top, kMostCode);
-    const uint64_t at = (uint64_t)((uint32_t)page * p.kv_heads + head);
-    if (threadIdx.x < p.row) {
-      int8_t* const to = p.bound_codes + at * (unsigned)(2 * p.row) + threadIdx.x;
-      to[0] = (int8_t)(mine ? code_of(lo, scale) : 0);
-      to[p.row] = (int8_t)(mine ? code_of(hi, scale) : 0);
+        for (int j = 0; j < kOwn; ++j) extremes[warp][0][j * 32 + lane] = lo[j], extremes[warp][1][j * 32 + lane] = hi[j];
+        __syncthreads();
+        if (share == 0) {
+          for (int w = warp + 1; w < warp + p.split; ++w)
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+              lo[j] = fminf(lo[j], extremes[w][0][j * 32 + lane]);
+              hi[j] = fmaxf(hi[j], extremes[w][1][j * 32 + lane]);
+            }
+        }
+        __syncthreads();
+      }
+      if (share != 0 || !mine) continue;  // (whole warps)
+      // the lane's channels: kOwn from part * 16 on, and those that it gave away before them
+      int channel = part * kPiece;
+#pragma unroll
+      for (int d = kTeam, n = kPiece / 2; d < 32; d <<= 1, n >>= 1) channel += lane & d ? n : 0;
+      float top = 0.f, lo_own[kOwn], hi_own[kOwn];
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) {
+        lo_own[j] = channel + j < p.head_dim ? lo[j] : 0.f;
+        hi_own[j] = channel + j < p.head_dim ? hi[j] : 0.f;
+        top = fmaxf(top, fmaxf(fabsf(lo_own[j]), fabsf(hi_own[j])));
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+      const Coder code = coder_of(top);
+      const uint64_t at = (uint64_t)((uint32_t)page * p.kv_heads + head);
+      if (real) {
+        int8_t* const to = p.bound_codes + at * (unsigned)(2 * p.row) + channel;
+        uint32_t least[(kOwn + 3) / 4], largest[(kOwn + 3) / 4];
+        code(lo_own, least);
+        code(hi_own, largest);
+        if constexpr (kOwn == 2) {
+          *reinterpret_cast<uint16_t*>(to) = (uint16_t)least[0];
+          *reinterpret_cast<uint16_t*>(to + p.row) = (uint16_t)largest[0];
+        } else {
+#pragma unroll
+          for (int j = 0; j < kOwn / 4; ++j) {
+            *reinterpret_cast<uint32_t*>(to + 4 * j) = least[j];
+            *reinterpret_cast<uint32_t*>(to + p.row + 4 * j) = largest[j];
+          }
+        }
+      }
+      if (lane == 0) p.bound_scales[at] = code.scale;
     }
-    if (threadIdx.x == 0) p.bound_scales[at] = scale;
-    __syncthreads();  // (before `extremes` and `tops` are written again)
   }
 }
 
@@ -179,12 +282,52 @@ static int cache_bound(const SplashCacheBoundArgs& a, cudaStream_t stream) {
   p.group_shift = log2_of(c.group);
   // n tokens make n / page_size + 1 pages whole at most
   const int64_t pages = a.newest / c.page_size + 1;
-  const dim3 grid((unsigned)(pages < a.n_table ? pages : a.n_table), (unsigned)c.kv_heads, (unsigned)(a.batch < 65535 ? a.batch : 65535));
-  const int team = c.row_k / 8, smem = 2 * (kBoundThreads / team) * c.row_k * (int)sizeof(float);  // 16 KB at most
+  p.slots = (int32_t)(pages < a.n_table ? pages : a.n_table);
+  // A warp has up to kWarpTokens of a page's tokens, as far as the warps of a block go.
+  p.split = 1;
+  while (p.split < kBoundWarps && p.split * kWarpTokens < c.page_size) p.split *= 2;
+  const int per_block = kBoundWarps / p.split;
+  const int64_t blocks = ((int64_t)p.slots * c.kv_heads + per_block - 1) / per_block;
+  const dim3 grid((unsigned)(blocks < INT32_MAX ? blocks : INT32_MAX), (unsigned)(a.batch < 65535 ? a.batch : 65535));
+  auto launch = [&](auto format) {
+    constexpr int kFormat = decltype(format)::value;
+    if (c.row_k <= 64)
+      cache_bound_kernel<kFormat, 4><<<grid, kBoundThreads, 0, stream>>>(p);
+    else if (c.row_k <= 128)
+      cache_bound_kernel<kFormat, 8><<<grid, kBoundThreads, 0, stream>>>(p);
+    else
+      cache_bound_kernel<kFormat, 16><<<grid, kBoundThreads, 0, stream>>>(p);
+  };
   if (c.format == SPLASH_CACHE_INT4)
-    cache_bound_kernel<SPLASH_CACHE_INT4><<<grid, kBoundThreads, smem, stream>>>(p);
+    launch(std::integral_constant<int, SPLASH_CACHE_INT4>{});
   else
-    cache_bound_kernel<SPLASH_CACHE_E4M3><<<grid, kBoundThreads, smem, stream>>>(p);
+    launch(std::integral_constant<int, SPLASH_CACHE_E4M3>{});
+  return cudaGetLastError() == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
+}
+
+// A thread has eight channels of one side of a page and head.
+__global__ void __launch_bounds__(kBoundThreads) cache_bound_values_kernel(const int8_t* codes, const float* scales, float* out, uint32_t sides,
+                                                                           int row, int vectors) {
+  const uint64_t step = (uint64_t)gridDim.x * kBoundThreads, all = (uint64_t)sides * (unsigned)vectors;
+  for (uint64_t at = (uint64_t)blockIdx.x * kBoundThreads + threadIdx.x; at < all; at += step) {
+    const uint32_t side = (uint32_t)(all >> 32 == 0 ? (uint32_t)at / (unsigned)vectors : at / (unsigned)vectors);
+    const uint32_t part = (uint32_t)(at - (uint64_t)side * (unsigned)vectors);
+    const float scale = __ldg(scales + side / 2);
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + (uint64_t)side * (unsigned)row + part * 8));
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = scale * (float)(int8_t)((j < 4 ? w.x : w.y) >> 8 * (j % 4) & 255u);
+    store8(out, SPLASH_F32, (int64_t)(at * 8), x);
+  }
+}
+
+static int cache_bound_values(const SplashKvCache& c, const SplashPageBounds& bounds, float* values, cudaStream_t stream) {
+  if (const int status = check_cache(c)) return status;
+  if (const int status = check_bounds(bounds)) return status;
+  if (values == nullptr || (reinterpret_cast<uintptr_t>(values) & 15u) != 0) return SPLASH_ERR_INVALID_ARGUMENT;
+  const int64_t sides = c.n_pages * c.kv_heads * 2, blocks = (sides * (c.head_dim / 8) + kBoundThreads - 1) / kBoundThreads;
+  cache_bound_values_kernel<<<(unsigned)(blocks < kSms * 16 ? blocks : kSms * 16), kBoundThreads, 0, stream>>>(bounds.codes, bounds.scales, values,
+                                                                                                         (uint32_t)sides, c.row_k, c.head_dim / 8);
   return cudaGetLastError() == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
 }
 
@@ -204,10 +347,11 @@ struct ChooseParams {
   int32_t dtype, batch, kv_heads, heads_per_kv, q_len, n_table, page_size, page_shift, head_dim, row, count, first, last;
 };
 
-constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;
-constexpr int kKeysOnChip = 32768;  // pages of a row whose scores shared memory holds
-constexpr int kMostCluster = 8;
-constexpr int kBins = 2048, kBinBits = 11;
+constexpr int kKeysOnChip = 8192;       // pages of a row whose scores, and numbers, shared memory holds
+constexpr int kChooseShared = 220 * 1024;  // for a CTA, beside some 6 KB of fixed size
+constexpr int kMostCluster = 8, kMostChooseWarps = 8, kFewPages = 1024;
+constexpr int kBins = 1024, kBinBits = 10;
+constexpr int kFew = 64;  // keys that are counted against each other
 // Scores as unsigned numbers of the same order; 0: no candidate, kAlways: taken before all others.
 constexpr uint32_t kNoCandidate = 0, kAlways = ~0u;
 __device__ __forceinline__ uint32_t key_of(float score) {
@@ -222,177 +366,222 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Shared memory of a CTA: q's codes [heads, to a multiple of 8][2 * row, and 64 bytes], then the keys (of the cluster's first CTA).
+// Shared memory of a CTA: q's codes [heads, to a multiple of 8][2 * row, and 64 bytes], then the keys and the pages' numbers
+// (of the cluster's first CTA).
 __host__ __device__ constexpr int choose_pitch(int row) { return 2 * row + 64; }
 __host__ __device__ constexpr int choose_heads(int heads) { return (heads + 7) / 8 * 8; }
 
-struct Found {  // of some of a row's pages
+struct Found {  // of a row's pages
   uint32_t least, most;  // keys but for kAlways
   int candidates, always;
 };
-__device__ __forceinline__ Found join(Found a, Found b) {
-  return {min(a.least, b.least), max(a.most, b.most), a.candidates + b.candidates, a.always + b.always};
-}
-__device__ __forceinline__ Found join_warp(Found f) {
-  return {__reduce_min_sync(~0u, f.least), __reduce_max_sync(~0u, f.most), __reduce_add_sync(~0u, f.candidates), __reduce_add_sync(~0u, f.always)};
-}
-
-// Sum over the threads of a CTA before this one; `total` of all.  One word of `scratch` a warp.
-__device__ __forceinline__ uint64_t sum_before(uint64_t mine, uint64_t* scratch, uint64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint64_t sum = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const uint64_t other = __shfl_up_sync(~0u, sum, d);
-    if (lane >= d) sum += other;
-  }
-  if (lane == 31) scratch[warp] = sum;
-  __syncthreads();
-  uint64_t before = sum - mine;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kChooseWarps; ++w) {
-    before += w < warp ? scratch[w] : 0;
-    total += scratch[w];
-  }
-  __syncthreads();
-  return before;
-}
 
 // A cluster (of one CTA and more) has a query and kv head: its CTAs score pages, tile by tile of 16, and the first one chooses.
-__global__ void __launch_bounds__(kChooseThreads) cache_choose_kernel(const __grid_constant__ ChooseParams p) {
+// kChunks: pieces of 64 numbers that the bounds of a page are; kOnChip: the scores are in shared memory.
+template <int kChunks, int kWarps, bool kOnChip>
+__global__ void __launch_bounds__(kWarps * 32, (kChunks <= 4 ? 16 : 8) / kWarps) cache_choose_kernel(const __grid_constant__ ChooseParams p) {
+  constexpr int kThreads = kWarps * 32, kRow = kChunks * 32, kPitch = choose_pitch(kRow);
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ uint64_t scratch[kChooseWarps];
-  __shared__ Found parts[kMostCluster * kChooseWarps];
-  __shared__ uint32_t bins[kBins];
-  __shared__ uint32_t found_bin[2];
+  __shared__ __align__(16) Found found;
+  __shared__ __align__(16) uint32_t bins[kBins];
+  __shared__ __align__(16) uint2 few[kFew];  // keys and their places
+  __shared__ __align__(16) uint32_t tops[kWarps], sums[kWarps];
+  __shared__ uint32_t counts[kWarps][2], picked[3], few_count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   uint32_t ctas, rank;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const uint32_t row = blockIdx.x / ctas;  // (sequence, kv head, query)
   const int i = row % (unsigned)p.q_len, head = row / (unsigned)p.q_len % (unsigned)p.kv_heads, b = row / (unsigned)p.q_len / (unsigned)p.kv_heads;
-  if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const int length = __ldg(p.lengths + b);
 
+  // ---- a warp's tiles: 16 pages each, their bounds as operands of the products ----
+  const int32_t* const table = p.page_table + b * p.table_stride;
+  const int step = (int)ctas * kWarps * 16;
+  const int first = ((int)rank + warp * (int)ctas) * 16;
+  // Numbers of pages for two tiles at a time: lane i has page i % 16 of tile turn + i / 16 (behind the table: not looked at).
+  auto look_up = [&](int turn) { return __ldg(table + min(first + (turn + (lane >> 4)) * step + (lane & 15), p.n_table - 1)); };
+  int numbers_now = look_up(0), numbers_next = look_up(2);
+  struct Tile {
+    uint4 a[kChunks], a8[kChunks];  // of rows g and g + 8
+    float scale;                    // of lanes 0 and 1 of four: row g's and row g + 8's
+    int page;                       // the same
+  };
+  auto load_tile = [&](Tile& tile, int numbers, int which) {  // (what is no candidate is read as page 0)
+    const int page0 = __shfl_sync(~0u, numbers, which * 16 + g), page1 = __shfl_sync(~0u, numbers, which * 16 + 8 + g);
+    const uint32_t at0 = (uint32_t)(in_pool(page0, p.n_pages) ? page0 : 0) * p.kv_heads + head;
+    const uint32_t at1 = (uint32_t)(in_pool(page1, p.n_pages) ? page1 : 0) * p.kv_heads + head;
+    const uint4* const from0 = reinterpret_cast<const uint4*>(p.bound_codes + (uint64_t)at0 * (2 * kRow)) + t4;
+    const uint4* const from1 = reinterpret_cast<const uint4*>(p.bound_codes + (uint64_t)at1 * (2 * kRow)) + t4;
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) tile.a[k] = __ldg(from0 + k * 4), tile.a8[k] = __ldg(from1 + k * 4);
+    tile.scale = __ldg(p.bound_scales + (t4 & 1 ? at1 : at0));
+    tile.page = t4 & 1 ? page1 : page0;
+  };
+  // a thread has eight channels of every kThreads / (kRow / 8)-th head; the first head's stay with it
+  constexpr int kVectors = kRow / 8, kAtOnce = kThreads / kVectors;
+  const int vectors = p.head_dim / 8, heads = choose_heads(p.heads_per_kv), d = tid % kVectors, h_first = tid / kVectors;
+  const bool in_row = d < vectors && h_first < kAtOnce;
+  const uint16_t* const q = static_cast<const uint16_t*>(p.q) + b * p.q_stride_b + (int64_t)head * p.heads_per_kv * p.q_stride_h + i * p.q_stride_s;
+  auto load_q = [&](int h) {  // (rows that make up eight repeat the first one)
+    return __ldg(reinterpret_cast<const uint4*>(q + (h < p.heads_per_kv ? h : 0) * p.q_stride_h + d * 8));
+  };
+  uint4 q_first = make_uint4(0, 0, 0, 0);
+  if (in_row) q_first = load_q(h_first);
+  for (int k = tid * 4; k < kBins; k += kThreads * 4) *reinterpret_cast<uint4*>(bins + k) = make_uint4(0, 0, 0, 0);
+  if (tid == 0) {
+    few_count = 0;
+    found = {~0u, 0u, 0, 0};
+  }
+  __syncwarp();
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const int64_t reach = (int64_t)p.n_table << p.page_shift;
-  const int position = (int)min(max((int64_t)__ldg(p.lengths + b) - p.q_len + i, (int64_t)-1), reach - 1);
+  const int position = (int)min(max((int64_t)length - p.q_len + i, (int64_t)-1), reach - 1);
   const int own = position >> p.page_shift, pages = own + 1;  // (-1 and 0 before the sequence)
 
   // ---- q in 8 bits ----
-  const int vectors = p.head_dim / 8, pitch = choose_pitch(p.row);
-  const uint16_t* const q = static_cast<const uint16_t*>(p.q) + b * p.q_stride_b + (int64_t)head * p.heads_per_kv * p.q_stride_h + i * p.q_stride_s;
-  auto load_q = [&](int at, float (&x)[8]) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(q + at / vectors * p.q_stride_h + at % vectors * 8));
+  auto numbers = [&](const uint4& w, float (&x)[8]) {
     unpack16(p.dtype, w.x, x[0], x[1]);
     unpack16(p.dtype, w.y, x[2], x[3]);
     unpack16(p.dtype, w.z, x[4], x[5]);
     unpack16(p.dtype, w.w, x[6], x[7]);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = as_number(x[k]);
   };
-  float x[8] = {}, top = 0.f;
-  for (int at = tid; at < vectors * p.heads_per_kv; at += kChooseThreads) {
-    load_q(at, x);
+  auto top_of = [&](const uint4& w) {  // the largest size as bits, which sizes are in the order of; infinity for what is no number
+    float x[8], top = 0.f;
+    numbers(w, x);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k]));
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-  float* const tops = reinterpret_cast<float*>(scratch);
+    for (int k = 0; k < 8; k += 2) top = largest_of(top, fabsf(x[k]), fabsf(x[k + 1]));
+    return min(__float_as_uint(top), 0x7f800000u);
+  };
+  uint32_t top = top_of(q_first);
+  if (in_row)
+    for (int h = h_first + kAtOnce; h < p.heads_per_kv; h += kAtOnce) top = max(top, top_of(load_q(h)));
+  top = __reduce_max_sync(~0u, top);
   if (lane == 0) tops[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kChooseWarps; ++w) top = fmaxf(top, tops[w]);
-  const float scale = __fdiv_rn(top, kMostCode);
-  const int heads = choose_heads(p.heads_per_kv), row_vectors = p.row / 8;
-  for (int at = tid; at < heads * row_vectors; at += kChooseThreads) {
-    const int h = at / row_vectors, d = at % row_vectors;
-    uint32_t negative[2] = {0, 0}, positive[2] = {0, 0};
-    if (d < vectors) {
-      load_q((h < p.heads_per_kv ? h : 0) * vectors + d, x);  // (rows that make up eight repeat the first one)
+  for (int w = 0; w < kWarps; ++w) top = max(top, tops[w]);
+  const bool finite = top < 0x7f800000u;
+  if (!finite) {  // (all threads alike) once more, with each number as what it counts as
+    float most = 0.f;
+    if (in_row)
+      for (int h = h_first; h < p.heads_per_kv; h += kAtOnce) {
+        float x[8];
+        numbers(load_q(h), x);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int code = code_of(x[k], scale);
-        negative[k / 4] |= (uint32_t)(min(code, 0) & 255) << 8 * (k % 4);
-        positive[k / 4] |= (uint32_t)max(code, 0) << 8 * (k % 4);
+        for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(as_number(x[k])));
       }
+    __syncthreads();
+    top = __reduce_max_sync(~0u, __float_as_uint(most));
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = max(top, tops[w]);
+  }
+  Tile tile;
+  if (first < pages) load_tile(tile, numbers_now, 0);
+  const Coder coder = coder_of(__uint_as_float(top));
+  if (h_first < kAtOnce) {
+    for (int h = h_first; h < heads; h += kAtOnce) {
+      uint32_t negative[2] = {0, 0}, positive[2] = {0, 0};
+      if (d < vectors) {
+        float x[8];
+        uint32_t codes[2];
+        numbers(h == h_first ? q_first : load_q(h), x);
+        if (!finite) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = as_number(x[k]);
+        }
+        coder(x, codes);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t below;  // of each byte its sign
+          asm("prmt.b32 %0, %1, 0, 0xba98;" : "=r"(below) : "r"(codes[k]));
+          negative[k] = codes[k] & below;
+          positive[k] = codes[k] & ~below;
+        }
+      }
+      *reinterpret_cast<uint2*>(smem + h * kPitch + d * 8) = make_uint2(negative[0], negative[1]);
+      *reinterpret_cast<uint2*>(smem + h * kPitch + kRow + d * 8) = make_uint2(positive[0], positive[1]);
     }
-    *reinterpret_cast<uint2*>(smem + h * pitch + d * 8) = make_uint2(negative[0], negative[1]);
-    *reinterpret_cast<uint2*>(smem + h * pitch + p.row + d * 8) = make_uint2(positive[0], positive[1]);
   }
   __syncthreads();
 
   // ---- scores ----
-  uint32_t* const own_keys = p.keys != nullptr ? p.keys + (uint64_t)row * p.n_table : reinterpret_cast<uint32_t*>(smem + heads * pitch);
+  uint32_t* own_keys;  // and, in shared memory, the pages' numbers behind them
+  if constexpr (kOnChip)
+    own_keys = reinterpret_cast<uint32_t*>(smem + heads * kPitch);
+  else
+    own_keys = p.keys + (uint64_t)row * p.n_table;
   uint32_t* to_keys = own_keys;
-  Found* to_parts = parts;
+  Found* to_found = &found;
   if (ctas > 1) {
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // (the first CTA is there)
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // (the first CTA is there)
     uint64_t at;
-    if (p.keys == nullptr) {
+    if constexpr (kOnChip) {
       asm("mapa.u64 %0, %1, 0;" : "=l"(at) : "l"(reinterpret_cast<uint64_t>(own_keys)));
       to_keys = reinterpret_cast<uint32_t*>(at);
     }
-    asm("mapa.u64 %0, %1, 0;" : "=l"(at) : "l"(reinterpret_cast<uint64_t>(to_parts)));
-    to_parts = reinterpret_cast<Found*>(at);
+    asm("mapa.u64 %0, %1, 0;" : "=l"(at) : "l"(reinterpret_cast<uint64_t>(to_found)));
+    to_found = reinterpret_cast<Found*>(at);
   }
-  Found found{~0u, 0u, 0, 0};
-  const int32_t* const table = p.page_table + b * p.table_stride;
-  const int step = (int)ctas * kChooseWarps * 16, chunks = p.row / 32;
-  auto look_up = [&](int index) {
-    const int page = index < pages ? __ldg(table + index) : -1;
-    return in_pool(page, p.n_pages) ? page : -1;
-  };
-  int first = ((int)rank + warp * (int)ctas) * 16;
-  int page0 = look_up(first + g), page1 = look_up(first + 8 + g);
-  for (; first < pages; first += step) {
-    const int next0 = look_up(first + step + g), next1 = look_up(first + step + 8 + g);
-    // (pages that are no candidates are read as page 0)
-    const uint64_t at0 = (uint64_t)max(page0, 0) * p.kv_heads + head, at1 = (uint64_t)max(page1, 0) * p.kv_heads + head;
-    const uint4* const from0 = reinterpret_cast<const uint4*>(p.bound_codes + at0 * (unsigned)(2 * p.row)) + t4;
-    const uint4* const from1 = reinterpret_cast<const uint4*>(p.bound_codes + at1 * (unsigned)(2 * p.row)) + t4;
-    const int mine = t4 & 1;  // lanes 0 and 1 of four have a page each
-    const float page_scale = __ldg(p.bound_scales + (mine ? at1 : at0));
+  uint32_t least = ~0u, most = 0;
+  int candidates = 0, always = 0;
+  for (int turn = 0, at = first; at < pages; ++turn, at += step) {
+    Tile next;
+    if (at + step < pages) load_tile(next, turn & 1 ? numbers_next : numbers_now, ~turn & 1);
+    if (turn & 1) {
+      numbers_now = numbers_next;
+      numbers_next = look_up(turn + 3);
+    }
     int best0 = INT32_MIN, best1 = INT32_MIN;
     for (int h0 = 0; h0 < heads; h0 += 8) {
-      const uint8_t* const codes = smem + (h0 + g) * pitch + t4 * 16;
-      int c[4] = {};
-#pragma unroll 4
-      for (int k = 0; k < chunks; ++k) {
-        const uint4 a = __ldg(from0 + k * 4), a8 = __ldg(from1 + k * 4);
-        const uint4 w = *reinterpret_cast<const uint4*>(codes + k * 64);
-        mma_s8(c, a.x, a8.x, a.y, a8.y, w.x, w.y);
-        mma_s8(c, a.z, a8.z, a.w, a8.w, w.z, w.w);
-      }
-      best0 = max(best0, max(c[0], c[1]));
-      best1 = max(best1, max(c[2], c[3]));
-    }
+      const uint8_t* const codes = smem + (h0 + g) * kPitch + t4 * 16;
+      int c[2][4] = {};  // (two chains)
 #pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      best0 = max(best0, __shfl_xor_sync(~0u, best0, d));
-      best1 = max(best1, __shfl_xor_sync(~0u, best1, d));
-    }
-    const int index = first + mine * 8 + g;
-    if (t4 < 2 && index < pages) {
-      uint32_t key = key_of((float)(mine ? best1 : best0) * page_scale);
-      if ((mine ? page1 : page0) < 0)
-        key = kNoCandidate;
-      else if (index < p.first || index > own - p.last)
-        key = kAlways;
-      to_keys[index] = key;
-      found.candidates += key != kNoCandidate;
-      found.always += key == kAlways;
-      if (key != kNoCandidate && key != kAlways) {
-        found.least = min(found.least, key);
-        found.most = max(found.most, key);
+      for (int k = 0; k < kChunks; ++k) {
+        const uint4 w = *reinterpret_cast<const uint4*>(codes + k * 64), &a = tile.a[k], &a8 = tile.a8[k];
+        mma_s8(c[0], a.x, a8.x, a.y, a8.y, w.x, w.y);
+        mma_s8(c[1], a.z, a8.z, a.w, a8.w, w.z, w.w);
       }
+      best0 = max(best0, max(c[0][0] + c[1][0], c[0][1] + c[1][1]));
+      best1 = max(best1, max(c[0][2] + c[1][2], c[0][3] + c[1][3]));
     }
-    page0 = next0;
-    page1 = next1;
+    // lanes 0 and 1 of four have a page each
+    best0 = max(best0, __shfl_xor_sync(~0u, best0, 2));
+    best1 = max(best1, __shfl_xor_sync(~0u, best1, 2));
+    int best = t4 & 1 ? best1 : best0;
+    best = max(best, __shfl_xor_sync(~0u, t4 & 1 ? best0 : best1, 1));
+    const int index = at + (t4 & 1) * 8 + g;
+    if (t4 < 2 && index < pages) {
+      uint32_t key = key_of((float)best * tile.scale);
+      if (!in_pool(tile.page, p.n_pages)) {
+        key = kNoCandidate;
+      } else if (index < p.first || index > own - p.last) {
+        key = kAlways;
+        ++always;
+        ++candidates;
+      } else {
+        least = min(least, key);
+        most = max(most, key);
+        ++candidates;
+      }
+      to_keys[index] = key;
+      if constexpr (kOnChip) to_keys[p.n_table + index] = (uint32_t)tile.page;
+    }
+    tile = next;
   }
   __syncwarp();
-  found = join_warp(found);
-  if (lane == 0) to_parts[rank * kChooseWarps + warp] = found;
+  least = __reduce_min_sync(~0u, least);
+  most = __reduce_max_sync(~0u, most);
+  candidates = __reduce_add_sync(~0u, candidates);
+  always = __reduce_add_sync(~0u, always);
+  if (lane == 0 && candidates > 0) {
+    atomicMin(&to_found->least, least);
+    atomicMax(&to_found->most, most);
+    atomicAdd(&to_found->candidates, candidates);
+    atomicAdd(&to_found->always, always);
+  }
   __syncwarp();
   if (ctas > 1) {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -401,82 +590,150 @@ __global__ void __launch_bounds__(kChooseThreads) cache_choose_kernel(const __gr
     __syncthreads();
   }
 
-  // ---- the least key that is taken, and how many of those equal to it ----
-  found = {~0u, 0u, 0, 0};
-  for (int w = lane; w < (int)ctas * kChooseWarps; w += 32) found = join(found, parts[w]);
-  found = join_warp(found);
-  uint32_t threshold = 1;  // all candidates
-  int wanted = p.count, equal = INT32_MAX;
-  if (found.candidates > wanted) {
-    wanted -= found.always;  // of the others; fewer than there are
-    // Digits of key - least, from the highest: of each the bin that the wanted-th largest key lies in.
-    const uint32_t range = found.most - found.least;
-    int bits = 32 - __clz(range);  // of the differences
-    uint32_t prefix = 0;           // of the difference, above `bits`
-    threshold = kAlways;
+  // ---- which are taken: keys whose difference from the least, without its low bits, is above `prefix`, and of those that are equal
+  // to it the first `equal` ones ----
+  const Found all_found = found;
+  uint32_t prefix = 0;
+  int bits = 32, equal = INT32_MAX;  // (all)
+  // of eight keys, kThreads (or 32) apart
+  auto load_keys = [&](int at, int until, int apart, uint32_t (&keys)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) keys[k] = at + k * apart < until ? own_keys[at + k * apart] : kNoCandidate;
+  };
+  auto ranked = [](uint32_t key) { return key != kNoCandidate && key != kAlways; };
+  auto high_of = [&](uint32_t key) { return bits == 32 ? 0u : (key - all_found.least) >> bits; };
+  bool by_few = false;
+  if (all_found.candidates > p.count) {
+    int wanted = p.count - all_found.always;  // of the ranked ones; fewer than there are
     equal = 0;
-    while (wanted > 0) {
-      const int shift = max(bits - kBinBits, 0);
-      for (int k = tid; k < kBins; k += kChooseThreads) bins[k] = 0;
-      __syncthreads();
-      for (int k = tid; k < pages; k += kChooseThreads) {
-        const uint32_t key = own_keys[k], difference = key - found.least;
-        if (key != kNoCandidate && key != kAlways && (bits == 32 ? 0 : difference >> bits) == prefix)
-          atomicAdd(&bins[difference >> shift & ((1u << (bits - shift)) - 1)], 1u);
-      }
-      __syncthreads();
-      // bins from the highest: a thread has kBins / kChooseThreads of them
-      constexpr int kEach = kBins / kChooseThreads;
-      uint32_t own_bins[kEach], sum = 0;
+    prefix = ~0u;  // (none of them)
+    bits = 0;
+    if (wanted > 0) {
+      // Digits of the difference, from the highest: of each the bin that the wanted-th largest key lies in.
+      bits = 32 - __clz(all_found.most - all_found.least);
+      prefix = 0;
+      while (true) {
+        const int shift = max(bits - kBinBits, 0);
+        const uint32_t mask = (1u << (bits - shift)) - 1;
+        for (int at = tid; at < pages; at += kThreads * 8) {
+          uint32_t keys[8];
+          load_keys(at, pages, kThreads, keys);
 #pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        own_bins[k] = bins[kBins - 1 - (tid * kEach + k)];
-        sum += own_bins[k];
-      }
-      uint64_t total;
-      uint32_t before = (uint32_t)sum_before(sum, scratch, total);
-      if (before < (uint32_t)wanted && before + sum >= (uint32_t)wanted) {
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-          if (before < (uint32_t)wanted && before + own_bins[k] >= (uint32_t)wanted) {
-            found_bin[0] = kBins - 1 - (tid * kEach + k);
-            found_bin[1] = before;
-          }
-          before += own_bins[k];
+          for (int k = 0; k < 8; ++k)
+            if (ranked(keys[k]) && high_of(keys[k]) == prefix) atomicAdd(&bins[(keys[k] - all_found.least) >> shift & mask], 1u);
         }
+        __syncthreads();
+        // bins from the highest, kEach a thread
+        constexpr int kEach = kBins / kThreads;
+        uint32_t each[kEach], sum = 0;
+#pragma unroll
+        for (int k = 0; k < kEach; k += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(bins + kBins - 4 - k - kEach * tid);
+          each[k] = v.w, each[k + 1] = v.z, each[k + 2] = v.y, each[k + 3] = v.x;
+          sum += v.x + v.y + v.z + v.w;
+        }
+        uint32_t before = sum;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+          const uint32_t other = __shfl_up_sync(~0u, before, s);
+          if (lane >= s) before += other;
+        }
+        if (lane == 31) sums[warp] = before;
+        __syncthreads();
+        before -= sum;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) before += w < warp ? sums[w] : 0;
+        if (before < (uint32_t)wanted && before + sum >= (uint32_t)wanted) {
+#pragma unroll
+          for (int k = 0; k < kEach; ++k) {
+            if (before < (uint32_t)wanted && before + each[k] >= (uint32_t)wanted) {
+              picked[0] = kBins - 1 - kEach * tid - k;
+              picked[1] = before;
+              picked[2] = each[k];
+            }
+            before += each[k];
+          }
+        }
+        __syncthreads();
+        prefix = prefix << (bits - shift) | picked[0];
+        wanted -= (int)picked[1];
+        bits = shift;
+        const int population = (int)picked[2];
+        by_few = population > wanted && population <= kFew;
+        if (bits == 0 || population <= kFew || population == wanted) break;
+        for (int k = tid; k < kBins; k += kThreads) bins[k] = 0;
+        __syncthreads();
       }
-      __syncthreads();
-      prefix = prefix << (bits - shift) | found_bin[0];
-      wanted -= (int)found_bin[1];
-      bits = shift;
-      if (bits == 0) {
-        threshold = found.least + prefix;
-        equal = wanted;
-        break;
-      }
-      __syncthreads();  // (before bins and found_bin are written again)
+      equal = wanted;
     }
   }
 
-  // ---- the pages taken, in order: a thread has a run of them ----
-  const int run = (pages + kChooseThreads - 1) / kChooseThreads, from = min(tid * run, pages), until = min(from + run, pages);
-  uint64_t counts = 0;  // taken whatever comes, and equal to the threshold
-  for (int k = from; k < until; ++k) {
-    const uint32_t key = own_keys[k];
-    counts += (key > threshold || key == kAlways ? 1ull : 0ull) | (key == threshold && key != kAlways ? 1ull << 32 : 0ull);
+  // ---- how many, and where: a warp has a run of pages ----
+  const int run = (pages + kThreads - 1) / kThreads * 32, from = min(warp * run, pages), until = min(from + run, pages);
+  const uint32_t below = (1u << lane) - 1;
+  uint32_t taken[8], alike[8];
+  auto look = [&](int at, uint32_t (&keys)[8]) {
+    load_keys(at + lane, until, 32, keys);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t high = high_of(keys[k]);
+      taken[k] = __ballot_sync(~0u, keys[k] == kAlways || (ranked(keys[k]) && high > prefix));
+      alike[k] = __ballot_sync(~0u, ranked(keys[k]) && high == prefix);
+    }
+  };
+  uint32_t n_taken = 0, n_alike = 0, keys[8];
+  for (int at = from; at < until; at += 256) {
+    look(at, keys);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      n_taken += __popc(taken[k]);
+      n_alike += __popc(alike[k]);
+      if (by_few && alike[k] >> lane & 1) few[atomicAdd(&few_count, 1u)] = make_uint2(keys[k], at + k * 32 + lane);
+    }
   }
-  uint64_t total;
-  const uint64_t before = sum_before(counts, scratch, total);
-  int equals = (int)(before >> 32), taken = (int)(uint32_t)before + min(equals, equal);
+  if (lane == 0) counts[warp][0] = n_taken, counts[warp][1] = by_few ? 0 : n_alike;
+  __syncthreads();
+  if (by_few) {  // a few that differ in lower bits are counted against each other; those taken are marked
+    const int population = (int)few_count;
+    if (tid < population) {
+      const uint2 mine = few[tid];
+      int above = 0;
+      for (int k = 0; k < population; ++k) {
+        const uint2 other = few[k];
+        above += other.x > mine.x || (other.x == mine.x && other.y < mine.y);
+      }
+      if (above < equal) {
+        own_keys[mine.y] = kAlways;
+        atomicAdd(&counts[mine.y / run][0], 1u);
+      }
+    }
+    equal = 0;
+    __syncthreads();
+  }
+  int place = 0, alikes = 0, all = 0, all_alike = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    place += w < warp ? (int)counts[w][0] : 0;
+    alikes += w < warp ? (int)counts[w][1] : 0;
+    all += (int)counts[w][0];
+    all_alike += (int)counts[w][1];
+  }
+  all += min(all_alike, equal);
   int32_t* const to = p.tables + (uint64_t)row * p.count;
-  for (int k = from; k < until; ++k) {
-    const uint32_t key = own_keys[k];
-    bool take = key > threshold || key == kAlways;
-    if (key == threshold && key != kAlways) take = equals++ < equal;
-    if (take) to[taken++] = __ldg(table + k);
+  for (int at = from; at < until; at += 256) {
+    if (run > 256) look(at, keys);  // (else they are there)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int index = at + k * 32 + lane;
+      if (by_few && alike[k] != 0) taken[k] |= __ballot_sync(~0u, alike[k] >> lane & 1 && own_keys[index] == kAlways);
+      const int alike_before = alikes + __popc(alike[k] & below);
+      if (taken[k] >> lane & 1 || (alike[k] >> lane & 1 && alike_before < equal))
+        to[place + __popc(taken[k] & below) + min(alike_before, equal)] = kOnChip ? (int)own_keys[p.n_table + index] : __ldg(table + index);
+      place += __popc(taken[k]);
+      alikes += __popc(alike[k]);
+    }
   }
-  const int all = (int)(uint32_t)total + min((int)(total >> 32), equal);
-  for (int k = all + tid; k < p.count; k += kChooseThreads) to[k] = -1;
+  for (int k = all + tid; k < p.count; k += kThreads) to[k] = -1;
   if (tid == 0) {
     // the query's own page, the last one, is there up to the query
     const bool has_own = pages > 0 && own_keys[own] != kNoCandidate;
@@ -500,9 +757,27 @@ static int check_choose(const SplashCacheChooseArgs& a) {
   return SPLASH_OK;
 }
 
+// Shared memory of a CTA but for the keys.
+static int choose_shared(int row, int64_t heads_per_kv) { return choose_heads((int)heads_per_kv) * choose_pitch(row); }
+
 static size_t choose_workspace(const SplashCacheChooseArgs& a) {
-  if (check_choose(a) != SPLASH_OK || a.n_table <= kKeysOnChip) return 0;
+  if (check_choose(a) != SPLASH_OK) return 0;
+  if (a.n_table <= kKeysOnChip && choose_shared(a.cache.row_k, a.q.size[1] / a.cache.kv_heads) + a.n_table * 8 <= kChooseShared) return 0;
   return (size_t)(a.q.size[0] * a.cache.kv_heads * a.q.size[2]) * a.n_table * sizeof(uint32_t);
+}
+
+template <int kChunks, int kWarps, bool kOnChip>
+static int launch_choose(const cudaLaunchConfig_t& config, const ChooseParams& p) {
+  const auto kernel = cache_choose_kernel<kChunks, kWarps, kOnChip>;
+  static std::atomic<uint64_t> ready{0};  // devices that know how much shared memory the kernel takes
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return SPLASH_ERR_CUDA;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kChooseShared) != cudaSuccess) return SPLASH_ERR_CUDA;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return cudaLaunchKernelEx(&config, kernel, p) == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
 }
 
 static int cache_choose(const SplashCacheChooseArgs& a, cudaStream_t stream) {
@@ -538,22 +813,13 @@ static int cache_choose(const SplashCacheChooseArgs& a, cudaStream_t stream) {
   p.last = a.last;
   const int64_t rows = a.q.size[0] * c.kv_heads * a.q.size[2];
   // As many CTAs a row as the GPU has room for, each with a tile for each of its warps.
+  const int warps = a.n_table <= kFewPages ? kMostChooseWarps / 2 : kMostChooseWarps;
   int ctas = 1;
-  while (ctas < kMostCluster && rows * ctas * 2 <= 2 * kSms && (int64_t)a.n_table > (int64_t)ctas * kChooseWarps * 16) ctas *= 2;
-  const int smem = choose_heads(p.heads_per_kv) * choose_pitch(p.row) + (p.keys == nullptr ? a.n_table * 4 : 0);
-  static std::atomic<uint64_t> ready{0};  // devices that know how much shared memory the kernel takes
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return SPLASH_ERR_CUDA;
-  const uint64_t bit = 1ull << (device & 63);
-  constexpr int kMostShared = 128 * choose_pitch(256) + kKeysOnChip * 4;
-  static_assert(kMostShared + 12 * 1024 <= 227 * 1024);
-  if (device > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(cache_choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return SPLASH_ERR_CUDA;
-    ready.fetch_or(bit, std::memory_order_relaxed);
-  }
+  while (ctas < kMostCluster && rows * ctas * 2 <= 2 * kSms && (int64_t)a.n_table > (int64_t)ctas * warps * 16) ctas *= 2;
+  const int smem = choose_shared(p.row, p.heads_per_kv) + (p.keys == nullptr ? a.n_table * 8 : 0);
   cudaLaunchConfig_t config{};
   config.gridDim = dim3((unsigned)(rows * ctas));
-  config.blockDim = dim3(kChooseThreads);
+  config.blockDim = dim3(warps * 32);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attribute{};
@@ -562,7 +828,20 @@ static int cache_choose(const SplashCacheChooseArgs& a, cudaStream_t stream) {
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, cache_choose_kernel, p) == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
+  auto launch = [&](auto chunks) {
+    constexpr int kChunks = decltype(chunks)::value;
+    constexpr int kMost = kMostChooseWarps;
+    return p.keys != nullptr        ? launch_choose<kChunks, kMost, false>(config, p)
+           : warps == kMost ? launch_choose<kChunks, kMost, true>(config, p)
+                            : launch_choose<kChunks, kMost / 2, true>(config, p);
+  };
+  switch (p.row) {
+    case 64: return launch(std::integral_constant<int, 2>{});
+    case 96: return launch(std::integral_constant<int, 3>{});
+    case 128: return launch(std::integral_constant<int, 4>{});
+    case 192: return launch(std::integral_constant<int, 6>{});
+    default: return launch(std::integral_constant<int, 8>{});
+  }
 }
 
 }  // namespace sb
@@ -571,6 +850,11 @@ extern "C" {
 
 int splash_cache_bound(const SplashCacheBoundArgs* args, void* cuda_stream) {
   return args == nullptr ? SPLASH_ERR_INVALID_ARGUMENT : sb::cache_bound(*args, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int splash_cache_bound_values(const SplashKvCache* cache, const SplashPageBounds* bounds, float* values, void* cuda_stream) {
+  return cache == nullptr || bounds == nullptr ? SPLASH_ERR_INVALID_ARGUMENT
+                                               : sb::cache_bound_values(*cache, *bounds, values, static_cast<cudaStream_t>(cuda_stream));
 }
 
 int splash_cache_choose(const SplashCacheChooseArgs* args, void* cuda_stream) {

@@ -115,15 +115,6 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
   return d;
 }
 
-// a / b, correctly rounded, for `inverse` = 1 / b, correctly rounded: a product, corrected by the remainder that a fused
-// multiply-add leaves (Markstein 1990, "Computation of elementary functions on the IBM RISC System/6000 processor").  It asks for
-// a b whose significand is not all ones, and for no underflow on the way.
-__device__ __forceinline__ float divide(float a, float b, float inverse) {
-  const float q = a * inverse;
-  return fmaf(fmaf(-q, b, a), inverse, q);
-}
-constexpr float kLeastDivisor = 0x1p-80f;  // below it the division of the hardware's own
-
 constexpr int kRowThreads = 256;
 constexpr int kWrite = 16;  // channels of a thread that writes
 

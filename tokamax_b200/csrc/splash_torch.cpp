@@ -294,14 +294,17 @@ struct PageLibrary {
   int (*attend)(const SplashCacheAttendArgs*, void*) = nullptr;
   size_t (*attend_workspace_bytes)(const SplashCacheAttendArgs*) = nullptr;
   int (*bound)(const SplashCacheBoundArgs*, void*) = nullptr;
+  int (*bound_values)(const SplashKvCache*, const SplashPageBounds*, float*, void*) = nullptr;
   int (*choose)(const SplashCacheChooseArgs*, void*) = nullptr;
   size_t (*choose_workspace_bytes)(const SplashCacheChooseArgs*) = nullptr;
 } page_lib;
 
-void bind_page_library(uintptr_t attend, uintptr_t attend_workspace_bytes, uintptr_t bound, uintptr_t choose, uintptr_t choose_workspace_bytes) {
+void bind_page_library(uintptr_t attend, uintptr_t attend_workspace_bytes, uintptr_t bound, uintptr_t bound_values, uintptr_t choose,
+                       uintptr_t choose_workspace_bytes) {
   page_lib.attend = reinterpret_cast<decltype(page_lib.attend)>(attend);
   page_lib.attend_workspace_bytes = reinterpret_cast<decltype(page_lib.attend_workspace_bytes)>(attend_workspace_bytes);
   page_lib.bound = reinterpret_cast<decltype(page_lib.bound)>(bound);
+  page_lib.bound_values = reinterpret_cast<decltype(page_lib.bound_values)>(bound_values);
   page_lib.choose = reinterpret_cast<decltype(page_lib.choose)>(choose);
   page_lib.choose_workspace_bytes = reinterpret_cast<decltype(page_lib.choose_workspace_bytes)>(choose_workspace_bytes);
 }
@@ -541,6 +544,16 @@ void cache_bound(const KvCache& cache, const PageBounds& bounds, const at::Tenso
   if (a.batch != 0) check_cache_call(on_stream_of(table, [&](void* stream) { return page_lib.bound(&a, stream); }), "splash_cache_bound");
 }
 
+at::Tensor cache_bound_values(const KvCache& cache, const PageBounds& bounds) {
+  const SplashKvCache& c = cache.desc;
+  require_not_traced();
+  require_bounds_of(bounds, cache);
+  const at::Tensor values = at::empty({c.n_pages, c.kv_heads, 2, c.head_dim}, bounds.scales.options());
+  check_cache_call(on_stream_of(values, [&](void* stream) { return page_lib.bound_values(&c, &bounds.desc, static_cast<float*>(values.data_ptr()), stream); }),
+                   "splash_cache_bound_values");
+  return values;
+}
+
 std::tuple<at::Tensor, at::Tensor> cache_choose(const KvCache& cache, const PageBounds& bounds, const at::Tensor& q_in, const at::Tensor& table_in,
                                                 const at::Tensor& lengths, int64_t count, int64_t first, int64_t last) {
   const SplashKvCache& c = cache.desc;
@@ -710,6 +723,7 @@ PYBIND11_MODULE(_splash_torch, m) {
   m.def("bind_rotary_library", &bind_rotary_library);
   pybind11::class_<PageBounds>(m, "PageBounds").def(pybind11::init<at::Tensor, at::Tensor>());
   m.def("cache_bound", torch::wrap_pybind_function(cache_bound));
+  m.def("cache_bound_values", torch::wrap_pybind_function(cache_bound_values));
   m.def("cache_choose", torch::wrap_pybind_function(cache_choose));
   pybind11::class_<RotaryTable, std::shared_ptr<RotaryTable>>(m, "RotaryTable").def(pybind11::init<at::Tensor, int, bool, double>());
   m.def("rotate", torch::wrap_pybind_function(rotate));

@@ -144,19 +144,21 @@ class PageBounds:
   ``[n_pages, kv_heads]``: ``value = scale * code``."""
   codes: torch.Tensor
   scales: torch.Tensor
-  head_dim: int
+  cache: KVCache = dataclasses.field(repr=False)
   native: object = dataclasses.field(repr=False)
 
   def values(self) -> torch.Tensor:
     """The bounds that the codes stand for, float32 ``[n_pages, kv_heads, 2, head_dim]``."""
-    return self.codes[..., :self.head_dim] * self.scales[:, :, None, None]
+    if not self.codes.is_cuda:
+      return self.codes[..., :self.cache.head_dim] * self.scales[:, :, None, None]
+    return _native.host().cache_bound_values(self.cache.native, self.native)
 
 
 def make_page_bounds(cache: KVCache) -> PageBounds:
   """Bounds for the pages of ``cache``, all of them 0; :func:`bound_pages` writes them as pages fill."""
   codes = torch.zeros((*cache.k_codes.shape[:2], 2, _row_k(cache)), dtype=torch.int8, device=cache.device)
   scales = torch.zeros(cache.k_codes.shape[:2], dtype=torch.float32, device=cache.device)
-  return PageBounds(codes, scales, cache.head_dim, _native.host().PageBounds(codes, scales))
+  return PageBounds(codes, scales, cache, _native.host().PageBounds(codes, scales))
 
 
 def _row_k(cache: KVCache) -> int:
