@@ -380,6 +380,18 @@ def test_items_cut_into_shares(fmt, group, dtype):
   _check_attend(store, tables, tokens, q_heads=4, t=2, soft_cap=20.0, sinks=sinks, dtype=dtype)
 
 
+@pytest.mark.parametrize("fmt,group", [("int4", 128), ("e4m3", None)])
+@pytest.mark.parametrize("batch,t,pages", [(1, 1, 20), (1, 1, 70), (1, 2, 700), (10, 1, 40), (10, 4, 40), (20, 8, 20), (50, 7, 12)])
+def test_items_of_clusters_of_every_size(fmt, group, batch, t, pages):
+  """Few items and many, tables with room for few tokens and many more than there are: a CTA an item, clusters of two to eight, and
+  shares.  Lengths from nothing to the whole table."""
+  store = Store([(37 * b * b + 1) % 300 for b in range(batch - 1)] + [640], heads=2, d=128, fmt=fmt, group=group, page=16)
+  tables, tokens = _random_tables(store, t, min(pages, 40))
+  tables = torch.nn.functional.pad(tables, (0, pages - min(pages, 40)), value=-1)
+  first = _check_attend(store, tables, tokens, q_heads=6, t=t)
+  assert torch.equal(first, _check_attend(store, tables, tokens, q_heads=6, t=t))
+
+
 def test_more_tables_than_a_cta_has_threads():
   store = Store([3 * i for i in range(70)], heads=3, d=64, page=16)
   tables, tokens = _random_tables(store, 1, 200)  # (3200 tokens of room: shares)

@@ -47,6 +47,7 @@
 // element type is a value at run time, so a kernel holds four forms of the product with P (masked or not, f16's second product or
 // not); 34 of the 50 kernels spill, up to 224 bytes a thread (most where groups of 32 keep many scales), the forms that are timed here
 // 0 (e4m3) to 36 (head dim 64 in groups of 32).
+#include <algorithm>
 #include <atomic>
 
 #include "cache_common.cuh"
@@ -57,6 +58,7 @@ namespace sb {
 // tokens, 8 items 12.5 : 10.6, 256 items 14.6 : 14.6, 1024 items 35.6 : 44.3).  Shares: four CTAs of 4 warps on an SM and two of 8
 // are alike where sequences are long, short ones want the smaller CTAs (64 x 200 .. 4096: 53.6 : 56.3).
 constexpr int kWarps = 4, kMostWarps = 8;
+constexpr int kMostCluster = 8;
 
 struct AttendParams {
   const uint8_t* k_codes;
@@ -79,7 +81,8 @@ struct AttendParams {
   // `queries` is what q has of them.  items: kv heads of a table times row tiles.
   int32_t batch, q_heads, kv_heads, heads_per_kv, q_len, queries, items, row_tiles, n_table, page_size, page_shift, dtype;
   int32_t head_dim, head_dim_v, window, item_cost;  // item_cost: in units
-  bool whole;  // every item is one CTA's
+  int32_t cluster;  // whole: CTAs of a cluster that share an item
+  bool whole;       // every item is one CTA's, or one cluster's
   bool by_head;
 };
 
@@ -408,7 +411,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   int64_t at, end, before, share_begin;  // in the measure of shares; before: what lies before sequence b
   int b;
   if (p.whole) {  // items in turn
-    at = blockIdx.x;
+    at = blockIdx.x / (unsigned)p.cluster;
     end = (int64_t)p.batch * per_sequence;
   } else {
     const Start start = find_start<kUnit>(p, reinterpret_cast<int64_t*>(smem));
@@ -435,7 +438,12 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       keys = keys_of<kUnit>(p, length);
       u0 = 0;
       u1 = keys.units;
-      at += gridDim.x;
+      if (p.cluster > 1) {
+        const int rank = blockIdx.x % (unsigned)p.cluster;
+        u0 = keys.units * rank / p.cluster;  // (units are below 2^26)
+        u1 = keys.units * (rank + 1) / p.cluster;
+      }
+      at += gridDim.x / (unsigned)p.cluster;
     } else {
       length = __ldg(p.lengths + b);
       keys = keys_of<kUnit>(p, length);
@@ -1077,6 +1085,16 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         for (int k = 0; k < 8; ++k) x[k] = fmaf(y[k], weight, x[k]);
         sum = fmaf(warp_sum[w * kRows + r], weight, sum);
       }
+      if (p.cluster > 1) {  // the CTA's sums, in the place of its first warp's (this thread's), for the others of the cluster
+        float4* const to = reinterpret_cast<float4*>(smem + Shape::kRing + (r * Shape::kV + d) * 4);
+        to[0] = make_float4(x[0], x[1], x[2], x[3]);
+        to[1] = make_float4(x[4], x[5], x[6], x[7]);
+        if (d == 0) {
+          factors[r] = most;
+          q_sums[r] = sum;
+        }
+        continue;
+      }
       if (!alone) {
         float4* const to = reinterpret_cast<float4*>(part + r * Shape::kV + d);
         to[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -1088,6 +1106,34 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         continue;
       }
       finish_row(p, rows, row0 + r, d, x, most, sum);
+    }
+    if (p.cluster > 1) {
+      // Each CTA finishes its part of the rows' channels, from the sums of all.
+      cluster_sync();
+      const int rank = blockIdx.x % (unsigned)p.cluster;
+      for (int id = rank * blockDim.x + tid; id < n_rows * (Shape::kV / 8); id += p.cluster * blockDim.x) {
+        const int r = id / (Shape::kV / 8), d = id % (Shape::kV / 8) * 8;
+        float x[8] = {}, m[kMostCluster], sum = 0.f, most = kNoMaximum;
+#pragma unroll
+        for (int c = 0; c < kMostCluster; ++c) {
+          m[c] = c < p.cluster ? __uint_as_float(cluster_ld_u32(cluster_addr(factors + r, c))) : kNoMaximum;
+          most = fmaxf(most, m[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < kMostCluster; ++c) {
+          if (c >= p.cluster) break;
+          const float weight = ex2(m[c] - most);
+          const uint32_t from = cluster_addr(smem + Shape::kRing + (r * Shape::kV + d) * 4, c);
+          const float4 lo = cluster_ld_v4(from), hi = cluster_ld_v4(from + 16);
+          const float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = fmaf(y[k], weight, x[k]);
+          sum = fmaf(__uint_as_float(cluster_ld_u32(cluster_addr(q_sums + r, c))), weight, sum);
+        }
+        finish_row(p, rows, row0 + r, d, x, most, sum);
+      }
+      cluster_sync();  // (nobody is read from any more)
+      continue;
     }
     __syncthreads();  // before q's place, the statistics and the ring are written again
   }
@@ -1215,23 +1261,33 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const int64_t items = (int64_t)p.items * p.batch;
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute attribute{};
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  config.stream = stream;
+  if (p.cluster > 1) {
+    config.gridDim = dim3((unsigned)(p.cluster * (items * p.cluster < ctas ? items : ctas / p.cluster)));
+    config.blockDim = dim3(kWarps * 32);
+    config.dynamicSmemBytes = Shape::smem(kWarps);
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = p.cluster;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    return cudaLaunchKernelEx(&config, kernel, p) == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
+  }
   const int warps = p.whole && items < 2 * kSms ? kMostWarps : kWarps;
   kernel<<<p.whole && items < ctas ? (int)items : ctas, warps * 32, Shape::smem(warps), stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return SPLASH_ERR_CUDA;
   if (p.whole) return SPLASH_OK;
-  cudaLaunchConfig_t config{};
+  config.dynamicSmemBytes = 0;
   // (as many blocks of an item as its rows and the GPU have room for, where items are few)
   const int rows = p.q_len * p.heads_per_kv < Shape::kRows ? p.q_len * p.heads_per_kv : Shape::kRows;
   const bool few = items < kSms / 2;
   config.gridDim = dim3((unsigned)p.items, (unsigned)(p.batch < 65535 ? p.batch : 65535),
                         (unsigned)(items >= 2 * kSms ? 1 : items * rows <= 8 * kSms ? rows : 8 * kSms / items));
   config.blockDim = dim3(kJoinThreads);
-  config.stream = stream;
-  cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
   const auto join = few ? cache_attend_join_kernel<Shape::kRows, Shape::kV, 4> : cache_attend_join_kernel<Shape::kRows, Shape::kV, 2>;
   const cudaError_t launched = cudaLaunchKernelEx(&config, join, p, ctas);
   return launched == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
@@ -1327,11 +1383,29 @@ static int check_attend(const SplashCacheAttendArgs& a, bool by_head) {
   return SPLASH_OK;
 }
 
+template <typename Shape>
+static int64_t items_of(const SplashCacheAttendArgs& a) {
+  const int64_t tiles = (a.q.size[2] * (a.q.size[1] / a.cache.kv_heads) + Shape::kRows - 1) / Shape::kRows;
+  return a.q.size[0] * a.cache.kv_heads * tiles;
+}
+
+// Tables by head are of much the same length (so many pages of a long sequence): an item is one cluster's, and there is no second
+// launch, unless the items are few and long.  As many CTAs as the GPU holds, each with a unit at least for each of its warps.
+template <typename Shape>
+static int cluster_of(const SplashCacheAttendArgs& a, bool by_head) {
+  const int64_t items = items_of<Shape>(a), reach = reach_of(a);
+  if (!by_head || items > INT32_MAX / kMostCluster) return 0;
+  if (items * kMostCluster < 2 * kSms && reach > kMostCluster * kWholeTokens) return 0;
+  int cluster = 1;
+  while (cluster < kMostCluster && items * cluster * 2 <= resident<Shape>() && reach >= 2 * cluster * kWarps * Shape::kUnit) cluster *= 2;
+  return cluster;
+}
+
 // Whether every item is given to one CTA: one launch, no sums in the workspace.
 template <typename Shape>
-static bool is_whole(const SplashCacheAttendArgs& a) {
-  const int64_t tiles = (a.q.size[2] * (a.q.size[1] / a.cache.kv_heads) + Shape::kRows - 1) / Shape::kRows;
-  const int64_t items = a.q.size[0] * a.cache.kv_heads * tiles;
+static bool is_whole(const SplashCacheAttendArgs& a, bool by_head) {
+  if (cluster_of<Shape>(a, by_head) > 0) return true;
+  const int64_t items = items_of<Shape>(a);
   const bool some = items >= kWholeItems && items < kMostWholeItems;
   return reach_of(a) <= (some ? 2 * kWholeTokens : kWholeTokens) && items <= INT32_MAX;
 }
@@ -1381,7 +1455,8 @@ static int cache_attend(const SplashCacheAttendArgs& args, bool by_head, cudaStr
   return with_shape(a, [&](auto shape) -> int {
     using Shape = decltype(shape);
     AttendParams own = p;
-    own.whole = is_whole<Shape>(a);
+    own.whole = is_whole<Shape>(a, by_head);
+    own.cluster = own.whole && by_head ? std::max(cluster_of<Shape>(a, true), 1) : 1;
     if (!own.whole) {
       const size_t parts = parts_bytes<Shape>();
       if (a.workspace == nullptr || (reinterpret_cast<uintptr_t>(a.workspace) & 15u) != 0 ||
@@ -1403,7 +1478,7 @@ static size_t cache_attend_workspace(const SplashCacheAttendArgs& args, bool by_
   size_t bytes = 0;
   with_shape(a, [&](auto shape) -> int {
     using Shape = decltype(shape);
-    if (!is_whole<Shape>(a)) bytes = parts_bytes<Shape>() + 8 * ((size_t)a.q.size[0] + 1);
+    if (!is_whole<Shape>(a, by_head)) bytes = parts_bytes<Shape>() + 8 * ((size_t)a.q.size[0] + 1);
     return 0;
   });
   return bytes;
