@@ -129,8 +129,6 @@ __device__ __forceinline__ uint32_t less_eight(uint32_t word, bool odd) {
   const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&pair), *reinterpret_cast<const __half2*>(&less));
   return *reinterpret_cast<const uint32_t*>(&x);
 }
-__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------------
 // sizes
@@ -405,7 +403,8 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   float* const warp_sum = warp_base + kMostWarps * kRows;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
-  grid_dependents_launch();  // the joining kernel may come up beside this one; it waits for its end
+  if (!p.whole) grid_dependents_launch();  // the joining kernel may come up beside this one; it waits for its end
+  grid_dependency_wait();    // (where this one has come up beside the kernel that chose its pages)
 
   const int per_sequence = p.items;
   int64_t at, end, before, share_begin;  // in the measure of shares; before: what lies before sequence b
@@ -1262,32 +1261,24 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   }
   const int64_t items = (int64_t)p.items * p.batch;
   cudaLaunchConfig_t config{};
-  cudaLaunchAttribute attribute{};
-  config.attrs = &attribute;
-  config.numAttrs = 1;
+  cudaLaunchAttribute attributes[2]{early_launch(), cluster_size(p.cluster)};
+  config.attrs = attributes;
   config.stream = stream;
-  if (p.cluster > 1) {
-    config.gridDim = dim3((unsigned)(p.cluster * (items * p.cluster < ctas ? items : ctas / p.cluster)));
-    config.blockDim = dim3(kWarps * 32);
-    config.dynamicSmemBytes = Shape::smem(kWarps);
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = p.cluster;
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    return cudaLaunchKernelEx(&config, kernel, p) == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
-  }
-  const int warps = p.whole && items < 2 * kSms ? kMostWarps : kWarps;
-  kernel<<<p.whole && items < ctas ? (int)items : ctas, warps * 32, Shape::smem(warps), stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return SPLASH_ERR_CUDA;
+  const int warps = p.whole && p.cluster == 1 && items < 2 * kSms ? kMostWarps : kWarps;
+  config.gridDim = dim3((unsigned)(!p.whole ? ctas : p.cluster * (items * p.cluster < ctas ? items : ctas / p.cluster)));
+  config.blockDim = dim3(warps * 32);
+  config.dynamicSmemBytes = Shape::smem(warps);
+  config.numAttrs = p.by_head ? p.cluster > 1 ? 2 : 1 : 0;
+  if (cudaLaunchKernelEx(&config, kernel, p) != cudaSuccess) return SPLASH_ERR_CUDA;
   if (p.whole) return SPLASH_OK;
   config.dynamicSmemBytes = 0;
+  config.numAttrs = 1;
   // (as many blocks of an item as its rows and the GPU have room for, where items are few)
   const int rows = p.q_len * p.heads_per_kv < Shape::kRows ? p.q_len * p.heads_per_kv : Shape::kRows;
   const bool few = items < kSms / 2;
   config.gridDim = dim3((unsigned)p.items, (unsigned)(p.batch < 65535 ? p.batch : 65535),
                         (unsigned)(items >= 2 * kSms ? 1 : items * rows <= 8 * kSms ? rows : 8 * kSms / items));
   config.blockDim = dim3(kJoinThreads);
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
   const auto join = few ? cache_attend_join_kernel<Shape::kRows, Shape::kV, 4> : cache_attend_join_kernel<Shape::kRows, Shape::kV, 2>;
   const cudaError_t launched = cudaLaunchKernelEx(&config, join, p, ctas);
   return launched == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;

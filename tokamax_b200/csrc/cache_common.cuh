@@ -80,6 +80,24 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
+// A kernel that is launched early comes up before the one ahead of it in the stream has ended (from when all of that one's CTAs have
+// said so); what the wait comes before sees all that the other has written.  Without such a launch both do nothing.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+inline cudaLaunchAttribute early_launch() {
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+inline cudaLaunchAttribute cluster_size(int ctas) {
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeClusterDimension;
+  a.val.clusterDim.x = ctas;
+  a.val.clusterDim.y = a.val.clusterDim.z = 1;
+  return a;
+}
+
 inline int log2_of(int power_of_two) {
   int n = 0;
   while ((1 << n) < power_of_two) ++n;

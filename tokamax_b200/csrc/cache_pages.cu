@@ -73,7 +73,7 @@ struct BoundParams {
   int32_t n_table, page_size, page_shift, kv_heads, head_dim, row, group_shift, slots, split;
 };
 
-constexpr int kBoundThreads = 256, kBoundWarps = kBoundThreads / 32;
+constexpr int kBoundThreads = 128, kBoundWarps = kBoundThreads / 32;
 constexpr int kPiece = 16;  // channels of a lane
 
 // Sixteen channels of a row in 32 bits, from their codes and the scales of their group.
@@ -95,10 +95,15 @@ struct RowPiece {
   __device__ __forceinline__ void get(float (&x)[kPiece]) const {
     const float s = __uint_as_float(scale & 0xffff0000u);
     if constexpr (kFormat == SPLASH_CACHE_INT4) {
-      // (2^23 + code has the code in its low bits; zero and product are 8 and 12 bits, their sum is rounded once)
+      // A code that stands 4 i bits up in a word is that of 2^(23 - 4 i) + code, for i up to 4: a mask and an exponent, one instruction.
+      // (Zero and product are 8 and 12 bits, their sum is rounded once.)
       const float zero = bf16_bits_to_float(scale);
 #pragma unroll
-      for (int j = 0; j < kPiece; ++j) x[j] = fmaf(s, __uint_as_float(w[j / 8] >> 4 * (j % 8) & 15u | 0x4b000000u) - 8388608.f, zero);
+      for (int j = 0; j < kPiece; ++j) {
+        const int i = j % 8 < 5 ? j % 8 : j % 8 - 5;
+        const uint32_t word = j % 8 < 5 ? w[j / 8] : w[j / 8] >> 20, exponent = 0x4b000000u - i * 0x02000000u;
+        x[j] = fmaf(s, __uint_as_float((word & 15u << 4 * i) | exponent) - __uint_as_float(exponent), zero);
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < kPiece / 2; ++j) {
@@ -117,12 +122,13 @@ constexpr int kWarpTokens = 128;
 // heads, the heads fastest; y: the sequence.  A team of kTeam lanes (the power of two that holds the row's width / 16) has a
 // token's row.
 template <int kFormat, int kTeam>
-__global__ void __launch_bounds__(kBoundThreads) cache_bound_kernel(const __grid_constant__ BoundParams p) {
+__global__ void __launch_bounds__(kBoundThreads, 4) cache_bound_kernel(const __grid_constant__ BoundParams p) {
   constexpr int kRows = 32 / kTeam;       // of a warp's load
-  constexpr int kAhead = 4;               // loads in flight
+  constexpr int kAhead = 8;               // loads in flight
   constexpr int kOwn = kPiece / kRows;    // channels of a lane once the rows are together
   static_assert(kOwn >= 2);
   __shared__ float extremes[kBoundWarps][2][32 * kOwn];
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % kTeam, team = lane / kTeam;
   const int share = warp % p.split;  // of the page's tokens
   const int64_t items = (int64_t)p.slots * p.kv_heads, step = (int64_t)gridDim.x * (kBoundWarps / p.split);
@@ -148,12 +154,11 @@ __global__ void __launch_bounds__(kBoundThreads) cache_bound_kernel(const __grid
         for (int t = t0; t < t1; t += kRows * kAhead) {
           RowPiece<kFormat> piece[kAhead];
 #pragma unroll
-          for (int i = 0; i < kAhead; ++i) {
-            const int at = t + i * kRows < t1 ? t + i * kRows : t;  // (one of them twice)
-            piece[i].load(codes + (int64_t)at * row_bytes, scales + (int64_t)at * scale_bytes);
-          }
+          for (int i = 0; i < kAhead; ++i)  // (tokens come in sixteens: two of a lane's at least)
+            if (t + i * kRows < t1) piece[i].load(codes + (int64_t)(t + i * kRows) * row_bytes, scales + (int64_t)(t + i * kRows) * scale_bytes);
 #pragma unroll
           for (int i = 0; i < kAhead; i += 2) {
+            if (t + i * kRows >= t1) break;
             float x[kPiece], y[kPiece];
             piece[i].get(x);
             piece[i + 1].get(y);
@@ -289,20 +294,22 @@ static int cache_bound(const SplashCacheBoundArgs& a, cudaStream_t stream) {
   const int per_block = kBoundWarps / p.split;
   const int64_t blocks = ((int64_t)p.slots * c.kv_heads + per_block - 1) / per_block;
   const dim3 grid((unsigned)(blocks < INT32_MAX ? blocks : INT32_MAX), (unsigned)(a.batch < 65535 ? a.batch : 65535));
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute attribute = early_launch();
+  config.gridDim = grid;
+  config.blockDim = dim3(kBoundThreads);
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
   auto launch = [&](auto format) {
     constexpr int kFormat = decltype(format)::value;
-    if (c.row_k <= 64)
-      cache_bound_kernel<kFormat, 4><<<grid, kBoundThreads, 0, stream>>>(p);
-    else if (c.row_k <= 128)
-      cache_bound_kernel<kFormat, 8><<<grid, kBoundThreads, 0, stream>>>(p);
-    else
-      cache_bound_kernel<kFormat, 16><<<grid, kBoundThreads, 0, stream>>>(p);
+    return c.row_k <= 64    ? cudaLaunchKernelEx(&config, cache_bound_kernel<kFormat, 4>, p)
+           : c.row_k <= 128 ? cudaLaunchKernelEx(&config, cache_bound_kernel<kFormat, 8>, p)
+                            : cudaLaunchKernelEx(&config, cache_bound_kernel<kFormat, 16>, p);
   };
-  if (c.format == SPLASH_CACHE_INT4)
-    launch(std::integral_constant<int, SPLASH_CACHE_INT4>{});
-  else
-    launch(std::integral_constant<int, SPLASH_CACHE_E4M3>{});
-  return cudaGetLastError() == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
+  const cudaError_t launched = c.format == SPLASH_CACHE_INT4 ? launch(std::integral_constant<int, SPLASH_CACHE_INT4>{})
+                                                             : launch(std::integral_constant<int, SPLASH_CACHE_E4M3>{});
+  return launched == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
 }
 
 // A thread has eight channels of one side of a page and head.
@@ -393,6 +400,7 @@ __global__ void __launch_bounds__(kWarps * 32, (kChunks <= 4 ? 16 : 8) / kWarps)
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const uint32_t row = blockIdx.x / ctas;  // (sequence, kv head, query)
   const int i = row % (unsigned)p.q_len, head = row / (unsigned)p.q_len % (unsigned)p.kv_heads, b = row / (unsigned)p.q_len / (unsigned)p.kv_heads;
+  grid_dependency_wait();
   const int length = __ldg(p.lengths + b);
 
   // ---- a warp's tiles: 16 pages each, their bounds as operands of the products ----
@@ -822,12 +830,9 @@ static int cache_choose(const SplashCacheChooseArgs& a, cudaStream_t stream) {
   config.blockDim = dim3(warps * 32);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = ctas;
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
+  cudaLaunchAttribute attributes[2]{early_launch(), cluster_size(ctas)};
+  config.attrs = attributes;
+  config.numAttrs = 2;
   auto launch = [&](auto chunks) {
     constexpr int kChunks = decltype(chunks)::value;
     constexpr int kMost = kMostChooseWarps;

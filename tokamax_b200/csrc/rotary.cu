@@ -172,11 +172,8 @@ static int launch_rotate(RotateParams& p, bool interleaved, cudaStream_t stream)
   p.lanes = p.dim / (2 * kPairs) + (p.head_dim - p.dim + 2 * kPairs - 1) / (2 * kPairs);
   p.rows_each = kRotateThreads / p.lanes;
   const int heads = p.side[0].heads + p.side[1].heads;
-  // As many heads a thread as leave the GPU some 32 warps an SM.
-  const int64_t threads = (int64_t)p.rows * p.lanes, most = (int64_t)kSms * 1024;
-  int64_t each = (threads * heads + most - 1) / most;
-  if (each > kRotateAhead) each = (each + kRotateAhead - 1) / kRotateAhead * kRotateAhead;
-  p.heads_each = (int)(each < heads ? each : heads);
+  // Four heads a thread, whose loads are in flight together, unless that leaves the GPU without threads.
+  p.heads_each = (int64_t)p.rows * p.lanes * heads < (int64_t)kSms * 2048 ? 1 : kRotateAhead;
   const dim3 grid((p.rows + p.rows_each - 1) / p.rows_each, (unsigned)((heads + p.heads_each - 1) / p.heads_each));
   const int block = p.rows_each * p.lanes;
   if (interleaved)
