@@ -10,6 +10,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -376,6 +377,14 @@ void check_cache_call(int status, const char* what) {
   throw python_error();
 }
 
+// Memory for results, from torch's allocator without its dispatcher (a microsecond less for each).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, at::Device device) { return at::detail::empty_cuda(sizes, type, device, std::nullopt); }
+// In the order of t's dense strides.
+at::Tensor fresh_like(const at::Tensor& t) {
+  return t.is_non_overlapping_and_dense() ? at::Tensor(at::detail::empty_strided_cuda(t.sizes(), t.strides(), t.scalar_type(), t.device()))
+                                          : fresh(t.sizes(), t.scalar_type(), t.device());
+}
+
 template <typename Fn>
 int on_stream_of(const at::Tensor& t, Fn&& call) {
   const WithoutGil release;
@@ -411,17 +420,21 @@ void cache_append(const KvCache& cache, const at::Tensor& k_in, const at::Tensor
   check_cache_call(on_stream_of(k, [&](void* stream) { return cache_lib.append(&a, stream); }), "splash_cache_append");
 }
 
+void require_pages(const at::Tensor& table, const at::Tensor& lengths, int64_t pages, const KvCache& cache) {
+  TORCH_CHECK_VALUE(table.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt, "the page table and the lengths are int32");
+  require_on_gpu(table, cache, "the page table");
+  require_on_gpu(lengths, cache, "lengths");
+  TORCH_CHECK_VALUE(pages >= 1 && pages <= INT32_MAX, "a page table of ", pages, " pages");
+}
+
 // A page table [B, pages] and the lengths [B] of the sequences, as the kernels take them.
 template <typename Args>
 at::Tensor set_pages(Args& a, const KvCache& cache, const at::Tensor& table_in, const at::Tensor& lengths) {
   TORCH_CHECK_VALUE(table_in.dim() == 2 && lengths.dim() == 1 && table_in.size(0) == lengths.size(0), "page table ", table_in.sizes(),
                     " and lengths ", lengths.sizes(), " do not match: expected [B, pages] and [B]");
-  TORCH_CHECK_VALUE(table_in.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt, "the page table and the lengths are int32");
-  require_on_gpu(table_in, cache, "the page table");
-  require_on_gpu(lengths, cache, "lengths");
+  require_pages(table_in, lengths, table_in.size(1), cache);
   TORCH_CHECK_VALUE(lengths.size(0) <= 1 || lengths.stride(0) == 1, "lengths are contiguous");
   const at::Tensor table = table_in.size(1) <= 1 || table_in.stride(1) == 1 ? table_in : table_in.contiguous();
-  TORCH_CHECK_VALUE(table.size(1) >= 1 && table.size(1) <= INT32_MAX, "a page table of ", table.size(1), " pages");
   a.cache = cache.desc;
   a.page_table = static_cast<const int32_t*>(table.data_ptr());
   a.table_stride = table.stride(0);
@@ -464,9 +477,14 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
                           table_in.size(1) == c.kv_heads && table_in.size(2) == q_in.size(2),
                       "page tables ", table_in.sizes(), " and lengths ", lengths.sizes(), " do not match: expected [B, kv_heads, T, pages] and [B, kv_heads, T]");
     TORCH_CHECK_VALUE(!window.has_value(), "local_window_size goes by places in the sequence, which tables of chosen pages do not say");
-    const int64_t rows = lengths.numel();
-    lengths = lengths.reshape({rows}).contiguous();
-    table = set_pages(a, cache, table_in.reshape({rows, table_in.size(3)}), lengths);
+    require_pages(table_in, lengths, table_in.size(3), cache);
+    table = table_in.contiguous();  // (rows one behind the other)
+    lengths = lengths.contiguous();
+    a.cache = cache.desc;
+    a.page_table = static_cast<const int32_t*>(table.data_ptr());
+    a.table_stride = table.size(3);
+    a.n_table = (int32_t)table.size(3);
+    a.lengths = static_cast<const int32_t*>(lengths.data_ptr());
   } else {
     table = set_pages(a, cache, table_in, lengths);
     TORCH_CHECK_VALUE(q_in.size(0) == lengths.size(0), "q of ", q_in.size(0), " sequences, lengths of ", lengths.size(0));
@@ -486,7 +504,7 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
   const at::Tensor q = usable(q_in);
   a.q = describe_row_tensor(q, "q", false);
   // (like q, it keeps q's dense stride order)
-  const at::Tensor o = c.head_dim_v == c.head_dim ? at::empty_like(q) : at::empty({b, heads, t, c.head_dim_v}, q.options());
+  const at::Tensor o = c.head_dim_v == c.head_dim ? fresh_like(q) : fresh({b, heads, t, c.head_dim_v}, q.scalar_type(), q.device());
   a.o = describe_row_tensor(o, "o", false);
   Maybe lse, max_logits;
   if (residuals) {
@@ -503,7 +521,7 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
   a.workspace_bytes = (by_head ? page_lib.attend_workspace_bytes : cache_lib.attend_workspace_bytes)(&a);
   at::Tensor workspace;
   if (a.workspace_bytes != 0) {
-    workspace = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
+    workspace = fresh({(int64_t)a.workspace_bytes}, at::kByte, q.device());
     a.workspace = workspace.data_ptr();
   }
   check_cache_call(on_stream_of(q, [&](void* stream) { return (by_head ? page_lib.attend : cache_lib.attend)(&a, stream); }),
@@ -548,7 +566,7 @@ at::Tensor cache_bound_values(const KvCache& cache, const PageBounds& bounds) {
   const SplashKvCache& c = cache.desc;
   require_not_traced();
   require_bounds_of(bounds, cache);
-  const at::Tensor values = at::empty({c.n_pages, c.kv_heads, 2, c.head_dim}, bounds.scales.options());
+  const at::Tensor values = fresh({c.n_pages, c.kv_heads, 2, c.head_dim}, at::kFloat, bounds.codes.device());
   check_cache_call(on_stream_of(values, [&](void* stream) { return page_lib.bound_values(&c, &bounds.desc, static_cast<float*>(values.data_ptr()), stream); }),
                    "splash_cache_bound_values");
   return values;
@@ -571,9 +589,8 @@ std::tuple<at::Tensor, at::Tensor> cache_choose(const KvCache& cache, const Page
   const at::Tensor q = usable(q_in);
   a.bounds = bounds.desc;
   a.q = describe_row_tensor(q, "q", false);
-  const auto options = table.options();
-  const at::Tensor tables = at::empty({q.size(0), c.kv_heads, q.size(2), count}, options);
-  const at::Tensor table_lengths = at::empty({q.size(0), c.kv_heads, q.size(2)}, options);
+  const at::Tensor tables = fresh({q.size(0), c.kv_heads, q.size(2), count}, at::kInt, q.device());
+  const at::Tensor table_lengths = fresh({q.size(0), c.kv_heads, q.size(2)}, at::kInt, q.device());
   if (tables.numel() == 0) return {tables, table_lengths};
   a.tables = static_cast<int32_t*>(tables.data_ptr());
   a.table_lengths = static_cast<int32_t*>(table_lengths.data_ptr());
@@ -612,9 +629,8 @@ std::tuple<at::Tensor, at::Tensor> rotated(const RotaryTable& table, const at::T
     if (i == 1 && !z.has_value()) continue;
     const at::Tensor& t = i == 0 ? x : *z;
     in[i] = usable(t);
-    out[i] = at::empty_like(in[i]);  // (in the order of the input's dense strides)
+    out[i] = fresh_like(in[i]);
     if (out[i].numel() == 0) continue;
-    if (usable(out[i]).data_ptr() != out[i].data_ptr()) out[i] = at::empty(in[i].sizes(), in[i].options());
     a.x[i] = describe_row_tensor(in[i], "rotate", true);
     a.y[i] = describe_row_tensor(out[i], "rotate", true);
   }
