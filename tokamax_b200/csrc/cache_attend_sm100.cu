@@ -168,7 +168,8 @@ struct AttendShape {
   static constexpr int kRing = (kStats + 3 * kMostWarps * kRows * 4 + 127) / 128 * 128;
   // of a warp: its two stages, and in their place its sums [kRows][kV] once they have run dry
   static constexpr int kWarpBytes = 2 * kStageBytes > kRows * kV * 4 ? 2 * kStageBytes : kRows * kV * 4;
-  static constexpr int smem(int warps) { return kRing + warps * kWarpBytes; }
+  __host__ __device__ static constexpr int smem(int warps) { return kRing + warps * kWarpBytes; }
+  static constexpr int smem_cluster() { return smem(kWarps) + (kRows * kV / 8 + kMostCluster) * 48; }  // (sums of a cluster's CTAs)
 };
 
 // Where in a stage 16-byte piece c of row r lies: so that eight consecutive rows' piece c are in eight different bank groups.
@@ -407,6 +408,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   grid_dependency_wait();    // (where this one has come up beside the kernel that chose its pages)
 
   const int per_sequence = p.items;
+  const int rank = p.cluster > 1 ? blockIdx.x % (unsigned)p.cluster : 0;
   int64_t at, end, before, share_begin;  // in the measure of shares; before: what lies before sequence b
   int b;
   if (p.whole) {  // items in turn
@@ -421,6 +423,9 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     before = start.before;
   }
   uint8_t* const ring = smem + Shape::kRing + warp * Shape::kWarpBytes;
+  // of a cluster: the sums of all its CTAs for the channels that this one finishes, [eight channels][CTA][eight sums, maximum, sum of P, 2]
+  float* const received = reinterpret_cast<float*>(smem + Shape::smem(kWarps));
+  if (p.cluster > 1) cluster_arrive();
   const uint32_t ring_at = smem_u32(ring);
   const int heads = p.heads_per_kv;
 
@@ -433,15 +438,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     if (p.whole) {
       b = (int)((unsigned)at / (unsigned)per_sequence);
       item = (int)((unsigned)at % (unsigned)per_sequence);
-      length = __ldg(p.lengths + b);
-      keys = keys_of<kUnit>(p, length);
-      u0 = 0;
-      u1 = keys.units;
-      if (p.cluster > 1) {
-        const int rank = blockIdx.x % (unsigned)p.cluster;
-        u0 = keys.units * rank / p.cluster;  // (units are below 2^26)
-        u1 = keys.units * (rank + 1) / p.cluster;
-      }
+      length = __ldg(p.lengths + b);  // (on its way: see below)
       at += gridDim.x / (unsigned)p.cluster;
     } else {
       length = __ldg(p.lengths + b);
@@ -541,6 +538,15 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         const int i = query_of(r), h = head * heads + first_row + r - i * heads;
         raw[pass] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + rows.b * p.q_stride_b + h * p.q_stride_h +
                                                          (rows.query + first_query + i) * p.q_stride_s + piece * 8));
+      }
+    }
+    if (p.whole) {
+      keys = keys_of<kUnit>(p, length);
+      u0 = 0;
+      u1 = keys.units;
+      if (p.cluster > 1) {
+        u0 = keys.units * rank / p.cluster;  // (units are below 2^26)
+        u1 = keys.units * (rank + 1) / p.cluster;
       }
     }
     start_item();
@@ -1065,6 +1071,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     }
     __syncthreads();
     // ---- and together ----
+    if (p.cluster > 1) cluster_wait();  // (the others are there)
     const bool alone = u0 == 0 && u1 == keys.units;
     // sums of this CTA: an item that began before its share in place 0, one that goes on behind it in place 1 (both: 0)
     float* const part = p.parts + ((int64_t)blockIdx.x * 2 + (is_last ? 1 : 0)) * (kRows * (Shape::kV + 2));
@@ -1084,14 +1091,11 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         for (int k = 0; k < 8; ++k) x[k] = fmaf(y[k], weight, x[k]);
         sum = fmaf(warp_sum[w * kRows + r], weight, sum);
       }
-      if (p.cluster > 1) {  // the CTA's sums, in the place of its first warp's (this thread's), for the others of the cluster
-        float4* const to = reinterpret_cast<float4*>(smem + Shape::kRing + (r * Shape::kV + d) * 4);
-        to[0] = make_float4(x[0], x[1], x[2], x[3]);
-        to[1] = make_float4(x[4], x[5], x[6], x[7]);
-        if (d == 0) {
-          factors[r] = most;
-          q_sums[r] = sum;
-        }
+      if (p.cluster > 1) {  // to the CTA that finishes these channels
+        const uint32_t to = cluster_addr(received + (id / p.cluster * p.cluster + rank) * 12, id % p.cluster);
+        cluster_st_v4(to, x[0], x[1], x[2], x[3]);
+        cluster_st_v4(to + 16, x[4], x[5], x[6], x[7]);
+        cluster_st_v4(to + 32, most, sum, 0.f, 0.f);
         continue;
       }
       if (!alone) {
@@ -1106,33 +1110,24 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       }
       finish_row(p, rows, row0 + r, d, x, most, sum);
     }
-    if (p.cluster > 1) {
-      // Each CTA finishes its part of the rows' channels, from the sums of all.
+    if (p.cluster > 1) {  // (a cluster has one item)
       cluster_sync();
-      const int rank = blockIdx.x % (unsigned)p.cluster;
-      for (int id = rank * blockDim.x + tid; id < n_rows * (Shape::kV / 8); id += p.cluster * blockDim.x) {
-        const int r = id / (Shape::kV / 8), d = id % (Shape::kV / 8) * 8;
-        float x[8] = {}, m[kMostCluster], sum = 0.f, most = kNoMaximum;
-#pragma unroll
-        for (int c = 0; c < kMostCluster; ++c) {
-          m[c] = c < p.cluster ? __uint_as_float(cluster_ld_u32(cluster_addr(factors + r, c))) : kNoMaximum;
-          most = fmaxf(most, m[c]);
-        }
-#pragma unroll
-        for (int c = 0; c < kMostCluster; ++c) {
-          if (c >= p.cluster) break;
-          const float weight = ex2(m[c] - most);
-          const uint32_t from = cluster_addr(smem + Shape::kRing + (r * Shape::kV + d) * 4, c);
-          const float4 lo = cluster_ld_v4(from), hi = cluster_ld_v4(from + 16);
+      for (int id = tid * p.cluster + rank; id < n_rows * (Shape::kV / 8); id += blockDim.x * p.cluster) {
+        const float* const from = received + id / p.cluster * p.cluster * 12;
+        float x[8] = {}, sum = 0.f, most = kNoMaximum;
+        for (int c = 0; c < p.cluster; ++c) most = fmaxf(most, from[c * 12 + 8]);
+#pragma unroll 4
+        for (int c = 0; c < p.cluster; ++c) {
+          const float weight = ex2(from[c * 12 + 8] - most);
+          const float4 lo = *reinterpret_cast<const float4*>(from + c * 12), hi = *reinterpret_cast<const float4*>(from + c * 12 + 4);
           const float y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[k] = fmaf(y[k], weight, x[k]);
-          sum = fmaf(__uint_as_float(cluster_ld_u32(cluster_addr(q_sums + r, c))), weight, sum);
+          sum = fmaf(from[c * 12 + 9], weight, sum);
         }
-        finish_row(p, rows, row0 + r, d, x, most, sum);
+        finish_row(p, rows, row0 + id / (Shape::kV / 8), id % (Shape::kV / 8) * 8, x, most, sum);
       }
-      cluster_sync();  // (nobody is read from any more)
-      continue;
+      return;
     }
     __syncthreads();  // before q's place, the statistics and the ring are written again
   }
@@ -1249,7 +1244,7 @@ __global__ void __launch_bounds__(kJoinThreads, kAhead > 2 ? 2 : 4) cache_attend
 template <typename Shape>
 static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   auto kernel = cache_attend_kernel<Shape>;
-  static_assert(Shape::smem(kMostWarps) <= 227 * 1024);
+  static_assert(Shape::smem(kMostWarps) <= 227 * 1024 && Shape::smem_cluster() <= Shape::smem(kMostWarps));
   static std::atomic<uint64_t> ready{0};  // devices that know how much shared memory the kernel takes
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return SPLASH_ERR_CUDA;
@@ -1267,7 +1262,7 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   const int warps = p.whole && p.cluster == 1 && items < 2 * kSms ? kMostWarps : kWarps;
   config.gridDim = dim3((unsigned)(!p.whole ? ctas : p.cluster * (items * p.cluster < ctas ? items : ctas / p.cluster)));
   config.blockDim = dim3(warps * 32);
-  config.dynamicSmemBytes = Shape::smem(warps);
+  config.dynamicSmemBytes = p.cluster > 1 ? Shape::smem_cluster() : Shape::smem(warps);
   config.numAttrs = p.by_head ? p.cluster > 1 ? 2 : 1 : 0;
   if (cudaLaunchKernelEx(&config, kernel, p) != cudaSuccess) return SPLASH_ERR_CUDA;
   if (p.whole) return SPLASH_OK;
