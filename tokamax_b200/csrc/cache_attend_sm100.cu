@@ -49,12 +49,13 @@
 // 0 (e4m3) to 36 (head dim 64 in groups of 32).
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "cache_common.cuh"
 
 namespace sb {
 
-// Warps of a CTA; kMostWarps where every item is one CTA's and there are fewer than two for an SM (us, 4 : 8 warps, up to 1024
+// Warps of a CTA; kMostWarps where every item is one CTA's and there are fewer than two for an SM (tables by head: see form_by_head) (us, 4 : 8 warps, up to 1024
 // tokens, 8 items 12.5 : 10.6, 256 items 14.6 : 14.6, 1024 items 35.6 : 44.3).  Shares: four CTAs of 4 warps on an SM and two of 8
 // are alike where sequences are long, short ones want the smaller CTAs (64 x 200 .. 4096: 53.6 : 56.3).
 constexpr int kWarps = 4, kMostWarps = 8;
@@ -169,7 +170,7 @@ struct AttendShape {
   // of a warp: its two stages, and in their place its sums [kRows][kV] once they have run dry
   static constexpr int kWarpBytes = 2 * kStageBytes > kRows * kV * 4 ? 2 * kStageBytes : kRows * kV * 4;
   __host__ __device__ static constexpr int smem(int warps) { return kRing + warps * kWarpBytes; }
-  static constexpr int smem_cluster() { return smem(kWarps) + (kRows * kV / 8 + kMostCluster) * 48; }  // (sums of a cluster's CTAs)
+  static constexpr int smem_cluster(int warps) { return smem(warps) + (kRows * kV / 8 + kMostCluster) * 48; }  // (sums of a cluster's CTAs)
 };
 
 // Where in a stage 16-byte piece c of row r lies: so that eight consecutive rows' piece c are in eight different bank groups.
@@ -424,7 +425,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   }
   uint8_t* const ring = smem + Shape::kRing + warp * Shape::kWarpBytes;
   // of a cluster: the sums of all its CTAs for the channels that this one finishes, [eight channels][CTA][eight sums, maximum, sum of P, 2]
-  float* const received = reinterpret_cast<float*>(smem + Shape::smem(kWarps));
+  float* const received = reinterpret_cast<float*>(smem + Shape::smem(warps));
   if (p.cluster > 1) cluster_arrive();
   const uint32_t ring_at = smem_u32(ring);
   const int heads = p.heads_per_kv;
@@ -1242,15 +1243,15 @@ __global__ void __launch_bounds__(kJoinThreads, kAhead > 2 ? 2 : 4) cache_attend
 // host
 // ------------------------------------------------------------------------------------------
 template <typename Shape>
-static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
+static int launch(const AttendParams& p, int warps, int ctas, cudaStream_t stream) {
   auto kernel = cache_attend_kernel<Shape>;
-  static_assert(Shape::smem(kMostWarps) <= 227 * 1024 && Shape::smem_cluster() <= Shape::smem(kMostWarps));
+  static_assert(Shape::smem_cluster(kMostWarps) <= 227 * 1024);
   static std::atomic<uint64_t> ready{0};  // devices that know how much shared memory the kernel takes
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return SPLASH_ERR_CUDA;
   const uint64_t bit = 1ull << (device & 63);
   if (device > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem(kMostWarps)) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem_cluster(kMostWarps)) != cudaSuccess)
       return SPLASH_ERR_CUDA;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
@@ -1259,10 +1260,10 @@ static int launch(const AttendParams& p, int ctas, cudaStream_t stream) {
   cudaLaunchAttribute attributes[2]{early_launch(), cluster_size(p.cluster)};
   config.attrs = attributes;
   config.stream = stream;
-  const int warps = p.whole && p.cluster == 1 && items < 2 * kSms ? kMostWarps : kWarps;
-  config.gridDim = dim3((unsigned)(!p.whole ? ctas : p.cluster * (items * p.cluster < ctas ? items : ctas / p.cluster)));
+  // (shares: as many CTAs as the GPU holds; clusters: as many as there are items, which one alone takes in turn)
+  config.gridDim = dim3((unsigned)(!p.whole ? ctas : p.cluster > 1 ? p.cluster * items : items < ctas ? items : ctas));
   config.blockDim = dim3(warps * 32);
-  config.dynamicSmemBytes = p.cluster > 1 ? Shape::smem_cluster() : Shape::smem(warps);
+  config.dynamicSmemBytes = p.cluster > 1 ? Shape::smem_cluster(warps) : Shape::smem(warps);
   config.numAttrs = p.by_head ? p.cluster > 1 ? 2 : 1 : 0;
   if (cudaLaunchKernelEx(&config, kernel, p) != cudaSuccess) return SPLASH_ERR_CUDA;
   if (p.whole) return SPLASH_OK;
@@ -1375,22 +1376,43 @@ static int64_t items_of(const SplashCacheAttendArgs& a) {
   return a.q.size[0] * a.cache.kv_heads * tiles;
 }
 
-// Tables by head are of much the same length (so many pages of a long sequence): an item is one cluster's, and there is no second
-// launch, unless the items are few and long.  As many CTAs as the GPU holds, each with a unit at least for each of its warps.
+// Tables by head are of much the same length (so many pages of long sequences): an item can be one cluster's, of 1, 2, 4 or 8 CTAs of
+// 4 or 8 warps, without shares to look for and a second launch.  What a call takes is estimated for each such form, in tokens of one
+// SM with all its warps (265 a us, eight rows of 128 channels in int4), and the least one taken:
+//   * an SM has ceil(CTAs / SMs) of an item's parts, as many at a time as it holds; with 4, 8 and 12 warps it gets to 0.57, 0.92 and 0.97
+//     of its rate, and another turn costs 4 us more (8 where it is clusters', which need room for all of their CTAs);
+//   * a cluster's barriers and sums 0.35 us for each doubling; a warp has a unit at least;
+//   * shares: equal for all SMs, and 4 us for the second launch and the search, 1.2 for each item of an SM.
+// us measured, shares | 1 CTA of 8 warps | the form taken: 8 items of 1024 tokens 11.6 | 9.6 | 7.3 (8 x 8), of 8192 13.6 | 42.6 | 11.4 (8 x 8);
+// 32 of 4096 14.8 | 23.8 | 11.3 (4 x 8); 96 of 3072 tokens 22.7 | 19.7 | 17.5 (4 x 4), 192 of 4096 38.3 | 37.6 | 32.4 (2 x 4), 256 of 4096
+// 45.7 | 37.6 | 37.6, 512 of 1024 23.1 | 27.0 | 23.1 (1 x 4).
+struct Form {
+  int cluster, warps;  // cluster 0: shares
+};
 template <typename Shape>
-static int cluster_of(const SplashCacheAttendArgs& a, bool by_head) {
-  const int64_t items = items_of<Shape>(a), reach = reach_of(a);
-  if (!by_head || items > INT32_MAX / kMostCluster) return 0;
-  if (items * kMostCluster < 2 * kSms && reach > kMostCluster * kWholeTokens) return 0;
-  int cluster = 1;
-  while (cluster < kMostCluster && items * cluster * 2 <= resident<Shape>() && reach >= 2 * cluster * kWarps * Shape::kUnit) cluster *= 2;
-  return cluster;
+static Form form_by_head(const SplashCacheAttendArgs& a) {
+  const double items = (double)items_of<Shape>(a), reach = (double)reach_of(a);
+  Form best{0, kWarps};
+  double least = 1100. + (1.05 * reach + 320.) * items / kSms;
+  if (items > INT32_MAX / kMostCluster) return best;
+  const auto rate = [](int warps) { return warps <= 4 ? 0.57 : warps <= 8 ? 0.92 : warps <= 12 ? 0.97 : 1.; };
+  for (int cluster = 1, doublings = 0; cluster <= kMostCluster; cluster *= 2, ++doublings) {
+    for (int warps = kWarps; warps <= kMostWarps; warps *= 2) {
+      if (cluster > 1 && reach < (double)cluster * warps * Shape::kUnit) continue;
+      const double held = std::max(Shape::kResident * kWarps / warps, 1), of_sm = std::ceil(items * cluster / kSms), part = reach / cluster;
+      const double turns = std::floor(of_sm / held), rest = of_sm - turns * held;
+      const double cost = turns * held * part / rate((int)held * warps) + (rest > 0. ? rest * part / rate((int)rest * warps) : 0.) +
+                          (cluster > 1 ? 2200. : 1000.) * (std::ceil(of_sm / held) - 1.) + 100. * doublings;
+      if (cost < least) least = cost, best = {cluster, warps};
+    }
+  }
+  return best;
 }
 
 // Whether every item is given to one CTA: one launch, no sums in the workspace.
 template <typename Shape>
 static bool is_whole(const SplashCacheAttendArgs& a, bool by_head) {
-  if (cluster_of<Shape>(a, by_head) > 0) return true;
+  if (by_head) return form_by_head<Shape>(a).cluster > 0;
   const int64_t items = items_of<Shape>(a);
   const bool some = items >= kWholeItems && items < kMostWholeItems;
   return reach_of(a) <= (some ? 2 * kWholeTokens : kWholeTokens) && items <= INT32_MAX;
@@ -1442,7 +1464,9 @@ static int cache_attend(const SplashCacheAttendArgs& args, bool by_head, cudaStr
     using Shape = decltype(shape);
     AttendParams own = p;
     own.whole = is_whole<Shape>(a, by_head);
-    own.cluster = own.whole && by_head ? std::max(cluster_of<Shape>(a, true), 1) : 1;
+    const int64_t items = items_of<Shape>(a);
+    const Form form = by_head ? form_by_head<Shape>(a) : Form{0, own.whole && items < 2 * kSms ? kMostWarps : kWarps};
+    own.cluster = std::max(form.cluster, 1);
     if (!own.whole) {
       const size_t parts = parts_bytes<Shape>();
       if (a.workspace == nullptr || (reinterpret_cast<uintptr_t>(a.workspace) & 15u) != 0 ||
@@ -1454,7 +1478,7 @@ static int cache_attend(const SplashCacheAttendArgs& args, bool by_head, cudaStr
     own.row_tiles = (p.q_len * p.heads_per_kv + Shape::kRows - 1) / Shape::kRows;
     own.items = a.cache.kv_heads * own.row_tiles;
     own.item_cost = item_tokens(Shape::kN) / Shape::kUnit;
-    return launch<Shape>(own, resident<Shape>(), stream);
+    return launch<Shape>(own, form.warps, resident<Shape>(), stream);
   });
 }
 
