@@ -584,7 +584,7 @@ int splash_cache_bound_values(const SplashKvCache* cache, const SplashPageBounds
  * infinities as for the bounds).  Sums are of whole numbers: the choice does not depend on their order.
  * tables [batch, kv_heads, q_len, count] int32: the pages taken, as numbers of the pool, in the order of the sequence, then -1;
  * table_lengths [batch, kv_heads, q_len] int32: the tokens up to the query's position that lie on them.
- * Bounds of the queries' own pages are not read.  workspace: splash_cache_choose_workspace_bytes, 16-byte aligned; need not be zeroed. */
+ * Bounds of pages that are always taken have no part.  workspace: splash_cache_choose_workspace_bytes, 16-byte aligned; need not be zeroed. */
 typedef struct SplashCacheChooseArgs {
   SplashKvCache cache;
   SplashPageBounds bounds;

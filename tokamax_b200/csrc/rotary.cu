@@ -173,7 +173,7 @@ static int launch_rotate(RotateParams& p, bool interleaved, cudaStream_t stream)
   p.rows_each = kRotateThreads / p.lanes;
   const int heads = p.side[0].heads + p.side[1].heads;
   // Four heads a thread, whose loads are in flight together, unless that leaves the GPU without threads.
-  p.heads_each = (int64_t)p.rows * p.lanes * heads < (int64_t)kSms * 2048 ? 1 : kRotateAhead;
+  p.heads_each = (int64_t)p.rows * p.lanes * heads < (int64_t)kSms * 2048 && heads <= 65535 ? 1 : kRotateAhead;
   const dim3 grid((p.rows + p.rows_each - 1) / p.rows_each, (unsigned)((heads + p.heads_each - 1) / p.heads_each));
   const int block = p.rows_each * p.lanes;
   if (interleaved)
