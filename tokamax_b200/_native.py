@@ -33,6 +33,7 @@ SOURCES = (
     "exchange.cu",
     "cache_rows.cu",
     "cache_attend_sm100.cu",
+    "cache_attend_tables_sm100.cu",
     "cache_pages.cu",
     "rotary.cu",
     "splash_xla_ffi.cc",  # handlers compile only where xla/ffi/api/ffi.h is on the include path
@@ -42,7 +43,7 @@ HOST_SOURCE = "splash_torch.cpp"  # the host side of a call: tensors in, tensors
 
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-lineinfo", "-O3", "-std=c++17",
+    "-lineinfo", "-O3", "-std=c++17", "--threads", "8",
     "-shared", "-Xcompiler", "-fPIC",
 )
 

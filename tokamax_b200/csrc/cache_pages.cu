@@ -4,7 +4,8 @@
 // Mathematics.  With least_c <= k_c <= largest_c for the keys of a page, q . k <= sum over c of max(q_c least_c, q_c largest_c) =
 // sum over c of min(q_c, 0) least_c + max(q_c, 0) largest_c, a product of rows of twice the head dim.  Both sides are held in 8 bits, so
 // that the sum is one of whole numbers: it has no rounding, and the choice is the same in any order of summation.  (The 8 bits are
-// rounded to the nearest: the sum is a score then, a bound within half a step a channel.)
+// rounded to the nearest: the sum is a score then, a bound within half a step a channel.)  Bounds of a page are 256 bytes a head
+// (head dim 128) beside the 9 KB of its keys and values: a choice among all pages costs 3 % of what attention over them would.
 #include <atomic>
 
 #include "cache_common.cuh"
@@ -118,6 +119,11 @@ struct RowPiece {
 
 constexpr int kWarpTokens = 128;
 
+// Bound by instructions and latency, not by memory (72 bytes a row of 128 channels in four bits): a channel of a key takes an extraction
+// (a mask with an exponent, 2 cycles of a scheduler), a sum, a fused multiply-add and half of two three-way extremes, 6.2 cycles, and a page
+// some 500 instructions beside.  A warp a page of 64 tokens, eight rows a lane in flight: 4 prompts of up to 8192 tokens, 8 heads
+// of 128, 9.6 us (26 with a block of 256 threads a page and its extremes by way of shared memory, 11.0 with four rows in flight, 11.9 with
+// 32 tokens a warp); the instructions alone 3.7, memory 1.6; 9.6 is two turns of the warps that there are for an SM.
 // `split` warps of a block have a page of a sequence and kv head; blockIdx.x: pages (from the first that has become whole) and
 // heads, the heads fastest; y: the sequence.  A team of kTeam lanes (the power of two that holds the row's width / 16) has a
 // token's row.
@@ -384,6 +390,13 @@ struct Found {  // of a row's pages
 };
 
 // A cluster (of one CTA and more) has a query and kv head: its CTAs score pages, tile by tile of 16, and the first one chooses.
+// The bounds of a page are a row of the products' first operand as they lie in memory: channels may come in any order as long as q's do
+// too, so that a lane's 16 bytes are the registers of two products.  The wanted-th largest of the scores is found by a histogram of
+// 1024 bins over their range; the few in its bin are counted against each other.
+// Bound by latency: of some 13000 cycles for 2048 pages, 8 CTAs a row (7.4 us) the first loads take 2000, q's codes 1600, two tiles of each
+// warp 2300, the cluster's barrier 1200, the histogram 1400, the few 2400 and the writing 1300, all of it chains of dependent steps at 20 % of the
+// instructions that an SM could issue.  32 sequences of 8192 .. 32768 tokens 9.5 us (21 MB of bounds: 3.3).  Tried: tiles through
+// shared memory by asynchronous copies 11.5, two and three tiles ahead 10.5, 8 warps for short rows (62 pages, 512 rows) 6.2 -> 10.2.
 // kChunks: pieces of 64 numbers that the bounds of a page are; kOnChip: the scores are in shared memory.
 template <int kChunks, int kWarps, bool kOnChip>
 __global__ void __launch_bounds__(kWarps * 32, (kChunks <= 4 ? 16 : 8) / kWarps) cache_choose_kernel(const __grid_constant__ ChooseParams p) {

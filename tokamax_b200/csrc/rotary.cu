@@ -5,8 +5,11 @@
 // whole turns exactly, at any position, with one integer multiplication, where a product in floating point loses the
 // fraction of a turn as positions grow (32 bits: 0.03 of a turn at 10^6).  The 32 high bits go to sincospi as half turns.
 //
-// Bound by memory: a value is read once and written once.  A thread has the same pairs of a token for some heads, so that an angle,
-// its sine and cosine are worked out once for them.
+// Bound by memory: a value is read once and written once.  A thread has the same eight pairs of a token for four heads: an angle, its
+// sine and cosine are worked out once for them, and eight loads of 16 bytes are in flight.  4 x 4096 tokens, 32 + 8 heads of 128, bf16:
+// 54.8 us, 6.1 TB/s (a plain copy of the same tensors 58.4, each input and output once at the copy rate 51.3); with two heads a
+// thread 70, with ten 59.6, forty 66.6; eight loads ahead 74.  2 x 8192 forward and back 104.7 (floor 102.6).  Interleaved 57.8.
+// Evicting loads and stores, and blocks of 128, +-1 %.
 #include "cache_common.cuh"
 
 namespace sb {
@@ -185,7 +188,8 @@ static int launch_rotate(RotateParams& p, bool interleaved, cudaStream_t stream)
 
 template <int kDType>
 static int pick_rotate(RotateParams& p, bool interleaved, cudaStream_t stream) {
-  // Eight pairs a lane, 16 bytes of a 16-bit type, where the pairs come in eights, else four or one.
+  // Eight pairs a lane, 16 bytes of a 16-bit type, where the pairs come in eights, else four or one (two bytes at a time: for widths
+  // such as 20 of 80 channels, which have no better alignment).
   if (p.dim % 16 == 0) return launch_rotate<kDType, 8>(p, interleaved, stream);
   if (p.dim % 8 == 0) return launch_rotate<kDType, 4>(p, interleaved, stream);
   return launch_rotate<kDType, 1>(p, interleaved, stream);
