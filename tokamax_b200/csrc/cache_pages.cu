@@ -71,7 +71,7 @@ struct BoundParams {
   const int32_t* page_table;
   const int32_t* lengths;
   int64_t table_stride, n_pages, newest, batch;
-  int32_t n_table, page_size, page_shift, kv_heads, head_dim, row, group_shift, slots, split;
+  int32_t n_table, page_size, page_shift, kv_heads, head_dim, row, group_shift, split;
 };
 
 constexpr int kBoundThreads = 128, kBoundWarps = kBoundThreads / 32;
@@ -103,7 +103,9 @@ struct RowPiece {
       for (int j = 0; j < kPiece; ++j) {
         const int i = j % 8 < 5 ? j % 8 : j % 8 - 5;
         const uint32_t word = j % 8 < 5 ? w[j / 8] : w[j / 8] >> 20, exponent = 0x4b000000u - i * 0x02000000u;
-        x[j] = fmaf(s, __uint_as_float((word & 15u << 4 * i) | exponent) - __uint_as_float(exponent), zero);
+        uint32_t above;  // (the compiler takes two instructions for it)
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(above) : "r"(word), "r"(15u << 4 * i), "r"(exponent));
+        x[j] = fmaf(s, __uint_as_float(above) - __uint_as_float(exponent), zero);
       }
     } else {
 #pragma unroll
@@ -117,15 +119,16 @@ struct RowPiece {
   }
 };
 
-constexpr int kWarpTokens = 128;
+constexpr int kWarpTokens = 64;
 
 // Bound by instructions and latency, not by memory (72 bytes a row of 128 channels in four bits): a channel of a key takes an extraction
-// (a mask with an exponent, 2 cycles of a scheduler), a sum, a fused multiply-add and half of two three-way extremes, 6.2 cycles, and a page
-// some 500 instructions beside.  A warp a page of 64 tokens, eight rows a lane in flight: 4 prompts of up to 8192 tokens, 8 heads
-// of 128, 9.6 us (26 with a block of 256 threads a page and its extremes by way of shared memory, 11.0 with four rows in flight, 11.9 with
-// 32 tokens a warp); the instructions alone 3.7, memory 1.6; 9.6 is two turns of the warps that there are for an SM.
-// `split` warps of a block have a page of a sequence and kv head; blockIdx.x: pages (from the first that has become whole) and
-// heads, the heads fastest; y: the sequence.  A team of kTeam lanes (the power of two that holds the row's width / 16) has a
+// (a mask with an exponent, 2 cycles of a scheduler), a sum, a fused multiply-add and two extremes, 6.1 cycles, and a page some 500
+// instructions beside.  A warp a page of 64 tokens, eight rows a lane in flight: 4 prompts of up to 8192 tokens, 8 heads of 128, 8.0 us (26
+// with a block of 256 threads a page and its extremes by way of shared memory, 9.6 with quotients of 64 bits for pages and heads and two
+// instructions for an extraction, 8.6 with four rows in flight, 10.3 with 32 tokens a warp); the instructions alone 3.6, memory 1.6.
+// Eight channels a lane, 16 to 32 warps on an SM, sums of two channels in an instruction: no faster.
+// `split` warps of a block have a page of a sequence and kv head; blockIdx.x: the page (from the first that has become whole), y: the
+// sequence, z: kv heads.  A team of kTeam lanes (the power of two that holds the row's width / 16) has a
 // token's row.
 template <int kFormat, int kTeam>
 __global__ void __launch_bounds__(kBoundThreads, 4) cache_bound_kernel(const __grid_constant__ BoundParams p) {
@@ -136,17 +139,15 @@ __global__ void __launch_bounds__(kBoundThreads, 4) cache_bound_kernel(const __g
   __shared__ float extremes[kBoundWarps][2][32 * kOwn];
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane % kTeam, team = lane / kTeam;
-  const int share = warp % p.split;  // of the page's tokens
-  const int64_t items = (int64_t)p.slots * p.kv_heads, step = (int64_t)gridDim.x * (kBoundWarps / p.split);
+  const int share = warp & (p.split - 1);  // of the page's tokens (`split` is a power of two)
+  const int head = (int)((blockIdx.z * blockDim.x + threadIdx.x) / (32u * p.split));
   const bool real = part * kPiece < p.row;  // (of teams of 96 and 192 channels some lanes have none)
   for (int64_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
     const int64_t length = min((int64_t)max(__ldg(p.lengths + b), 0), (int64_t)p.n_table << p.page_shift);
     const int64_t first = max(length - p.newest, (int64_t)0) >> p.page_shift, whole = length >> p.page_shift;
-    for (int64_t item0 = (int64_t)blockIdx.x * (kBoundWarps / p.split); item0 < items; item0 += step) {
-      if (first + item0 / p.kv_heads >= whole) break;  // (all warps of the block alike)
-      const int64_t item = item0 + warp / p.split, index = first + item / p.kv_heads;
-      const int head = (int)(item % p.kv_heads);
-      const int page = item < items && index < whole ? __ldg(p.page_table + b * p.table_stride + index) : -1;
+    const int64_t index = first + blockIdx.x;
+    if (index < whole) {  // (all warps of the block alike)
+      const int page = head < p.kv_heads ? __ldg(p.page_table + b * p.table_stride + index) : -1;
       const bool mine = in_pool(page, p.n_pages);
       float lo[kPiece], hi[kPiece];
 #pragma unroll
@@ -293,17 +294,16 @@ static int cache_bound(const SplashCacheBoundArgs& a, cudaStream_t stream) {
   p.group_shift = log2_of(c.group);
   // n tokens make n / page_size + 1 pages whole at most
   const int64_t pages = a.newest / c.page_size + 1;
-  p.slots = (int32_t)(pages < a.n_table ? pages : a.n_table);
   // A warp has up to kWarpTokens of a page's tokens, as far as the warps of a block go.
   p.split = 1;
   while (p.split < kBoundWarps && p.split * kWarpTokens < c.page_size) p.split *= 2;
-  const int per_block = kBoundWarps / p.split;
-  const int64_t blocks = ((int64_t)p.slots * c.kv_heads + per_block - 1) / per_block;
-  const dim3 grid((unsigned)(blocks < INT32_MAX ? blocks : INT32_MAX), (unsigned)(a.batch < 65535 ? a.batch : 65535));
+  const int most = kBoundWarps / p.split, heads = c.kv_heads < most ? c.kv_heads : most;  // of a block
+  const dim3 grid((unsigned)(pages < a.n_table ? pages : a.n_table), (unsigned)(a.batch < 65535 ? a.batch : 65535),
+                  (unsigned)((c.kv_heads + heads - 1) / heads));
   cudaLaunchConfig_t config{};
   cudaLaunchAttribute attribute = early_launch();
   config.gridDim = grid;
-  config.blockDim = dim3(kBoundThreads);
+  config.blockDim = dim3(heads * p.split * 32);
   config.stream = stream;
   config.attrs = &attribute;
   config.numAttrs = 1;

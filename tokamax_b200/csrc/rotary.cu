@@ -3,7 +3,7 @@
 // Mathematics.  Pair i of a row's first channels, as a complex number, times factor * exp(2 pi I * position * turns[i]); the gradient is
 // the product with the conjugate.  Angles are fixed-point fractions of a whole turn, 64 bits: position * turns modulo 2^64 drops
 // whole turns exactly, at any position, with one integer multiplication, where a product in floating point loses the
-// fraction of a turn as positions grow (32 bits: 0.03 of a turn at 10^6).  The 32 high bits go to sincospi as half turns.
+// fraction of a turn as positions grow (32 bits: 0.06 radians at 10^6).  The 32 high bits go to sincospi as half turns.
 //
 // Bound by memory: a value is read once and written once.  A thread has the same eight pairs of a token for four heads: an angle, its
 // sine and cosine are worked out once for them, and eight loads of 16 bytes are in flight.  4 x 4096 tokens, 32 + 8 heads of 128, bf16:
