@@ -360,8 +360,8 @@ struct ChooseParams {
   int32_t dtype, batch, kv_heads, heads_per_kv, q_len, n_table, page_size, page_shift, head_dim, row, count, first, last;
 };
 
-constexpr int kKeysOnChip = 8192;       // pages of a row whose scores, and numbers, shared memory holds
-constexpr int kChooseShared = 220 * 1024;  // for a CTA, beside some 6 KB of fixed size
+constexpr int kKeysOnChip = 8192;         // pages of a row whose scores, and numbers, shared memory holds
+constexpr int kMostHeads = 128;           // q heads of a kv head
 constexpr int kMostCluster = 8, kMostChooseWarps = 8, kFewPages = 1024;
 constexpr int kBins = 1024, kBinBits = 10;
 constexpr int kFew = 64;  // keys that are counted against each other
@@ -394,8 +394,8 @@ struct Found {  // of a row's pages
 // too, so that a lane's 16 bytes are the registers of two products.  The wanted-th largest of the scores is found by a histogram of
 // 1024 bins over their range; the few in its bin are counted against each other.
 // Bound by latency: of some 13000 cycles for 2048 pages, 8 CTAs a row (7.4 us) the first loads take 2000, q's codes 1600, two tiles of each
-// warp 2300, the cluster's barrier 1200, the histogram 1400, the few 2400 and the writing 1300, all of it chains of dependent steps at 20 % of the
-// instructions that an SM could issue.  32 sequences of 8192 .. 32768 tokens 9.5 us (21 MB of bounds: 3.3).  Tried: tiles through
+// warp 2400, the cluster's barrier 1300, the histogram 1600, the few 2200 and the writing 1700, all of it chains of dependent steps at 20 % of
+// the instructions that an SM could issue.  32 sequences of 8192 .. 32768 tokens 9.5 us (21 MB of bounds: 3.3).  Tried: tiles through
 // shared memory by asynchronous copies 11.5, two and three tiles ahead 10.5, 8 warps for short rows (62 pages, 512 rows) 6.2 -> 10.2.
 // kChunks: pieces of 64 numbers that the bounds of a page are; kOnChip: the scores are in shared memory.
 template <int kChunks, int kWarps, bool kOnChip>
@@ -773,29 +773,28 @@ static int check_choose(const SplashCacheChooseArgs& a) {
   if (a.first < 0 || a.last < 1 || (int64_t)a.first + a.last > a.count) return SPLASH_ERR_INVALID_ARGUMENT;
   // (as splash_cache_attend_tables takes them; rows of q that shared memory has room for)
   if (a.q.size[0] > (1 << 24) || a.q.size[2] > (1 << 20) || a.q.size[0] * c.kv_heads * a.q.size[2] > (1 << 24) ||
-      (int64_t)a.count * c.page_size > (1 << 30) || a.q.size[1] / c.kv_heads > 128)
+      (int64_t)a.count * c.page_size > (1 << 30) || a.q.size[1] / c.kv_heads > kMostHeads)
     return SPLASH_ERR_TOO_LARGE;
   return SPLASH_OK;
 }
 
-// Shared memory of a CTA but for the keys.
-static int choose_shared(int row, int64_t heads_per_kv) { return choose_heads((int)heads_per_kv) * choose_pitch(row); }
-
 static size_t choose_workspace(const SplashCacheChooseArgs& a) {
   if (check_choose(a) != SPLASH_OK) return 0;
-  if (a.n_table <= kKeysOnChip && choose_shared(a.cache.row_k, a.q.size[1] / a.cache.kv_heads) + a.n_table * 8 <= kChooseShared) return 0;
+  if (a.n_table <= kKeysOnChip) return 0;
   return (size_t)(a.q.size[0] * a.cache.kv_heads * a.q.size[2]) * a.n_table * sizeof(uint32_t);
 }
 
 template <int kChunks, int kWarps, bool kOnChip>
 static int launch_choose(const cudaLaunchConfig_t& config, const ChooseParams& p) {
   const auto kernel = cache_choose_kernel<kChunks, kWarps, kOnChip>;
+  constexpr int kMostShared = kMostHeads * choose_pitch(kChunks * 32) + (kOnChip ? kKeysOnChip * 8 : 0);
+  static_assert(kMostShared + 8 * 1024 <= 227 * 1024);
   static std::atomic<uint64_t> ready{0};  // devices that know how much shared memory the kernel takes
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return SPLASH_ERR_CUDA;
   const uint64_t bit = 1ull << (device & 63);
   if (device > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kChooseShared) != cudaSuccess) return SPLASH_ERR_CUDA;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return SPLASH_ERR_CUDA;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   return cudaLaunchKernelEx(&config, kernel, p) == cudaSuccess ? SPLASH_OK : SPLASH_ERR_CUDA;
@@ -837,7 +836,7 @@ static int cache_choose(const SplashCacheChooseArgs& a, cudaStream_t stream) {
   const int warps = a.n_table <= kFewPages ? kMostChooseWarps / 2 : kMostChooseWarps;
   int ctas = 1;
   while (ctas < kMostCluster && rows * ctas * 2 <= 2 * kSms && (int64_t)a.n_table > (int64_t)ctas * warps * 16) ctas *= 2;
-  const int smem = choose_shared(p.row, p.heads_per_kv) + (p.keys == nullptr ? a.n_table * 8 : 0);
+  const int smem = choose_heads(p.heads_per_kv) * choose_pitch(p.row) + (p.keys == nullptr ? a.n_table * 8 : 0);
   cudaLaunchConfig_t config{};
   config.gridDim = dim3((unsigned)(rows * ctas));
   config.blockDim = dim3(warps * 32);
