@@ -429,6 +429,16 @@ def test_tables_through_their_strides_and_nothing_at_all():
   assert call(q[:0], tables[:0], tokens[:0]).shape == (0, 4, 2, 64)
 
 
+def test_outputs_lie_as_the_queries_do():
+  store = Store([200, 90], heads=2, d=64, page=16)
+  tables, tokens = (x.to(DEV) for x in _random_tables(store, 3, 5))
+  q = torch.randn(2, 3, 8, 64, device=DEV, dtype=torch.bfloat16)[:, :, :4].transpose(1, 2)  # a part of a projection
+  for pages in ((tables, tokens), (store.table, store.lengths)):
+    out = kv_cache.attend(store.cache, q, *pages, logits_scale=0.1)
+    assert out.stride() == torch.empty_like(q).stride() and out.transpose(1, 2).is_contiguous()
+    assert torch.equal(out, kv_cache.attend(store.cache, q.contiguous(), *pages, logits_scale=0.1))
+
+
 @pytest.mark.parametrize("fmt,group", FORMATS)
 def test_a_choice_of_all_pages_is_attention_over_the_whole(fmt, group):
   """The same keys in the same order: bf16 outputs differ by roundings of sums of 32 bits at most, a step of bf16 where one is beside a tie."""

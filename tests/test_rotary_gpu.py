@@ -1,5 +1,7 @@
 """Rotary positions against products of complex numbers in 64 bits, and their gradients."""
+import copy
 import math
+import pickle
 
 import numpy as np
 import pytest
@@ -106,6 +108,41 @@ def test_operands_through_their_strides():
   assert torch.equal(rotary.rotate(rot, positions, wide), want[0][:1, :1].expand(2, 4, -1, -1))
   flipped = q.transpose(2, 3).contiguous().transpose(2, 3)  # tokens contiguous
   assert torch.equal(rotary.rotate(rot, positions, flipped), want[0])
+
+
+def test_results_of_parts_of_a_projection_lie_as_the_projection_does():
+  rot = rotary.make_rotary(64, device=DEV)
+  qkv = torch.randn(2, 30, 8, 64, device=DEV, dtype=torch.bfloat16)
+  q, k = qkv[:, :, :6].transpose(1, 2), qkv[:, :, 6:].transpose(1, 2)
+  out_q, out_k = rotary.rotate(rot, torch.arange(30, device=DEV), q, k)
+  assert out_q.transpose(1, 2).is_contiguous() and out_k.transpose(1, 2).is_contiguous()
+  assert out_q.stride() == torch.empty_like(q).stride()
+
+
+def test_a_module_that_holds_one_is_copied_and_pickled():
+  rot = rotary.make_rotary(32, base=500.0, interleaved=True, factor=1.5, device=DEV)
+  q, positions = _rows(1, 2, 9, 48, torch.float32, 5), torch.arange(9, device=DEV) * 1000
+  want = rotary.rotate(rot, positions, q)
+  for other in (copy.deepcopy(rot), copy.copy(rot), pickle.loads(pickle.dumps(rot))):
+    assert torch.equal(rotary.rotate(other, positions, q), want)
+  assert copy.deepcopy(rot).turns.data_ptr() != rot.turns.data_ptr()
+
+
+def test_rows_without_gradients_stay_so():
+  rot = rotary.make_rotary(64, device=DEV)
+  positions = torch.arange(5, device=DEV)
+  q, k = _rows(1, 2, 5, 64, torch.float32, 6).requires_grad_(), _rows(1, 1, 5, 64, torch.float32, 7)
+  out_q, out_k = rotary.rotate(rot, positions, q, k)
+  assert out_q.requires_grad and not out_k.requires_grad
+  (out_q.sum() + out_k.sum()).backward()
+  grad, q.grad = q.grad, None
+  rotary.rotate(rot, positions, q).sum().backward()
+  assert torch.equal(q.grad, grad)
+  out_k, out_q = rotary.rotate(rot, positions, k, q)
+  assert out_q.requires_grad and not out_k.requires_grad
+  q.grad = None
+  out_q.sum().backward()
+  assert torch.equal(q.grad, grad) and k.grad is None
 
 
 def test_nothing_at_all():

@@ -59,9 +59,9 @@
 
 namespace sb {
 
-// Warps of a CTA; kMostWarps where every item is one CTA's and there are fewer than two for an SM (tables by head: see form_by_head) (us, 4 : 8 warps, up to 1024
-// tokens, 8 items 12.5 : 10.6, 256 items 14.6 : 14.6, 1024 items 35.6 : 44.3).  Shares: four CTAs of 4 warps on an SM and two of 8
-// are alike where sequences are long, short ones want the smaller CTAs (64 x 200 .. 4096: 53.6 : 56.3).
+// Warps of a CTA; kMostWarps where every item is one CTA's and there are fewer than two for an SM (us, 4 : 8 warps, up to 1024
+// tokens, 8 items 12.5 : 10.6, 256 items 14.6 : 14.6, 1024 items 35.6 : 44.3; tables by head: form_by_head).  Shares: four CTAs of 4
+// warps on an SM and two of 8 are alike where sequences are long, short ones want the smaller CTAs (64 x 200 .. 4096: 53.6 : 56.3).
 constexpr int kWarps = 4, kMostWarps = 8;
 constexpr int kMostCluster = 8;
 
@@ -1398,7 +1398,7 @@ static int64_t items_of(const SplashCacheAttendArgs& a) {
 //   * a cluster's barriers and sums 0.35 us for each doubling; a warp has a unit at least;
 //   * shares: equal for all SMs, and 4 us for the second launch and the search, 1.2 for each item of an SM.
 // us measured, shares | 1 CTA of 8 warps | the form taken: 8 items of 1024 tokens 11.6 | 9.6 | 7.3 (8 x 8), of 8192 13.6 | 42.6 | 11.4 (8 x 8);
-// 32 of 4096 14.8 | 23.8 | 11.3 (4 x 8); 96 of 3072 tokens 22.7 | 19.7 | 17.5 (4 x 4), 192 of 4096 38.3 | 37.6 | 32.4 (2 x 4), 256 of 4096
+// 32 of 4096 14.8 | 23.8 | 11.3 (4 x 8), 192 of 4096 38.3 | 37.6 | 32.4 (2 x 4), 256 of 4096
 // 45.7 | 37.6 | 37.6, 512 of 1024 23.1 | 27.0 | 23.1 (1 x 4).
 struct Form {
   int cluster, warps;  // cluster 0: shares

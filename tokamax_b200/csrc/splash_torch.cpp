@@ -10,6 +10,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <ATen/ATen.h>
+#include <ATen/ExpandUtils.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
@@ -379,10 +380,10 @@ void check_cache_call(int status, const char* what) {
 
 // Memory for results, from torch's allocator without its dispatcher (a microsecond less for each).
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, at::Device device) { return at::detail::empty_cuda(sizes, type, device, std::nullopt); }
-// In the order of t's dense strides.
+// In the order of t's strides, dense.
 at::Tensor fresh_like(const at::Tensor& t) {
-  return t.is_non_overlapping_and_dense() ? at::Tensor(at::detail::empty_strided_cuda(t.sizes(), t.strides(), t.scalar_type(), t.device()))
-                                          : fresh(t.sizes(), t.scalar_type(), t.device());
+  if (t.is_non_overlapping_and_dense()) return at::detail::empty_strided_cuda(t.sizes(), t.strides(), t.scalar_type(), t.device());
+  return at::detail::empty_strided_cuda(t.sizes(), at::infer_dense_strides(t.sizes(), t.strides()), t.scalar_type(), t.device());
 }
 
 template <typename Fn>
@@ -662,6 +663,10 @@ struct Rotation : torch::autograd::Function<Rotation> {
     ctx->save_for_backward({positions});
     ctx->saved_data["call"] = c10::IValue::make_capsule(call);
     ctx->set_materialize_grads(false);
+    variable_list constant;  // (rows that no gradient is asked of stay so: a cache takes no others)
+    if (!x.requires_grad()) constant.push_back(y);
+    if (z.has_value() && !z->requires_grad()) constant.push_back(w);
+    ctx->mark_non_differentiable(constant);
     return z.has_value() ? variable_list{y, w} : variable_list{y};
   }
 

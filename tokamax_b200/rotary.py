@@ -97,6 +97,13 @@ class Rotary:
   turns: torch.Tensor
   native: object = dataclasses.field(repr=False)
 
+  def __reduce__(self):  # (a module that holds one can be copied and pickled)
+    return _of_turns, (self.dim, self.interleaved, self.factor, self.turns)
+
+
+def _of_turns(dim: int, interleaved: bool, factor: float, turns: torch.Tensor) -> Rotary:
+  return Rotary(dim, interleaved, factor, turns, _native.host().RotaryTable(turns, dim, interleaved, factor))
+
 
 def make_rotary(dim: int, *, base: float = 10000.0, scaling: Scaling | None = None, frequency=None, factor: float | None = None,
                 interleaved: bool = False, device="cuda") -> Rotary:
@@ -116,7 +123,7 @@ def make_rotary(dim: int, *, base: float = 10000.0, scaling: Scaling | None = No
     raise ValueError(f"factor must be finite, got {factor}")
   parts = [round(Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64 for f in freq.tolist()]  # (whole turns are none)
   turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in parts], dtype=torch.int64, device=device)
-  return Rotary(dim, interleaved, factor, turns, _native.host().RotaryTable(turns, dim, interleaved, factor))
+  return _of_turns(dim, interleaved, factor, turns)
 
 
 def rotate(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None = None):
@@ -124,7 +131,8 @@ def rotate(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Te
   the rotated q alone.
 
   ``positions [B, T]`` or ``[T]`` (int32 or int64), any numbers.  Rows are read through their strides, the ``[B, T, H, D]`` of a projection,
-  transposed, is not copied, and results lie as the inputs do.  Products are of 32 bits, rounded to the type once.
+  transposed, is not copied, and results lie as the inputs do.  (Strides that are no multiples of eight, or rows that begin between
+  two boundaries of 16 bytes: a contiguous copy is turned.)  Products are of 32 bits, rounded to the type once.
 
   Gradients go to q and k: the rotation back, which keeps nothing of a call but its positions.  Tangents of forward mode and
   ``torch.jit.trace`` are refused."""
