@@ -210,3 +210,42 @@ def test_the_oracle_bounds_logits():
   logits = (k @ q.T).amax((1, 2))
   off = 0.5 * scales * q.abs().sum(-1).max() + 0.5 * q.abs().max() / 127 * k.abs().amax((1, 2)) * 64
   assert (score >= logits - off * (1 + 2.0 ** -20)).all() and not math.isinf(float(score.max()))
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(q=torch.zeros(1, 3, 1, 64)), "does not match a cache"), (dict(q=torch.zeros(1, 4, 1, 32)), "does not match a cache"),
+    (dict(q=torch.zeros(4, 1, 64)), "does not match a cache"), (dict(q=torch.zeros(1, 0, 1, 64)), "does not match a cache"),
+    (dict(q=torch.zeros(2, 4, 1, 64)), "q of 2 sequences, lengths of 1"), (dict(table=torch.zeros(1, 4)), "are int32"),
+    (dict(table=torch.zeros(4, dtype=torch.int32)), r"expected \[B, pages\] and \[B\]"), (dict(table=torch.zeros(1, 0, dtype=torch.int32)), "of 0 pages"),
+    (dict(lengths=torch.ones(2, dtype=torch.int32)), r"expected \[B, pages\] and \[B\]"), (dict(lengths=torch.ones(1)), "are int32"),
+    (dict(q=torch.zeros(2, 4, 1, 64), table=torch.zeros(2, 4, dtype=torch.int32), lengths=torch.ones(4, dtype=torch.int32)[::2]), "lengths are contiguous"),
+    *((bad, "expected first >= 0, last >= 1 and count >= first") for bad in (
+        dict(count=0), dict(count=1), dict(count=2, first=2), dict(first=-1), dict(last=0), dict(count=1 << 32), dict(last=1 << 33, count=1 << 34)))])
+def test_what_a_choice_is_refused_for(kw, message):
+  """Each for its own reason, wherever the operands are."""
+  with pytest.raises(ValueError, match=message):
+    _choose(**kw)
+
+
+def test_what_bounds_are_refused_for():
+  cache = _cache()
+  bounds, table, lengths = kv_cache.make_page_bounds(cache), torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+  for bad, message in (((table, lengths, -1), "newest is not negative"), ((table, lengths.repeat(2), 1), r"expected \[B, pages\] and \[B\]"),
+                       ((table[:, :0], lengths, 1), "of 0 pages"), ((table.long(), lengths, 1), "are int32")):
+    with pytest.raises(ValueError, match=message):
+      kv_cache.bound_pages(cache, bounds, *bad)
+
+
+TABLES_THAT_DO_NOT_MATCH = [
+    ((1, 2, 1, 4), (1, 2), None, "do not match: expected .B, kv_heads, T, pages."), ((1, 2, 1, 4), (1, 2, 2), None, "do not match: expected .B, kv_heads"),
+    ((1, 1, 1, 4), (1, 1, 1), None, "do not match: expected .B, kv_heads"), ((2, 2, 1, 4), (2, 2, 1), None, "do not match: expected .B, kv_heads"),
+    ((1, 2, 3, 4), (1, 2, 3), None, "do not match: expected .B, kv_heads"), ((1, 2, 1, 4), (1, 2, 1), 5, "local_window_size goes by places"),
+    ((1, 2, 1, 0), (1, 2, 1), None, "of 0 pages"), ((1, 2, 4), (1, 2), None, r"expected \[B, pages\] and \[B\]"),
+    ((2, 4), (2,), None, "q of 1 sequences, lengths of 2")]
+
+
+@pytest.mark.parametrize("table,lengths,window,message", TABLES_THAT_DO_NOT_MATCH)
+def test_what_tables_are_refused_for(table, lengths, window, message):
+  with pytest.raises(ValueError, match=message):
+    kv_cache.attend(_cache(), torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16), torch.zeros(table, dtype=torch.int32),
+                    torch.ones(lengths, dtype=torch.int32), local_window_size=window)

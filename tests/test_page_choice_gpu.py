@@ -7,6 +7,7 @@ import torch
 from oracle import kv_cache_ref
 from oracle import pages_ref
 from test_kv_cache_gpu import ROUNDOFF, Store
+from test_page_choice_cpu import TABLES_THAT_DO_NOT_MATCH
 from tokamax_b200 import _native
 from tokamax_b200 import kv_cache
 
@@ -539,3 +540,24 @@ def test_refusals():
     kv_cache.choose_pages(store.cache, bounds, q.expand(-1, 4, -1, -1).repeat(1, 65, 1, 1), store.table, store.lengths, 4)
   with pytest.raises(ValueError, match="count"):
     kv_cache.choose_pages(store.cache, bounds, q, store.table, store.lengths, 1)
+
+
+@pytest.mark.parametrize("table,lengths,window,message", TABLES_THAT_DO_NOT_MATCH)
+def test_what_tables_are_refused_for(table, lengths, window, message):
+  """The kernel takes the extents of tables and lengths from q and the cache: what does not match them is not looked at."""
+  cache = kv_cache.make_kv_cache(5, 16, 2, 64, device=DEV)
+  with pytest.raises(ValueError, match=message):
+    kv_cache.attend(cache, torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(table, dtype=torch.int32, device=DEV),
+                    torch.ones(lengths, dtype=torch.int32, device=DEV), local_window_size=window)
+
+
+@pytest.mark.parametrize("kw", [dict(count=0), dict(count=1), dict(count=2, first=2), dict(first=-1), dict(last=0), dict(count=1 << 32),
+                                dict(last=1 << 33, count=1 << 34)])
+def test_counts_that_are_refused(kw):
+  cache = kv_cache.make_kv_cache(5, 16, 2, 64, device=DEV)
+  i = torch.ones(1, dtype=torch.int32, device=DEV)
+  with pytest.raises(ValueError, match="expected first >= 0, last >= 1 and count >= first"):
+    kv_cache.choose_pages(cache, kv_cache.make_page_bounds(cache), torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16, device=DEV), i[:, None], i,
+                          **dict(dict(count=3), **kw))
+  with pytest.raises(ValueError, match="q of 2 sequences, lengths of 1"):
+    kv_cache.choose_pages(cache, kv_cache.make_page_bounds(cache), torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16, device=DEV), i[:, None], i, 3)

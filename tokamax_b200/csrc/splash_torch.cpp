@@ -421,20 +421,27 @@ void cache_append(const KvCache& cache, const at::Tensor& k_in, const at::Tensor
   check_cache_call(on_stream_of(k, [&](void* stream) { return cache_lib.append(&a, stream); }), "splash_cache_append");
 }
 
-void require_pages(const at::Tensor& table, const at::Tensor& lengths, int64_t pages, const KvCache& cache) {
+// What can be said of page tables and lengths wherever they are; calls make all such checks before they ask for the device.
+void require_pages(const at::Tensor& table, const at::Tensor& lengths, int64_t pages) {
   TORCH_CHECK_VALUE(table.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt, "the page table and the lengths are int32");
-  require_on_gpu(table, cache, "the page table");
-  require_on_gpu(lengths, cache, "lengths");
   TORCH_CHECK_VALUE(pages >= 1 && pages <= INT32_MAX, "a page table of ", pages, " pages");
 }
+// [B, pages] and [B]
+void require_pages_of_sequences(const at::Tensor& table, const at::Tensor& lengths) {
+  TORCH_CHECK_VALUE(table.dim() == 2 && lengths.dim() == 1 && table.size(0) == lengths.size(0), "page table ", table.sizes(), " and lengths ",
+                    lengths.sizes(), " do not match: expected [B, pages] and [B]");
+  require_pages(table, lengths, table.size(1));
+  TORCH_CHECK_VALUE(lengths.size(0) <= 1 || lengths.stride(0) == 1, "lengths are contiguous");
+}
+void require_pages_on_gpu(const at::Tensor& table, const at::Tensor& lengths, const KvCache& cache) {
+  require_on_gpu(table, cache, "the page table");
+  require_on_gpu(lengths, cache, "lengths");
+}
 
-// A page table [B, pages] and the lengths [B] of the sequences, as the kernels take them.
+// A page table [B, pages] and the lengths [B] of the sequences (require_pages_of_sequences), as the kernels take them.
 template <typename Args>
 at::Tensor set_pages(Args& a, const KvCache& cache, const at::Tensor& table_in, const at::Tensor& lengths) {
-  TORCH_CHECK_VALUE(table_in.dim() == 2 && lengths.dim() == 1 && table_in.size(0) == lengths.size(0), "page table ", table_in.sizes(),
-                    " and lengths ", lengths.sizes(), " do not match: expected [B, pages] and [B]");
-  require_pages(table_in, lengths, table_in.size(1), cache);
-  TORCH_CHECK_VALUE(lengths.size(0) <= 1 || lengths.stride(0) == 1, "lengths are contiguous");
+  require_pages_on_gpu(table_in, lengths, cache);
   const at::Tensor table = table_in.size(1) <= 1 || table_in.stride(1) == 1 ? table_in : table_in.contiguous();
   a.cache = cache.desc;
   a.page_table = static_cast<const int32_t*>(table.data_ptr());
@@ -449,8 +456,9 @@ std::tuple<at::Tensor, at::Tensor> cache_read(const KvCache& cache, const at::Te
   const SplashKvCache& c = cache.desc;
   require_not_traced();
   SplashCacheReadArgs a{};
-  const at::Tensor table = set_pages(a, cache, table_in, lengths);
+  require_pages_of_sequences(table_in, lengths);
   TORCH_CHECK_VALUE(max_len >= 0, "max_len is not negative, got ", max_len);
+  const at::Tensor table = set_pages(a, cache, table_in, lengths);
   const auto options = cache.k_codes.options().dtype(type);
   const at::Tensor k = at::empty({lengths.size(0), c.kv_heads, max_len, c.head_dim}, options);
   const at::Tensor v = at::empty({lengths.size(0), c.kv_heads, max_len, c.head_dim_v}, options);
@@ -478,7 +486,8 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
                           table_in.size(1) == c.kv_heads && table_in.size(2) == q_in.size(2),
                       "page tables ", table_in.sizes(), " and lengths ", lengths.sizes(), " do not match: expected [B, kv_heads, T, pages] and [B, kv_heads, T]");
     TORCH_CHECK_VALUE(!window.has_value(), "local_window_size goes by places in the sequence, which tables of chosen pages do not say");
-    require_pages(table_in, lengths, table_in.size(3), cache);
+    require_pages(table_in, lengths, table_in.size(3));
+    require_pages_on_gpu(table_in, lengths, cache);
     table = table_in.contiguous();  // (rows one behind the other)
     lengths = lengths.contiguous();
     a.cache = cache.desc;
@@ -487,8 +496,9 @@ std::tuple<at::Tensor, Maybe, Maybe> cache_attend(const KvCache& cache, const at
     a.n_table = (int32_t)table.size(3);
     a.lengths = static_cast<const int32_t*>(lengths.data_ptr());
   } else {
-    table = set_pages(a, cache, table_in, lengths);
+    require_pages_of_sequences(table_in, lengths);
     TORCH_CHECK_VALUE(q_in.size(0) == lengths.size(0), "q of ", q_in.size(0), " sequences, lengths of ", lengths.size(0));
+    table = set_pages(a, cache, table_in, lengths);
   }
   TORCH_CHECK_VALUE(!window.has_value() || (*window >= 0 && *window <= INT32_MAX), "local_window_size is not negative");
   TORCH_CHECK_VALUE(!soft_cap.has_value() || (float)*soft_cap > 0, "logits_soft_cap is positive (in 32 bits), got ", *soft_cap);
@@ -554,9 +564,10 @@ void require_bounds_of(const PageBounds& bounds, const KvCache& cache) {
 void cache_bound(const KvCache& cache, const PageBounds& bounds, const at::Tensor& table_in, const at::Tensor& lengths, int64_t newest) {
   require_not_traced();
   SplashCacheBoundArgs a{};
+  require_pages_of_sequences(table_in, lengths);
+  TORCH_CHECK_VALUE(newest >= 0, "newest is not negative, got ", newest);
   const at::Tensor table = set_pages(a, cache, table_in, lengths);
   require_bounds_of(bounds, cache);
-  TORCH_CHECK_VALUE(newest >= 0, "newest is not negative, got ", newest);
   a.bounds = bounds.desc;
   a.batch = lengths.size(0);
   a.newest = newest;
@@ -581,10 +592,11 @@ std::tuple<at::Tensor, at::Tensor> cache_choose(const KvCache& cache, const Page
   TORCH_CHECK_VALUE(q_in.dim() == 4 && q_in.size(3) == c.head_dim && q_in.size(1) % c.kv_heads == 0 && q_in.size(1) > 0, "q ", q_in.sizes(),
                     " does not match a cache of ", c.kv_heads, " heads of ", c.head_dim, " channels: expected [B, heads, T, D]");
   SplashCacheChooseArgs a{};
-  const at::Tensor table = set_pages(a, cache, table_in, lengths);
+  require_pages_of_sequences(table_in, lengths);
   TORCH_CHECK_VALUE(q_in.size(0) == lengths.size(0), "q of ", q_in.size(0), " sequences, lengths of ", lengths.size(0));
   TORCH_CHECK_VALUE(first >= 0 && last >= 1 && first <= INT32_MAX && last <= INT32_MAX && count <= INT32_MAX && first + last <= count,
                     "expected first >= 0, last >= 1 and count >= first + last, got first ", first, ", last ", last, ", count ", count);
+  const at::Tensor table = set_pages(a, cache, table_in, lengths);
   require_bounds_of(bounds, cache);
   require_on_gpu(q_in, cache, "q");
   const at::Tensor q = usable(q_in);
