@@ -224,6 +224,27 @@ def test_positions_that_change_before_the_backward_are_noticed():
     out.sum().backward()
 
 
+def test_saved_positions_go_through_hooks():
+  """What a hook gives back is read if it is positions still, on the device, and refused before a kernel follows its address if not."""
+  rot = rotary.make_rotary(64, device=DEV)
+  positions = torch.arange(12, device=DEV).view(2, 6) * 100
+  q, g = _rows(2, 2, 6, 64, torch.float32, 0).requires_grad_(True), _rows(2, 2, 6, 64, torch.float32, 1)
+
+  def gradient(unpack):
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), unpack):
+      out = rotary.rotate(rot, positions, q)
+    return torch.autograd.grad(out, q, g)[0]
+
+  want = gradient(lambda t: t.to(DEV))
+  assert torch.equal(want, torch.autograd.grad(rotary.rotate(rot, positions, q), q, g)[0])
+  assert torch.equal(want, gradient(lambda t: t.to(DEV).int()))
+  assert torch.equal(want, gradient(lambda t: t.t().contiguous().to(DEV).t()))
+  for unpack, message in ((lambda t: t, "positions are on cpu"), (lambda t: t.to(DEV).half(), "int32 or int64"), (lambda t: t.to(DEV)[:, :5], "do not match"),
+                          (lambda t: t.to(DEV)[0, 0], "expected q and k")):
+    with pytest.raises(ValueError, match=message):
+      gradient(unpack)
+
+
 def test_shared_heads_and_broadcast_inputs():
   """Gradients of a head that is expanded add up; a gradient that is expanded itself is read."""
   rot = rotary.make_rotary(64, device=DEV)

@@ -633,6 +633,18 @@ struct RotaryTable {
   double factor;
 };
 
+// Positions [B, T] as the kernel reads them, which takes their extents from the rows: int32 or int64, tokens one behind the other.
+at::Tensor usable_positions(const at::Tensor& given, const at::Tensor& x) {
+  const auto type = given.scalar_type();
+  TORCH_CHECK_VALUE(type == at::kInt || type == at::kLong, "positions are int32 or int64, got ", type);
+  TORCH_CHECK_VALUE(x.dim() == 4 && (given.dim() == 1 || given.dim() == 2), "expected q and k of [B, heads, T, D] and positions of [B, T] or [T]");
+  const at::Tensor positions = given.dim() == 1 ? given.unsqueeze(0) : given;
+  TORCH_CHECK_VALUE((positions.size(0) == 1 || positions.size(0) == x.size(0)) && positions.size(1) == x.size(2), "positions ", given.sizes(),
+                    " do not match q ", x.sizes());
+  TORCH_CHECK_VALUE(positions.device() == x.device(), "positions are on ", positions.device(), ", q on ", x.device());
+  return positions.size(1) > 1 && positions.stride(1) != 1 ? positions.contiguous() : positions;
+}
+
 // x and, where there is one, z, turned by their positions (or back).
 std::tuple<at::Tensor, at::Tensor> rotated(const RotaryTable& table, const at::Tensor& positions, const at::Tensor& x, const Maybe& z, bool inverse) {
   at::Tensor out[2];
@@ -683,7 +695,7 @@ struct Rotation : torch::autograd::Function<Rotation> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    const at::Tensor positions = ctx->get_saved_variables()[0];
+    const at::Tensor saved = ctx->get_saved_variables()[0];
     const auto call = c10::static_intrusive_pointer_cast<RotaryCall>(ctx->saved_data["call"].toCapsule());
     auto back = c10::make_intrusive<RotaryCall>();
     back->table = call->table;
@@ -692,6 +704,8 @@ struct Rotation : torch::autograd::Function<Rotation> {
     const at::Tensor dy = ctx->needs_input_grad(1) ? grads[0] : at::Tensor();
     const at::Tensor dw = grads.size() > 1 && ctx->needs_input_grad(2) ? grads[1] : at::Tensor();
     if (dy.defined() || dw.defined()) {
+      // (hooks of saved tensors may give back anything)
+      const at::Tensor positions = usable_positions(saved, dy.defined() ? dy : dw);
       const variable_list out = Rotation::apply(positions, dy.defined() ? dy : dw, dy.defined() && dw.defined() ? Maybe(dw) : Maybe(), back);
       if (dy.defined()) found[0] = out[0];
       if (dw.defined()) found[1] = out[dy.defined() ? 1 : 0];
@@ -702,12 +716,7 @@ struct Rotation : torch::autograd::Function<Rotation> {
 
 std::tuple<at::Tensor, Maybe> rotate(const std::shared_ptr<RotaryTable>& table, const at::Tensor& positions_in, const at::Tensor& q, const Maybe& k) {
   TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "rotate cannot be recorded by torch.jit.trace");
-  const auto type = positions_in.scalar_type();
-  TORCH_CHECK_VALUE(type == at::kInt || type == at::kLong, "positions are int32 or int64, got ", type);
-  TORCH_CHECK_VALUE(q.dim() == 4 && (positions_in.dim() == 1 || positions_in.dim() == 2), "expected q and k of [B, heads, T, D] and positions of [B, T] or [T]");
-  at::Tensor positions = positions_in.dim() == 1 ? positions_in.unsqueeze(0) : positions_in;
-  TORCH_CHECK_VALUE((positions.size(0) == 1 || positions.size(0) == q.size(0)) && positions.size(1) == q.size(2), "positions ", positions_in.sizes(),
-                    " do not match q ", q.sizes());
+  const at::Tensor positions = usable_positions(positions_in, q);
   const at::Tensor* const both[2] = {&q, k.has_value() ? &*k : nullptr};
   for (int i = 0; i < 2; ++i) {
     const at::Tensor* const t = both[i];
@@ -728,8 +737,6 @@ std::tuple<at::Tensor, Maybe> rotate(const std::shared_ptr<RotaryTable>& table, 
     TORCH_CHECK(device.is_cuda(), i == 0 ? "q" : "k", " is on ", device, ": the kernels need a CUDA device");
     TORCH_CHECK_VALUE(device == table->turns.device(), i == 0 ? "q" : "k", " is on ", device, ", the rotary table on ", table->turns.device());
   }
-  TORCH_CHECK_VALUE(positions.device() == q.device(), "positions are on ", positions.device(), ", q on ", q.device());
-  if (positions.size(1) > 1 && positions.stride(1) != 1) positions = positions.contiguous();
   if (!(at::GradMode::is_enabled() && (q.requires_grad() || (k.has_value() && k->requires_grad())))) {
     const auto [y, w] = rotated(*table, positions, q, k, false);
     return {y, k.has_value() ? Maybe(w) : Maybe()};
