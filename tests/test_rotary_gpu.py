@@ -6,6 +6,7 @@ import pickle
 import numpy as np
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from oracle import rotary_ref
 from tokamax_b200 import rotary
@@ -312,6 +313,19 @@ def test_offsets_beyond_32_bits():
   positions[:, -5:] = torch.arange(5, device=DEV) + 100
   out = rotary.rotate(rot, positions, q)
   assert torch.equal(out[:, :, -5:], rotary.rotate(rot, positions[:, -5:], q[:, :, -5:].contiguous())) and not out[:, :, :-5].any()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_rows_without_memory_are_refused(grad):
+  """They have an address of nothing; a call would give back memory that nobody wrote."""
+  rot, positions = rotary.make_rotary(64, device=DEV), torch.arange(3, device=DEV)
+  q = torch.randn(2, 4, 3, 64, device=DEV).requires_grad_(grad)
+  with pytest.raises((ValueError, RuntimeError)):
+    torch.func.functionalize(lambda x: rotary.rotate(rot, positions, x))(q)
+  with FakeTensorMode(allow_non_fake_inputs=True) as mode, pytest.raises((ValueError, RuntimeError)):
+    rotary.rotate(rot, positions, mode.from_tensor(q))
+  with FakeTensorMode(allow_non_fake_inputs=True) as mode, pytest.raises((ValueError, RuntimeError)):
+    rotary.rotate(rot, positions, q, mode.from_tensor(q))
 
 
 def test_refusals():

@@ -366,6 +366,7 @@ SplashTensor describe_row_tensor(const at::Tensor& t, const char* name, bool f32
   require_row_type(type, name, f32_too);
   d.dtype = type == at::kBFloat16 ? SPLASH_BF16 : type == at::kHalf ? SPLASH_F16 : SPLASH_F32;
   d.data = t.data_ptr();
+  TORCH_CHECK_VALUE(d.data != nullptr || t.numel() == 0, name, ": a tensor without memory (a fake or a functional one?)");
   for (int i = 0; i < 4; ++i) d.size[i] = t.size(i), d.stride[i] = t.stride(i);
   return d;
 }
@@ -650,16 +651,18 @@ std::tuple<at::Tensor, at::Tensor> rotated(const RotaryTable& table, const at::T
   at::Tensor out[2];
   SplashRotateArgs a{};
   at::Tensor in[2];
+  bool any = false;
   for (int i = 0; i < 2; ++i) {
     if (i == 1 && !z.has_value()) continue;
     const at::Tensor& t = i == 0 ? x : *z;
     in[i] = usable(t);
     out[i] = fresh_like(in[i]);
     if (out[i].numel() == 0) continue;
+    any = true;
     a.x[i] = describe_row_tensor(in[i], "rotate", true);
     a.y[i] = describe_row_tensor(out[i], "rotate", true);
   }
-  if (a.x[0].data != nullptr || a.x[1].data != nullptr) {
+  if (any) {
     a.positions = positions.data_ptr();
     a.positions_are_64 = positions.scalar_type() == at::kLong;
     a.position_stride = positions.size(0) == 1 ? 0 : positions.stride(0);
