@@ -8,6 +8,7 @@ import subprocess
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from oracle import pages_ref
 from tokamax_b200 import _native
@@ -65,6 +66,17 @@ def test_calls_are_not_recorded():
   for call in (lambda x: _choose(q=x), lambda x: kv_cache.bound_pages(cache, bounds, i[None], i, 1) or x):
     with pytest.raises(NotImplementedError, match="recorded"):
       torch.jit.trace(call, q, check_trace=False)
+
+
+def test_calls_are_not_recorded_by_make_fx():
+  cache = _cache()
+  bounds, i = kv_cache.make_page_bounds(cache), torch.zeros(1, dtype=torch.int32)
+  q = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
+  for call in (lambda x: _choose(q=x), lambda x: kv_cache.bound_pages(cache, bounds, i[None], i, 1) or x,
+               lambda x: kv_cache.attend(cache, x, i[None], i), lambda x: kv_cache.append(cache, x, x, i[None]) or x,
+               lambda x: kv_cache.read(cache, i[None], i, 1)):
+    with pytest.raises(NotImplementedError, match="recorded by make_fx"):
+      make_fx(call)(q)
 
 
 def test_queries_with_a_derivative_are_refused():

@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from oracle import rotary_ref
 from tokamax_b200 import _native
@@ -98,6 +99,12 @@ def test_calls_are_not_recorded_and_tangents_refused():
   for dtype in (torch.float64, torch.int32, torch.complex64):
     with pytest.raises(NotImplementedError, match="not built"):
       _call(q=q.to(dtype))
+
+
+def test_calls_are_not_recorded_by_make_fx():
+  """A graph of it would give back what this call's rows became, whatever it is given."""
+  with pytest.raises(NotImplementedError, match="recorded by make_fx"):
+    make_fx(lambda x: _call(q=x))(torch.zeros(1, 2, 3, 16))
 
 
 def _args():

@@ -14,6 +14,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
@@ -350,10 +351,14 @@ void require_no_grad(const at::Tensor& t, const char* name) {
                               " has a tangent of forward mode: the cache's operators have none");
 }
 
-// A recorded graph would hold what allocates the results and not the launch that writes them.
-void require_not_traced() {
-  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "the cache's operators cannot be recorded by torch.jit.trace");
+// A recorded graph (of torch.jit.trace or make_fx) would hold results of this call, or what allocates them, and not the launch that
+// writes them.
+void require_not_recorded(const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), what, " cannot be recorded by torch.jit.trace");
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(), what,
+                              " cannot be recorded by make_fx");
 }
+void require_not_traced() { require_not_recorded("the cache's operators"); }
 
 void require_row_type(at::ScalarType type, const char* name, bool f32_too) {
   TORCH_CHECK_NOT_IMPLEMENTED(type == at::kBFloat16 || type == at::kHalf || (f32_too && type == at::kFloat), name, ": ", type,
@@ -718,7 +723,7 @@ struct Rotation : torch::autograd::Function<Rotation> {
 };
 
 std::tuple<at::Tensor, Maybe> rotate(const std::shared_ptr<RotaryTable>& table, const at::Tensor& positions_in, const at::Tensor& q, const Maybe& k) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "rotate cannot be recorded by torch.jit.trace");
+  require_not_recorded("rotate");
   const at::Tensor positions = usable_positions(positions_in, q);
   const at::Tensor* const both[2] = {&q, k.has_value() ? &*k : nullptr};
   for (int i = 0; i < 2; ++i) {

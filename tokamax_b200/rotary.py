@@ -134,7 +134,7 @@ def rotate(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Te
   transposed, is not copied, and results lie as the inputs do.  (Strides that are no multiples of eight, or rows that begin between
   two boundaries of 16 bytes: a contiguous copy is turned.)  Products are of 32 bits, rounded to the type once.
 
-  Gradients go to q and k: the rotation back, which keeps nothing of a call but its positions.  Tangents of forward mode and
-  ``torch.jit.trace`` are refused."""
+  Gradients go to q and k: the rotation back, which keeps nothing of a call but its positions.  Tangents of forward mode,
+  the transforms of ``torch.func``, ``torch.jit.trace`` and ``make_fx`` are refused; ``torch.compile`` runs the call as it is."""
   out_q, out_k = _native.host().rotate(rotary.native, positions, q, k)
   return out_q if k is None else (out_q, out_k)
