@@ -520,6 +520,21 @@ def test_two_graphs_with_workspaces_side_by_side():
   assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_compiled_calls_give_the_same_and_transforms_are_refused():
+  store = Store([700, 300], heads=2, d=64, page=16)
+  bounds, q = kv_cache.make_page_bounds(store.cache), torch.randn(2, 4, 1, 64, device=DEV, dtype=torch.bfloat16)
+
+  def step(q):
+    kv_cache.bound_pages(store.cache, bounds, store.table, store.lengths, 700)
+    return kv_cache.attend(store.cache, q, *kv_cache.choose_pages(store.cache, bounds, q, store.table, store.lengths, 8), logits_scale=0.1) * 2.0
+
+  assert torch.equal(torch.compile(step, backend="eager")(q), step(q))
+  choose = lambda x: kv_cache.choose_pages(store.cache, bounds, x, store.table, store.lengths, 8)  # noqa: E731
+  for transform in (lambda: torch.func.vmap(choose)(q[None]), lambda: torch.func.grad(lambda x: step(x).sum())(q)):
+    with pytest.raises((RuntimeError, NotImplementedError)):
+      transform()
+
+
 def test_refusals():
   store = Store([20], heads=2, d=64)
   bounds, other = kv_cache.make_page_bounds(store.cache), kv_cache.make_page_bounds(Store([20, 20], heads=2, d=64).cache)

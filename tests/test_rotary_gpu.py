@@ -303,6 +303,33 @@ def test_a_captured_training_step():
   assert torch.equal(got, step())
 
 
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_calls_give_the_same(backend):
+  rot, positions = rotary.make_rotary(64, device=DEV), torch.arange(6, device=DEV)
+
+  def step(q, k):
+    out_q, out_k = rotary.rotate(rot, positions, q * 0.5, k)
+    return out_q.sum(1) + 2.0 * out_k.sum(1)
+
+  results = []
+  for call in (step, torch.compile(step, backend=backend)):
+    q, k = _rows(2, 4, 6, 64, torch.float32, 0).requires_grad_(True), _rows(2, 2, 6, 64, torch.float32, 1, False).requires_grad_(True)
+    out = call(q, k)
+    results.append((out, *torch.autograd.grad(out.square().sum(), (q, k))))
+  assert all(torch.equal(a, b) for a, b in zip(*results))
+  with torch.no_grad():
+    assert torch.equal(torch.compile(step, backend=backend)(q, k), out)
+
+
+def test_transforms_are_refused():
+  rot, positions, q = rotary.make_rotary(64, device=DEV), torch.arange(6, device=DEV), _rows(2, 4, 6, 64, torch.float32, 0)
+  call = lambda x: rotary.rotate(rot, positions, x)  # noqa: E731
+  for transform in (lambda: torch.func.grad(lambda x: call(x).sum())(q), lambda: torch.func.vjp(call, q), lambda: torch.func.jvp(call, (q,), (q,)),
+                    lambda: torch.func.vmap(call)(q[None]), lambda: torch.func.vmap(lambda p: rotary.rotate(rot, p, q))(positions[None])):
+    with pytest.raises((RuntimeError, NotImplementedError)):
+      transform()
+
+
 def test_offsets_beyond_32_bits():
   """The last rows of a tensor of over 2^32 bytes."""
   rot = rotary.make_rotary(64, device=DEV)
