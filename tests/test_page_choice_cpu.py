@@ -198,6 +198,13 @@ def test_workspaces():
   assert lib.splash_cache_attend_tables(C.byref(b), None) == -1
 
 
+def test_up_to_8192_pages_need_no_workspace():
+  lib, a = _native.lib(), _args("SplashCacheChooseArgs")
+  for n_table, size in ((8192, 0), (8193, 2 * 3 * 8193 * 4)):
+    a.n_table = n_table
+    assert lib.splash_cache_choose_workspace_bytes(C.byref(a)) == size
+
+
 def test_structs_have_the_layout_the_c_header_gives_them(tmp_path):
   root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
   structs = {"SplashPageBounds": "scales", "SplashCacheBoundArgs": "newest", "SplashCacheChooseArgs": "workspace_bytes", "SplashRotateArgs": "factor"}

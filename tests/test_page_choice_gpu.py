@@ -247,6 +247,25 @@ def test_wide_tables(n_table):
   assert small[0].shape == (2, 1, 2, 40)
 
 
+@pytest.mark.parametrize("d,group", [(64, 2), (80, 9), (128, 4), (160, 5), (256, 2), (256, 128)])
+@pytest.mark.parametrize("n_table", [1024, 1025, 8191, 8192, 8193, 20000])
+def test_tables_on_both_sides_of_each_limit_in_every_width(n_table, d, group):
+  """Four warps a CTA up to 1024 pages, eight above; scores on the chip up to 8192, in a workspace above; a cluster a row where rows are
+  few, a CTA where they are many.  128 q heads of 256 channels and 8192 pages are the most shared memory that a CTA asks for."""
+  pool = Pool([16 * 300 + 4], heads=1, d=d, seed=n_table)
+  table = torch.arange(n_table, dtype=torch.int32) * 7 % pool.cache.n_pages
+  q, count = pool.q(group, 1)[:1].to(DEV), 500
+  score = pages_ref.scores(q[0, :, 0].cpu(), pool.codes[table.long(), 0], pool.scales[table.long(), 0])
+  for pages in (n_table, n_table - 333):
+    order = score[:pages].clone()
+    order[0] = order[-1] = math.inf
+    taken = torch.sort(torch.sort(order, descending=True, stable=True).indices[:count]).values
+    for rows in (1, 300):  # (sequences of the same pages)
+      lengths = torch.full((rows,), pages * 16 - 3, dtype=torch.int32, device=DEV)
+      tables, tokens = kv_cache.choose_pages(pool.cache, pool.bounds, q.expand(rows, -1, -1, -1), table[None].expand(rows, -1).to(DEV), lengths, count)
+      assert torch.equal(tables.cpu(), table[taken].expand(rows, 1, 1, -1)) and (tokens == count * 16 - 3).all()
+
+
 def test_drafted_tokens_choose_as_they_would_one_by_one():
   pool = Pool([1000, 37, 64])
   q = pool.q(4, 5).to(DEV)
