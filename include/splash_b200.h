@@ -610,8 +610,9 @@ size_t splash_cache_choose_workspace_bytes(const SplashCacheChooseArgs* args);
  * Pair i of a row's first `dim` channels, (x[i], x[i + dim / 2]) or, interleaved, (x[2i], x[2i + 1]), is turned by position *
  * turns[i] and multiplied by `factor`; the other channels are copied:
  *   y0 = factor * (x0 cos a - x1 sin a), y1 = factor * (x1 cos a + x0 sin a)
- * turns [dim / 2]: 2^64ths of a whole turn for each token, so that the angle of any position (a 64-bit product, whose overflow
- * is whole turns) has no error but that of `turns`.  inverse: by the negative angle, which is the gradient's way back.
+ * turns [dim / 2]: 2^64ths of a whole turn for each token, so that a position's product with them (64 bits, whose overflow is whole
+ * turns) has no error but that of `turns`.  Sine and cosine are taken of its upper 32 bits, rounded to 24: up to 2^-26 of a turn off, for fp32
+ * rows 2^-28, at any position.  inverse: by the negative angle, which is the gradient's way back.
  * x and y: up to two tensors each ([batch, heads, tokens, head_dim], one type of bf16, f16, f32; the same sizes but for heads; data
  * NULL: none), strides multiples of 8 elements; x may be y.  Products and sums are of 32 bits.
  * ---------------------------------------------------------------------------------------- */

@@ -75,6 +75,20 @@ def test_far_positions_and_scalings(scaling):
   _check(rotary.rotate(rot, positions.int(), q), q, positions, freq, factor=factor)
 
 
+def test_sines_and_cosines_of_f32_rows_are_right_to_their_last_places():
+  """Pairs (1, 0) become cosine and sine.  An angle is cut off at 2^-32 of a turn (pi 2^-31), what it is beyond whole quarters rounded to
+  24 bits (2^-24 of it, and so at most of a sine that is near 0, or of one above 0.7), sine and cosine to 2 units in the last place
+  (2^-22): below pi 2^-31 + 2^-21 of each."""
+  freq = [math.pi / 2 * (n % 4) + 1e-4 * n * n for n in range(1, 33)]  # close to the axes, and farther from them as positions grow
+  positions = torch.arange(-300, 300, device=DEV)
+  q = torch.zeros(1, 1, 600, 64, device=DEV)
+  q[..., :32] = 1.0
+  out = rotary.rotate(rotary.make_rotary(64, frequency=freq, device=DEV), positions, q)[0, 0].cpu().double()
+  angle = rotary_ref.angles(positions.cpu(), freq)
+  for got, want in ((out[:, :32], angle.cos()), (out[:, 32:], angle.sin())):
+    assert ((got - want).abs() <= math.pi * 2.0 ** -31 + 2.0 ** -21 * want.abs() + 1e-15).all()
+
+
 def test_given_frequencies_whole_turns_and_the_factor():
   freq = np.array([0.0, math.pi / 2, 2 * math.pi, -1.0])  # none, a quarter, (almost) a whole one, backwards
   rot = rotary.make_rotary(8, frequency=torch.tensor(freq), factor=-2.0, device=DEV)

@@ -3,12 +3,16 @@
 // Mathematics.  Pair i of a row's first channels, as a complex number, times factor * exp(2 pi I * position * turns[i]); the gradient is
 // the product with the conjugate.  Angles are fixed-point fractions of a whole turn, 64 bits: position * turns modulo 2^64 drops
 // whole turns exactly, at any position, with one integer multiplication, where a product in floating point loses the
-// fraction of a turn as positions grow (32 bits: 0.06 radians at 10^6).  The 32 high bits go to sincospi as half turns.
+// fraction of a turn as positions grow (32 bits: 0.06 radians at 10^6).  The 32 high bits go to sincospi as half turns, in 24 bits: up to
+// 2^-25 of a half turn off, 1e-7 of a pair, which rows of 16 bits do not see.  For rows of 32 bits whole quarters of a turn are taken off first:
+// what is left has 24 bits of its own, and sine and cosine are right to their last places at any angle.
 //
 // Bound by memory: a value is read once and written once.  A thread has the same eight pairs of a token for four heads: an angle, its
 // sine and cosine are worked out once for them, and eight loads of 16 bytes are in flight.  4 x 4096 tokens, 32 + 8 heads of 128, bf16:
 // 54.8 us, 6.1 TB/s (a plain copy of the same tensors 58.4, each input and output once at the copy rate 51.3); with two heads a
-// thread 70, with ten 59.6, forty 66.6; eight loads ahead 74.  2 x 8192 forward and back 104.7 (floor 102.6).  Interleaved 57.8.
+// thread 70, with ten 59.6, forty 66.6; eight loads ahead 74.  2 x 8192 forward and back 104.7 (floor 102.6).  Interleaved 55.0.  f32 105.5 (floor
+// 102.6), interleaved 125.  80 channels, bf16 (floor 32.1): all of them turned 37.3; 72 or 40, whose pairs come in fours, 40; 20, whose pairs go one
+// by one, two bytes a load, 101.
 // Evicting loads and stores, and blocks of 128, +-1 %.
 #include "cache_common.cuh"
 
@@ -113,8 +117,18 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
                                                             : (int64_t)__ldg(static_cast<const int32_t*>(p.positions) + at));
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      const int32_t angle = (int32_t)(position * __ldg(p.turns + lane * kPairs + i) >> 32);  // 2^-31 of a half turn
-      sincospif((float)angle * 0x1p-31f, &sine[i], &cosine[i]);
+      const uint32_t angle = (uint32_t)(position * __ldg(p.turns + lane * kPairs + i) >> 32);  // 2^-31 of a half turn
+      if constexpr (kDType == SPLASH_F32) {
+        const uint32_t quarters = (angle + 0x20000000u) >> 30;  // (to the nearest)
+        float s, c;
+        sincospif((float)(int32_t)(angle - (quarters << 30)) * 0x1p-31f, &s, &c);
+        sine[i] = quarters & 1 ? c : s;
+        cosine[i] = quarters & 1 ? s : c;
+        if (quarters & 2) sine[i] = -sine[i];
+        if ((quarters + 1) & 2) cosine[i] = -cosine[i];
+      } else {
+        sincospif((float)(int32_t)angle * 0x1p-31f, &sine[i], &cosine[i]);
+      }
       sine[i] *= p.factor * p.sign;
       cosine[i] *= p.factor;
     }

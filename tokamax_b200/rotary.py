@@ -8,7 +8,9 @@ splash kernels and for the cache of :mod:`tokamax_b200.kv_cache`:
   q, k = rotary.rotate(rot, positions, q, k)
 
 A pair of channels is turned by its position times a frequency.  Angles are fractions of a whole turn in 64 bits, which wrap
-as turns do: a pair's frequency is held to 2^-65 of a turn a token, and the angle of a token at position 10^9 to 3e-11 of a turn.
+as turns do: a pair's frequency is held to 2^-65 of a turn a token, and its product with a position of 10^9 to 3e-11 of a turn.  Sine and
+cosine are taken of the upper 32 bits in 24 bits: up to 1.5e-8 of a turn off, at any position, for rows of 16 bits, 4e-9 for
+float32 rows.
 """
 from __future__ import annotations
 
