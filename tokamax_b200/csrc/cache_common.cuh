@@ -76,9 +76,6 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
 
 // A kernel that is launched early comes up before the one ahead of it in the stream has ended (from when all of that one's CTAs have
 // said so); what the wait comes before sees all that the other has written.  Without such a launch both do nothing.

@@ -357,7 +357,7 @@ struct ChooseParams {
   int32_t* table_lengths;
   uint32_t* keys;  // scores of a row's pages, [rows][n_table], where shared memory has no room for them; else NULL
   int64_t q_stride_b, q_stride_h, q_stride_s, table_stride, n_pages;
-  int32_t dtype, batch, kv_heads, heads_per_kv, q_len, n_table, page_size, page_shift, head_dim, row, count, first, last;
+  int32_t dtype, kv_heads, heads_per_kv, q_len, n_table, page_size, page_shift, head_dim, row, count, first, last;
 };
 
 constexpr int kKeysOnChip = 8192;         // pages of a row whose scores, and numbers, shared memory holds
@@ -819,7 +819,6 @@ static int cache_choose(const SplashCacheChooseArgs& a, cudaStream_t stream) {
   p.table_stride = a.table_stride;
   p.n_pages = c.n_pages;
   p.dtype = a.q.dtype;
-  p.batch = (int32_t)a.q.size[0];
   p.kv_heads = c.kv_heads;
   p.heads_per_kv = (int32_t)(a.q.size[1] / c.kv_heads);
   p.q_len = (int32_t)a.q.size[2];
