@@ -60,6 +60,14 @@ def test_tables_that_cannot_be_made(kw):
     rotary.make_rotary(**dict(dict(dim=8, device="cpu"), **kw))
 
 
+@pytest.mark.parametrize("kw", [dict(factor=1e39), dict(factor=-math.inf), dict(scaling=rotary.Scaling("by_parts", original=9, attention=1e300))])
+def test_factors_that_32_bits_do_not_hold_are_refused(kw):
+  """The kernels' factor is one: infinity times a sine of 0 would be NaN."""
+  with pytest.raises(ValueError, match="finite in 32 bits"):
+    rotary.make_rotary(8, device="cpu", **kw)
+  assert rotary.make_rotary(8, device="cpu", factor=3e38).factor == 3e38
+
+
 def test_turns():
   """The part of a turn that a token is, to 2^-65, whole turns left out."""
   freq = [1.0, 2 * math.pi + 0.25, -0.125, 0.0]

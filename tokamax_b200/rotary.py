@@ -121,8 +121,8 @@ def make_rotary(dim: int, *, base: float = 10000.0, scaling: Scaling | None = No
     if freq.shape != (dim // 2,) or not np.isfinite(freq).all():
       raise ValueError(f"expected {dim // 2} finite frequencies, got {freq.shape}")
   factor = attention if factor is None else float(factor)
-  if not math.isfinite(factor):
-    raise ValueError(f"factor must be finite, got {factor}")
+  if not abs(factor) <= torch.finfo(torch.float32).max:
+    raise ValueError(f"factor must be finite in 32 bits, got {factor}")
   parts = [round(Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64 for f in freq.tolist()]  # (whole turns are none)
   turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in parts], dtype=torch.int64, device=device)
   return _of_turns(dim, interleaved, factor, turns)
