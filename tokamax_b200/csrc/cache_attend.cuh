@@ -290,6 +290,13 @@ __device__ __forceinline__ int64_t share_of(int64_t total, int ctas) {  // a uni
   return share > kWarps ? share : kWarps;
 }
 
+// (What a kernel of sequences' tables works out from other parameters it is not given again: the compiler finds other registers for it,
+// and some calls take 1 to 3 % longer.)
+template <bool kByHead>
+__device__ __forceinline__ int items_of_table(const AttendParams& p) {
+  return kByHead ? p.items : p.kv_heads * p.row_tiles;
+}
+
 struct Start {  // where a CTA's share begins
   int64_t total, before;  // cost of all items, and of those of the sequences before b
   int64_t share;
@@ -298,10 +305,10 @@ struct Start {  // where a CTA's share begins
 
 // All threads of a CTA of kWarps; `scratch`: kWarps + 2 words of shared memory of 8 bytes.  Sequences go by the threads of a
 // CTA at a time; a second look is taken only where there are more of them than that.
-template <int kUnit>
+template <int kUnit, bool kByHead>
 __device__ Start find_start(const AttendParams& p, int64_t* scratch) {
   constexpr int kThreads = kWarps * 32;
-  const int64_t per_sequence = p.items;
+  const int64_t per_sequence = items_of_table<kByHead>(p);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t* const found = scratch + kWarps;
   const bool keep = blockIdx.x == 0;  // this CTA writes down where the sequences start
@@ -376,6 +383,7 @@ __device__ __forceinline__ Rows rows_of(const AttendParams& p, int b, int item) 
 }
 
 // Eight channels of a row, from the sums of all its keys.
+template <bool kByHead>
 __device__ __forceinline__ void finish_row(const AttendParams& p, const Rows& rows, int row, int d, float (&x)[8], float m, float l) {
   const int b = rows.b, i = rows.query + row / p.heads_per_kv, h = rows.head * p.heads_per_kv + row % p.heads_per_kv;
   float weight = 1.f;
@@ -389,7 +397,7 @@ __device__ __forceinline__ void finish_row(const AttendParams& p, const Rows& ro
   for (int k = 0; k < 8; ++k) x[k] *= weight;
   if (d < p.head_dim_v) store8(p.o, p.dtype, b * p.o_stride_b + h * p.o_stride_h + i * p.o_stride_s + d, x);
   if (d == 0) {
-    const int64_t to = ((int64_t)b * p.q_heads + h) * p.queries + i;
+    const int64_t to = ((int64_t)b * p.q_heads + h) * (kByHead ? p.queries : p.q_len) + i;
     if (p.lse != nullptr) p.lse[to] = l == 0.f ? p.mask_value : (m + __log2f(l)) * kLn2;
     if (p.max_logits != nullptr) p.max_logits[to] = l == 0.f ? p.mask_value : m * kLn2;
   }
@@ -414,7 +422,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
   if (!kByHead || !p.whole) grid_dependents_launch();  // the joining kernel may come up beside this one; it waits for its end
   if (kByHead) grid_dependency_wait();     // (where this one has come up beside the kernel that chose its pages)
 
-  const int per_sequence = p.items;
+  const int per_sequence = items_of_table<kByHead>(p);
   const bool clustered = kByHead && p.cluster > 1;
   const int rank = clustered ? blockIdx.x % (unsigned)p.cluster : 0;
   int64_t at, end, before, share_begin;  // in the measure of shares; before: what lies before sequence b
@@ -423,7 +431,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     at = kByHead ? blockIdx.x / (unsigned)p.cluster : blockIdx.x;
     end = (int64_t)p.batch * per_sequence;
   } else {
-    const Start start = find_start<kUnit>(p, reinterpret_cast<int64_t*>(smem));
+    const Start start = find_start<kUnit, kByHead>(p, reinterpret_cast<int64_t*>(smem));
     __syncthreads();  // (its scratch is about to be q's place)
     at = share_begin = (int64_t)blockIdx.x * start.share;
     end = min(at + start.share, start.total);
@@ -483,7 +491,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
     const int u = u0 + warp + (turn + lane / kTiles) * warps, token = keys.lo + u * kUnit + lane % kTiles * 16;
     const int page = u < u1 && token < keys.hi ? __ldg(p.page_table + b * p.table_stride + (token >> p.page_shift)) : -1;
     if (page < 0 || page >= p.n_pages) return kNowhere;
-    const uint32_t first = (uint32_t)(page * p.kv_heads + head) << (p.page_shift - 4);
+    const uint32_t first = (uint32_t)(page * p.kv_heads + (kByHead ? head : item / p.row_tiles)) << (p.page_shift - 4);
     return first + ((token & (p.page_size - 1)) >> 4);
   };
   uint32_t places, next_places;
@@ -531,7 +539,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
 
   while (next_item()) {
     const Rows rows = rows_of<kByHead>(p, b, item);
-    head = rows.head;
+    if (kByHead) head = rows.head;
     const int row0 = item % p.row_tiles * kRows;
     const int n_rows = min(kRows, p.q_len * heads - row0);
 
@@ -550,7 +558,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
       const int r = (pass * warps + warp) * kAtOnce + lane / kLanes;
       raw[pass] = make_uint4(0, 0, 0, 0);
       if (r < n_rows && piece * 8 < p.head_dim) {
-        const int i = query_of(r), h = head * heads + first_row + r - i * heads;
+        const int i = query_of(r), h = rows.head * heads + first_row + r - i * heads;
         raw[pass] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + rows.b * p.q_stride_b + h * p.q_stride_h +
                                                          (rows.query + first_query + i) * p.q_stride_s + piece * 8));
       }
@@ -1123,7 +1131,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
         }
         continue;
       }
-      finish_row(p, rows, row0 + r, d, x, most, sum);
+      finish_row<kByHead>(p, rows, row0 + r, d, x, most, sum);
     }
     if (clustered) {  // (a cluster has one item)
       cluster_sync();
@@ -1140,7 +1148,7 @@ __global__ void __maxnreg__(Shape::kMostRegisters) cache_attend_kernel(const __g
           for (int k = 0; k < 8; ++k) x[k] = fmaf(y[k], weight, x[k]);
           sum = fmaf(from[c * 12 + 9], weight, sum);
         }
-        finish_row(p, rows, row0 + id / (Shape::kV / 8), id % (Shape::kV / 8) * 8, x, most, sum);
+        finish_row<kByHead>(p, rows, row0 + id / (Shape::kV / 8), id % (Shape::kV / 8) * 8, x, most, sum);
       }
       return;
     }
@@ -1171,7 +1179,7 @@ __global__ void __launch_bounds__(kJoinThreads, kAhead > 2 ? 2 : 4) cache_attend
   const int lot = threadIdx.x / kEach, d = threadIdx.x % kEach * 8;
   const int64_t share = share_of(p.starts[p.batch], ctas);
   for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
-    const int64_t before = p.starts[b], cost = quotient(p.starts[b + 1] - before, p.items);
+    const int64_t before = p.starts[b], cost = quotient(p.starts[b + 1] - before, items_of_table<kByHead>(p));
     const int64_t first = before + blockIdx.x * cost + p.item_cost;  // unit of this item
     const int64_t c0 = quotient(first, share), c1 = cost > 0 ? quotient(first + cost - p.item_cost - 1, share) : c0 - 1;
     if (c0 == c1) continue;  // written already
@@ -1248,7 +1256,7 @@ __global__ void __launch_bounds__(kJoinThreads, kAhead > 2 ? 2 : 4) cache_attend
         }
         __syncthreads();
       }
-      if (mine && slice == 0) finish_row(p, rows, row0 + r, d, x, most, sum);
+      if (mine && slice == 0) finish_row<kByHead>(p, rows, row0 + r, d, x, most, sum);
     }
   }
 }
@@ -1259,14 +1267,14 @@ __global__ void __launch_bounds__(kJoinThreads, kAhead > 2 ? 2 : 4) cache_attend
 template <typename Shape, bool kByHead>
 static int launch(const AttendParams& p, int warps, int ctas, cudaStream_t stream) {
   auto kernel = cache_attend_kernel<Shape, kByHead>;
-  static_assert(Shape::smem_cluster(kMostWarps) <= 227 * 1024);
+  constexpr int kMostShared = kByHead ? Shape::smem_cluster(kMostWarps) : Shape::smem(kMostWarps);
+  static_assert(kMostShared <= 227 * 1024);
   static std::atomic<uint64_t> ready{0};  // devices that know how much shared memory the kernel takes
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return SPLASH_ERR_CUDA;
   const uint64_t bit = 1ull << (device & 63);
   if (device > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem_cluster(kMostWarps)) != cudaSuccess)
-      return SPLASH_ERR_CUDA;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return SPLASH_ERR_CUDA;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const int64_t items = (int64_t)p.items * p.batch;
