@@ -1400,7 +1400,7 @@ static int64_t items_of(const SplashCacheAttendArgs& a) {
 
 // Tables by head are of much the same length (so many pages of long sequences): an item can be one cluster's, of 1, 2, 4 or 8 CTAs of
 // 4 or 8 warps, without shares to look for and a second launch.  What a call takes is estimated for each such form, in tokens of one
-// SM with all its warps (265 a us, eight rows of 128 channels in int4), and the least one taken:
+// SM with all its warps (265 a us, eight rows of 128 channels in int4: measured there alone, other shapes go by it too), and the least one taken:
 //   * an SM has ceil(CTAs / SMs) of an item's parts, as many at a time as it holds; with 4, 8 and 12 warps it gets to 0.57, 0.92 and 0.97
 //     of its rate, and another turn costs 4 us more (8 where it is clusters', which need room for all of their CTAs);
 //   * a cluster's barriers and sums 0.35 us for each doubling; a warp has a unit at least;

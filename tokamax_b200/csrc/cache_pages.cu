@@ -126,7 +126,8 @@ constexpr int kWarpTokens = 64;
 // instructions beside.  A warp a page of 64 tokens, eight rows a lane in flight: 4 prompts of up to 8192 tokens, 8 heads of 128, 8.0 us (26
 // with a block of 256 threads a page and its extremes by way of shared memory, 9.6 with quotients of 64 bits for pages and heads and two
 // instructions for an extraction, 8.6 with four rows in flight, 10.3 with 32 tokens a warp); the instructions alone 3.6, memory 1.6.
-// Eight channels a lane, 16 to 32 warps on an SM, sums of two channels in an instruction: no faster.
+// Eight channels a lane, 16 to 32 warps on an SM, sums of two channels in an instruction: no faster.  e4m3 rows are twice as wide: eight in flight
+// spill 88 to 100 bytes a thread (3 x 517 tokens behind 1999 .. 6001, 3.5 us).
 // `split` warps of a block have a page of a sequence and kv head; blockIdx.x: the page (from the first that has become whole), y: the
 // sequence, z: kv heads.  A team of kTeam lanes (the power of two that holds the row's width / 16) has a
 // token's row.
